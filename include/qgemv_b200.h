@@ -91,7 +91,10 @@ static inline uint32_t qg_meta_bytes_per_block(int fmt) {
 /* Error word bits (set by kernels, read and cleared by qg_get_error). */
 #define QG_ERR_WAIT_TIMEOUT 0x1u /* a bounded wait (TMA barrier, exchange word) ran out */
 #define QG_ERR_POSITION 0x2u     /* a decode position read from device memory was past the
-                                    KV cache or the step graph's context bucket */
+                                    KV cache or the step graph's context bucket; a token's
+                                    position past the rotation table */
+#define QG_ERR_PAGE 0x4u         /* a paged cache was given a page id outside its pool, or a
+                                    slot, sequence or length outside its page table */
 
 /* ===========================================================================
  * 1. Drop-in launchers (reference: runtime/kernels/decode/decode_kernels.h)
@@ -478,6 +481,72 @@ typedef struct qg_decoder_stage_views {
 } qg_decoder_stage_views;
 cudaError_t qg_decoder_stage_buffers(qg_decoder dec, qg_decoder_stage_views* views);
 cudaError_t qg_decoder_destroy(qg_decoder dec);
+
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache for batched decode (no reference counterpart: the reference's
+ * page_words / active_pages launchers write one word per page and its attention kernels
+ * are synthetic).  Keys and values of many sequences live in two pools of fixed-size
+ * pages; a sequence is the list of its pages.  Three operators share it:
+ *   qg_qk_norm_rope_append  per-head RMSNorm and rotation of new queries and keys, keys
+ *                           and values written to their slots, in one pass;
+ *   qg_paged_attn           one new token per sequence attends to its slots;
+ *   qg_kv_evict             a sequence is cut back to a budget of slots by the attention
+ *                           weight that its slots received.
+ *
+ * Slot s of sequence b lies in page table[b * table_stride + s / page_size] at place
+ * s % page_size, for s < table_pages * page_size.  Element (page, head, place, i) of
+ * either pool is at page * page_stride + head * head_stride + place * slot_stride + i
+ * (strides in elements, multiples of 8; 64-bit offsets), so pages may be ordered
+ * [head][place][dim] or [place][head][dim].  head_dim is a multiple of 8 up to 256,
+ * page_size any number >= 1; the pools are 16-B aligned.
+ *
+ * Device data that does not fit the cache never leads to an access outside it: a page id
+ * outside [0, num_pages) or a slot, sequence or length past the table sets QG_ERR_PAGE
+ * (qg_get_error), writes to it are dropped and reads from it give zero rows.
+ * ------------------------------------------------------------------------- */
+typedef enum qg_dtype { QG_F32 = 0, QG_F16 = 1, QG_BF16 = 2 } qg_dtype;
+
+typedef struct qg_kv_pages {
+  void *k, *v;
+  int dtype;                 /* QG_F16 or QG_BF16 */
+  uint32_t num_pages, page_size, n_kv_heads, head_dim;
+  uint64_t page_stride, head_stride, slot_stride;
+  const int32_t* table;      /* [batch][table_stride] page ids */
+  uint32_t batch, table_pages, table_stride;
+} qg_kv_pages;
+
+/* New queries, keys and values of `tokens` tokens.  For token t and each query and key
+ * head x of head_dim values:
+ *   x <- x / sqrt(mean(x^2) + eps) * norm        (q_norm / k_norm; NULL: not normalised)
+ *   (a, b) <- (a cos - b sin, a sin + b cos)     for the pairs of the first rot_dim values
+ * with the cosines and sines of row positions[t] of `rope` ([rope_rows][rot_dim] fp32:
+ * rot_dim / 2 cosines, then the sines; 16-B aligned).  Pair i is (2i, 2i + 1) for
+ * QG_PAIRS_ADJACENT, (i, i + rot_dim / 2) for QG_PAIRS_HALVES; rot_dim is 0 (no rotation,
+ * rope unused) or a multiple of 16 up to head_dim.  All in fp32, rounded once: queries
+ * to q_out (same type as q; may be q itself), keys and values to slot slots[t] (NULL: the
+ * position) of sequence seqs[t] (NULL: t).  positions[t] < 0 marks a padding row: its
+ * q_out is zero, nothing is appended, slots[t] and seqs[t] are not read.  slots[t] < 0
+ * appends nothing.  A position past the table sets QG_ERR_POSITION and gives a padding
+ * row.  Two tokens of one call must not name the same slot.
+ * q, k, v: heads of a token are contiguous, token t starts at t * {q,k,v}_stride elements
+ * (multiples of 16 bytes; so the three may be one fused projection); 16-B aligned. */
+#define QG_PAIRS_ADJACENT 0
+#define QG_PAIRS_HALVES 1
+typedef struct qg_append {
+  const void *q, *k, *v;
+  void* q_out;
+  int dtype;                 /* of q, k, v and q_out: QG_F32, QG_F16 or QG_BF16 */
+  uint32_t tokens, n_q_heads;
+  uint64_t q_stride, k_stride, v_stride, q_out_stride;
+  const float *q_norm, *k_norm;
+  float eps;
+  const float* rope;
+  uint32_t rope_rows, rot_dim;
+  int pairs;
+  const int32_t *positions, *slots, *seqs;
+} qg_append;
+cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
+                                   cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------
  * GGUF ingest (host code; the reference's reader is runtime/apps/gguf_probe/main.cpp:124-631):

@@ -1,0 +1,177 @@
+"""Paged key-value cache for batched decode: torch front end of the qg_kv_pages entry points
+(include/qgemv_b200.h has the formulas).
+
+* `PagedCache` -- the key and value pools, seen as [page, head, place, dim], and the page
+  list of every sequence.
+* `qk_norm_rope_append` -- normalise and rotate new queries and keys, write keys and values
+  to their slots.
+
+Device memory and streams only; every computation happens in the library.  Every call takes
+`stream` (default: the current one) and allocates what it returns on that stream, unless the
+caller passes the output; tensors of other streams are the caller's to order.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int, c_uint32, c_uint64, c_void_p
+
+import torch
+
+from ._lib import CudaError, lib
+
+QG_ERR_POSITION = 0x2
+QG_ERR_PAGE = 0x4
+
+DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # qg_dtype
+PAIRS = {"adjacent": 0, "halves": 1}
+
+
+class KvPagesC(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int),
+                ("num_pages", c_uint32), ("page_size", c_uint32), ("n_kv_heads", c_uint32),
+                ("head_dim", c_uint32), ("page_stride", c_uint64), ("head_stride", c_uint64),
+                ("slot_stride", c_uint64), ("table", c_void_p), ("batch", c_uint32),
+                ("table_pages", c_uint32), ("table_stride", c_uint32)]
+
+
+class AppendC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+                ("dtype", c_int), ("tokens", c_uint32), ("n_q_heads", c_uint32),
+                ("q_stride", c_uint64), ("k_stride", c_uint64), ("v_stride", c_uint64),
+                ("q_out_stride", c_uint64), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("eps", c_float), ("rope", c_void_p), ("rope_rows", c_uint32),
+                ("rot_dim", c_uint32), ("pairs", c_int), ("positions", c_void_p),
+                ("slots", c_void_p), ("seqs", c_void_p)]
+
+
+def _fail(message: str):
+    raise ValueError(message)
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """Call an entry point with `device` current."""
+    fn = getattr(lib(), name)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            code = fn(*args)
+    else:
+        code = fn(*args)
+    if code != 0:
+        raise CudaError(name, code)
+
+
+def _handle(stream, device: torch.device) -> int:
+    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+
+
+def _new(stream, shape, dtype, device) -> torch.Tensor:
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _ints(t: torch.Tensor | None, n: int, name: str, device: torch.device) -> int | None:
+    """Address of a contiguous int32 vector of n entries."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
+        _fail(f"{name}: a contiguous int32 tensor of {n} entries on {device} is needed")
+    return t.data_ptr()
+
+
+def _floats(t: torch.Tensor | None, shape: tuple, name: str, device: torch.device) -> int | None:
+    """Address of a contiguous fp32 tensor of a shape."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        _fail(f"{name}: a contiguous float32 tensor of shape {shape} on {device} is needed")
+    return t.data_ptr()
+
+
+def _heads(t: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str, device: torch.device) -> int:
+    """Stride from row to row of a [rows, heads, dim] tensor whose rows are contiguous."""
+    if t.dtype != dtype or t.device != device or t.dim() != 3 or tuple(t.shape) != (rows, heads, dim):
+        _fail(f"{name}: a {dtype} tensor of shape {(rows, heads, dim)} on {device} is needed")
+    stride = t.stride()
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
+        _fail(f"{name}: the heads of one row must be contiguous")
+    return stride[0] if rows > 1 else heads * dim
+
+
+class PagedCache:
+    """Pools `k` and `v` [pages, kv heads, page size, head dim] (fp16 or bf16, any strides
+    with contiguous dims, the same for both) and `table` [sequences, pages per sequence]
+    (int32).  The caller owns them: it hands out pages by writing the table."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
+        def steps(t):  # a dimension of one entry has no step
+            return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+
+        if k.dim() != 4 or k.shape != v.shape or steps(k) != steps(v) or k.dtype != v.dtype:
+            _fail("k and v: two [pages, heads, page size, dim] tensors of one type and layout are needed")
+        if not k.is_cuda or k.device != v.device or k.device != table.device:
+            _fail("k, v and table have to be on one CUDA device (there is no CPU path)")
+        if k.dtype not in (torch.float16, torch.bfloat16) or steps(k)[3] != 1:
+            _fail("k and v: float16 or bfloat16 with contiguous dims are needed")
+        if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+            _fail("table: an int32 tensor [sequences, pages per sequence] is needed")
+        self.k, self.v, self.table = k, v, table
+        self.device, self.dtype = k.device, k.dtype
+        self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.batch, self.table_pages = table.shape
+        self.capacity = self.table_pages * self.page_size
+        stride = steps(k)
+        self.c = KvPagesC(k.data_ptr(), v.data_ptr(), DTYPE_CODES[k.dtype], self.num_pages,
+                          self.page_size, self.n_kv_heads, self.head_dim, stride[0], stride[1],
+                          stride[2], table.data_ptr(), self.batch, self.table_pages,
+                          table.stride(0) if self.batch > 1 else self.table_pages)
+        self._ref = ctypes.byref(self.c)
+
+    @staticmethod
+    def empty(num_pages: int, n_kv_heads: int, page_size: int, head_dim: int, batch: int,
+              table_pages: int, dtype=torch.float16, device="cuda") -> "PagedCache":
+        """A cache of zeroed pools whose table names no page yet (every entry -1)."""
+        shape = (num_pages, n_kv_heads, page_size, head_dim)
+        return PagedCache(torch.zeros(shape, dtype=dtype, device=device),
+                          torch.zeros(shape, dtype=dtype, device=device),
+                          torch.full((batch, table_pages), -1, dtype=torch.int32, device=device))
+
+
+def rope_table(rows: int, rot_dim: int, base: float = 500000.0, device="cuda") -> torch.Tensor:
+    """[rows, rot_dim] fp32: the cosines, then the sines, of row * base^(-2i / rot_dim),
+    angles in 64 bits."""
+    inv = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    angle = torch.arange(rows, dtype=torch.float64)[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+def qk_norm_rope_append(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        rope: torch.Tensor | None, positions: torch.Tensor, *,
+                        slots: torch.Tensor | None = None, seqs: torch.Tensor | None = None,
+                        q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                        eps: float = 1e-5, pairs: str = "adjacent",
+                        q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """qg_qk_norm_rope_append: q [tokens, q heads, dim], k and v [tokens, kv heads, dim] of one
+    type (views of a fused projection are fine); returns the rotated queries."""
+    dev, dim, kv = cache.device, cache.head_dim, cache.n_kv_heads
+    if q.dtype not in DTYPE_CODES or q.dim() != 3:
+        _fail("q: a [tokens, heads, dim] tensor of float32, float16 or bfloat16 is needed")
+    tokens, heads = q.shape[0], q.shape[1]
+    if pairs not in PAIRS:
+        _fail("pairs is 'adjacent' or 'halves'")
+    if q_out is None:
+        q_out = _new(stream, (tokens, heads, dim), q.dtype, dev)
+    rows, rot = (rope.shape[0], rope.shape[1]) if rope is not None else (0, 0)
+    a = AppendC(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), DTYPE_CODES[q.dtype],
+                tokens, heads, _heads(q, tokens, heads, dim, q.dtype, "q", dev),
+                _heads(k, tokens, kv, dim, q.dtype, "k", dev),
+                _heads(v, tokens, kv, dim, q.dtype, "v", dev),
+                _heads(q_out, tokens, heads, dim, q.dtype, "q_out", dev),
+                _floats(q_norm, (dim,), "q_norm", dev), _floats(k_norm, (dim,), "k_norm", dev), eps,
+                _floats(rope, (rows, rot), "rope", dev), rows, rot, PAIRS[pairs],
+                _ints(positions, tokens, "positions", dev), _ints(slots, tokens, "slots", dev),
+                _ints(seqs, tokens, "seqs", dev))
+    _call("qg_qk_norm_rope_append", dev, cache._ref, ctypes.byref(a), _handle(stream, dev))
+    return q_out
