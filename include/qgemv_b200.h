@@ -548,6 +548,43 @@ typedef struct qg_append {
 cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
                                    cudaStream_t stream);
 
+/* Attention of one new token per sequence.  Sequence b holds lens[b] slots (at most
+ * max_len, which bounds the work the launch is sized for); with window > 0 only its last
+ * `window` slots are seen.  For query head h of kv head h / (n_q_heads / n_kv_heads):
+ *   s_j = scale * q . k_j,  m = max_j s_j,  l = sum_j exp(s_j - m)
+ *   out = sum_j exp(s_j - m) v_j / l,  lse = m + ln(l)    (lse may be NULL)
+ * over the seen slots; with none (length 0) out is 0 and lse -inf.  Slots past the length
+ * are never read as numbers, whatever they hold; an infinite or NaN value in a seen V row
+ * makes that column of the output infinite or NaN.  With weight_out each seen slot's share
+ * is summed over the query heads of its kv head:
+ *   weight_out[b][kv][j] = weight_in[b][kv][j] + sum_h exp(s_hj - m_h) / l_h
+ * for every j < lens[b] (unseen slots: weight_in alone), rows of weight_stride floats;
+ * weight_in may be weight_out, or NULL for zero; slots at or past lens[b] are left alone.
+ * Scores, statistics and sums are fp32; results are deterministic.  q, out:
+ * [batch][n_q_heads][head_dim] with sequence strides in elements (multiples of 16 bytes);
+ * 16-B aligned.  `workspace`: 256-B aligned, qg_paged_attn_workspace_bytes long, its
+ * first QG_PAGED_ATTN_ZEROED bytes zero before its first use (every call leaves them
+ * zero); calls that overlap need one each. */
+#define QG_PAGED_ATTN_ZEROED 4096u
+typedef struct qg_attn {
+  const void* q;
+  void* out;
+  int dtype;                 /* of q and out */
+  uint32_t n_q_heads;
+  uint64_t q_stride, out_stride;
+  const int32_t* lens;
+  uint32_t max_len, window;
+  float scale;
+  float* lse;                /* [batch][n_q_heads] */
+  const float* weight_in;
+  float* weight_out;         /* [batch][n_kv_heads][weight_stride] */
+  uint32_t weight_stride;
+} qg_attn;
+cudaError_t qg_paged_attn_workspace_bytes(const qg_kv_pages* cache, uint32_t n_q_heads,
+                                          uint32_t max_len, int weights, size_t* bytes);
+cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* a, void* workspace,
+                          cudaStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * GGUF ingest (host code; the reference's reader is runtime/apps/gguf_probe/main.cpp:124-631):
  * header, metadata (general.alignment, general.architecture), tensor infos, the data

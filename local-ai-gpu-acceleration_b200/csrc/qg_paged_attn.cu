@@ -1,0 +1,733 @@
+// qg_paged_attn.cu -- qg_paged_attn: attention of one new token per sequence over a paged
+// key-value cache (declared in include/qgemv_b200.h).
+//
+// Mathematics.  One pass over a sequence's slots with the running maximum m, sum l and
+// weighted value sum o of a softmax, in log2 units: s = (q . k) * scale * log2 e,
+//   m' = max(m, s),  l' = l 2^(m - m') + 2^(s - m'),  o' = o 2^(m - m') + 2^(s - m') v;
+// two passes over disjoint slots join by the same rule, so a sequence is cut anywhere.
+//
+// Bound by memory: a slot's K and V rows are read once for all query heads of their kv head,
+// at 1 to 16 multiply-adds a byte.  The dot products still go to the matrix pipe, because on
+// the CUDA cores a group of 8 heads would need 8 fp32 FMAs and conversions for every 2 bytes.
+// mma.sync (m16n8k16) keeps scores, probabilities and sums in the registers of the warp that
+// loads the slots; its rate is far above the few per cent that the memory can feed, so
+// tcgen05 with its trip through tensor memory has nothing to win here.
+//
+// Work.  The unit is a block of 64 slots of one (sequence, kv head, head tile); all blocks of
+// the batch, whatever the lengths, form one line that is cut into equal ranges, one a CTA
+// (two CTAs an SM).  In a range, warp w owns slots [16 w, 16 w + 16) of every block and runs
+// on its own: it fetches its rows through its own ring of stages (cp.async, 16 bytes a lane,
+// any page size and layout; a tile's page ids are read one tile ahead) and keeps its own
+// (m, l, o).  Where a (sequence, head) ends inside the range the four warps join through
+// shared memory; where it was cut by the range, the CTA leaves a record, and the CTA that
+// arrives last joins the records in CTA order, so results do not depend on timing.
+//
+// Matrix fragments.  Rows of the A operand are query heads.  Eight heads fill rows 0-7 and
+// the rounding errors of their values rows 8-15: q = hi + lo in the cache's type, so one mma
+// gives (hi + lo) . k, fp16 pairs carrying 22 bits and bf16 pairs 16.  (A fp32 q with a bf16
+// cache takes a third term, 24 bits, in a second mma.)  q is first scaled by a power of two
+// per head to a largest value in [1, 2), so neither term leaves fp16's range.  The scores'
+// accumulators are laid out like the A operand of the next product, so probabilities go back
+// in without a shuffle, again as hi + lo; they carry a factor 2^14 (removed with l), which
+// keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
+// Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
+// matrix pipe truncates when it accumulates, and o lives for thousands of tiles.
+#include <math_constants.h>
+
+#include <algorithm>
+#include <mutex>
+#include <set>
+#include <type_traits>
+
+#include "qg_paged.cuh"
+
+namespace qg {
+namespace {
+
+constexpr uint32_t kWarps = 4;
+constexpr uint32_t kAttnThreads = kWarps * 32;
+constexpr uint32_t kTile = 16;                // slots of one warp's tile
+constexpr uint32_t kBlock = kTile * kWarps;   // slots of a block
+constexpr uint32_t kMaxCtas = 512;            // counters in the workspace's zeroed bytes
+static_assert(kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "one counter per CTA");
+constexpr float kShareBits = 14.f;            // log2 of the factor that probabilities carry
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  int dtype;
+  uint64_t q_stride, out_stride;
+  const int32_t* lens;
+  uint32_t max_len, window;
+  uint32_t n_q, group, tiles;  // query heads, per kv head, head tiles per kv head
+  float scale_log2;
+  float* lse;
+  uint32_t* arrived;           // [kMaxCtas], zero between calls
+  float* records;              // [cta][2] partial results
+  float* scores;               // [batch][n_q][score_stride], log2 units, or NULL
+  float* norm;                 // [batch][n_q]: log2 of the full sum, with scores
+  uint32_t score_stride;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// (x, y) as TERMS pairs of the 16-bit type whose sum is (x, y) to 11 (8) bits a term.
+template <typename T, int N>
+__device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    term[i] = pack2(x, y, T());
+    const float2 f = unpack2(term[i], T());
+    x -= f.x;
+    y -= f.y;
+  }
+}
+
+// Where a range of blocks is: sequence, kv head x head tile, block.
+struct Cursor {
+  uint64_t at;                       // block's place in the line
+  uint32_t b, h, j, j0, j1;          // j in [j0, j1)
+  uint32_t start, len;               // the sequence's seen slots are [start, len)
+
+  __device__ __forceinline__ void bounds(const PagedView& c, const AttnArgs& a) {
+    len = paged_len(a.lens[b], min(a.max_len, c.capacity));
+    start = a.window != 0u && len > a.window ? len - a.window : 0u;
+    j0 = start / kBlock;
+    j1 = max((len + kBlock - 1u) / kBlock, j0 + 1u);  // an empty sequence has one empty block
+  }
+  __device__ __forceinline__ void next(const PagedView& c, const AttnArgs& a, uint64_t end) {
+    ++at;
+    if (++j == j1) {
+      if (++h == c.n_kv * a.tiles) {
+        h = 0;
+        ++b;
+        if (at < end) bounds(c, a);
+      }
+      j = j0;
+    }
+  }
+};
+
+// T: cache type.  DP: head_dim rounded up to 64, 128 or 256.  MT: tiles of 8 heads.
+// EXTRA: third terms of q and of the probabilities (fp32 queries over a bf16 cache).
+template <typename T, int DP, int MT, bool EXTRA>
+struct AttnShape {
+  static constexpr uint32_t kHeads = 8u * MT;
+  static constexpr uint32_t kStage = 2u * kTile * DP * 2u;  // one warp's K and V tile
+  static constexpr uint32_t kStages = DP == 64 ? 6 : 3;
+  static constexpr uint32_t kRing = kWarps * kStages * kStage;
+  static constexpr uint32_t kQRows = MT * (EXTRA ? 24u : 16u);
+  static constexpr uint32_t kQBytes = kQRows * DP * 2u;
+  static constexpr uint32_t kSmem = kRing + kQBytes;
+  static constexpr uint32_t kRecord = kHeads * (DP + 2u);  // m[], l[], o[][]
+  static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
+  static_assert(kHeads * DP * 4u <= kStage, "a warp's sums join in its free stage");
+};
+
+template <typename T, int DP, int MT, bool EXTRA>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCtasPerSm)
+    paged_attn_kernel(const PagedView c, const AttnArgs a) {
+  using Shape = AttnShape<T, DP, MT, EXTRA>;
+  constexpr uint32_t kStages = Shape::kStages, kHeads = Shape::kHeads;
+  constexpr int kTerms = EXTRA ? 3 : 2;
+  constexpr uint32_t kChunks = DP / 8;  // 16-byte pieces of a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float join_m[kWarps][kHeads], join_l[kWarps][kHeads], q_mult[kHeads];
+  __shared__ uint64_t sum64[kWarps];
+  __shared__ uint32_t first_at[3];
+  __shared__ uint32_t is_last;
+
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
+  const uint32_t chunks = c.dim / 8u;
+  uint8_t* const ring = smem + warp * (kStages * Shape::kStage);
+  const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(smem + Shape::kRing);
+
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's range of the line of blocks
+  const uint32_t lines = c.n_kv * a.tiles;
+  uint64_t total = 0;
+  for (uint32_t b = tid; b < c.batch; b += kAttnThreads) {
+    Cursor s;
+    s.b = b;
+    s.bounds(c, a);
+    total += s.j1 - s.j0;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  if (lane == 0u) sum64[warp] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kWarps; ++w) total += sum64[w];
+  total *= lines;
+  const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), total);
+  if (blockIdx.x >= ctas) return;
+  const uint64_t r0 = blockIdx.x * total / ctas, r1 = (blockIdx.x + 1u) * total / ctas;
+  for (uint64_t base = 0, b0 = 0; b0 < c.batch; b0 += kAttnThreads) {
+    const uint32_t b = static_cast<uint32_t>(b0) + tid;
+    Cursor s;
+    uint64_t n = 0;
+    if (b < c.batch) {
+      s.b = b;
+      s.bounds(c, a);
+      n = s.j1 - s.j0;
+    }
+    uint64_t upto = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint64_t o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= static_cast<uint32_t>(off)) upto += o;
+    }
+    __syncthreads();
+    if (lane == 31u) sum64[warp] = upto;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += sum64[w];
+      all += sum64[w];
+    }
+    upto += base;
+    if (n != 0u && r0 >= (upto - n) * lines && r0 < upto * lines) {
+      const uint64_t in = r0 - (upto - n) * lines;
+      first_at[0] = b;
+      first_at[1] = static_cast<uint32_t>(in / n);
+      first_at[2] = static_cast<uint32_t>(in % n);
+    }
+    base += all;
+    if (base * lines > r0) break;
+  }
+  __syncthreads();
+  Cursor use;
+  use.at = r0;
+  use.b = first_at[0];
+  use.h = first_at[1];
+  use.bounds(c, a);
+  use.j = use.j0 + first_at[2];
+  Cursor ahead = use;
+
+  if (DP != c.dim) {  // the pieces past head_dim are never written: zero them once
+    for (uint32_t i = lane; i < kStages * Shape::kStage / 16u; i += 32u) {
+      const uint32_t r = (i / kChunks) % kTile, ch = (i % kChunks) ^ (r & 7u);
+      if (ch >= chunks) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncwarp();
+  }
+
+  // ---- fetching: lane l knows the row of slot l % 16 of the next tile
+  uint64_t row = kNoRow;
+  auto look_up = [&]() {
+    row = kNoRow;
+    if (ahead.at < r1) {
+      const uint32_t slot = ahead.j * kBlock + warp * kTile + (lane & 15u);
+      if (slot >= ahead.start && slot < ahead.len) {
+        row = paged_row(c, c.table + static_cast<size_t>(ahead.b) * c.table_stride, slot, ahead.h / a.tiles);
+      }
+      ahead.next(c, a, r1);
+    }
+  };
+  auto fetch = [&](uint32_t stage) {
+    const uint32_t to = ring_at + stage * Shape::kStage;
+#pragma unroll
+    for (uint32_t i = 0; i < kTile * kChunks / 32u; ++i) {
+      const uint32_t r = (i * 32u + lane) / kChunks, ch = (i * 32u + lane) % kChunks;
+      const uint64_t at = __shfl_sync(0xffffffffu, row, r);
+      if (ch < chunks) {
+        const uint64_t src = at == kNoRow ? 0u : at + ch * 16u;
+        const uint32_t n = at == kNoRow ? 0u : 16u;  // unseen slots arrive as zero rows
+        const uint32_t dst = to + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4);
+        cp_async_16(dst, c.k + src, n);
+        cp_async_16(dst + kTile * DP * 2u, c.v + src, n);
+      }
+    }
+  };
+  look_up();
+#pragma unroll
+  for (uint32_t s = 0; s < kStages; ++s) {
+    fetch(s);
+    cp_async_commit();
+    look_up();
+  }
+
+  uint32_t qa[MT][DP / 16][4], qx[MT][EXTRA ? DP / 16 : 1][2];
+  float o[MT][DP / 8][2], m[MT], l[MT], mult[MT];
+  uint32_t stage = 0;
+  bool fresh = true;
+
+  while (use.at < r1) {
+    const uint32_t kv = use.h / a.tiles, ht = use.h - kv * a.tiles;
+    const uint32_t heads = min(kHeads, a.group - ht * kHeads);
+    const uint32_t head0 = kv * a.group + ht * kHeads;
+
+    if (fresh) {  // ---- the queries of a new (sequence, head tile)
+      fresh = false;
+      constexpr uint32_t kPer = DP / 32;
+      for (uint32_t r = warp; r < kHeads; r += kWarps) {
+        float x[kPer];
+        float top = 0.f;
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; ++e) {
+          const uint32_t d = lane * kPer + e;
+          x[e] = 0.f;
+          if (r < heads && d < c.dim) {
+            const uint64_t at = use.b * a.q_stride + static_cast<uint64_t>(head0 + r) * c.dim + d;
+            x[e] = a.dtype == QG_F32   ? static_cast<const float*>(a.q)[at]
+                   : a.dtype == QG_F16 ? __half2float(static_cast<const __half*>(a.q)[at])
+                                       : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
+          }
+          top = fmaxf(top, fabsf(x[e]));
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        int power = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // top in [2^power, 2^(power + 1))
+        power = top == 0.f ? 0 : max(-100, min(100, power));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+        if (lane == 0u) q_mult[r] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; e += 2) {
+          uint32_t term[kTerms];
+          split_terms<T>(x[e] * down, x[e + 1] * down, term);
+          const uint32_t d = lane * kPer + e;
+#pragma unroll
+          for (int i = 0; i < kTerms; ++i) {
+            const uint32_t qr = (r / 8u) * (EXTRA ? 24u : 16u) + i * 8u + (r & 7u);
+            *reinterpret_cast<uint32_t*>(smem + Shape::kRing + qr * (DP * 2u) + (((d / 8u) ^ (qr & 7u)) << 4) +
+                                         (d & 7u) * 2u) = term[i];
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint32_t r0q = i * (EXTRA ? 24u : 16u);
+#pragma unroll
+        for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t r = r0q + (lane & 7u) + ((lane >> 3) & 1u) * 8u, ch = 2u * kk + (lane >> 4);
+          ldsm_x4(qa[i][kk], q_at + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4));
+          if constexpr (EXTRA) {
+            const uint32_t rx = r0q + 16u + g;
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+              qx[i][kk][e] = *reinterpret_cast<const uint32_t*>(smem + Shape::kRing + rx * (DP * 2u) +
+                                                                (((2u * kk + e) ^ (rx & 7u)) << 4) + t4 * 4u);
+            }
+          }
+        }
+        mult[i] = q_mult[i * 8 + g];
+        m[i] = -CUDART_INF_F;
+        l[i] = 0.f;
+#pragma unroll
+        for (uint32_t n = 0; n < DP / 8; ++n) o[i][n][0] = o[i][n][1] = 0.f;
+      }
+    }
+
+    // ---- one tile: scores, probabilities, weighted values
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t slot0 = use.j * kBlock + warp * kTile;
+    const uint32_t k_at = ring_at + stage * Shape::kStage, v_at = k_at + kTile * DP * 2u;
+    if (slot0 < use.len && slot0 + kTile > use.start) {
+      float s[MT][2][4], sx[MT][2][EXTRA ? 4 : 1];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][0][e] = s[i][1][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < (EXTRA ? 4 : 1); ++e) sx[i][0][e] = sx[i][1][e] = 0.f;
+      }
+#pragma unroll
+      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+        uint32_t kb[4];
+        const uint32_t r = (lane & 7u) + ((lane >> 4) << 3), ch = 2u * kk + ((lane >> 3) & 1u);
+        ldsm_x4(kb, k_at + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma(s[i][0], qa[i][kk][0], qa[i][kk][1], qa[i][kk][2], qa[i][kk][3], kb[0], kb[1], T());
+          mma(s[i][1], qa[i][kk][0], qa[i][kk][1], qa[i][kk][2], qa[i][kk][3], kb[2], kb[3], T());
+          if constexpr (EXTRA) {
+            mma(sx[i][0], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[0], kb[1], T());
+            mma(sx[i][1], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[2], kb[3], T());
+          }
+        }
+      }
+      const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
+      uint32_t p0[MT][kTerms], p1[MT][kTerms];
+      float fade[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        // this thread's head is 8 i + g; its slots 2 t4, 2 t4 + 1 and 8 more
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float hi = s[i][e >> 1][e & 1];
+          float lo = s[i][e >> 1][(e & 1) + 2];
+          if constexpr (EXTRA) lo += sx[i][e >> 1][e & 1];
+          // an infinite key: the errors' products are not numbers, the first term's sum is right
+          x[e] = (fabsf(hi) == CUDART_INF_F ? hi : hi + lo) * mult[i];
+          const uint32_t slot = slot0 + (e >> 1) * 8u + 2u * t4 + (e & 1);
+          if (!whole && (slot < use.start || slot >= use.len)) x[e] = -CUDART_INF_F;
+        }
+        if (a.scores != nullptr && i * 8u + g < heads) {
+          float* to = a.scores + (static_cast<size_t>(use.b) * a.n_q + head0 + i * 8u + g) * a.score_stride + slot0;
+          *reinterpret_cast<float2*>(to + 2u * t4) = make_float2(x[0], x[1]);
+          *reinterpret_cast<float2*>(to + 8u + 2u * t4) = make_float2(x[2], x[3]);
+        }
+        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(m[i], top);
+        const float from = now == -CUDART_INF_F ? 0.f : now;
+        fade[i] = exp2_fast(m[i] - from);
+        m[i] = now;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = exp2_fast(x[e] - from + kShareBits);
+        l[i] = fmaf(l[i], fade[i], (x[0] + x[1]) + (x[2] + x[3]));
+        split_terms<T>(x[0], x[1], p0[i]);
+        split_terms<T>(x[2], x[3], p1[i]);
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < DP / 16; ++n) {
+        uint32_t vb[4];
+        const uint32_t r = (lane & 7u) + ((lane >> 3) & 1u) * 8u, ch = 2u * n + (lane >> 4);
+        ldsm_x4_trans(vb, v_at + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+          for (uint32_t e = 0; e < 2; ++e) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma(d, p0[i][0], p0[i][1], p1[i][0], p1[i][1], vb[2 * e], vb[2 * e + 1], T());
+            if constexpr (EXTRA) mma(d, p0[i][kTerms - 1], 0u, p1[i][kTerms - 1], 0u, vb[2 * e], vb[2 * e + 1], T());
+            o[i][2 * n + e][0] = fmaf(o[i][2 * n + e][0], fade[i], d[0] + d[2]);
+            o[i][2 * n + e][1] = fmaf(o[i][2 * n + e][1], fade[i], d[1] + d[3]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+
+    // ---- the end of a (sequence, head tile), or of the range inside one
+    if (use.j + 1u == use.j1 || use.at + 1u == r1) {
+      fresh = true;
+      const uint64_t seg0 = use.at - (use.j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
+      const bool mine = seg0 >= r0 && seg1 <= r1;
+      // each warp's sums into the stage it has just used, float4 pieces swizzled by head
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float sum = l[i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (t4 == 0u) {
+          join_m[warp][i * 8 + g] = m[i];
+          join_l[warp][i * 8 + g] = sum;
+        }
+        float2* to = reinterpret_cast<float2*>(ring + stage * Shape::kStage) + (i * 8u + g) * (DP / 2u);
+#pragma unroll
+        for (uint32_t n = 0; n < DP / 8; ++n) {
+          to[(n * 4u + t4) ^ ((g & 3u) << 2)] = make_float2(o[i][n][0], o[i][n][1]);
+        }
+      }
+      __syncthreads();
+      float* record = a.records + (static_cast<size_t>(blockIdx.x) * 2u + (seg0 < r0 ? 0u : 1u)) * Shape::kRecord;
+      auto finish = [&](uint32_t h, uint32_t ch, float top, float sum, float4 v) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+        const size_t at = use.b * a.out_stride + static_cast<size_t>(head0 + h) * c.dim + ch * 4u;
+        if (ch * 4u < c.dim) {
+          if (a.dtype == QG_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+          } else if (a.dtype == QG_F16) {
+            *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) =
+                make_uint2(pack2(v.x, v.y, __half()), pack2(v.z, v.w, __half()));
+          } else {
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+                make_uint2(pack2(v.x, v.y, __nv_bfloat16()), pack2(v.z, v.w, __nv_bfloat16()));
+          }
+        }
+        if (ch == 0u) {
+          const size_t hi = static_cast<size_t>(use.b) * a.n_q + head0 + h;
+          const float full = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
+          if (a.lse != nullptr) a.lse[hi] = full * 0.69314718055994530942f;
+          if (a.norm != nullptr) a.norm[hi] = full;
+        }
+      };
+      for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
+        const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);
+        float top = join_m[0][h];
+#pragma unroll
+        for (uint32_t w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w][h]);
+        const float from = top == -CUDART_INF_F ? 0.f : top;
+        float sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+          const float f = exp2_fast(join_m[w][h] - from);
+          const float4 x = reinterpret_cast<const float4*>(smem + (w * kStages + stage) * Shape::kStage)
+              [h * (DP / 4u) + (ch ^ ((h & 3u) << 1))];
+          sum = fmaf(join_l[w][h], f, sum);
+          v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y);
+          v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+        }
+        if (mine) {
+          finish(h, ch, top, sum, v);
+        } else {
+          if (ch == 0u) {
+            record[h] = top;
+            record[kHeads + h] = sum;
+          }
+          reinterpret_cast<float4*>(record + 2u * kHeads)[h * (DP / 4u) + ch] = v;
+        }
+      }
+      if (!mine) {
+        // the CTAs that share this head: those that own its first to its last block
+        const uint64_t c0 = ((seg0 + 1u) * ctas - 1u) / total, c1 = (seg1 * ctas - 1u) / total;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0u) {
+          const uint32_t others = static_cast<uint32_t>(c1 - c0);
+          const uint32_t before = atomicAdd(a.arrived + c0, 1u);
+          is_last = before == others;
+          if (is_last != 0u) a.arrived[c0] = 0u;
+        }
+        __syncthreads();
+        if (is_last != 0u) {
+          __threadfence();
+          for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
+            const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);
+            float top = -CUDART_INF_F, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint64_t p = c0; p <= c1; ++p) {
+              const float* rec = a.records + (p * 2u + (p == c0 ? 1u : 0u)) * Shape::kRecord;
+              const float pm = __ldcg(rec + h), pl = __ldcg(rec + kHeads + h);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + 2u * kHeads) + h * (DP / 4u) + ch);
+              const float now = fmaxf(top, pm);
+              const float from = now == -CUDART_INF_F ? 0.f : now;
+              const float f0 = exp2_fast(top - from), f1 = exp2_fast(pm - from);
+              top = now;
+              sum = fmaf(sum, f0, pl * f1);
+              v.x = fmaf(v.x, f0, x.x * f1), v.y = fmaf(v.y, f0, x.y * f1);
+              v.z = fmaf(v.z, f0, x.z * f1), v.w = fmaf(v.w, f0, x.w * f1);
+            }
+            finish(h, ch, top, sum, v);
+          }
+        }
+      }
+      __syncthreads();  // the stages and joins are free again
+    }
+
+    fetch(stage);
+    cp_async_commit();
+    look_up();
+    stage = stage + 1u == kStages ? 0u : stage + 1u;
+    use.next(c, a, r1);
+  }
+  cp_async_wait<0>();
+}
+
+// weight_out = weight_in + the slot's shares summed over the heads of its kv head.
+__global__ void __launch_bounds__(256) attn_weight_kernel(const PagedView c, const AttnArgs a,
+                                                          const float* weight_in, float* weight_out,
+                                                          uint32_t weight_stride) {
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t kv = blockIdx.y, b = blockIdx.z, j = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t len = paged_len(a.lens[b], min(a.max_len, c.capacity));
+  if (j >= len) return;
+  const uint32_t start = a.window != 0u && len > a.window ? len - a.window : 0u;
+  const size_t at = (static_cast<size_t>(b) * c.n_kv + kv) * weight_stride + j;
+  float w = weight_in != nullptr ? weight_in[at] : 0.f;
+  if (j >= start) {
+    const size_t head = static_cast<size_t>(b) * a.n_q + kv * a.group;
+    float sum = 0.f;
+    for (uint32_t h = 0; h < a.group; ++h) {
+      sum += exp2_fast(a.scores[(head + h) * a.score_stride + j] - a.norm[head + h]);
+    }
+    w += sum;
+  }
+  weight_out[at] = w;
+}
+
+// ---- host side
+
+struct AttnPlan {
+  uint32_t dp, mt, tiles, record;
+  size_t records_at, scores_at, norm_at, bytes;
+};
+
+constexpr size_t round_up(size_t v) { return (v + 255u) & ~static_cast<size_t>(255u); }
+
+bool plan_attn(const PagedView& c, uint32_t n_q, uint32_t max_len, bool weights,
+               bool extra, AttnPlan* p) {
+  if (n_q == 0u || n_q > 65535u || n_q % c.n_kv != 0u || max_len == 0u || max_len > 0x7fffffffu) return false;
+  const uint32_t group = n_q / c.n_kv;
+  p->dp = c.dim <= 64u ? 64u : c.dim <= 128u ? 128u : 256u;
+  // two tiles of 8 heads share a pass over the slots where their registers allow it
+  p->mt = group > 8u && (p->dp == 64u || (p->dp == 128u && !extra)) ? 2u : 1u;
+  p->tiles = (group + 8u * p->mt - 1u) / (8u * p->mt);
+  p->record = 8u * p->mt * (p->dp + 2u);
+  p->records_at = QG_PAGED_ATTN_ZEROED;
+  p->scores_at = round_up(p->records_at + static_cast<size_t>(kMaxCtas) * 2u * p->record * 4u);
+  const size_t stride = (max_len + kBlock - 1u) / kBlock * kBlock;
+  p->norm_at = round_up(p->scores_at + (weights ? static_cast<size_t>(c.batch) * n_q * stride * 4u : 0u));
+  p->bytes = round_up(p->norm_at + (weights ? static_cast<size_t>(c.batch) * n_q * 4u : 0u));
+  return true;
+}
+
+int sm_count() {
+  static std::mutex mu;
+  static int cache[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 0 || dev >= 64) return device_sm_count();
+  if (cache[dev] == 0) cache[dev] = device_sm_count();
+  return cache[dev];
+}
+
+template <typename T, int DP, int MT, bool EXTRA>
+cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, cudaStream_t stream) {
+  using Shape = AttnShape<T, DP, MT, EXTRA>;
+  const auto kernel = paged_attn_kernel<T, DP, MT, EXTRA>;
+  {
+    static std::mutex mu;
+    static std::set<int> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done.count(dev) == 0u) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+      if (e != cudaSuccess) return e;
+      done.insert(dev);
+    }
+  }
+  const uint64_t blocks = static_cast<uint64_t>(c.batch) * c.n_kv * a.tiles *
+                          ((std::min(a.max_len, c.capacity) + kBlock - 1u) / kBlock);
+  const uint64_t fit = static_cast<uint64_t>(sm_count()) * Shape::kCtasPerSm;
+  const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
+  return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a);
+}
+
+template <typename T>
+cudaError_t launch_attn(const AttnPlan& p, bool extra, const PagedView& c, const AttnArgs& a,
+                        cudaStream_t stream) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (extra) {
+      if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, true>(c, a, stream);
+      if (p.dp == 64u) return launch_attn<T, 64, 1, true>(c, a, stream);
+      if (p.dp == 128u) return launch_attn<T, 128, 1, true>(c, a, stream);
+      return launch_attn<T, 256, 1, true>(c, a, stream);
+    }
+  }
+  if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, false>(c, a, stream);
+  if (p.dp == 64u) return launch_attn<T, 64, 1, false>(c, a, stream);
+  if (p.dp == 128u && p.mt == 2u) return launch_attn<T, 128, 2, false>(c, a, stream);
+  if (p.dp == 128u) return launch_attn<T, 128, 1, false>(c, a, stream);
+  return launch_attn<T, 256, 1, false>(c, a, stream);
+}
+
+}  // namespace
+}  // namespace qg
+
+extern "C" cudaError_t qg_paged_attn_workspace_bytes(const qg_kv_pages* cache, uint32_t n_q_heads,
+                                                     uint32_t max_len, int weights, size_t* bytes) {
+  using namespace qg;
+  PagedView c;
+  AttnPlan p0, p1;
+  if (bytes == nullptr || !paged_view(cache, &c)) return cudaErrorInvalidValue;
+  // the type of the queries is not known here: the larger of both forms
+  if (!plan_attn(c, n_q_heads, max_len, weights != 0, false, &p0) ||
+      !plan_attn(c, n_q_heads, max_len, weights != 0, true, &p1)) {
+    return cudaErrorInvalidValue;
+  }
+  *bytes = std::max(p0.bytes, p1.bytes);
+  return cudaSuccess;
+}
+
+extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p, void* workspace,
+                                     cudaStream_t stream) {
+  using namespace qg;
+  PagedView c;
+  if (!paged_view(cache, &c) || p == nullptr || !dtype_ok(p->dtype)) return cudaErrorInvalidValue;
+  const bool weights = p->weight_out != nullptr;
+  const bool extra = cache->dtype == QG_BF16 && p->dtype == QG_F32;
+  AttnPlan plan;
+  if (!plan_attn(c, p->n_q_heads, p->max_len, weights, extra, &plan)) return cudaErrorInvalidValue;
+  const uint64_t piece = 16u / dtype_bytes(p->dtype);
+  if (p->q == nullptr || p->out == nullptr || p->lens == nullptr || workspace == nullptr ||
+      p->q_stride % piece != 0u || p->out_stride % piece != 0u || !aligned16(p->q) || !aligned16(p->out) ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0u ||
+      (weights && p->weight_stride < p->max_len) || (!weights && p->weight_in != nullptr)) {
+    return cudaErrorInvalidValue;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  AttnArgs a{};
+  a.q = p->q;
+  a.out = p->out;
+  a.dtype = p->dtype;
+  a.q_stride = p->q_stride;
+  a.out_stride = p->out_stride;
+  a.lens = p->lens;
+  a.max_len = p->max_len;
+  a.window = p->window;
+  a.n_q = p->n_q_heads;
+  a.group = p->n_q_heads / c.n_kv;
+  a.tiles = plan.tiles;
+  a.scale_log2 = p->scale * 1.44269504088896340736f;
+  a.lse = p->lse;
+  a.arrived = reinterpret_cast<uint32_t*>(ws);
+  a.records = reinterpret_cast<float*>(ws + plan.records_at);
+  a.scores = weights ? reinterpret_cast<float*>(ws + plan.scores_at) : nullptr;
+  a.norm = weights ? reinterpret_cast<float*>(ws + plan.norm_at) : nullptr;
+  a.score_stride = (p->max_len + kBlock - 1u) / kBlock * kBlock;
+  const cudaError_t e = cache->dtype == QG_F16 ? launch_attn<__half>(plan, extra, c, a, stream)
+                                               : launch_attn<__nv_bfloat16>(plan, extra, c, a, stream);
+  if (e != cudaSuccess || !weights) return e;
+  const dim3 grid((std::min(p->max_len, c.capacity) + 255u) / 256u, c.n_kv, c.batch);
+  return launch_k(attn_weight_kernel, grid, 256, 0, stream, c, a, p->weight_in, p->weight_out,
+                  p->weight_stride);
+}

@@ -5,6 +5,7 @@
   list of every sequence.
 * `qk_norm_rope_append` -- normalise and rotate new queries and keys, write keys and values
   to their slots.
+* `AttentionPlan`, `attend` -- one new token per sequence attends to its sequence's slots.
 
 Device memory and streams only; every computation happens in the library.  Every call takes
 `stream` (default: the current one) and allocates what it returns on that stream, unless the
@@ -43,6 +44,14 @@ class AppendC(ctypes.Structure):
                 ("eps", c_float), ("rope", c_void_p), ("rope_rows", c_uint32),
                 ("rot_dim", c_uint32), ("pairs", c_int), ("positions", c_void_p),
                 ("slots", c_void_p), ("seqs", c_void_p)]
+
+
+class AttnC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("dtype", c_int), ("n_q_heads", c_uint32),
+                ("q_stride", c_uint64), ("out_stride", c_uint64), ("lens", c_void_p),
+                ("max_len", c_uint32), ("window", c_uint32), ("scale", c_float),
+                ("lse", c_void_p), ("weight_in", c_void_p), ("weight_out", c_void_p),
+                ("weight_stride", c_uint32)]
 
 
 def _fail(message: str):
@@ -175,3 +184,53 @@ def qk_norm_rope_append(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: 
                 _ints(seqs, tokens, "seqs", dev))
     _call("qg_qk_norm_rope_append", dev, cache._ref, ctypes.byref(a), _handle(stream, dev))
     return q_out
+
+
+class AttentionPlan:
+    """The workspace of `attend` for a cache, a number of query heads and lengths up to
+    max_len (default: all that a table row names).  Calls that may overlap need a plan each."""
+
+    def __init__(self, cache: PagedCache, n_q_heads: int, max_len: int | None = None,
+                 weights: bool = False):
+        self.cache, self.n_q_heads, self.weights = cache, n_q_heads, weights
+        self.max_len = cache.capacity if max_len is None else max_len
+        n = ctypes.c_size_t(0)
+        _call("qg_paged_attn_workspace_bytes", cache.device, cache._ref, n_q_heads, self.max_len,
+              int(weights), ctypes.byref(n))
+        self.workspace = torch.zeros(n.value, dtype=torch.uint8, device=cache.device)
+
+
+def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: int = 0,
+           scale: float | None = None, out: torch.Tensor | None = None,
+           lse: torch.Tensor | None = None, return_lse: bool = False,
+           weight_in: torch.Tensor | None = None, weight_out: torch.Tensor | None = None,
+           stream=None):
+    """qg_paged_attn: q [sequences, q heads, dim] attends to lens[b] slots of sequence b (scale
+    defaults to dim^-1/2); returns out like q, or (out, lse [sequences, q heads]).
+    weight_out [sequences, kv heads, >= max_len] receives weight_in plus each slot's shares
+    (a plan with weights; weight_in may be weight_out)."""
+    cache = plan.cache
+    dev, dim, batch, heads = cache.device, cache.head_dim, cache.batch, plan.n_q_heads
+    if q.dtype not in DTYPE_CODES:
+        _fail("q: float32, float16 or bfloat16 is needed")
+    if out is None:
+        out = _new(stream, (batch, heads, dim), q.dtype, dev)
+    if lse is None and return_lse:
+        lse = _new(stream, (batch, heads), torch.float32, dev)
+    width = 0
+    if weight_out is not None:
+        if not plan.weights:
+            _fail("weight_out needs a plan with weights")
+        width = weight_out.shape[-1]
+    elif weight_in is not None:
+        _fail("weight_in without weight_out")
+    shape = (batch, cache.n_kv_heads, width)
+    a = AttnC(q.data_ptr(), out.data_ptr(), DTYPE_CODES[q.dtype], heads,
+              _heads(q, batch, heads, dim, q.dtype, "q", dev),
+              _heads(out, batch, heads, dim, q.dtype, "out", dev), _ints(lens, batch, "lens", dev),
+              plan.max_len, window, dim ** -0.5 if scale is None else scale,
+              _floats(lse, (batch, heads), "lse", dev), _floats(weight_in, shape, "weight_in", dev),
+              _floats(weight_out, shape, "weight_out", dev), width)
+    _call("qg_paged_attn", dev, cache._ref, ctypes.byref(a), plan.workspace.data_ptr(),
+          _handle(stream, dev))
+    return (out, lse) if lse is not None else out
