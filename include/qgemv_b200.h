@@ -585,6 +585,33 @@ cudaError_t qg_paged_attn_workspace_bytes(const qg_kv_pages* cache, uint32_t n_q
 cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* a, void* workspace,
                           cudaStream_t stream);
 
+/* Eviction by accumulated attention weight.  A sequence of lens[b] <= budget slots keeps
+ * them all.  A longer one keeps, for each kv head, its first `sink` slots, its last
+ * `recent` slots (sink + recent <= budget) and, of the slots between, the
+ * budget - sink - recent with the largest weight; equal weights go to the lower slot, a
+ * NaN weight ranks below every other.  The kept slots move, in ascending order, to the
+ * front: slot kept[b][kv][i] to slot i, keys, values and weights alike, bit for bit; their
+ * rotation stays that of their own positions.  kept rows hold `budget` entries, the ones
+ * past the new length -1.  lens_out[b] = min(lens[b], budget).  weight_out entries from
+ * the new length to max_len are zero, so slots appended later start from nothing.
+ * new_table ([batch][new_table_stride], new_table_pages entries, at least
+ * min(budget, max_len) slots) names the pages that receive the rows; they must be
+ * distinct from every page that the call reads.  NULL moves within the old pages (the
+ * freed pages are the tail of each row); no page may then belong to two sequences.
+ * weight_out may be weight, lens_out lens.
+ * lens[b] at most max_len; weight rows of weight_stride floats. */
+typedef struct qg_evict {
+  const int32_t* lens;
+  int32_t* lens_out;
+  const float* weight;       /* [batch][n_kv_heads][weight_stride] */
+  float* weight_out;
+  uint32_t max_len, weight_stride, budget, sink, recent;
+  int32_t* kept;             /* [batch][n_kv_heads][budget] */
+  const int32_t* new_table;
+  uint32_t new_table_pages, new_table_stride;
+} qg_evict;
+cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, cudaStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * GGUF ingest (host code; the reference's reader is runtime/apps/gguf_probe/main.cpp:124-631):
  * header, metadata (general.alignment, general.architecture), tensor infos, the data

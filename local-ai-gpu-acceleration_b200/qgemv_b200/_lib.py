@@ -94,6 +94,7 @@ SIGNATURES: dict[str, list] = {
     "qg_qk_norm_rope_append": [P, P, P],
     "qg_paged_attn_workspace_bytes": [P, U32, U32, c_int, P],
     "qg_paged_attn": [P, P, P, P],
+    "qg_kv_evict": [P, P, P],
     "qg_gguf_open": [ctypes.c_char_p, P],
     "qg_gguf_summary": [P, P],
     "qg_gguf_tensor": [P, U64, P],

@@ -6,6 +6,7 @@
 * `qk_norm_rope_append` -- normalise and rotate new queries and keys, write keys and values
   to their slots.
 * `AttentionPlan`, `attend` -- one new token per sequence attends to its sequence's slots.
+* `evict` -- sequences are cut back to a budget of slots by the weight that `attend` summed.
 
 Device memory and streams only; every computation happens in the library.  Every call takes
 `stream` (default: the current one) and allocates what it returns on that stream, unless the
@@ -52,6 +53,14 @@ class AttnC(ctypes.Structure):
                 ("max_len", c_uint32), ("window", c_uint32), ("scale", c_float),
                 ("lse", c_void_p), ("weight_in", c_void_p), ("weight_out", c_void_p),
                 ("weight_stride", c_uint32)]
+
+
+class EvictC(ctypes.Structure):
+    _fields_ = [("lens", c_void_p), ("lens_out", c_void_p), ("weight", c_void_p),
+                ("weight_out", c_void_p), ("max_len", c_uint32), ("weight_stride", c_uint32),
+                ("budget", c_uint32), ("sink", c_uint32), ("recent", c_uint32),
+                ("kept", c_void_p), ("new_table", c_void_p), ("new_table_pages", c_uint32),
+                ("new_table_stride", c_uint32)]
 
 
 def _fail(message: str):
@@ -234,3 +243,37 @@ def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: 
     _call("qg_paged_attn", dev, cache._ref, ctypes.byref(a), plan.workspace.data_ptr(),
           _handle(stream, dev))
     return (out, lse) if lse is not None else out
+
+
+def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: int, *, sink: int = 0,
+          recent: int = 0, new_table: torch.Tensor | None = None, lens_out: torch.Tensor | None = None,
+          weight_out: torch.Tensor | None = None, kept: torch.Tensor | None = None, stream=None):
+    """qg_kv_evict: keep `budget` slots per kv head of every longer sequence -- the first `sink`,
+    the last `recent`, and the heaviest between them by weight [sequences, kv heads, >= longest
+    length].  Rows move to the front of the same pages, lens and weight are updated; or, with
+    new_table [sequences, pages], to those pages, lens and weight left as they are.  Returns
+    (kept [sequences, kv heads, budget], new lens); the new weights are in weight_out."""
+    dev, batch, kv = cache.device, cache.batch, cache.n_kv_heads
+    if weight.dim() != 3:
+        _fail("weight: [sequences, kv heads, slots] is needed")
+    width = weight.shape[2]
+    if lens_out is None:
+        lens_out = lens if new_table is None else _new(stream, (batch,), torch.int32, dev)
+    if weight_out is None:
+        weight_out = weight if new_table is None else _new(stream, weight.shape, torch.float32, dev)
+    if kept is None:
+        kept = _new(stream, (batch, kv, budget), torch.int32, dev)
+    to, pages, step = None, 0, 0
+    if new_table is not None:
+        if (new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != batch
+                or new_table.device != dev or (new_table.shape[1] > 1 and new_table.stride(1) != 1)):
+            _fail("new_table: an int32 tensor [sequences, pages per sequence] is needed")
+        to, pages = new_table.data_ptr(), new_table.shape[1]
+        step = new_table.stride(0) if batch > 1 else pages
+    shape = (batch, kv, width)
+    e = EvictC(_ints(lens, batch, "lens", dev), _ints(lens_out, batch, "lens_out", dev),
+               _floats(weight, shape, "weight", dev), _floats(weight_out, shape, "weight_out", dev),
+               width, width, budget, sink, recent, _ints(kept, batch * kv * budget, "kept", dev),
+               to, pages, step)
+    _call("qg_kv_evict", dev, cache._ref, ctypes.byref(e), _handle(stream, dev))
+    return kept, lens_out
