@@ -67,55 +67,63 @@ def _fail(message: str):
     raise ValueError(message)
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """Call an entry point with `device` current."""
-    fn = getattr(lib(), name)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+def _call(fn, index: int, *args) -> None:
+    """Call an entry point with device `index` current."""
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
             code = fn(*args)
     else:
         code = fn(*args)
     if code != 0:
-        raise CudaError(name, code)
+        raise CudaError(fn.__name__, code)
 
 
-def _handle(stream, device: torch.device) -> int:
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+def _handle(stream, index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
-def _new(stream, shape, dtype, device) -> torch.Tensor:
+def _new(shape: tuple, dtype, device, stream) -> torch.Tensor:
+    """A new tensor on the stream that will write it."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _ints(t: torch.Tensor | None, n: int, name: str, device: torch.device) -> int | None:
-    """Address of a contiguous int32 vector of n entries."""
+def _like(t: torch.Tensor, stream) -> torch.Tensor:
+    """The same for a tensor like t (half the time of _new)."""
+    if stream is None:
+        return torch.empty_like(t)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t)
+
+
+def _ints(t: torch.Tensor | None, n: int, name: str, index: int) -> int | None:
+    """Address of a contiguous int32 tensor of n entries."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
-        _fail(f"{name}: a contiguous int32 tensor of {n} entries on {device} is needed")
+    if t.dtype is not torch.int32 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+        _fail(f"{name}: a contiguous int32 tensor of {n} entries on cuda:{index} is needed")
     return t.data_ptr()
 
 
-def _floats(t: torch.Tensor | None, shape: tuple, name: str, device: torch.device) -> int | None:
+def _floats(t: torch.Tensor | None, shape: tuple, name: str, index: int) -> int | None:
     """Address of a contiguous fp32 tensor of a shape."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        _fail(f"{name}: a contiguous float32 tensor of shape {shape} on {device} is needed")
+    if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        _fail(f"{name}: a contiguous float32 tensor of shape {shape} on cuda:{index} is needed")
     return t.data_ptr()
 
 
-def _heads(t: torch.Tensor, rows: int, heads: int, dim: int, dtype, name: str, device: torch.device) -> int:
+def _heads(t: torch.Tensor, shape: tuple, dtype, name: str, index: int) -> int:
     """Stride from row to row of a [rows, heads, dim] tensor whose rows are contiguous."""
-    if t.dtype != dtype or t.device != device or t.dim() != 3 or tuple(t.shape) != (rows, heads, dim):
-        _fail(f"{name}: a {dtype} tensor of shape {(rows, heads, dim)} on {device} is needed")
-    stride = t.stride()
-    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        _fail(f"{name}: a {dtype} tensor of shape {shape} on cuda:{index} is needed")
+    row, head, one = t.stride()
+    if one != 1 or (shape[1] > 1 and head != shape[2]):
         _fail(f"{name}: the heads of one row must be contiguous")
-    return stride[0] if rows > 1 else heads * dim
+    return row if shape[0] > 1 else shape[1] * shape[2]
 
 
 class PagedCache:
@@ -136,7 +144,7 @@ class PagedCache:
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             _fail("table: an int32 tensor [sequences, pages per sequence] is needed")
         self.k, self.v, self.table = k, v, table
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self.index = k.device, k.dtype, k.get_device()
         self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.batch, self.table_pages = table.shape
         self.capacity = self.table_pages * self.page_size
@@ -173,25 +181,26 @@ def qk_norm_rope_append(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: 
                         q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """qg_qk_norm_rope_append: q [tokens, q heads, dim], k and v [tokens, kv heads, dim] of one
     type (views of a fused projection are fine); returns the rotated queries."""
-    dev, dim, kv = cache.device, cache.head_dim, cache.n_kv_heads
-    if q.dtype not in DTYPE_CODES or q.dim() != 3:
+    index, dim, kv, dtype = cache.index, cache.head_dim, cache.n_kv_heads, q.dtype
+    if dtype not in DTYPE_CODES or q.dim() != 3:
         _fail("q: a [tokens, heads, dim] tensor of float32, float16 or bfloat16 is needed")
-    tokens, heads = q.shape[0], q.shape[1]
+    tokens, heads, _ = q.shape
     if pairs not in PAIRS:
         _fail("pairs is 'adjacent' or 'halves'")
+    q_shape, kv_shape = (tokens, heads, dim), (tokens, kv, dim)
+    q_stride = _heads(q, q_shape, dtype, "q", index)
     if q_out is None:
-        q_out = _new(stream, (tokens, heads, dim), q.dtype, dev)
-    rows, rot = (rope.shape[0], rope.shape[1]) if rope is not None else (0, 0)
-    a = AppendC(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), DTYPE_CODES[q.dtype],
-                tokens, heads, _heads(q, tokens, heads, dim, q.dtype, "q", dev),
-                _heads(k, tokens, kv, dim, q.dtype, "k", dev),
-                _heads(v, tokens, kv, dim, q.dtype, "v", dev),
-                _heads(q_out, tokens, heads, dim, q.dtype, "q_out", dev),
-                _floats(q_norm, (dim,), "q_norm", dev), _floats(k_norm, (dim,), "k_norm", dev), eps,
-                _floats(rope, (rows, rot), "rope", dev), rows, rot, PAIRS[pairs],
-                _ints(positions, tokens, "positions", dev), _ints(slots, tokens, "slots", dev),
-                _ints(seqs, tokens, "seqs", dev))
-    _call("qg_qk_norm_rope_append", dev, cache._ref, ctypes.byref(a), _handle(stream, dev))
+        q_out = _like(q, stream)
+    out_stride = _heads(q_out, q_shape, dtype, "q_out", index)
+    rows, rot = (0, 0) if rope is None else rope.shape
+    a = AppendC(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), DTYPE_CODES[dtype],
+                tokens, heads, q_stride, _heads(k, kv_shape, dtype, "k", index),
+                _heads(v, kv_shape, dtype, "v", index), out_stride,
+                _floats(q_norm, (dim,), "q_norm", index), _floats(k_norm, (dim,), "k_norm", index), eps,
+                _floats(rope, (rows, rot), "rope", index), rows, rot, PAIRS[pairs],
+                _ints(positions, tokens, "positions", index), _ints(slots, tokens, "slots", index),
+                _ints(seqs, tokens, "seqs", index))
+    _call(lib().qg_qk_norm_rope_append, index, cache._ref, ctypes.byref(a), _handle(stream, index))
     return q_out
 
 
@@ -204,9 +213,10 @@ class AttentionPlan:
         self.cache, self.n_q_heads, self.weights = cache, n_q_heads, weights
         self.max_len = cache.capacity if max_len is None else max_len
         n = ctypes.c_size_t(0)
-        _call("qg_paged_attn_workspace_bytes", cache.device, cache._ref, n_q_heads, self.max_len,
+        _call(lib().qg_paged_attn_workspace_bytes, cache.index, cache._ref, n_q_heads, self.max_len,
               int(weights), ctypes.byref(n))
         self.workspace = torch.zeros(n.value, dtype=torch.uint8, device=cache.device)
+        self.lse = torch.empty(cache.batch, n_q_heads, device=cache.device)  # what new ones are made like
 
 
 def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: int = 0,
@@ -218,14 +228,16 @@ def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: 
     defaults to dim^-1/2); returns out like q, or (out, lse [sequences, q heads]).
     weight_out [sequences, kv heads, >= max_len] receives weight_in plus each slot's shares
     (a plan with weights; weight_in may be weight_out)."""
-    cache = plan.cache
-    dev, dim, batch, heads = cache.device, cache.head_dim, cache.batch, plan.n_q_heads
-    if q.dtype not in DTYPE_CODES:
+    cache, heads, dtype = plan.cache, plan.n_q_heads, q.dtype
+    index, dim, batch = cache.index, cache.head_dim, cache.batch
+    if dtype not in DTYPE_CODES:
         _fail("q: float32, float16 or bfloat16 is needed")
+    shape = (batch, heads, dim)
+    q_stride = _heads(q, shape, dtype, "q", index)
     if out is None:
-        out = _new(stream, (batch, heads, dim), q.dtype, dev)
+        out = _like(q, stream)
     if lse is None and return_lse:
-        lse = _new(stream, (batch, heads), torch.float32, dev)
+        lse = _like(plan.lse, stream)
     width = 0
     if weight_out is not None:
         if not plan.weights:
@@ -233,16 +245,16 @@ def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: 
         width = weight_out.shape[-1]
     elif weight_in is not None:
         _fail("weight_in without weight_out")
-    shape = (batch, cache.n_kv_heads, width)
-    a = AttnC(q.data_ptr(), out.data_ptr(), DTYPE_CODES[q.dtype], heads,
-              _heads(q, batch, heads, dim, q.dtype, "q", dev),
-              _heads(out, batch, heads, dim, q.dtype, "out", dev), _ints(lens, batch, "lens", dev),
+    w_shape = (batch, cache.n_kv_heads, width)
+    a = AttnC(q.data_ptr(), out.data_ptr(), DTYPE_CODES[dtype], heads, q_stride,
+              _heads(out, shape, dtype, "out", index), _ints(lens, batch, "lens", index),
               plan.max_len, window, dim ** -0.5 if scale is None else scale,
-              _floats(lse, (batch, heads), "lse", dev), _floats(weight_in, shape, "weight_in", dev),
-              _floats(weight_out, shape, "weight_out", dev), width)
-    _call("qg_paged_attn", dev, cache._ref, ctypes.byref(a), plan.workspace.data_ptr(),
-          _handle(stream, dev))
-    return (out, lse) if lse is not None else out
+              _floats(lse, (batch, heads), "lse", index),
+              _floats(weight_in, w_shape, "weight_in", index),
+              _floats(weight_out, w_shape, "weight_out", index), width)
+    _call(lib().qg_paged_attn, index, cache._ref, ctypes.byref(a), plan.workspace.data_ptr(),
+          _handle(stream, index))
+    return out if lse is None else (out, lse)
 
 
 def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: int, *, sink: int = 0,
@@ -253,27 +265,27 @@ def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: i
     length].  Rows move to the front of the same pages, lens and weight are updated; or, with
     new_table [sequences, pages], to those pages, lens and weight left as they are.  Returns
     (kept [sequences, kv heads, budget], new lens); the new weights are in weight_out."""
-    dev, batch, kv = cache.device, cache.batch, cache.n_kv_heads
+    index, batch, kv = cache.index, cache.batch, cache.n_kv_heads
     if weight.dim() != 3:
         _fail("weight: [sequences, kv heads, slots] is needed")
     width = weight.shape[2]
     if lens_out is None:
-        lens_out = lens if new_table is None else _new(stream, (batch,), torch.int32, dev)
+        lens_out = lens if new_table is None else _like(lens, stream)
     if weight_out is None:
-        weight_out = weight if new_table is None else _new(stream, weight.shape, torch.float32, dev)
+        weight_out = weight if new_table is None else _like(weight, stream)
     if kept is None:
-        kept = _new(stream, (batch, kv, budget), torch.int32, dev)
+        kept = _new((batch, kv, budget), torch.int32, cache.device, stream)
     to, pages, step = None, 0, 0
     if new_table is not None:
-        if (new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != batch
-                or new_table.device != dev or (new_table.shape[1] > 1 and new_table.stride(1) != 1)):
+        if (new_table.dtype is not torch.int32 or new_table.dim() != 2 or new_table.shape[0] != batch
+                or new_table.get_device() != index or (new_table.shape[1] > 1 and new_table.stride(1) != 1)):
             _fail("new_table: an int32 tensor [sequences, pages per sequence] is needed")
         to, pages = new_table.data_ptr(), new_table.shape[1]
         step = new_table.stride(0) if batch > 1 else pages
     shape = (batch, kv, width)
-    e = EvictC(_ints(lens, batch, "lens", dev), _ints(lens_out, batch, "lens_out", dev),
-               _floats(weight, shape, "weight", dev), _floats(weight_out, shape, "weight_out", dev),
-               width, width, budget, sink, recent, _ints(kept, batch * kv * budget, "kept", dev),
+    e = EvictC(_ints(lens, batch, "lens", index), _ints(lens_out, batch, "lens_out", index),
+               _floats(weight, shape, "weight", index), _floats(weight_out, shape, "weight_out", index),
+               width, width, budget, sink, recent, _ints(kept, batch * kv * budget, "kept", index),
                to, pages, step)
-    _call("qg_kv_evict", dev, cache._ref, ctypes.byref(e), _handle(stream, dev))
+    _call(lib().qg_kv_evict, index, cache._ref, ctypes.byref(e), _handle(stream, index))
     return kept, lens_out
