@@ -560,7 +560,10 @@ cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
  *   weight_out[b][kv][j] = weight_in[b][kv][j] + sum_h exp(s_hj - m_h) / l_h
  * for every j < lens[b] (unseen slots: weight_in alone), rows of weight_stride floats;
  * weight_in may be weight_out, or NULL for zero; slots at or past lens[b] are left alone.
- * Scores, statistics and sums are fp32; results are deterministic.  q, out:
+ * Scores, statistics and sums are fp32; results are deterministic.  The cache's strides
+ * have to nest, as they do in every dense or padded layout: slot_stride and head_stride, the
+ * smaller at least head_dim, one a multiple of the other, page_stride a multiple of both and
+ * below 2^39 (strides of a dimension of one entry are not looked at).  q, out:
  * [batch][n_q_heads][head_dim] with sequence strides in elements (multiples of 16 bytes);
  * 16-B aligned.  `workspace`: 256-B aligned, qg_paged_attn_workspace_bytes long, its
  * first QG_PAGED_ATTN_ZEROED bytes zero before its first use (every call leaves them

@@ -16,9 +16,13 @@
 // Work.  The unit is a block of 64 slots of one (sequence, kv head, head tile); all blocks of
 // the batch, whatever the lengths, form one line that is cut into equal ranges, one a CTA
 // (two CTAs an SM).  In a range, warp w owns slots [16 w, 16 w + 16) of every block and runs
-// on its own: it fetches its rows through its own ring of stages (cp.async, 16 bytes a lane,
-// any page size and layout; a tile's page ids are read one tile ahead) and keeps its own
-// (m, l, o).  Where a (sequence, head) ends inside the range the four warps join through
+// on its own: it fetches its rows through its own ring of stages and keeps its own (m, l, o).
+// Rows arrive as TMA boxes of gcd(16, page_size) slots x 64 values, swizzled for ldmatrix, so
+// no box crosses a page, whatever the page size, and values past head_dim, slots of no page
+// and slots past the sequence's last box are the tensor map's zeros; a tile's page ids are
+// read one tile ahead.  Only rows that share a box with the sequence's ends can hold what is
+// not the sequence's: their V rows are cleared in shared memory, their scores are masked.
+// Where a (sequence, head) ends inside the range the four warps join through
 // shared memory; where it was cut by the range, the CTA leaves a record, and the CTA that
 // arrives last joins the records in CTA order, so results do not depend on timing.
 //
@@ -32,6 +36,8 @@
 // keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
 // Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
 // matrix pipe truncates when it accumulates, and o lives for thousands of tiles.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math_constants.h>
 
 #include <algorithm>
@@ -67,6 +73,13 @@ struct AttnArgs {
   float* scores;               // [batch][n_q][score_stride], log2 units, or NULL
   float* norm;                 // [batch][n_q]: log2 of the full sum, with scores
   uint32_t score_stride;
+  uint32_t box, boxes;         // slots of a box, boxes of a tile's 16 slots
+  bool heads_inside;           // a page's heads lie inside its slots ([place][head][dim])
+};
+
+// K and V pools as [page][.][.][dim] tensors; the middle two in the order of their strides.
+struct AttnMaps {
+  CUtensorMap k, v;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -75,13 +88,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One box of a pool's tensor map (a kernel parameter) into shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                            int32_t page, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(page), "r"(bar), "l"(policy)
+      : "memory");
 }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
@@ -161,7 +175,8 @@ struct AttnShape {
   static constexpr uint32_t kRing = kWarps * kStages * kStage;
   static constexpr uint32_t kQRows = MT * (EXTRA ? 24u : 16u);
   static constexpr uint32_t kQBytes = kQRows * DP * 2u;
-  static constexpr uint32_t kSmem = kRing + kQBytes;
+  static constexpr uint32_t kSmem = kRing + kQBytes + 1024u;  // the ring starts on 1024 bytes
+  static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
   static constexpr uint32_t kRecord = kHeads * (DP + 2u);  // m[], l[], o[][]
   static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
   static_assert(kHeads * DP * 4u <= kStage, "a warp's sums join in its free stage");
@@ -169,21 +184,26 @@ struct AttnShape {
 
 template <typename T, int DP, int MT, bool EXTRA>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCtasPerSm)
-    paged_attn_kernel(const PagedView c, const AttnArgs a) {
+    paged_attn_kernel(const PagedView c, const AttnArgs a, const __grid_constant__ AttnMaps maps) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
   constexpr uint32_t kStages = Shape::kStages, kHeads = Shape::kHeads;
   constexpr int kTerms = EXTRA ? 3 : 2;
-  constexpr uint32_t kChunks = DP / 8;  // 16-byte pieces of a row
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr uint32_t kPanels = Shape::kPanels, kPanel = kTile * 128u;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ float join_m[kWarps][kHeads], join_l[kWarps][kHeads], q_mult[kHeads];
+  __shared__ __align__(8) uint64_t full[kWarps][kStages];
   __shared__ uint64_t sum64[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
 
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
-  const uint32_t chunks = c.dim / 8u;
+  uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* const ring = smem + warp * (kStages * Shape::kStage);
   const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(smem + Shape::kRing);
+  if (lane == 0u) {
+    for (uint32_t i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1u);
+    fence_mbar_init();
+  }
 
   pdl_wait();
   pdl_trigger();
@@ -251,38 +271,42 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   use.j = use.j0 + first_at[2];
   Cursor ahead = use;
 
-  if (DP != c.dim) {  // the pieces past head_dim are never written: zero them once
-    for (uint32_t i = lane; i < kStages * Shape::kStage / 16u; i += 32u) {
-      const uint32_t r = (i / kChunks) % kTile, ch = (i % kChunks) ^ (r & 7u);
-      if (ch >= chunks) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    __syncwarp();
-  }
-
-  // ---- fetching: lane l knows the row of slot l % 16 of the next tile
-  uint64_t row = kNoRow;
+  // ---- fetching: lane l knows the page and place of slot l % 16 of the next tile
+  const uint64_t policy = l2_evict_first_policy();
+  int32_t page = 0, place = 0, head = 0;
+  bool more = false;
   auto look_up = [&]() {
-    row = kNoRow;
-    if (ahead.at < r1) {
+    more = ahead.at < r1;
+    if (more) {
       const uint32_t slot = ahead.j * kBlock + warp * kTile + (lane & 15u);
-      if (slot >= ahead.start && slot < ahead.len) {
-        row = paged_row(c, c.table + static_cast<size_t>(ahead.b) * c.table_stride, slot, ahead.h / a.tiles);
+      const uint32_t box0 = slot & ~(a.box - 1u);
+      const uint32_t at = div_by(slot, c.page);
+      page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
+      place = static_cast<int32_t>(slot - at * c.page.d);
+      head = static_cast<int32_t>(ahead.h / a.tiles);
+      if (box0 < ahead.len && box0 + a.box > ahead.start) {
+        const uint32_t id = static_cast<uint32_t>(c.table[static_cast<size_t>(ahead.b) * c.table_stride + at]);
+        if (id < c.num_pages) {
+          page = static_cast<int32_t>(id);
+        } else {
+          atomicOr(&g_error_word, QG_ERR_PAGE);
+        }
       }
       ahead.next(c, a, r1);
     }
   };
   auto fetch = [&](uint32_t stage) {
-    const uint32_t to = ring_at + stage * Shape::kStage;
-#pragma unroll
-    for (uint32_t i = 0; i < kTile * kChunks / 32u; ++i) {
-      const uint32_t r = (i * 32u + lane) / kChunks, ch = (i * 32u + lane) % kChunks;
-      const uint64_t at = __shfl_sync(0xffffffffu, row, r);
-      if (ch < chunks) {
-        const uint64_t src = at == kNoRow ? 0u : at + ch * 16u;
-        const uint32_t n = at == kNoRow ? 0u : 16u;  // unseen slots arrive as zero rows
-        const uint32_t dst = to + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4);
-        cp_async_16(dst, c.k + src, n);
-        cp_async_16(dst + kTile * DP * 2u, c.v + src, n);
+    if (!more) return;
+    const uint32_t to = ring_at + stage * Shape::kStage, bar = smem_addr(&full[warp][stage]);
+    if (lane == 0u) mbar_arrive_expect_tx(&full[warp][stage], Shape::kStage);
+    __syncwarp();
+    for (uint32_t i0 = 0; i0 < a.boxes * kPanels * 2u; i0 += 32u) {
+      const uint32_t i = i0 + lane, panel = (i >> 1) % kPanels, r = (i >> 1) / kPanels * a.box;
+      const int32_t pg = __shfl_sync(0xffffffffu, page, r & 15u), pl = __shfl_sync(0xffffffffu, place, r & 15u);
+      if (r < kTile) {
+        const uint32_t dst = to + ((i & 1u) * kPanels + panel) * kPanel + r * 128u;
+        tma_load_4d(dst, (i & 1u) != 0u ? &maps.v : &maps.k, static_cast<int32_t>(panel * 64u),
+                    a.heads_inside ? head : pl, a.heads_inside ? pl : head, pg, bar, policy);
       }
     }
   };
@@ -290,14 +314,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
   for (uint32_t s = 0; s < kStages; ++s) {
     fetch(s);
-    cp_async_commit();
     look_up();
   }
+  // ldmatrix rows and 16-byte pieces of this lane (K: 8 slots x 2 pieces x 2; V, transposed:
+  // 16 slots x 2 pieces); piece 2 n of a panel is at lane_at ^ (n << 5)
+  const uint32_t kr = (lane & 7u) + ((lane >> 4) << 3), vr = (lane & 7u) + ((lane >> 3) & 1u) * 8u;
+  const uint32_t k_lane = kr * 128u + ((((lane >> 3) & 1u) ^ (kr & 7u)) << 4);
+  const uint32_t v_lane = kPanels * kPanel + vr * 128u + (((lane >> 4) ^ (vr & 7u)) << 4);
 
   uint32_t qa[MT][DP / 16][4], qx[MT][EXTRA ? DP / 16 : 1][2];
   float o[MT][DP / 8][2], m[MT], l[MT], mult[MT];
-  uint32_t stage = 0;
-  bool fresh = true;
+  uint32_t stage = 0, parity = 0;
+  bool fresh = true, arrives = true;
 
   while (use.at < r1) {
     const uint32_t kv = use.h / a.tiles, ht = use.h - kv * a.tiles;
@@ -367,11 +395,22 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     }
 
     // ---- one tile: scores, probabilities, weighted values
-    cp_async_wait<kStages - 1>();
-    __syncwarp();
+    arrives = arrives && __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], parity));
     const uint32_t slot0 = use.j * kBlock + warp * kTile;
-    const uint32_t k_at = ring_at + stage * Shape::kStage, v_at = k_at + kTile * DP * 2u;
-    if (slot0 < use.len && slot0 + kTile > use.start) {
+    const uint32_t tile_at = ring_at + stage * Shape::kStage;
+    const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
+    bool written = false;  // by this warp, where the next box will land
+    if (arrives && slot0 < use.len && slot0 + kTile > use.start) {
+      if (!whole) {  // V rows beside the sequence's ends: 0 x NaN must not reach the sums
+        written = true;
+        for (uint32_t i = lane; i < kTile * DP / 8u; i += 32u) {
+          const uint32_t r = i / 8u % kTile;
+          if (slot0 + r < use.start || slot0 + r >= use.len) {
+            reinterpret_cast<uint4*>(ring + stage * Shape::kStage + kPanels * kPanel)[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        __syncwarp();
+      }
       float s[MT][2][4], sx[MT][2][EXTRA ? 4 : 1];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -383,8 +422,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
       for (uint32_t kk = 0; kk < DP / 16; ++kk) {
         uint32_t kb[4];
-        const uint32_t r = (lane & 7u) + ((lane >> 4) << 3), ch = 2u * kk + ((lane >> 3) & 1u);
-        ldsm_x4(kb, k_at + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4));
+        ldsm_x4(kb, tile_at + (k_lane ^ ((kk & 3u) << 5)) + kk / 4u * kPanel);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           mma(s[i][0], qa[i][kk][0], qa[i][kk][1], qa[i][kk][2], qa[i][kk][3], kb[0], kb[1], T());
@@ -395,7 +433,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
           }
         }
       }
-      const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
       uint32_t p0[MT][kTerms], p1[MT][kTerms];
       float fade[MT];
 #pragma unroll
@@ -433,8 +470,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
       for (uint32_t n = 0; n < DP / 16; ++n) {
         uint32_t vb[4];
-        const uint32_t r = (lane & 7u) + ((lane >> 3) & 1u) * 8u, ch = 2u * n + (lane >> 4);
-        ldsm_x4_trans(vb, v_at + r * (DP * 2u) + ((ch ^ (r & 7u)) << 4));
+        ldsm_x4_trans(vb, tile_at + (v_lane ^ ((n & 3u) << 5)) + n / 4u * kPanel);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -452,7 +488,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 
     // ---- the end of a (sequence, head tile), or of the range inside one
     if (use.j + 1u == use.j1 || use.at + 1u == r1) {
-      fresh = true;
+      fresh = written = true;
       const uint64_t seg0 = use.at - (use.j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
       const bool mine = seg0 >= r0 && seg1 <= r1;
       // each warp's sums into the stage it has just used, float4 pieces swizzled by head
@@ -559,13 +595,19 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
       __syncthreads();  // the stages and joins are free again
     }
 
-    fetch(stage);
-    cp_async_commit();
+    if (written) fence_proxy_async_smem();
+    __syncwarp();
+    if (arrives) fetch(stage);
     look_up();
-    stage = stage + 1u == kStages ? 0u : stage + 1u;
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1u;
+    }
     use.next(c, a, r1);
   }
-  cp_async_wait<0>();
+  if (!arrives) {  // a wait ran out (QG_ERR_WAIT_TIMEOUT is set): let what is in flight land
+    for (uint32_t i = 0; i < kStages; ++i) mbar_wait_bounded(&full[warp][(stage + i) % kStages], parity ^ 1u);
+  }
 }
 
 // weight_out = weight_in + the slot's shares summed over the heads of its kv head.
@@ -628,8 +670,54 @@ int sm_count() {
   return cache[dev];
 }
 
+// cuTensorMapEncodeTiled from the driver (looked up once; no link-time dependency on libcuda).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    const bool found = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                                        &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(found ? p : nullptr);
+  }();
+  return fn;
+}
+
+// Strides of a tensor map nest: each is a multiple of the one inside it (a dimension of one
+// entry takes whatever fits).  False where the pools' do not.
+struct PoolStrides {
+  uint64_t inner, outer, page;  // bytes
+  bool heads_inside;
+};
+bool pool_strides(const qg_kv_pages* cache, PoolStrides* s) {
+  uint64_t head = cache->head_stride * 2u, slot = cache->slot_stride * 2u;
+  const uint64_t row = cache->head_dim * 2u;
+  s->heads_inside = cache->n_kv_heads != 1u && (cache->page_size == 1u || head < slot);
+  if (cache->n_kv_heads == 1u) head = cache->page_size == 1u ? row : slot;
+  if (cache->page_size == 1u) slot = head;
+  s->inner = s->heads_inside ? head : slot;
+  s->outer = s->heads_inside ? slot : head;
+  s->page = cache->num_pages == 1u ? s->outer : cache->page_stride * 2u;
+  return s->inner >= row && s->inner % 16u == 0u && s->outer >= s->inner && s->outer % s->inner == 0u &&
+         s->page >= s->outer && s->page % s->outer == 0u && s->page < (1ull << 40);
+}
+
+bool encode_pool(CUtensorMap* map, void* pool, const qg_kv_pages* cache, const PoolStrides& s, uint32_t box_slots) {
+  const auto encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const uint32_t inner = s.heads_inside ? cache->n_kv_heads : cache->page_size;
+  const uint32_t outer = s.heads_inside ? cache->page_size : cache->n_kv_heads;
+  const cuuint64_t dims[4] = {cache->head_dim, inner, outer, cache->num_pages};
+  const cuuint64_t strides[3] = {s.inner, s.outer, s.page};
+  const cuuint32_t box[4] = {64u, s.heads_inside ? 1u : box_slots, s.heads_inside ? box_slots : 1u, 1u};
+  const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+  return encode(map, cache->dtype == QG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP, int MT, bool EXTRA>
-cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, const AttnMaps& maps, cudaStream_t stream) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
   const auto kernel = paged_attn_kernel<T, DP, MT, EXTRA>;
   {
@@ -649,25 +737,25 @@ cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, cudaStream_t stre
                           ((std::min(a.max_len, c.capacity) + kBlock - 1u) / kBlock);
   const uint64_t fit = static_cast<uint64_t>(sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
-  return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a);
+  return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);
 }
 
 template <typename T>
 cudaError_t launch_attn(const AttnPlan& p, bool extra, const PagedView& c, const AttnArgs& a,
-                        cudaStream_t stream) {
+                        const AttnMaps& maps, cudaStream_t stream) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     if (extra) {
-      if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, true>(c, a, stream);
-      if (p.dp == 64u) return launch_attn<T, 64, 1, true>(c, a, stream);
-      if (p.dp == 128u) return launch_attn<T, 128, 1, true>(c, a, stream);
-      return launch_attn<T, 256, 1, true>(c, a, stream);
+      if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, true>(c, a, maps, stream);
+      if (p.dp == 64u) return launch_attn<T, 64, 1, true>(c, a, maps, stream);
+      if (p.dp == 128u) return launch_attn<T, 128, 1, true>(c, a, maps, stream);
+      return launch_attn<T, 256, 1, true>(c, a, maps, stream);
     }
   }
-  if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, false>(c, a, stream);
-  if (p.dp == 64u) return launch_attn<T, 64, 1, false>(c, a, stream);
-  if (p.dp == 128u && p.mt == 2u) return launch_attn<T, 128, 2, false>(c, a, stream);
-  if (p.dp == 128u) return launch_attn<T, 128, 1, false>(c, a, stream);
-  return launch_attn<T, 256, 1, false>(c, a, stream);
+  if (p.dp == 64u && p.mt == 2u) return launch_attn<T, 64, 2, false>(c, a, maps, stream);
+  if (p.dp == 64u) return launch_attn<T, 64, 1, false>(c, a, maps, stream);
+  if (p.dp == 128u && p.mt == 2u) return launch_attn<T, 128, 2, false>(c, a, maps, stream);
+  if (p.dp == 128u) return launch_attn<T, 128, 1, false>(c, a, maps, stream);
+  return launch_attn<T, 256, 1, false>(c, a, maps, stream);
 }
 
 }  // namespace
@@ -704,8 +792,18 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
       (weights && p->weight_stride < p->max_len) || (!weights && p->weight_in != nullptr)) {
     return cudaErrorInvalidValue;
   }
+  PoolStrides strides;
+  if (!pool_strides(cache, &strides)) return cudaErrorInvalidValue;
+  const uint32_t box = 1u << std::min(4, __builtin_ctz(cache->page_size));  // gcd(16, page_size)
+  AttnMaps maps;
+  if (!encode_pool(&maps.k, cache->k, cache, strides, box) || !encode_pool(&maps.v, cache->v, cache, strides, box)) {
+    return cudaErrorNotSupported;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AttnArgs a{};
+  a.box = box;
+  a.boxes = kTile / box;
+  a.heads_inside = strides.heads_inside;
   a.q = p->q;
   a.out = p->out;
   a.dtype = p->dtype;
@@ -724,8 +822,8 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
   a.scores = weights ? reinterpret_cast<float*>(ws + plan.scores_at) : nullptr;
   a.norm = weights ? reinterpret_cast<float*>(ws + plan.norm_at) : nullptr;
   a.score_stride = (p->max_len + kBlock - 1u) / kBlock * kBlock;
-  const cudaError_t e = cache->dtype == QG_F16 ? launch_attn<__half>(plan, extra, c, a, stream)
-                                               : launch_attn<__nv_bfloat16>(plan, extra, c, a, stream);
+  const cudaError_t e = cache->dtype == QG_F16 ? launch_attn<__half>(plan, extra, c, a, maps, stream)
+                                               : launch_attn<__nv_bfloat16>(plan, extra, c, a, maps, stream);
   if (e != cudaSuccess || !weights) return e;
   const dim3 grid((std::min(p->max_len, c.capacity) + 255u) / 256u, c.n_kv, c.batch);
   return launch_k(attn_weight_kernel, grid, 256, 0, stream, c, a, p->weight_in, p->weight_out,

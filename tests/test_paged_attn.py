@@ -293,7 +293,7 @@ def _args():
 
 @pytest.mark.parametrize("what,field,value", [
     ("c", "k", None), ("c", "dtype", 0), ("c", "head_dim", 12), ("c", "slot_stride", 4), ("c", "page_size", 0),
-    ("c", "table_pages", 2 ** 31 - 1),
+    ("c", "table_pages", 2 ** 31 - 1), ("c", "head_stride", 1032), ("c", "slot_stride", 56), ("c", "page_stride", 1536),
     ("a", "q", None), ("a", "q", 8), ("a", "out", None), ("a", "out", 24), ("a", "dtype", -1), ("a", "dtype", 3),
     ("a", "n_q_heads", 0), ("a", "n_q_heads", 3), ("a", "q_stride", 4), ("a", "out_stride", 260), ("a", "lens", None),
     ("a", "max_len", 0), ("a", "max_len", 2 ** 31), ("a", "weight_in", 64), ("a", "weight_out", 64),
