@@ -13,14 +13,14 @@
 // loads the slots; its rate is far above the few per cent that the memory can feed, so
 // tcgen05 with its trip through tensor memory has nothing to win here.
 //
-// Work.  The unit is a block of 64 slots of one (sequence, kv head, head tile); all blocks of
+// Work.  The unit is a block of 128 slots of one (sequence, kv head, head tile); all blocks of
 // the batch, whatever the lengths, form one line that is cut into equal ranges, one a CTA
-// (two CTAs an SM).  In a range, warp w owns slots [16 w, 16 w + 16) of every block and runs
-// on its own: it fetches its rows through its own ring of stages and keeps its own (m, l, o).
-// Rows arrive as TMA boxes of gcd(16, page_size) slots x 64 values, swizzled for ldmatrix, so
-// no box crosses a page, whatever the page size, and values past head_dim, slots of no page
-// and slots past the sequence's last box are the tensor map's zeros; a tile's page ids are
-// read one tile ahead.  Only rows that share a box with the sequence's ends can hold what is
+// (two CTAs an SM).  In a range, warp w owns slots [32 w, 32 w + 32) of every block and runs
+// on its own: it fetches its K and V tiles in turn through its own ring and keeps its own
+// (m, l, o).  Tiles arrive as TMA boxes of gcd(32, page_size) slots x 64 values, swizzled for
+// ldmatrix, so no box crosses a page, whatever the page size, and values past head_dim, slots
+// of no page and slots past the sequence's last box are the tensor map's zeros; page ids are
+// read 32 boxes at a time, ahead of their use.  Only rows that share a box with the sequence's ends can hold what is
 // not the sequence's: their V rows are cleared in shared memory, their scores are masked.
 // Where a (sequence, head) ends inside the range the four warps join through
 // shared memory; where it was cut by the range, the CTA leaves a record, and the CTA that
@@ -34,7 +34,7 @@
 // accumulators are laid out like the A operand of the next product, so probabilities go back
 // in without a shuffle, again as hi + lo; they carry a factor 2^14 (removed with l), which
 // keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
-// Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
+// Each 32-slot tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
 // matrix pipe truncates when it accumulates, and o lives for thousands of tiles.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -52,7 +52,8 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kAttnThreads = kWarps * 32;
-constexpr uint32_t kTile = 16;                // slots of one warp's tile
+constexpr uint32_t kTile = 32;                // slots of one warp's tile
+constexpr uint32_t kLogTile = 5;
 constexpr uint32_t kBlock = kTile * kWarps;   // slots of a block
 constexpr uint32_t kMaxCtas = 512;            // counters in the workspace's zeroed bytes
 static_assert(kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "one counter per CTA");
@@ -73,7 +74,7 @@ struct AttnArgs {
   float* scores;               // [batch][n_q][score_stride], log2 units, or NULL
   float* norm;                 // [batch][n_q]: log2 of the full sum, with scores
   uint32_t score_stride;
-  uint32_t box, boxes;         // slots of a box, boxes of a tile's 16 slots
+  uint32_t log_boxes;          // log2 of the boxes of a tile
   bool heads_inside;           // a page's heads lie inside its slots ([place][head][dim])
 };
 
@@ -140,11 +141,10 @@ __device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N
   }
 }
 
-// Where a range of blocks is: sequence, kv head x head tile, block.
-struct Cursor {
-  uint64_t at;                       // block's place in the line
-  uint32_t b, h, j, j0, j1;          // j in [j0, j1)
-  uint32_t start, len;               // the sequence's seen slots are [start, len)
+// One (sequence, kv head x head tile) of the line: its seen slots [start, len) are blocks
+// [j0, j1); j is the next one.
+struct Segment {
+  uint32_t b, h, j, j0, j1, start, len;
 
   __device__ __forceinline__ void bounds(const PagedView& c, const AttnArgs& a) {
     len = paged_len(a.lens[b], min(a.max_len, c.capacity));
@@ -152,16 +152,14 @@ struct Cursor {
     j0 = start / kBlock;
     j1 = max((len + kBlock - 1u) / kBlock, j0 + 1u);  // an empty sequence has one empty block
   }
-  __device__ __forceinline__ void next(const PagedView& c, const AttnArgs& a, uint64_t end) {
-    ++at;
-    if (++j == j1) {
-      if (++h == c.n_kv * a.tiles) {
-        h = 0;
-        ++b;
-        if (at < end) bounds(c, a);
-      }
-      j = j0;
+  // The one after it, if `more` blocks of the range are left.
+  __device__ __forceinline__ void next(const PagedView& c, const AttnArgs& a, bool more) {
+    if (++h == c.n_kv * a.tiles) {
+      h = 0;
+      ++b;
+      if (more) bounds(c, a);
     }
+    j = j0;
   }
 };
 
@@ -170,49 +168,50 @@ struct Cursor {
 template <typename T, int DP, int MT, bool EXTRA>
 struct AttnShape {
   static constexpr uint32_t kHeads = 8u * MT;
-  static constexpr uint32_t kStage = 2u * kTile * DP * 2u;  // one warp's K and V tile
-  static constexpr uint32_t kStages = DP == 64 ? 6 : 3;
-  static constexpr uint32_t kRing = kWarps * kStages * kStage;
+  static constexpr uint32_t kUnit = kTile * DP * 2u;        // a warp's K or V tile
+  static constexpr uint32_t kUnits = DP == 64 ? 6 : 3;      // of its ring
+  static constexpr uint32_t kRing = kWarps * kUnits * kUnit;
   static constexpr uint32_t kQRows = MT * (EXTRA ? 24u : 16u);
   static constexpr uint32_t kQBytes = kQRows * DP * 2u;
   static constexpr uint32_t kSmem = kRing + kQBytes + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
-  static constexpr uint32_t kRecord = kHeads * (DP + 2u);  // m[], l[], o[][]
+  static constexpr uint32_t kRecord = kHeads * (DP + 2u);   // m[], l[], o[][]
   static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
-  static_assert(kHeads * DP * 4u <= kStage, "a warp's sums join in its free stage");
+  static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
 
 template <typename T, int DP, int MT, bool EXTRA>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCtasPerSm)
     paged_attn_kernel(const PagedView c, const AttnArgs a, const __grid_constant__ AttnMaps maps) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
-  constexpr uint32_t kStages = Shape::kStages, kHeads = Shape::kHeads;
+  constexpr uint32_t kUnits = Shape::kUnits, kUnit = Shape::kUnit, kHeads = Shape::kHeads;
   constexpr int kTerms = EXTRA ? 3 : 2;
+  constexpr int kSteps = kTile / 16;    // 16-slot steps of a product over slots
   constexpr uint32_t kPanels = Shape::kPanels, kPanel = kTile * 128u;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float join_m[kWarps][kHeads], join_l[kWarps][kHeads], q_mult[kHeads];
-  __shared__ __align__(8) uint64_t full[kWarps][kStages];
+  __shared__ __align__(8) uint64_t full[kWarps][kUnits];
   __shared__ uint64_t sum64[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
 
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  uint8_t* const ring = smem + warp * (kStages * Shape::kStage);
+  uint8_t* const ring = smem + warp * (kUnits * kUnit);
   const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(smem + Shape::kRing);
   if (lane == 0u) {
-    for (uint32_t i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1u);
+    for (uint32_t i = 0; i < kUnits; ++i) mbar_init(&full[warp][i], 1u);
     fence_mbar_init();
   }
 
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's range of the line of blocks
+  // ---- this CTA's range [r0, r1) of the line of blocks
   const uint32_t lines = c.n_kv * a.tiles;
   uint64_t total = 0;
   for (uint32_t b = tid; b < c.batch; b += kAttnThreads) {
-    Cursor s;
+    Segment s;
     s.b = b;
     s.bounds(c, a);
     total += s.j1 - s.j0;
@@ -230,7 +229,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   const uint64_t r0 = blockIdx.x * total / ctas, r1 = (blockIdx.x + 1u) * total / ctas;
   for (uint64_t base = 0, b0 = 0; b0 < c.batch; b0 += kAttnThreads) {
     const uint32_t b = static_cast<uint32_t>(b0) + tid;
-    Cursor s;
+    Segment s;
     uint64_t n = 0;
     if (b < c.batch) {
       s.b = b;
@@ -263,77 +262,112 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     if (base * lines > r0) break;
   }
   __syncthreads();
-  Cursor use;
-  use.at = r0;
+  Segment use;
   use.b = first_at[0];
   use.h = first_at[1];
   use.bounds(c, a);
   use.j = use.j0 + first_at[2];
-  Cursor ahead = use;
+  uint32_t left = static_cast<uint32_t>(r1 - r0);  // blocks, this one included (below 2^31)
 
-  // ---- fetching: lane l knows the page and place of slot l % 16 of the next tile
+  // ---- fetching.  A set of page ids covers the next 32 boxes of this warp's tiles, a box a
+  // lane; the set after it is read while this one is used.
   const uint64_t policy = l2_evict_first_policy();
-  int32_t page = 0, place = 0, head = 0;
-  bool more = false;
+  const uint32_t boxes = 1u << a.log_boxes, log_box = kLogTile - a.log_boxes;
+  Segment ahead = use;
+  uint32_t ahead_left = left;
+  int32_t page = 0, place = 0, head = 0, next_page = 0, next_place = 0, next_head = 0;
+  uint32_t at_tile = 0, tiles = 0, next_tiles = 0;  // of the set
   auto look_up = [&]() {
-    more = ahead.at < r1;
-    if (more) {
-      const uint32_t slot = ahead.j * kBlock + warp * kTile + (lane & 15u);
-      const uint32_t box0 = slot & ~(a.box - 1u);
-      const uint32_t at = div_by(slot, c.page);
-      page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
-      place = static_cast<int32_t>(slot - at * c.page.d);
-      head = static_cast<int32_t>(ahead.h / a.tiles);
-      if (box0 < ahead.len && box0 + a.box > ahead.start) {
-        const uint32_t id = static_cast<uint32_t>(c.table[static_cast<size_t>(ahead.b) * c.table_stride + at]);
-        if (id < c.num_pages) {
-          page = static_cast<int32_t>(id);
-        } else {
-          atomicOr(&g_error_word, QG_ERR_PAGE);
+    next_tiles = min(min(32u >> a.log_boxes, ahead.j1 - ahead.j), ahead_left);
+    if (next_tiles == 0u) return;
+    const uint32_t t = lane >> a.log_boxes;
+    const uint32_t slot = (ahead.j + t) * kBlock + warp * kTile + ((lane & (boxes - 1u)) << log_box);
+    const uint32_t at = div_by(slot, c.page);
+    next_page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
+    next_place = static_cast<int32_t>(slot - at * c.page.d);
+    next_head = static_cast<int32_t>(ahead.h / a.tiles);
+    if (t < next_tiles && slot < ahead.len && slot + (1u << log_box) > ahead.start) {
+      const uint32_t id = static_cast<uint32_t>(c.table[static_cast<size_t>(ahead.b) * c.table_stride + at]);
+      if (id < c.num_pages) {
+        next_page = static_cast<int32_t>(id);
+      } else {
+        atomicOr(&g_error_word, QG_ERR_PAGE);
+      }
+    }
+    ahead.j += next_tiles;
+    ahead_left -= next_tiles;
+    if (ahead.j == ahead.j1) ahead.next(c, a, ahead_left != 0u);
+  };
+  auto next_set = [&]() {
+    page = next_page;
+    place = next_place;
+    head = next_head;
+    tiles = next_tiles;
+    at_tile = 0;
+    look_up();
+  };
+  // the K (before its V) or V tile of the next block into unit u
+  auto fetch = [&](uint32_t u, bool is_v) {
+    if (!is_v && at_tile == tiles) next_set();
+    if (at_tile == tiles) return;  // the range is fetched
+    const uint32_t to = ring_at + u * kUnit, bar = smem_addr(&full[warp][u]);
+    if (lane == 0u) mbar_arrive_expect_tx(&full[warp][u], kUnit);
+    __syncwarp();
+    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+#pragma unroll
+    for (uint32_t p = 0; p < kPanels; p += (kPanels == 1u ? 1u : 2u)) {
+      // lanes: boxes of one panel, or of two where both fit a warp
+      const uint32_t sub = kPanels == 1u ? lane : lane >> 1, panel = kPanels == 1u ? 0u : p + (lane & 1u);
+      constexpr uint32_t kOnce = kPanels == 1u ? 32u : 16u;
+      for (uint32_t s0 = 0; s0 < boxes; s0 += kOnce) {
+        const uint32_t from = ((at_tile << a.log_boxes) + s0 + sub) & 31u;
+        const int32_t pg = __shfl_sync(0xffffffffu, page, from), pl = __shfl_sync(0xffffffffu, place, from);
+        if (s0 + sub < boxes) {
+          tma_load_4d(to + panel * kPanel + ((s0 + sub) << log_box) * 128u, map, static_cast<int32_t>(panel * 64u),
+                      a.heads_inside ? head : pl, a.heads_inside ? pl : head, pg, bar, policy);
         }
       }
-      ahead.next(c, a, r1);
     }
-  };
-  auto fetch = [&](uint32_t stage) {
-    if (!more) return;
-    const uint32_t to = ring_at + stage * Shape::kStage, bar = smem_addr(&full[warp][stage]);
-    if (lane == 0u) mbar_arrive_expect_tx(&full[warp][stage], Shape::kStage);
-    __syncwarp();
-    for (uint32_t i0 = 0; i0 < a.boxes * kPanels * 2u; i0 += 32u) {
-      const uint32_t i = i0 + lane, panel = (i >> 1) % kPanels, r = (i >> 1) / kPanels * a.box;
-      const int32_t pg = __shfl_sync(0xffffffffu, page, r & 15u), pl = __shfl_sync(0xffffffffu, place, r & 15u);
-      if (r < kTile) {
-        const uint32_t dst = to + ((i & 1u) * kPanels + panel) * kPanel + r * 128u;
-        tma_load_4d(dst, (i & 1u) != 0u ? &maps.v : &maps.k, static_cast<int32_t>(panel * 64u),
-                    a.heads_inside ? head : pl, a.heads_inside ? pl : head, pg, bar, policy);
-      }
-    }
+    if (is_v) ++at_tile;
   };
   look_up();
 #pragma unroll
-  for (uint32_t s = 0; s < kStages; ++s) {
-    fetch(s);
-    look_up();
-  }
+  for (uint32_t u = 0; u < kUnits; ++u) fetch(u, (u & 1u) != 0u);
+  bool fetch_v = (kUnits & 1u) != 0u;  // what the next free unit receives
+
   // ldmatrix rows and 16-byte pieces of this lane (K: 8 slots x 2 pieces x 2; V, transposed:
   // 16 slots x 2 pieces); piece 2 n of a panel is at lane_at ^ (n << 5)
   const uint32_t kr = (lane & 7u) + ((lane >> 4) << 3), vr = (lane & 7u) + ((lane >> 3) & 1u) * 8u;
   const uint32_t k_lane = kr * 128u + ((((lane >> 3) & 1u) ^ (kr & 7u)) << 4);
-  const uint32_t v_lane = kPanels * kPanel + vr * 128u + (((lane >> 4) ^ (vr & 7u)) << 4);
+  const uint32_t v_lane = vr * 128u + (((lane >> 4) ^ (vr & 7u)) << 4);
 
   uint32_t qa[MT][DP / 16][4], qx[MT][EXTRA ? DP / 16 : 1][2];
   float o[MT][DP / 8][2], m[MT], l[MT], mult[MT];
-  uint32_t stage = 0, parity = 0;
-  bool fresh = true, arrives = true;
+  uint32_t unit = 0, parity = 0;
+  bool arrives = true;
+  auto await_unit = [&]() {
+    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[warp][unit], parity))) {
+      arrives = arrives && __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][unit], parity));
+    }
+  };
+  auto release_unit = [&](bool written) {
+    if (written) fence_proxy_async_smem();
+    __syncwarp();
+    if (arrives) fetch(unit, fetch_v);
+    fetch_v = !fetch_v;
+    if (++unit == kUnits) {
+      unit = 0;
+      parity ^= 1u;
+    }
+  };
 
-  while (use.at < r1) {
+  while (left != 0u) {
     const uint32_t kv = use.h / a.tiles, ht = use.h - kv * a.tiles;
     const uint32_t heads = min(kHeads, a.group - ht * kHeads);
     const uint32_t head0 = kv * a.group + ht * kHeads;
+    const uint32_t from_j = use.j, to_j = min(use.j1, use.j + left);
 
-    if (fresh) {  // ---- the queries of a new (sequence, head tile)
-      fresh = false;
+    {  // ---- the queries
       constexpr uint32_t kPer = DP / 32;
       for (uint32_t r = warp; r < kHeads; r += kWarps) {
         float x[kPer];
@@ -394,104 +428,139 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
       }
     }
 
-    // ---- one tile: scores, probabilities, weighted values
-    arrives = arrives && __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], parity));
-    const uint32_t slot0 = use.j * kBlock + warp * kTile;
-    const uint32_t tile_at = ring_at + stage * Shape::kStage;
-    const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
-    bool written = false;  // by this warp, where the next box will land
-    if (arrives && slot0 < use.len && slot0 + kTile > use.start) {
-      if (!whole) {  // V rows beside the sequence's ends: 0 x NaN must not reach the sums
-        written = true;
-        for (uint32_t i = lane; i < kTile * DP / 8u; i += 32u) {
-          const uint32_t r = i / 8u % kTile;
-          if (slot0 + r < use.start || slot0 + r >= use.len) {
-            reinterpret_cast<uint4*>(ring + stage * Shape::kStage + kPanels * kPanel)[i] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        __syncwarp();
-      }
-      float s[MT][2][4], sx[MT][2][EXTRA ? 4 : 1];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][0][e] = s[i][1][e] = 0.f;
-#pragma unroll
-        for (int e = 0; e < (EXTRA ? 4 : 1); ++e) sx[i][0][e] = sx[i][1][e] = 0.f;
-      }
-#pragma unroll
-      for (uint32_t kk = 0; kk < DP / 16; ++kk) {
-        uint32_t kb[4];
-        ldsm_x4(kb, tile_at + (k_lane ^ ((kk & 3u) << 5)) + kk / 4u * kPanel);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          mma(s[i][0], qa[i][kk][0], qa[i][kk][1], qa[i][kk][2], qa[i][kk][3], kb[0], kb[1], T());
-          mma(s[i][1], qa[i][kk][0], qa[i][kk][1], qa[i][kk][2], qa[i][kk][3], kb[2], kb[3], T());
-          if constexpr (EXTRA) {
-            mma(sx[i][0], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[0], kb[1], T());
-            mma(sx[i][1], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[2], kb[3], T());
-          }
-        }
-      }
-      uint32_t p0[MT][kTerms], p1[MT][kTerms];
+    for (; use.j < to_j; ++use.j) {
+      const uint32_t slot0 = use.j * kBlock + warp * kTile;
+      const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
+      const bool seen = slot0 < use.len && slot0 + kTile > use.start;
+      // ---- scores
+      uint32_t p[MT][kSteps][2][kTerms];  // probabilities: [16-slot step][8-slot half][term]
       float fade[MT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        // this thread's head is 8 i + g; its slots 2 t4, 2 t4 + 1 and 8 more
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float hi = s[i][e >> 1][e & 1];
-          float lo = s[i][e >> 1][(e & 1) + 2];
-          if constexpr (EXTRA) lo += sx[i][e >> 1][e & 1];
-          // an infinite key: the errors' products are not numbers, the first term's sum is right
-          x[e] = (fabsf(hi) == CUDART_INF_F ? hi : hi + lo) * mult[i];
-          const uint32_t slot = slot0 + (e >> 1) * 8u + 2u * t4 + (e & 1);
-          if (!whole && (slot < use.start || slot >= use.len)) x[e] = -CUDART_INF_F;
-        }
-        if (a.scores != nullptr && i * 8u + g < heads) {
-          float* to = a.scores + (static_cast<size_t>(use.b) * a.n_q + head0 + i * 8u + g) * a.score_stride + slot0;
-          *reinterpret_cast<float2*>(to + 2u * t4) = make_float2(x[0], x[1]);
-          *reinterpret_cast<float2*>(to + 8u + 2u * t4) = make_float2(x[2], x[3]);
-        }
-        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(m[i], top);
-        const float from = now == -CUDART_INF_F ? 0.f : now;
-        fade[i] = exp2_fast(m[i] - from);
-        m[i] = now;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = exp2_fast(x[e] - from + kShareBits);
-        l[i] = fmaf(l[i], fade[i], (x[0] + x[1]) + (x[2] + x[3]));
-        split_terms<T>(x[0], x[1], p0[i]);
-        split_terms<T>(x[2], x[3], p1[i]);
-      }
-#pragma unroll
-      for (uint32_t n = 0; n < DP / 16; ++n) {
-        uint32_t vb[4];
-        ldsm_x4_trans(vb, tile_at + (v_lane ^ ((n & 3u) << 5)) + n / 4u * kPanel);
+      await_unit();
+      if (seen && arrives) {
+        float s[MT][2 * kSteps][4], sx[MT][2 * kSteps][EXTRA ? 4 : 1];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
-          for (uint32_t e = 0; e < 2; ++e) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma(d, p0[i][0], p0[i][1], p1[i][0], p1[i][1], vb[2 * e], vb[2 * e + 1], T());
-            if constexpr (EXTRA) mma(d, p0[i][kTerms - 1], 0u, p1[i][kTerms - 1], 0u, vb[2 * e], vb[2 * e + 1], T());
-            o[i][2 * n + e][0] = fmaf(o[i][2 * n + e][0], fade[i], d[0] + d[2]);
-            o[i][2 * n + e][1] = fmaf(o[i][2 * n + e][1], fade[i], d[1] + d[3]);
+          for (int n = 0; n < 2 * kSteps; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < (EXTRA ? 4 : 1); ++e) sx[i][n][e] = 0.f;
+          }
+        }
+        const uint32_t k_at = ring_at + unit * kUnit;
+#pragma unroll
+        for (uint32_t kk = 0; kk < DP / 16; ++kk) {
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            uint32_t kb[4];
+            ldsm_x4(kb, k_at + (k_lane ^ ((kk & 3u) << 5)) + kk / 4u * kPanel + st * 2048u);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const uint32_t* q = qa[i][kk];
+              mma(s[i][2 * st], q[0], q[1], q[2], q[3], kb[0], kb[1], T());
+              mma(s[i][2 * st + 1], q[0], q[1], q[2], q[3], kb[2], kb[3], T());
+              if constexpr (EXTRA) {
+                mma(sx[i][2 * st], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[0], kb[1], T());
+                mma(sx[i][2 * st + 1], qx[i][kk][0], 0u, qx[i][kk][1], 0u, kb[2], kb[3], T());
+              }
+            }
+          }
+        }
+        // ---- probabilities: this thread's head is 8 i + g, its slots 8 n + 2 t4 and one more
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          float x[2 * kSteps][2];
+          float top = -CUDART_INF_F;
+#pragma unroll
+          for (int n = 0; n < 2 * kSteps; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float hi = s[i][n][e];
+              float lo = s[i][n][e + 2];
+              if constexpr (EXTRA) lo += sx[i][n][e];
+              // an infinite key: the errors' products are not numbers, the first term's sum is right
+              x[n][e] = (fabsf(hi) == CUDART_INF_F ? hi : hi + lo) * mult[i];
+              const uint32_t slot = slot0 + n * 8u + 2u * t4 + e;
+              if (!whole && (slot < use.start || slot >= use.len)) x[n][e] = -CUDART_INF_F;
+            }
+            if (a.scores != nullptr && i * 8u + g < heads) {
+              const size_t row = static_cast<size_t>(use.b) * a.n_q + head0 + i * 8u + g;
+              *reinterpret_cast<float2*>(a.scores + row * a.score_stride + slot0 + n * 8u + 2u * t4) =
+                  make_float2(x[n][0], x[n][1]);
+            }
+            top = fmaxf(top, fmaxf(x[n][0], x[n][1]));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float now = fmaxf(m[i], top);
+          const float from = now == -CUDART_INF_F ? 0.f : now;
+          fade[i] = exp2_fast(m[i] - from);
+          m[i] = now;
+          const float base = kShareBits - from;
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < 2 * kSteps; ++n) {
+            x[n][0] = exp2_fast(x[n][0] + base);
+            x[n][1] = exp2_fast(x[n][1] + base);
+            sum += x[n][0] + x[n][1];
+            split_terms<T>(x[n][0], x[n][1], p[i][n / 2][n % 2]);
+          }
+          l[i] = fmaf(l[i], fade[i], sum);
+        }
+      }
+      release_unit(false);
+
+      // ---- weighted values
+      await_unit();
+      bool written = false;  // by this warp, where the next box will land
+      if (seen && arrives) {
+        if (!whole) {  // V rows beside the sequence's ends: 0 x NaN must not reach the sums
+          written = true;
+          for (uint32_t i = lane; i < kTile * DP / 8u; i += 32u) {
+            const uint32_t slot = slot0 + i / 8u % kTile;
+            if (slot < use.start || slot >= use.len) {
+              reinterpret_cast<uint4*>(ring + unit * kUnit)[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          __syncwarp();
+        }
+        const uint32_t v_at = ring_at + unit * kUnit;
+#pragma unroll
+        for (uint32_t n = 0; n < DP / 16; ++n) {
+          uint32_t vb[kSteps][4];
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            ldsm_x4_trans(vb[st], v_at + (v_lane ^ ((n & 3u) << 5)) + n / 4u * kPanel + st * 2048u);
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int st = 0; st < kSteps; ++st) {
+                const auto& ps = p[i][st];
+                mma(d, ps[0][0], ps[0][1], ps[1][0], ps[1][1], vb[st][2 * e], vb[st][2 * e + 1], T());
+                if constexpr (EXTRA) {
+                  mma(d, ps[0][kTerms - 1], 0u, ps[1][kTerms - 1], 0u, vb[st][2 * e], vb[st][2 * e + 1], T());
+                }
+              }
+              o[i][2 * n + e][0] = fmaf(o[i][2 * n + e][0], fade[i], d[0] + d[2]);
+              o[i][2 * n + e][1] = fmaf(o[i][2 * n + e][1], fade[i], d[1] + d[3]);
+            }
           }
         }
       }
+      __syncwarp();
+      if (use.j + 1u < to_j) release_unit(written);  // the last one is where the warp joins
     }
-    __syncwarp();
+    left -= to_j - from_j;
 
-    // ---- the end of a (sequence, head tile), or of the range inside one
-    if (use.j + 1u == use.j1 || use.at + 1u == r1) {
-      fresh = written = true;
-      const uint64_t seg0 = use.at - (use.j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
-      const bool mine = seg0 >= r0 && seg1 <= r1;
-      // each warp's sums into the stage it has just used, float4 pieces swizzled by head
+    // ---- the end of the segment, or of the range inside it
+    {
+      const bool mine = from_j == use.j0 && to_j == use.j1;
+      // each warp's sums into the unit it has just used, float4 pieces swizzled by head
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         float sum = l[i];
@@ -501,14 +570,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
           join_m[warp][i * 8 + g] = m[i];
           join_l[warp][i * 8 + g] = sum;
         }
-        float2* to = reinterpret_cast<float2*>(ring + stage * Shape::kStage) + (i * 8u + g) * (DP / 2u);
+        float2* to = reinterpret_cast<float2*>(ring + unit * kUnit) + (i * 8u + g) * (DP / 2u);
 #pragma unroll
         for (uint32_t n = 0; n < DP / 8; ++n) {
           to[(n * 4u + t4) ^ ((g & 3u) << 2)] = make_float2(o[i][n][0], o[i][n][1]);
         }
       }
       __syncthreads();
-      float* record = a.records + (static_cast<size_t>(blockIdx.x) * 2u + (seg0 < r0 ? 0u : 1u)) * Shape::kRecord;
+      float* record = a.records + (static_cast<size_t>(blockIdx.x) * 2u + (from_j == use.j0 ? 1u : 0u)) * Shape::kRecord;
       auto finish = [&](uint32_t h, uint32_t ch, float top, float sum, float4 v) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
@@ -526,9 +595,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         }
         if (ch == 0u) {
           const size_t hi = static_cast<size_t>(use.b) * a.n_q + head0 + h;
-          const float full = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
-          if (a.lse != nullptr) a.lse[hi] = full * 0.69314718055994530942f;
-          if (a.norm != nullptr) a.norm[hi] = full;
+          const float full_sum = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
+          if (a.lse != nullptr) a.lse[hi] = full_sum * 0.69314718055994530942f;
+          if (a.norm != nullptr) a.norm[hi] = full_sum;
         }
       };
       for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
@@ -542,7 +611,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w) {
           const float f = exp2_fast(join_m[w][h] - from);
-          const float4 x = reinterpret_cast<const float4*>(smem + (w * kStages + stage) * Shape::kStage)
+          const float4 x = reinterpret_cast<const float4*>(smem + (w * kUnits + unit) * kUnit)
               [h * (DP / 4u) + (ch ^ ((h & 3u) << 1))];
           sum = fmaf(join_l[w][h], f, sum);
           v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y);
@@ -560,6 +629,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
       }
       if (!mine) {
         // the CTAs that share this head: those that own its first to its last block
+        const uint64_t seg0 = r1 - left - (to_j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
         const uint64_t c0 = ((seg0 + 1u) * ctas - 1u) / total, c1 = (seg1 * ctas - 1u) / total;
         __threadfence();
         __syncthreads();
@@ -576,8 +646,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
             const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);
             float top = -CUDART_INF_F, sum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint64_t p = c0; p <= c1; ++p) {
-              const float* rec = a.records + (p * 2u + (p == c0 ? 1u : 0u)) * Shape::kRecord;
+            for (uint64_t q = c0; q <= c1; ++q) {
+              const float* rec = a.records + (q * 2u + (q == c0 ? 1u : 0u)) * Shape::kRecord;
               const float pm = __ldcg(rec + h), pl = __ldcg(rec + kHeads + h);
               const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + 2u * kHeads) + h * (DP / 4u) + ch);
               const float now = fmaxf(top, pm);
@@ -592,21 +662,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
           }
         }
       }
-      __syncthreads();  // the stages and joins are free again
+      __syncthreads();  // the units, the joins and the queries are free again
     }
-
-    if (written) fence_proxy_async_smem();
-    __syncwarp();
-    if (arrives) fetch(stage);
-    look_up();
-    if (++stage == kStages) {
-      stage = 0;
-      parity ^= 1u;
-    }
-    use.next(c, a, r1);
+    release_unit(true);
+    if (use.j == use.j1) use.next(c, a, left != 0u);
   }
   if (!arrives) {  // a wait ran out (QG_ERR_WAIT_TIMEOUT is set): let what is in flight land
-    for (uint32_t i = 0; i < kStages; ++i) mbar_wait_bounded(&full[warp][(stage + i) % kStages], parity ^ 1u);
+    for (uint32_t i = 0; i < kUnits; ++i) {
+      const uint32_t u = unit + i < kUnits ? unit + i : unit + i - kUnits;
+      mbar_wait_bounded(&full[warp][u], unit + i < kUnits ? parity : parity ^ 1u);
+    }
   }
 }
 
@@ -737,6 +802,7 @@ cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, const AttnMaps& m
                           ((std::min(a.max_len, c.capacity) + kBlock - 1u) / kBlock);
   const uint64_t fit = static_cast<uint64_t>(sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
+  if (blocks / grid >= (1ull << 31)) return cudaErrorInvalidValue;  // a CTA counts its blocks in 32 bits
   return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);
 }
 
@@ -794,15 +860,15 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
   }
   PoolStrides strides;
   if (!pool_strides(cache, &strides)) return cudaErrorInvalidValue;
-  const uint32_t box = 1u << std::min(4, __builtin_ctz(cache->page_size));  // gcd(16, page_size)
+  const uint32_t log_box = std::min<uint32_t>(kLogTile, __builtin_ctz(cache->page_size));  // gcd(kTile, page_size)
+  const uint32_t box = 1u << log_box;
   AttnMaps maps;
   if (!encode_pool(&maps.k, cache->k, cache, strides, box) || !encode_pool(&maps.v, cache->v, cache, strides, box)) {
     return cudaErrorNotSupported;
   }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AttnArgs a{};
-  a.box = box;
-  a.boxes = kTile / box;
+  a.log_boxes = kLogTile - log_box;
   a.heads_inside = strides.heads_inside;
   a.q = p->q;
   a.out = p->out;
