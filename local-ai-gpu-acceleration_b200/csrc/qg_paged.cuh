@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t paged_len(int32_t len, uint32_t most) {
   return static_cast<uint32_t>(len);
 }
 
-// Element types: loads and stores of 8 consecutive values as fp32.
+// Pairs of 16-bit values as fp32 and back.
 __device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
@@ -76,43 +76,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <typename T>
-struct Raw8 {  // 8 elements as loaded
-  uint4 w;
-  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2(u[i], T());
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-};
-template <>
-struct Raw8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = reinterpret_cast<const float4*>(p)[0];
-    b = reinterpret_cast<const float4*>(p)[1];
-  }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  }
-};
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack2(x[0], x[1], T()), pack2(x[2], x[3], T()),
-                                            pack2(x[4], x[5], T()), pack2(x[6], x[7], T()));
-}
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
 // Host side.
