@@ -528,6 +528,7 @@ typedef struct qg_kv_pages {
  * q_out is zero, nothing is appended, slots[t] and seqs[t] are not read.  slots[t] < 0
  * appends nothing.  A position past the table sets QG_ERR_POSITION and gives a padding
  * row.  Two tokens of one call must not name the same slot.
+ * n_q_heads + 2 * n_kv_heads is at most 65535.
  * q, k, v: heads of a token are contiguous, token t starts at t * {q,k,v}_stride elements
  * (multiples of 16 bytes; so the three may be one fused projection); 16-B aligned. */
 #define QG_PAIRS_ADJACENT 0

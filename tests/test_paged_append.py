@@ -210,7 +210,7 @@ def _args():
     ("a", "q", None), ("a", "q", 72), ("a", "q_out", None), ("a", "q_out", 72), ("a", "k", None), ("a", "v", 72),
     ("a", "dtype", 3), ("a", "q_stride", 252), ("a", "v_stride", 124), ("a", "positions", None),
     ("a", "rope", None), ("a", "rope", 72), ("a", "rope_rows", 0), ("a", "rot_dim", 8), ("a", "rot_dim", 80),
-    ("a", "pairs", 2), ("a", "q_norm", 72), ("a", "k_norm", 72),
+    ("a", "pairs", 2), ("a", "q_norm", 72), ("a", "k_norm", 72), ("a", "n_q_heads", 65532),
 ])
 def test_append_refuses_bad_arguments(what, field, value):
     """Returned before any launch (and any CUDA call)."""
