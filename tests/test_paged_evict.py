@@ -97,6 +97,24 @@ def test_evict_keeps_the_heaviest(cuda, lens, budget, sink, recent, heads, dim, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_weights_apart_from_rows(cuda, in_place):
+    """Rows in place with new weights elsewhere, and rows elsewhere with weights in place: the
+    first kept slots do not move, their weights still have to."""
+    rng = np.random.default_rng(3)
+    lens, budget = [1500, 700, 90], 600
+    c = make_cache(rng, 3, 94 if in_place else 134, 16, 2, 128, torch.float16)
+    c, table = paged.PagedCache(c.k, c.v, c.table[:, :94]), c.table[:, :94] if in_place else c.table[:, 94:]
+    old = {"k": c.k.clone(), "v": c.v.clone()}
+    w = weights(rng, (3, 2, 1500), lens)
+    w[:, :, :300] += 1e5  # the first slots stay where they are
+    w0, ln, out = w.clone(), int32(lens), torch.full_like(w, 9.0) if in_place else w
+    kept, new = paged.evict(c, ln, w, budget, recent=10, new_table=None if in_place else table, weight_out=out)
+    check(c, old, table, kept, w0, out, lens, new, budget, 0, 10)
+    assert not in_place or torch.equal(w, w0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["zeros", "alike", "special", "narrow", "rising", "falling"])
 @pytest.mark.parametrize("n", [1000, 60000])  # keys held in shared memory, and read again
 def test_evict_ties_and_special_weights(cuda, kind, n):
