@@ -2,14 +2,14 @@
 // of slots by the attention weight that their slots received (declared in
 // include/qgemv_b200.h).  Two launches:
 //
-//  * evict_select_kernel, one CTA per (kv head, sequence): the budget-th largest key by radix
-//    selection (11 + 11 + 10 bits of an order-preserving integer image of the weights, the
-//    slots that always stay above every weight; histograms in shared memory), then the kept
-//    slots in ascending order: every warp counts its stretch of the slots, one scan over the
-//    warps, every warp writes its stretch.  Keys equal to the threshold are taken from the
-//    lowest slot on.  After the first pass the keys of the threshold's bin, where they fit,
-//    are listed and the other passes read the list alone.  Bound by instruction issue (one
-//    SM works for each (head, sequence)), so a lane takes 4 slots at a time.
+//  * evict_select_kernel, a cluster of 1 to 8 CTAs per (kv head, sequence), each with a
+//    stretch of the slots: the budget-th largest key by radix selection (11 + 11 + 10 bits of
+//    an order-preserving integer image of the weights, the slots that always stay above every
+//    weight; histograms in shared memory, added over the cluster through distributed shared
+//    memory), then the kept slots in ascending order: every warp counts its stretch, one scan
+//    over the warps and CTAs, every warp writes its stretch.  Keys equal to the threshold are
+//    taken from the lowest slot on.  Bound by instruction issue: some 100 instructions a warp
+//    for each 32 slots, which is why the cluster grows while SMs are free.
 //  * evict_move_kernel: rows kept[i] -> i, K and V of a row with one look-up; a lane looks up
 //    one row's places and the warp moves 32 rows through them.  In place a CTA walks i
 //    upwards and reads a chunk of rows before it writes it: kept[] ascends and
@@ -17,8 +17,9 @@
 //    independent, so 64-byte column slices walk side by side.  Into other pages there is no
 //    such order: whole rows, split over CTAs.  Bound by memory: the kept rows once in and
 //    once out.
-#include <algorithm>
+#include <cooperative_groups.h>
 
+#include <algorithm>
 #include <mutex>
 #include <set>
 
@@ -30,8 +31,8 @@ namespace {
 constexpr uint32_t kSelectThreads = 1024;
 constexpr uint32_t kSelectWarps = kSelectThreads / 32;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kListed = 4096;             // keys of one bin that fit the list
-constexpr uint32_t kCachedKeys = 48u * 1024u;  // slots whose keys fit in shared memory (192 KB)
+constexpr uint32_t kCachedKeys = 48u * 1024u;  // keys that fit in a CTA's shared memory (192 KB)
+constexpr uint32_t kMaxCluster = 8;            // CTAs of a cluster on every device
 constexpr uint32_t kStays = 0xffffffffu;       // key of a slot that always stays
 
 struct EvictArgs {
@@ -49,53 +50,67 @@ struct EvictArgs {
 
 // An integer that orders like the weight: NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (isnan(w)) return 0u;
   const uint32_t u = __float_as_uint(w + 0.f);
-  return (u & 0x80000000u) != 0u ? ~u : u | 0x80000000u;
+  const uint32_t key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return isnan(w) ? 0u : key;
+}
+constexpr uint32_t kZeroKey = 0x80000000u;     // of weight 0, the one that many slots share
+
+// blockIdx.x: rank in the cluster.  A CTA's stretch is a multiple of 32 slots a warp.
+__host__ __device__ constexpr uint32_t stretch(uint32_t n, uint32_t ctas) {
+  const uint32_t unit = kSelectWarps * 32u;
+  return ((n + ctas - 1u) / ctas + unit - 1u) / unit * unit;
 }
 
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const PagedView c, const EvictArgs a,
                                                                       bool cached) {
-  extern __shared__ uint4 keys4[];  // cached: the keys of all slots, then zeros to a multiple of 4
-  __shared__ uint32_t bins[kBins], list[kListed];
+  extern __shared__ uint32_t keys[];  // cached: the keys of this CTA's stretch
+  __shared__ uint32_t bins[kBins];
   __shared__ uint32_t warp_a[kSelectWarps], warp_b[kSelectWarps];
-  __shared__ uint32_t found_bin, found_left, found_count, listed;
+  __shared__ uint32_t found_bin, found_left, totals[2];
+  auto cluster = cooperative_groups::this_cluster();
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t kv = blockIdx.x, b = blockIdx.y;
-  uint32_t* const keys = reinterpret_cast<uint32_t*>(keys4);
+  const uint32_t kv = blockIdx.y, b = blockIdx.z, rank = blockIdx.x, ctas = gridDim.x;
   pdl_wait();
   pdl_trigger();
   const uint32_t n = paged_len(a.lens[b], min(a.max_len, c.capacity));
   const float* w = a.weight + (static_cast<size_t>(b) * c.n_kv + kv) * a.weight_stride;
   int32_t* kept = a.kept + (static_cast<size_t>(b) * c.n_kv + kv) * a.budget;
   if (n <= a.budget) {
-    for (uint32_t i = tid; i < a.budget; i += kSelectThreads) kept[i] = i < n ? static_cast<int32_t>(i) : -1;
+    for (uint32_t i = rank * kSelectThreads + tid; i < a.budget; i += ctas * kSelectThreads) {
+      kept[i] = i < n ? static_cast<int32_t>(i) : -1;
+    }
     return;
   }
   const uint32_t lo = a.sink, hi = n - a.recent;  // the slots that are chosen from
+  const uint32_t s0 = min(rank * stretch(n, ctas), n), s1 = min(s0 + stretch(n, ctas), n);
   auto slot_key = [&](uint32_t i) { return i < lo || i >= hi ? kStays : weight_key(w[i]); };
-  if (tid == 0u) listed = 0u;
+  auto key_at = [&](uint32_t i) { return cached ? keys[i - s0] : slot_key(i); };
 
-  // One histogram step: a warp's keys that count go to bins[]; the first one's bin in one
-  // addition, so weights that are all alike do not queue up.
-  auto count_keys = [&](uint32_t bin, bool counts) {
-    const uint32_t live = __ballot_sync(0xffffffffu, counts);
-    if (live == 0u) return;
-    const uint32_t lead = __ffs(live) - 1u;
-    const uint32_t lead_bin = __shfl_sync(0xffffffffu, bin, lead);
-    const uint32_t same = __ballot_sync(0xffffffffu, counts && bin == lead_bin);
-    if (lane == lead) {
-      atomicAdd(&bins[bin], static_cast<uint32_t>(__popc(same)));
-    } else if (counts && bin != lead_bin) {
+  // Histograms count one key at a time, but for slots that never had weight: those are
+  // counted in a register and added once a warp, so they do not queue up at one bin.
+  uint32_t zeros = 0;
+  auto count_key = [&](uint32_t key, uint32_t bin) {
+    if (key == kZeroKey) {
+      ++zeros;
+    } else {
       atomicAdd(&bins[bin], 1u);
     }
   };
   uint32_t left = a.budget;  // of the keys that match the prefix, how many stay
-  // The bin of the left-th largest counted key, with how many of its keys stay.
-  auto find_bin = [&]() {
-    __syncthreads();
+  // Adds the warps' zeros, then finds the bin of the left-th largest key that was counted.
+  auto find_bin = [&](uint32_t zero_bin) {
+    zeros = __reduce_add_sync(0xffffffffu, zeros);
+    if (lane == 0u && zeros != 0u) atomicAdd(&bins[zero_bin], zeros);
+    zeros = 0u;
+    cluster.sync();
     // thread t holds bins 2 t and 2 t + 1; upto: keys in them and in higher bins
-    const uint32_t b0 = bins[2u * tid], b1 = bins[2u * tid + 1u];
+    uint32_t b0 = 0, b1 = 0;
+    for (uint32_t r = 0; r < ctas; ++r) {
+      const uint2 x = reinterpret_cast<const uint2*>(cluster.map_shared_rank(bins, r))[tid];
+      b0 += x.x;
+      b1 += x.y;
+    }
     uint32_t upto = b0 + b1;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -104,131 +119,94 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     }
     if (lane == 0u) warp_a[warp] = upto;
     __syncthreads();
-    for (uint32_t x = warp + 1u; x < kSelectWarps; ++x) upto += warp_a[x];
+    upto += __reduce_add_sync(0xffffffffu, lane > warp ? warp_a[lane] : 0u);
     const uint32_t above1 = upto - b0 - b1, above0 = upto - b0;
     if (above1 < left && left <= above1 + b1) {
-      found_bin = 2u * tid + 1u, found_left = left - above1, found_count = b1;
+      found_bin = 2u * tid + 1u, found_left = left - above1;
     } else if (above0 < left && left <= above0 + b0) {
-      found_bin = 2u * tid, found_left = left - above0, found_count = b0;
+      found_bin = 2u * tid, found_left = left - above0;
     }
-    __syncthreads();
+    cluster.sync();  // every CTA has read the bins
     left = found_left;
   };
   auto clear_bins = [&]() {
-    __syncthreads();
-    for (uint32_t i = tid; i < kBins; i += kSelectThreads) bins[i] = 0u;
+    reinterpret_cast<uint2*>(bins)[tid] = make_uint2(0u, 0u);
     __syncthreads();
   };
 
   // ---- the threshold: bits 31-21 over all slots, then 20-10 and 9-0 over those that match
   clear_bins();
-  for (uint32_t i0 = 0; i0 < n; i0 += 4u * kSelectThreads) {
-    uint32_t key[4];
+  constexpr uint32_t kAhead = 8;  // weights in flight per thread
+  for (uint32_t i0 = s0; i0 < s1; i0 += kAhead * kSelectThreads) {
+    uint32_t key[kAhead];
 #pragma unroll
-    for (uint32_t u = 0; u < 4u; ++u) {
+    for (uint32_t u = 0; u < kAhead; ++u) {
       const uint32_t i = i0 + u * kSelectThreads + tid;
-      key[u] = i < n ? slot_key(i) : 0u;
+      if (i < s1) key[u] = slot_key(i);
     }
 #pragma unroll
-    for (uint32_t u = 0; u < 4u; ++u) {
+    for (uint32_t u = 0; u < kAhead; ++u) {
       const uint32_t i = i0 + u * kSelectThreads + tid;
-      if (cached && i < ((n + 3u) & ~3u)) keys[i] = key[u];
-      count_keys(key[u] >> 21, i < n);
-    }
-  }
-  find_bin();
-  uint32_t threshold = found_bin << 21;
-  const bool short_list = found_count <= kListed;
-  // four slots' keys from slot i (a multiple of 4); slots past n are 0 and never asked for
-  auto four_keys = [&](uint32_t i) {
-    if (cached) return keys4[i / 4u];
-    uint4 k;
-    k.x = i < n ? slot_key(i) : 0u;
-    k.y = i + 1u < n ? slot_key(i + 1u) : 0u;
-    k.z = i + 2u < n ? slot_key(i + 2u) : 0u;
-    k.w = i + 3u < n ? slot_key(i + 3u) : 0u;
-    return k;
-  };
-  if (short_list) {
-    for (uint32_t i = 4u * tid; i < n; i += 4u * kSelectThreads) {
-      const uint4 k = four_keys(i);
-      const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (uint32_t u = 0; u < 4u; ++u) {
-        if (i + u < n && key[u] >> 21 == found_bin) list[atomicAdd(&listed, 1u)] = key[u];
+      if (i < s1) {
+        if (cached) keys[i - s0] = key[u];
+        count_key(key[u], key[u] >> 21);
       }
     }
   }
+  find_bin(kZeroKey >> 21);
+  uint32_t threshold = found_bin << 21;
 #pragma unroll
   for (uint32_t pass = 0; pass < 2u; ++pass) {
     const uint32_t shift = pass == 0u ? 10u : 0u, width = pass == 0u ? 2048u : 1024u;
-    const uint32_t above = pass == 0u ? 21u : 10u;  // bits from here on are settled
+    const uint32_t settled = pass == 0u ? 21u : 10u;  // bits from here on match
     clear_bins();
-    const uint32_t m = short_list ? listed : n;
-    for (uint32_t i0 = 0; i0 < m; i0 += kSelectThreads) {
-      const uint32_t i = i0 + tid;
-      const uint32_t key = i >= m ? 0u : short_list ? list[i] : cached ? keys[i] : slot_key(i);
-      count_keys((key >> shift) & (width - 1u), i < m && (key ^ threshold) >> above == 0u);
+    for (uint32_t i = s0 + tid; i < s1; i += kSelectThreads) {
+      const uint32_t key = key_at(i);
+      if ((key ^ threshold) >> settled == 0u) count_key(key, (key >> shift) & (width - 1u));
     }
-    find_bin();
+    find_bin((kZeroKey >> shift) & (width - 1u));
     threshold |= found_bin << shift;
   }
 
   // ---- the kept slots in ascending order: larger keys, and the first `left` equal ones
-  const uint32_t per = ((n + kSelectWarps - 1u) / kSelectWarps + 127u) & ~127u;
-  const uint32_t from = min(warp * per, n), to = min(from + per, n);
+  const uint32_t per = stretch(n, ctas) / kSelectWarps;
+  const uint32_t from = min(s0 + warp * per, s1), to = min(from + per, s1);
   uint32_t more = 0, ties = 0;
-  for (uint32_t i = from + 4u * lane; i < to; i += 128u) {
-    const uint4 k = four_keys(i);
-    const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-    for (uint32_t u = 0; u < 4u; ++u) {
-      more += i + u < n && key[u] > threshold;
-      ties += i + u < n && key[u] == threshold;
-    }
+  for (uint32_t i = from + lane; i < to; i += 32u) {
+    const uint32_t key = key_at(i);
+    more += key > threshold;
+    ties += key == threshold;
   }
   more = __reduce_add_sync(0xffffffffu, more);
   ties = __reduce_add_sync(0xffffffffu, ties);
-  __syncthreads();
   if (lane == 0u) warp_a[warp] = more, warp_b[warp] = ties;
   __syncthreads();
-  more = ties = 0;
-  for (uint32_t x = 0; x < warp; ++x) {
-    more += warp_a[x];
-    ties += warp_b[x];
+  const uint32_t in_a = warp_a[lane], in_b = warp_b[lane];
+  if (warp == 0u) {
+    const uint32_t all_a = __reduce_add_sync(0xffffffffu, in_a), all_b = __reduce_add_sync(0xffffffffu, in_b);
+    if (lane == 0u) totals[0] = all_a, totals[1] = all_b;
   }
-  for (uint32_t i0 = from; i0 < to; i0 += 128u) {
-    const uint32_t i = i0 + 4u * lane;
-    const uint4 k = i < to ? four_keys(i) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t key[4] = {k.x, k.y, k.z, k.w};
-    uint32_t mine = 0;  // larger keys in the low half, equal ones in the high half
-#pragma unroll
-    for (uint32_t u = 0; u < 4u; ++u) {
-      if (i + u < to) mine += key[u] > threshold ? 1u : key[u] == threshold ? 0x10000u : 0u;
-    }
-    uint32_t before = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= static_cast<uint32_t>(off)) before += o;
-    }
-    const uint32_t all = __shfl_sync(0xffffffffu, before, 31);
-    before -= mine;
-    uint32_t m = more + (before & 0xffffu), t = ties + (before >> 16);
-#pragma unroll
-    for (uint32_t u = 0; u < 4u; ++u) {
-      if (i + u >= to) break;
-      if (key[u] > threshold) {
-        kept[m + min(t, left)] = static_cast<int32_t>(i + u);
-        ++m;
-      } else if (key[u] == threshold) {
-        if (t < left) kept[m + t] = static_cast<int32_t>(i + u);
-        ++t;
-      }
-    }
-    more += all & 0xffffu;
-    ties += all >> 16;
+  more = __reduce_add_sync(0xffffffffu, lane < warp ? in_a : 0u);
+  ties = __reduce_add_sync(0xffffffffu, lane < warp ? in_b : 0u);
+  cluster.sync();
+  for (uint32_t r = 0; r < rank; ++r) {
+    const uint32_t* t = cluster.map_shared_rank(totals, r);
+    more += t[0];
+    ties += t[1];
   }
+  const uint32_t below = (1u << lane) - 1u;
+  for (uint32_t i0 = from; i0 < to; i0 += 32u) {
+    const uint32_t i = i0 + lane;
+    const uint32_t key = i < to ? key_at(i) : 0u;
+    const uint32_t mb = __ballot_sync(0xffffffffu, i < to && key > threshold);
+    const uint32_t tb = __ballot_sync(0xffffffffu, i < to && key == threshold);
+    const uint32_t m = more + __popc(mb & below), t = ties + __popc(tb & below);
+    const bool stays = ((mb | (t < left ? tb : 0u)) >> lane & 1u) != 0u;
+    if (stays) kept[m + min(t, left)] = static_cast<int32_t>(i);
+    more += __popc(mb);
+    ties += __popc(tb);
+  }
+  cluster.sync();  // no CTA leaves while another may read its totals
 }
 
 constexpr uint32_t kMoveThreads = 256;
@@ -378,9 +356,26 @@ extern "C" cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, 
   a.parts = ordered ? 1u : (most + kMoveRows - 1u) / kMoveRows;
   cudaError_t err = select_smem_attr();
   if (err != cudaSuccess) return err;
-  const bool cached = e->max_len <= kCachedKeys;
-  err = launch_k(evict_select_kernel, dim3(c.n_kv, c.batch), kSelectThreads,
-                 cached ? (e->max_len + 3u) / 4u * 16u : 0u, stream, c, a, cached);
+  // CTAs of a selection: while SMs are free and a stretch keeps two slots a thread
+  uint32_t ctas = 1;
+  const uint64_t lines = static_cast<uint64_t>(c.n_kv) * c.batch, sms = static_cast<uint64_t>(device_sm_count());
+  while (ctas < kMaxCluster && lines * ctas * 2u <= sms && e->max_len >= ctas * 2u * 2u * kSelectThreads) ctas *= 2u;
+  const uint32_t slots = stretch(e->max_len, ctas);
+  const bool cached = slots <= kCachedKeys;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, c.n_kv, c.batch);
+  cfg.blockDim = kSelectThreads;
+  cfg.dynamicSmemBytes = cached ? slots * 4u : 0u;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  err = cudaLaunchKernelEx(&cfg, evict_select_kernel, c, a, cached);
   if (err != cudaSuccess) return err;
   const dim3 grid(a.slices * a.parts, c.n_kv, c.batch);
   if (ordered) return launch_k(evict_move_kernel<true, kSliceLanes>, grid, kMoveThreads, 0, stream, c, a);
