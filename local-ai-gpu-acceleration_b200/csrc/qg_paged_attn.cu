@@ -13,18 +13,20 @@
 // loads the slots; its rate is far above the few per cent that the memory can feed, so
 // tcgen05 with its trip through tensor memory has nothing to win here.
 //
-// Work.  The unit is a block of 128 slots of one (sequence, kv head, head tile); all blocks of
+// Work.  The unit is a block of 128 slots (64 at head size 256) of one (sequence, kv head, head
+// tile); all blocks of
 // the batch, whatever the lengths, form one line that is cut into equal ranges, one a CTA
-// (two CTAs an SM).  In a range, warp w owns slots [32 w, 32 w + 32) of every block and runs
+// (two CTAs an SM).  In a range, warp w owns a quarter, a tile, of every block and runs
 // on its own: it fetches its K and V tiles in turn through its own ring and keeps its own
-// (m, l, o).  Tiles arrive as TMA boxes of gcd(32, page_size) slots x 64 values, swizzled for
+// (m, l, o).  Tiles arrive as TMA boxes of gcd(tile, page_size) slots x 64 values, swizzled for
 // ldmatrix, so no box crosses a page, whatever the page size, and values past head_dim, slots
 // of no page and slots past the sequence's last box are the tensor map's zeros; page ids are
 // read 32 boxes at a time, ahead of their use.  Only rows that share a box with the sequence's ends can hold what is
 // not the sequence's: their V rows are cleared in shared memory, their scores are masked.
 // Where a (sequence, head) ends inside the range the four warps join through
-// shared memory; where it was cut by the range, the CTA leaves a record, and the CTA that
-// arrives last joins the records in CTA order, so results do not depend on timing.
+// shared memory; where it was cut by the range, the CTA leaves a record.  The CTA
+// that arrives last joins a head's records (more than 48 in groups of 16 first, each by its
+// last CTA), always in CTA order, so results do not depend on timing.
 //
 // Matrix fragments.  Rows of the A operand are query heads.  Eight heads fill rows 0-7 and
 // the rounding errors of their values rows 8-15: q = hi + lo in the cache's type, so one mma
@@ -34,7 +36,7 @@
 // accumulators are laid out like the A operand of the next product, so probabilities go back
 // in without a shuffle, again as hi + lo; they carry a factor 2^14 (removed with l), which
 // keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
-// Each 32-slot tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
+// Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
 // matrix pipe truncates when it accumulates, and o lives for thousands of tiles.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -52,11 +54,15 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kAttnThreads = kWarps * 32;
-constexpr uint32_t kTile = 32;                // slots of one warp's tile
-constexpr uint32_t kLogTile = 5;
-constexpr uint32_t kBlock = kTile * kWarps;   // slots of a block
-constexpr uint32_t kMaxCtas = 512;            // counters in the workspace's zeroed bytes
-static_assert(kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "one counter per CTA");
+// Slots of one warp's tile: 8 KB of K at head sizes 128 and 256, 4 KB at 64.
+constexpr uint32_t log_tile(uint32_t dp) { return dp == 256u ? 4u : 5u; }
+constexpr uint32_t block_slots(uint32_t dp) { return kWarps << log_tile(dp); }
+constexpr uint32_t kMaxCtas = 512;
+constexpr uint32_t kJoinAll = 48;             // records of a head that are joined at once
+constexpr uint32_t kJoin = 16;                // records of a group where there are more
+constexpr uint32_t kInFlight = 16;            // records whose sums are asked for together
+static_assert(2u * kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "two counters per CTA");
+static_assert(kMaxCtas / kJoin <= 64u && kJoinAll <= 64u, "two records a lane");
 constexpr float kShareBits = 14.f;            // log2 of the factor that probabilities carry
 
 struct AttnArgs {
@@ -69,7 +75,7 @@ struct AttnArgs {
   uint32_t n_q, group, tiles;  // query heads, per kv head, head tiles per kv head
   float scale_log2;
   float* lse;
-  uint32_t* arrived;           // [kMaxCtas], zero between calls
+  uint32_t* arrived;           // [2][kMaxCtas], zero between calls
   float* records;              // [cta][2] partial results
   float* scores;               // [batch][n_q][score_stride], log2 units, or NULL
   float* norm;                 // [batch][n_q]: log2 of the full sum, with scores
@@ -143,6 +149,7 @@ __device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N
 
 // One (sequence, kv head x head tile) of the line: its seen slots [start, len) are blocks
 // [j0, j1); j is the next one.
+template <uint32_t kBlock>
 struct Segment {
   uint32_t b, h, j, j0, j1, start, len;
 
@@ -167,6 +174,8 @@ struct Segment {
 // EXTRA: third terms of q and of the probabilities (fp32 queries over a bf16 cache).
 template <typename T, int DP, int MT, bool EXTRA>
 struct AttnShape {
+  static constexpr uint32_t kTile = 1u << log_tile(DP);
+  static constexpr uint32_t kBlock = block_slots(DP);
   static constexpr uint32_t kHeads = 8u * MT;
   static constexpr uint32_t kUnit = kTile * DP * 2u;        // a warp's K or V tile
   static constexpr uint32_t kUnits = DP == 64 ? 6 : 3;      // of its ring
@@ -176,7 +185,10 @@ struct AttnShape {
   static constexpr uint32_t kSmem = kRing + kQBytes + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
   static constexpr uint32_t kRecord = kHeads * (DP + 2u);   // m[], l[], o[][]
-  static constexpr int kCtasPerSm = DP == 256 ? 1 : 2;
+  static constexpr int kCtasPerSm = 2;
+  // What a segment costs beside its blocks, in blocks: queries in, sums out (about 3 us, a
+  // block of 64 KB at an SM's half of the memory's rate).
+  static constexpr uint32_t kHeader = DP == 64 ? 2 : 1;
   static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
 
@@ -184,6 +196,8 @@ template <typename T, int DP, int MT, bool EXTRA>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCtasPerSm)
     paged_attn_kernel(const PagedView c, const AttnArgs a, const __grid_constant__ AttnMaps maps) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
+  using Seg = Segment<Shape::kBlock>;
+  constexpr uint32_t kTile = Shape::kTile, kBlock = Shape::kBlock, kLogTile = log_tile(DP);
   constexpr uint32_t kUnits = Shape::kUnits, kUnit = Shape::kUnit, kHeads = Shape::kHeads;
   constexpr int kTerms = EXTRA ? 3 : 2;
   constexpr int kSteps = kTile / 16;    // 16-slot steps of a product over slots
@@ -194,6 +208,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   __shared__ uint64_t sum64[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
+  __shared__ float share[kHeads][64];
 
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -203,39 +218,37 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     for (uint32_t i = 0; i < kUnits; ++i) mbar_init(&full[warp][i], 1u);
     fence_mbar_init();
   }
+  if (tid < 2u) {  // the tensor maps are kernel parameters: nothing to wait for
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tid == 0u ? &maps.k : &maps.v)) : "memory");
+  }
 
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's range [r0, r1) of the line of blocks
+  // ---- this CTA's range [r0, r1) of the line of units (blocks, and headers before each segment's)
   const uint32_t lines = c.n_kv * a.tiles;
-  uint64_t total = 0;
-  for (uint32_t b = tid; b < c.batch; b += kAttnThreads) {
-    Segment s;
+  auto blocks_of = [&](uint32_t b) {
+    Seg s;
     s.b = b;
     s.bounds(c, a);
-    total += s.j1 - s.j0;
+    return s.j1 - s.j0;
+  };
+  uint64_t total = 0;  // blocks of one line of every sequence, then of all lines
+  if (c.batch > kAttnThreads) {
+    for (uint32_t b = tid; b < c.batch; b += kAttnThreads) total += blocks_of(b);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (lane == 0u) sum64[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) total += sum64[w];
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-  if (lane == 0u) sum64[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < kWarps; ++w) total += sum64[w];
-  total *= lines;
-  const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), total);
-  if (blockIdx.x >= ctas) return;
-  const uint64_t r0 = blockIdx.x * total / ctas, r1 = (blockIdx.x + 1u) * total / ctas;
+  uint64_t ctas = 0, r0 = 0, r1 = 0;
+  uint32_t header = 0;  // units of a segment that stand for its cost beside its blocks
   for (uint64_t base = 0, b0 = 0; b0 < c.batch; b0 += kAttnThreads) {
     const uint32_t b = static_cast<uint32_t>(b0) + tid;
-    Segment s;
-    uint64_t n = 0;
-    if (b < c.batch) {
-      s.b = b;
-      s.bounds(c, a);
-      n = s.j1 - s.j0;
-    }
+    const uint64_t n = b < c.batch ? blocks_of(b) : 0u;
     uint64_t upto = n;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -251,29 +264,66 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
       if (w < warp) upto += sum64[w];
       all += sum64[w];
     }
-    upto += base;
-    if (n != 0u && r0 >= (upto - n) * lines && r0 < upto * lines) {
-      const uint64_t in = r0 - (upto - n) * lines;
+    if (b0 == 0u) {
+      if (c.batch <= kAttnThreads) total = all;
+      // fewer blocks than CTAs: a block each; otherwise segments cost more than their blocks
+      if (total * lines > gridDim.x) header = Shape::kHeader;
+      total = (total + static_cast<uint64_t>(header) * c.batch) * lines;
+      ctas = min(static_cast<uint64_t>(gridDim.x), total);
+      if (blockIdx.x >= ctas) return;
+      r0 = blockIdx.x * total / ctas;
+      r1 = (blockIdx.x + 1u) * total / ctas;
+    }
+    const uint64_t units = n + header;
+    upto += base + static_cast<uint64_t>(header) * (b + 1u);
+    if (n != 0u && r0 >= (upto - units) * lines && r0 < upto * lines) {
+      const uint64_t in = r0 - (upto - units) * lines;
       first_at[0] = b;
-      first_at[1] = static_cast<uint32_t>(in / n);
-      first_at[2] = static_cast<uint32_t>(in % n);
+      first_at[1] = static_cast<uint32_t>(in / units);
+      first_at[2] = static_cast<uint32_t>(in % units);
     }
     base += all;
-    if (base * lines > r0) break;
+    if ((base + static_cast<uint64_t>(header) * (b0 + kAttnThreads)) * lines > r0) break;
   }
   __syncthreads();
-  Segment use;
+  Seg use;
   use.b = first_at[0];
   use.h = first_at[1];
   use.bounds(c, a);
-  use.j = use.j0 + first_at[2];
-  uint32_t left = static_cast<uint32_t>(r1 - r0);  // blocks, this one included (below 2^31)
+  uint32_t left = static_cast<uint32_t>(r1 - r0);  // units of the range from use.j on (below 2^31)
+  auto skip_header = [&](uint32_t& units, uint32_t done) { units -= min(units, header - min(done, header)); };
+  skip_header(left, first_at[2]);
+  use.j = use.j0 + (first_at[2] - min(first_at[2], header));
+
+  // a segment's queries as this lane splits them: rows warp, warp + 4, .. of its head tile
+  constexpr uint32_t kPer = DP / 32, kQRowsPerWarp = kHeads / kWarps;
+  float q_raw[kQRowsPerWarp][kPer];
+  auto load_queries = [&](const Seg& s) {
+    const uint32_t kv = s.h / a.tiles, ht = s.h - kv * a.tiles;
+    const uint32_t heads = a.group - ht * kHeads;  // or more than the tile has
+#pragma unroll
+    for (uint32_t i = 0; i < kQRowsPerWarp; ++i) {
+      const uint32_t r = warp + i * kWarps;
+      const uint64_t row = s.b * a.q_stride + static_cast<uint64_t>(kv * a.group + ht * kHeads + r) * c.dim;
+#pragma unroll
+      for (uint32_t e = 0; e < kPer; ++e) {
+        const uint32_t d = lane * kPer + e;
+        q_raw[i][e] = 0.f;
+        if (r < heads && d < c.dim) {
+          q_raw[i][e] = a.dtype == QG_F32   ? static_cast<const float*>(a.q)[row + d]
+                        : a.dtype == QG_F16 ? __half2float(static_cast<const __half*>(a.q)[row + d])
+                                            : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[row + d]);
+        }
+      }
+    }
+  };
+  if (left != 0u) load_queries(use);
 
   // ---- fetching.  A set of page ids covers the next 32 boxes of this warp's tiles, a box a
   // lane; the set after it is read while this one is used.
   const uint64_t policy = l2_evict_first_policy();
   const uint32_t boxes = 1u << a.log_boxes, log_box = kLogTile - a.log_boxes;
-  Segment ahead = use;
+  Seg ahead = use;
   uint32_t ahead_left = left;
   int32_t page = 0, place = 0, head = 0, next_page = 0, next_place = 0, next_head = 0;
   uint32_t at_tile = 0, tiles = 0, next_tiles = 0;  // of the set
@@ -296,7 +346,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     }
     ahead.j += next_tiles;
     ahead_left -= next_tiles;
-    if (ahead.j == ahead.j1) ahead.next(c, a, ahead_left != 0u);
+    if (ahead.j == ahead.j1) {
+      skip_header(ahead_left, 0u);
+      ahead.next(c, a, ahead_left != 0u);
+    }
   };
   auto next_set = [&]() {
     page = next_page;
@@ -368,22 +421,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     const uint32_t from_j = use.j, to_j = min(use.j1, use.j + left);
 
     {  // ---- the queries
-      constexpr uint32_t kPer = DP / 32;
-      for (uint32_t r = warp; r < kHeads; r += kWarps) {
-        float x[kPer];
+#pragma unroll
+      for (uint32_t row = 0; row < kQRowsPerWarp; ++row) {
+        const uint32_t r = warp + row * kWarps;
+        const float(&x)[kPer] = q_raw[row];
         float top = 0.f;
 #pragma unroll
-        for (uint32_t e = 0; e < kPer; ++e) {
-          const uint32_t d = lane * kPer + e;
-          x[e] = 0.f;
-          if (r < heads && d < c.dim) {
-            const uint64_t at = use.b * a.q_stride + static_cast<uint64_t>(head0 + r) * c.dim + d;
-            x[e] = a.dtype == QG_F32   ? static_cast<const float*>(a.q)[at]
-                   : a.dtype == QG_F16 ? __half2float(static_cast<const __half*>(a.q)[at])
-                                       : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
-          }
-          top = fmaxf(top, fabsf(x[e]));
-        }
+        for (uint32_t e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         int power = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // top in [2^power, 2^(power + 1))
@@ -558,6 +602,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     left -= to_j - from_j;
 
     // ---- the end of the segment, or of the range inside it
+    Seg after = use;
+    const uint64_t here = r1 - left;  // the unit after this segment's part
+    if (use.j == use.j1) {
+      skip_header(left, 0u);
+      after.next(c, a, left != 0u);
+    }
+    if (left != 0u) load_queries(after);  // on their way while this segment joins
     {
       const bool mine = from_j == use.j0 && to_j == use.j1;
       // each warp's sums into the unit it has just used, float4 pieces swizzled by head
@@ -628,44 +679,95 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         }
       }
       if (!mine) {
-        // the CTAs that share this head: those that own its first to its last block
-        const uint64_t seg0 = r1 - left - (to_j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
-        const uint64_t c0 = ((seg0 + 1u) * ctas - 1u) / total, c1 = (seg1 * ctas - 1u) / total;
-        __threadfence();
-        __syncthreads();
-        if (tid == 0u) {
-          const uint32_t others = static_cast<uint32_t>(c1 - c0);
-          const uint32_t before = atomicAdd(a.arrived + c0, 1u);
-          is_last = before == others;
-          if (is_last != 0u) a.arrived[c0] = 0u;
-        }
-        __syncthreads();
-        if (is_last != 0u) {
+        // the CTAs that share this head own its first to its last block, in order
+        const uint64_t seg0 = here - (to_j - use.j0), seg1 = seg0 + (use.j1 - use.j0);
+        const uint32_t c0 = static_cast<uint32_t>(((seg0 + 1u) * ctas - 1u) / total);
+        const uint32_t count = static_cast<uint32_t>((seg1 * ctas - 1u) / total) - c0 + 1u;
+        const uint32_t per = count <= kJoinAll ? count : kJoin;
+        const uint32_t index = blockIdx.x - c0, group = index / per;
+        const uint32_t groups = (count + per - 1u) / per, members = min(per, count - group * per);
+        auto record_of = [&](uint32_t cta) {
+          return a.records + (static_cast<size_t>(cta) * 2u + (cta == c0 ? 1u : 0u)) * Shape::kRecord;
+        };
+        // whether this CTA is the last of `n` to arrive; the others' records can then be read
+        auto last_of = [&](uint32_t* counter, uint32_t n) {
           __threadfence();
+          __syncthreads();
+          if (tid == 0u) {
+            is_last = atomicAdd(counter, 1u) == n - 1u;
+            if (is_last != 0u) *counter = 0u;
+          }
+          __syncthreads();
+          if (is_last != 0u) __threadfence();
+          return is_last != 0u;
+        };
+        // joins the n <= 64 records of CTAs first, first + step, ..; put(head, piece, m, l, o)
+        auto join_records = [&](uint32_t first, uint32_t step, uint32_t n, auto put) {
+          for (uint32_t h = warp; h < heads; h += kWarps) {  // two records a lane
+            float pm[2], sum[2];
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+              const uint32_t q = lane + 32u * e;
+              const float* rec = record_of(first + min(q, n - 1u) * step);
+              pm[e] = q < n ? __ldcg(rec + h) : -CUDART_INF_F;
+              sum[e] = q < n ? __ldcg(rec + kHeads + h) : 0.f;
+            }
+            float top = fmaxf(pm[0], pm[1]);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float from = top == -CUDART_INF_F ? 0.f : top;
+            const float f0 = exp2_fast(pm[0] - from), f1 = exp2_fast(pm[1] - from);
+            float all = fmaf(sum[0], f0, sum[1] * f1);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+            share[h][lane] = f0;
+            share[h][lane + 32u] = f1;
+            if (lane == 0u) join_m[0][h] = top, join_l[0][h] = all;
+          }
+          __syncthreads();
           for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
             const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);
-            float top = -CUDART_INF_F, sum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint64_t q = c0; q <= c1; ++q) {
-              const float* rec = a.records + (q * 2u + (q == c0 ? 1u : 0u)) * Shape::kRecord;
-              const float pm = __ldcg(rec + h), pl = __ldcg(rec + kHeads + h);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + 2u * kHeads) + h * (DP / 4u) + ch);
-              const float now = fmaxf(top, pm);
-              const float from = now == -CUDART_INF_F ? 0.f : now;
-              const float f0 = exp2_fast(top - from), f1 = exp2_fast(pm - from);
-              top = now;
-              sum = fmaf(sum, f0, pl * f1);
-              v.x = fmaf(v.x, f0, x.x * f1), v.y = fmaf(v.y, f0, x.y * f1);
-              v.z = fmaf(v.z, f0, x.z * f1), v.w = fmaf(v.w, f0, x.w * f1);
+            for (uint32_t q0 = 0; q0 < n; q0 += kInFlight) {
+              float4 x[kInFlight];
+#pragma unroll
+              for (uint32_t q = 0; q < kInFlight; ++q) {
+                x[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q0 + q < n) {
+                  x[q] = __ldcg(reinterpret_cast<const float4*>(record_of(first + (q0 + q) * step) + 2u * kHeads) + i);
+                }
+              }
+#pragma unroll
+              for (uint32_t q = 0; q < kInFlight; ++q) {
+                const float f = share[h][q0 + q];
+                v.x = fmaf(x[q].x, f, v.x), v.y = fmaf(x[q].y, f, v.y);
+                v.z = fmaf(x[q].z, f, v.z), v.w = fmaf(x[q].w, f, v.w);
+              }
             }
-            finish(h, ch, top, sum, v);
+            put(h, ch, join_m[0][h], join_l[0][h], v);
+          }
+        };
+        auto to_record = [&](float* rec) {
+          return [=](uint32_t h, uint32_t ch, float top, float sum, float4 v) {
+            if (ch == 0u) rec[h] = top, rec[kHeads + h] = sum;
+            reinterpret_cast<float4*>(rec + 2u * kHeads)[h * (DP / 4u) + ch] = v;
+          };
+        };
+        // few records are joined at once, many in groups, then the groups' records
+        const uint32_t g0 = c0 + group * per;
+        if (members == 1u || last_of(a.arrived + g0, members)) {
+          if (groups == 1u) {
+            join_records(g0, 1u, members, finish);
+          } else {
+            if (members > 1u) join_records(g0, 1u, members, to_record(record_of(g0)));
+            if (last_of(a.arrived + kMaxCtas + c0, groups)) join_records(c0, per, groups, finish);
           }
         }
       }
       __syncthreads();  // the units, the joins and the queries are free again
     }
     release_unit(true);
-    if (use.j == use.j1) use.next(c, a, left != 0u);
+    use = after;
   }
   if (!arrives) {  // a wait ran out (QG_ERR_WAIT_TIMEOUT is set): let what is in flight land
     for (uint32_t i = 0; i < kUnits; ++i) {
@@ -676,32 +778,47 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 }
 
 // weight_out = weight_in + the slot's shares summed over the heads of its kv head.
-__global__ void __launch_bounds__(256) attn_weight_kernel(const PagedView c, const AttnArgs a,
-                                                          const float* weight_in, float* weight_out,
-                                                          uint32_t weight_stride) {
+constexpr uint32_t kWeightThreads = 128, kWeightSlots = 4;  // of a thread, a block's width apart
+
+__global__ void __launch_bounds__(kWeightThreads) attn_weight_kernel(const PagedView c, const AttnArgs a,
+                                                                     const float* weight_in, float* weight_out,
+                                                                     uint32_t weight_stride) {
   pdl_wait();
   pdl_trigger();
-  const uint32_t kv = blockIdx.y, b = blockIdx.z, j = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t kv = blockIdx.y, b = blockIdx.z, j0 = blockIdx.x * (kWeightThreads * kWeightSlots) + threadIdx.x;
   const uint32_t len = paged_len(a.lens[b], min(a.max_len, c.capacity));
-  if (j >= len) return;
+  if (j0 - threadIdx.x >= len) return;
   const uint32_t start = a.window != 0u && len > a.window ? len - a.window : 0u;
-  const size_t at = (static_cast<size_t>(b) * c.n_kv + kv) * weight_stride + j;
-  float w = weight_in != nullptr ? weight_in[at] : 0.f;
-  if (j >= start) {
-    const size_t head = static_cast<size_t>(b) * a.n_q + kv * a.group;
-    float sum = 0.f;
-    for (uint32_t h = 0; h < a.group; ++h) {
-      sum += exp2_fast(a.scores[(head + h) * a.score_stride + j] - a.norm[head + h]);
-    }
-    w += sum;
+  const size_t head = static_cast<size_t>(b) * a.n_q + kv * a.group;
+  const size_t row = (static_cast<size_t>(b) * c.n_kv + kv) * weight_stride;
+  float old[kWeightSlots], sum[kWeightSlots];
+#pragma unroll
+  for (uint32_t u = 0; u < kWeightSlots; ++u) {
+    const uint32_t j = j0 + u * kWeightThreads;
+    old[u] = weight_in != nullptr && j < len ? weight_in[row + j] : 0.f;
+    sum[u] = 0.f;
   }
-  weight_out[at] = w;
+#pragma unroll 2
+  for (uint32_t h = 0; h < a.group; ++h) {
+    const float full = a.norm[head + h];
+    const float* scores = a.scores + (head + h) * a.score_stride;
+#pragma unroll
+    for (uint32_t u = 0; u < kWeightSlots; ++u) {
+      const uint32_t j = j0 + u * kWeightThreads;
+      if (j >= start && j < len) sum[u] += exp2_fast(scores[j] - full);
+    }
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < kWeightSlots; ++u) {
+    const uint32_t j = j0 + u * kWeightThreads;
+    if (j < len) weight_out[row + j] = old[u] + sum[u];
+  }
 }
 
 // ---- host side
 
 struct AttnPlan {
-  uint32_t dp, mt, tiles, record;
+  uint32_t dp, mt, tiles, record, score_stride;
   size_t records_at, scores_at, norm_at, bytes;
 };
 
@@ -718,7 +835,9 @@ bool plan_attn(const PagedView& c, uint32_t n_q, uint32_t max_len, bool weights,
   p->record = 8u * p->mt * (p->dp + 2u);
   p->records_at = QG_PAGED_ATTN_ZEROED;
   p->scores_at = round_up(p->records_at + static_cast<size_t>(kMaxCtas) * 2u * p->record * 4u);
-  const size_t stride = (max_len + kBlock - 1u) / kBlock * kBlock;
+  const uint32_t block = block_slots(p->dp);
+  const size_t stride = (max_len + block - 1u) / block * block;
+  p->score_stride = static_cast<uint32_t>(stride);
   p->norm_at = round_up(p->scores_at + (weights ? static_cast<size_t>(c.batch) * n_q * stride * 4u : 0u));
   p->bytes = round_up(p->norm_at + (weights ? static_cast<size_t>(c.batch) * n_q * 4u : 0u));
   return true;
@@ -799,10 +918,10 @@ cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, const AttnMaps& m
     }
   }
   const uint64_t blocks = static_cast<uint64_t>(c.batch) * c.n_kv * a.tiles *
-                          ((std::min(a.max_len, c.capacity) + kBlock - 1u) / kBlock);
+                          ((std::min(a.max_len, c.capacity) + Shape::kBlock - 1u) / Shape::kBlock);
   const uint64_t fit = static_cast<uint64_t>(sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
-  if (blocks / grid >= (1ull << 31)) return cudaErrorInvalidValue;  // a CTA counts its blocks in 32 bits
+  if (blocks / grid >= (1ull << 29)) return cudaErrorInvalidValue;  // a CTA counts its units in 32 bits
   return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);
 }
 
@@ -860,7 +979,8 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
   }
   PoolStrides strides;
   if (!pool_strides(cache, &strides)) return cudaErrorInvalidValue;
-  const uint32_t log_box = std::min<uint32_t>(kLogTile, __builtin_ctz(cache->page_size));  // gcd(kTile, page_size)
+  // a box is gcd(tile, page_size) slots
+  const uint32_t log_box = std::min<uint32_t>(log_tile(plan.dp), __builtin_ctz(cache->page_size));
   const uint32_t box = 1u << log_box;
   AttnMaps maps;
   if (!encode_pool(&maps.k, cache->k, cache, strides, box) || !encode_pool(&maps.v, cache->v, cache, strides, box)) {
@@ -868,7 +988,7 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
   }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   AttnArgs a{};
-  a.log_boxes = kLogTile - log_box;
+  a.log_boxes = log_tile(plan.dp) - log_box;
   a.heads_inside = strides.heads_inside;
   a.q = p->q;
   a.out = p->out;
@@ -887,11 +1007,12 @@ extern "C" cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* p,
   a.records = reinterpret_cast<float*>(ws + plan.records_at);
   a.scores = weights ? reinterpret_cast<float*>(ws + plan.scores_at) : nullptr;
   a.norm = weights ? reinterpret_cast<float*>(ws + plan.norm_at) : nullptr;
-  a.score_stride = (p->max_len + kBlock - 1u) / kBlock * kBlock;
+  a.score_stride = plan.score_stride;
   const cudaError_t e = cache->dtype == QG_F16 ? launch_attn<__half>(plan, extra, c, a, maps, stream)
                                                : launch_attn<__nv_bfloat16>(plan, extra, c, a, maps, stream);
   if (e != cudaSuccess || !weights) return e;
-  const dim3 grid((std::min(p->max_len, c.capacity) + 255u) / 256u, c.n_kv, c.batch);
-  return launch_k(attn_weight_kernel, grid, 256, 0, stream, c, a, p->weight_in, p->weight_out,
+  constexpr uint32_t kSpan = kWeightThreads * kWeightSlots;
+  const dim3 grid((std::min(p->max_len, c.capacity) + kSpan - 1u) / kSpan, c.n_kv, c.batch);
+  return launch_k(attn_weight_kernel, grid, kWeightThreads, 0, stream, c, a, p->weight_in, p->weight_out,
                   p->weight_stride);
 }
