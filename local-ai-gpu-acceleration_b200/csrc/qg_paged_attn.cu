@@ -297,23 +297,22 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 
   // a segment's queries as this lane splits them: rows warp, warp + 4, .. of its head tile
   constexpr uint32_t kPer = DP / 32, kQRowsPerWarp = kHeads / kWarps;
-  float q_raw[kQRowsPerWarp][kPer];
+  uint32_t q_raw[kQRowsPerWarp][kPer];  // fp32 words, or pairs of 16-bit values in the first half
   auto load_queries = [&](const Seg& s) {
     const uint32_t kv = s.h / a.tiles, ht = s.h - kv * a.tiles;
     const uint32_t heads = a.group - ht * kHeads;  // or more than the tile has
+    const uint32_t bytes = a.dtype == QG_F32 ? 4u : 2u;
 #pragma unroll
     for (uint32_t i = 0; i < kQRowsPerWarp; ++i) {
       const uint32_t r = warp + i * kWarps;
       const uint64_t row = s.b * a.q_stride + static_cast<uint64_t>(kv * a.group + ht * kHeads + r) * c.dim;
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.q) +
+                                                             (row + lane * kPer) * bytes);
+      const bool has = r < heads && lane * kPer < c.dim;  // dim is a multiple of 8, kPer divides it
 #pragma unroll
       for (uint32_t e = 0; e < kPer; ++e) {
-        const uint32_t d = lane * kPer + e;
-        q_raw[i][e] = 0.f;
-        if (r < heads && d < c.dim) {
-          q_raw[i][e] = a.dtype == QG_F32   ? static_cast<const float*>(a.q)[row + d]
-                        : a.dtype == QG_F16 ? __half2float(static_cast<const __half*>(a.q)[row + d])
-                                            : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[row + d]);
-        }
+        q_raw[i][e] = 0u;
+        if (has && (e < kPer / 2u || a.dtype == QG_F32)) q_raw[i][e] = at[e];
       }
     }
   };
@@ -424,7 +423,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
       for (uint32_t row = 0; row < kQRowsPerWarp; ++row) {
         const uint32_t r = warp + row * kWarps;
-        const float(&x)[kPer] = q_raw[row];
+        float x[kPer];
+        if (a.dtype == QG_F32) {
+#pragma unroll
+          for (uint32_t e = 0; e < kPer; ++e) x[e] = __uint_as_float(q_raw[row][e]);
+        } else {
+#pragma unroll
+          for (uint32_t e = 0; e < kPer / 2u; ++e) {
+            const float2 f = a.dtype == QG_F16 ? unpack2(q_raw[row][e], __half()) : unpack2(q_raw[row][e], __nv_bfloat16());
+            x[2u * e] = f.x;
+            x[2u * e + 1u] = f.y;
+          }
+        }
         float top = 0.f;
 #pragma unroll
         for (uint32_t e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[e]));
@@ -691,33 +701,56 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         };
         // whether this CTA is the last of `n` to arrive; the others' records can then be read
         auto last_of = [&](uint32_t* counter, uint32_t n) {
-          __threadfence();
           __syncthreads();
           if (tid == 0u) {
+            __threadfence();  // this CTA's records, ordered before by the barrier, are out
             is_last = atomicAdd(counter, 1u) == n - 1u;
             if (is_last != 0u) *counter = 0u;
+            __threadfence();
           }
           __syncthreads();
-          if (is_last != 0u) __threadfence();
           return is_last != 0u;
         };
         // joins the n <= 64 records of CTAs first, first + step, ..; put(head, piece, m, l, o)
         auto join_records = [&](uint32_t first, uint32_t step, uint32_t n, auto put) {
-          for (uint32_t h = warp; h < heads; h += kWarps) {  // two records a lane
-            float pm[2], sum[2];
+          constexpr uint32_t kItems = kHeads * (DP / 4u) / kAttnThreads;      // float4 pieces of a thread
+          constexpr uint32_t kOnce = kItems < 2u ? 1u : 2u;                   // .. that it works on together
+          float4 x[kOnce][kInFlight];
+          auto ask = [&](uint32_t i0, uint32_t q0) {
 #pragma unroll
-            for (uint32_t e = 0; e < 2; ++e) {
-              const uint32_t q = lane + 32u * e;
-              const float* rec = record_of(first + min(q, n - 1u) * step);
-              pm[e] = q < n ? __ldcg(rec + h) : -CUDART_INF_F;
-              sum[e] = q < n ? __ldcg(rec + kHeads + h) : 0.f;
+            for (uint32_t q = 0; q < kInFlight; ++q) {
+              const float4* rec = reinterpret_cast<const float4*>(record_of(first + (q0 + q) * step) + 2u * kHeads);
+#pragma unroll
+              for (uint32_t e = 0; e < kOnce; ++e) {
+                const uint32_t i = (i0 + e) * kAttnThreads + tid;
+                x[e][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q0 + q < n && i < heads * (DP / 4u)) x[e][q] = __ldcg(rec + i);
+              }
             }
-            float top = fmaxf(pm[0], pm[1]);
+          };
+          ask(0u, 0u);
+          constexpr uint32_t kHeadsPerWarp = kHeads / kWarps;
+          float pm[kHeadsPerWarp][2], pl[kHeadsPerWarp][2];  // two records a lane
+#pragma unroll
+          for (uint32_t e = 0; e < 2; ++e) {
+            const uint32_t q = lane + 32u * e;
+            const float* rec = record_of(first + min(q, n - 1u) * step);
+#pragma unroll
+            for (uint32_t i = 0; i < kHeadsPerWarp; ++i) {
+              const uint32_t h = warp + i * kWarps;
+              pm[i][e] = q < n && h < heads ? __ldcg(rec + h) : -CUDART_INF_F;
+              pl[i][e] = q < n && h < heads ? __ldcg(rec + kHeads + h) : 0.f;
+            }
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < kHeadsPerWarp; ++i) {
+            const uint32_t h = warp + i * kWarps;
+            float top = fmaxf(pm[i][0], pm[i][1]);
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
             const float from = top == -CUDART_INF_F ? 0.f : top;
-            const float f0 = exp2_fast(pm[0] - from), f1 = exp2_fast(pm[1] - from);
-            float all = fmaf(sum[0], f0, sum[1] * f1);
+            const float f0 = exp2_fast(pm[i][0] - from), f1 = exp2_fast(pm[i][1] - from);
+            float all = fmaf(pl[i][0], f0, pl[i][1] * f1);
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
             share[h][lane] = f0;
@@ -725,26 +758,28 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
             if (lane == 0u) join_m[0][h] = top, join_l[0][h] = all;
           }
           __syncthreads();
-          for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
-            const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (uint32_t i0 = 0; i0 < kItems; i0 += kOnce) {
+            float4 v[kOnce];
+#pragma unroll
+            for (uint32_t e = 0; e < kOnce; ++e) v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
             for (uint32_t q0 = 0; q0 < n; q0 += kInFlight) {
-              float4 x[kInFlight];
+              if (i0 + q0 != 0u) ask(i0, q0);
 #pragma unroll
               for (uint32_t q = 0; q < kInFlight; ++q) {
-                x[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (q0 + q < n) {
-                  x[q] = __ldcg(reinterpret_cast<const float4*>(record_of(first + (q0 + q) * step) + 2u * kHeads) + i);
+#pragma unroll
+                for (uint32_t e = 0; e < kOnce; ++e) {
+                  const float f = share[((i0 + e) * kAttnThreads + tid) / (DP / 4u)][q0 + q];
+                  v[e].x = fmaf(x[e][q].x, f, v[e].x), v[e].y = fmaf(x[e][q].y, f, v[e].y);
+                  v[e].z = fmaf(x[e][q].z, f, v[e].z), v[e].w = fmaf(x[e][q].w, f, v[e].w);
                 }
               }
-#pragma unroll
-              for (uint32_t q = 0; q < kInFlight; ++q) {
-                const float f = share[h][q0 + q];
-                v.x = fmaf(x[q].x, f, v.x), v.y = fmaf(x[q].y, f, v.y);
-                v.z = fmaf(x[q].z, f, v.z), v.w = fmaf(x[q].w, f, v.w);
-              }
             }
-            put(h, ch, join_m[0][h], join_l[0][h], v);
+#pragma unroll
+            for (uint32_t e = 0; e < kOnce; ++e) {
+              const uint32_t i = (i0 + e) * kAttnThreads + tid, h = i / (DP / 4u);
+              if (h < heads) put(h, i % (DP / 4u), join_m[0][h], join_l[0][h], v[e]);
+            }
           }
         };
         auto to_record = [&](float* rec) {
