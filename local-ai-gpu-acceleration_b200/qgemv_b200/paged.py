@@ -67,19 +67,24 @@ def _fail(message: str):
     raise ValueError(message)
 
 
+# The checks below run on every call and on small batches take as long as the kernels, so each
+# reads an attribute once and calls nothing it does not need.
+_F32, _I32 = torch.float32, torch.int32
+_device_now = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_byref = ctypes.byref
+_empty_like = torch.empty_like
+
+
 def _call(fn, index: int, *args) -> None:
     """Call an entry point with device `index` current."""
-    if torch._C._cuda_getDevice() != index:
+    if _device_now() != index:
         with torch.cuda.device(index):
             code = fn(*args)
     else:
         code = fn(*args)
     if code != 0:
         raise CudaError(fn.__name__, code)
-
-
-def _handle(stream, index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
 def _new(shape: tuple, dtype, device, stream) -> torch.Tensor:
@@ -93,25 +98,21 @@ def _new(shape: tuple, dtype, device, stream) -> torch.Tensor:
 def _like(t: torch.Tensor, stream) -> torch.Tensor:
     """The same for a tensor like t (half the time of _new)."""
     if stream is None:
-        return torch.empty_like(t)
+        return _empty_like(t)
     with torch.cuda.stream(stream):
-        return torch.empty_like(t)
+        return _empty_like(t)
 
 
-def _ints(t: torch.Tensor | None, n: int, name: str, index: int) -> int | None:
+def _ints(t: torch.Tensor, n: int, name: str, index: int) -> int:
     """Address of a contiguous int32 tensor of n entries."""
-    if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not _I32 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
         _fail(f"{name}: a contiguous int32 tensor of {n} entries on cuda:{index} is needed")
     return t.data_ptr()
 
 
-def _floats(t: torch.Tensor | None, shape: tuple, name: str, index: int) -> int | None:
+def _floats(t: torch.Tensor, shape: tuple, name: str, index: int) -> int:
     """Address of a contiguous fp32 tensor of a shape."""
-    if t is None:
-        return None
-    if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not _F32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
         _fail(f"{name}: a contiguous float32 tensor of shape {shape} on cuda:{index} is needed")
     return t.data_ptr()
 
@@ -120,10 +121,11 @@ def _heads(t: torch.Tensor, shape: tuple, dtype, name: str, index: int) -> int:
     """Stride from row to row of a [rows, heads, dim] tensor whose rows are contiguous."""
     if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
         _fail(f"{name}: a {dtype} tensor of shape {shape} on cuda:{index} is needed")
+    rows, heads, dim = shape
     row, head, one = t.stride()
-    if one != 1 or (shape[1] > 1 and head != shape[2]):
+    if one != 1 or (head != dim and heads > 1):
         _fail(f"{name}: the heads of one row must be contiguous")
-    return row if shape[0] > 1 else shape[1] * shape[2]
+    return row if rows > 1 else heads * dim
 
 
 class PagedCache:
@@ -184,23 +186,27 @@ def qk_norm_rope_append(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: 
     index, dim, kv, dtype = cache.index, cache.head_dim, cache.n_kv_heads, q.dtype
     if dtype not in DTYPE_CODES or q.dim() != 3:
         _fail("q: a [tokens, heads, dim] tensor of float32, float16 or bfloat16 is needed")
-    tokens, heads, _ = q.shape
     if pairs not in PAIRS:
         _fail("pairs is 'adjacent' or 'halves'")
+    tokens, heads, _ = q.shape
     q_shape, kv_shape = (tokens, heads, dim), (tokens, kv, dim)
     q_stride = _heads(q, q_shape, dtype, "q", index)
     if q_out is None:
-        q_out = _like(q, stream)
-    out_stride = _heads(q_out, q_shape, dtype, "q_out", index)
+        q_out, out_stride = _like(q, stream), heads * dim
+    else:
+        out_stride = _heads(q_out, q_shape, dtype, "q_out", index)
     rows, rot = (0, 0) if rope is None else rope.shape
     a = AppendC(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), DTYPE_CODES[dtype],
                 tokens, heads, q_stride, _heads(k, kv_shape, dtype, "k", index),
                 _heads(v, kv_shape, dtype, "v", index), out_stride,
-                _floats(q_norm, (dim,), "q_norm", index), _floats(k_norm, (dim,), "k_norm", index), eps,
-                _floats(rope, (rows, rot), "rope", index), rows, rot, PAIRS[pairs],
-                _ints(positions, tokens, "positions", index), _ints(slots, tokens, "slots", index),
-                _ints(seqs, tokens, "seqs", index))
-    _call(lib().qg_qk_norm_rope_append, index, cache._ref, ctypes.byref(a), _handle(stream, index))
+                None if q_norm is None else _floats(q_norm, (dim,), "q_norm", index),
+                None if k_norm is None else _floats(k_norm, (dim,), "k_norm", index), eps,
+                None if rope is None else _floats(rope, (rows, rot), "rope", index), rows, rot,
+                PAIRS[pairs], _ints(positions, tokens, "positions", index),
+                None if slots is None else _ints(slots, tokens, "slots", index),
+                None if seqs is None else _ints(seqs, tokens, "seqs", index))
+    _call(lib().qg_qk_norm_rope_append, index, cache._ref, _byref(a),
+          _raw_stream(index) if stream is None else stream.cuda_stream)
     return q_out
 
 
@@ -211,11 +217,13 @@ class AttentionPlan:
     def __init__(self, cache: PagedCache, n_q_heads: int, max_len: int | None = None,
                  weights: bool = False):
         self.cache, self.n_q_heads, self.weights = cache, n_q_heads, weights
+        self.shape = (cache.batch, n_q_heads, cache.head_dim)
         self.max_len = cache.capacity if max_len is None else max_len
         n = ctypes.c_size_t(0)
         _call(lib().qg_paged_attn_workspace_bytes, cache.index, cache._ref, n_q_heads, self.max_len,
-              int(weights), ctypes.byref(n))
+              int(weights), _byref(n))
         self.workspace = torch.zeros(n.value, dtype=torch.uint8, device=cache.device)
+        self.workspace_at = self.workspace.data_ptr()
         self.lse = torch.empty(cache.batch, n_q_heads, device=cache.device)  # what new ones are made like
 
 
@@ -228,32 +236,36 @@ def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: 
     defaults to dim^-1/2); returns out like q, or (out, lse [sequences, q heads]).
     weight_out [sequences, kv heads, >= max_len] receives weight_in plus each slot's shares
     (a plan with weights; weight_in may be weight_out)."""
-    cache, heads, dtype = plan.cache, plan.n_q_heads, q.dtype
-    index, dim, batch = cache.index, cache.head_dim, cache.batch
+    cache, shape, dtype = plan.cache, plan.shape, q.dtype
+    index = cache.index
+    batch, heads, dim = shape
     if dtype not in DTYPE_CODES:
         _fail("q: float32, float16 or bfloat16 is needed")
-    shape = (batch, heads, dim)
     q_stride = _heads(q, shape, dtype, "q", index)
     if out is None:
-        out = _like(q, stream)
-    if lse is None and return_lse:
+        out, out_stride = _like(q, stream), heads * dim
+    else:
+        out_stride = _heads(out, shape, dtype, "out", index)
+    if lse is not None:
+        _floats(lse, (batch, heads), "lse", index)
+    elif return_lse:
         lse = _like(plan.lse, stream)
-    width = 0
+    width, w_in, w_out = 0, None, None
     if weight_out is not None:
         if not plan.weights:
             _fail("weight_out needs a plan with weights")
         width = weight_out.shape[-1]
+        w_out = _floats(weight_out, (batch, cache.n_kv_heads, width), "weight_out", index)
+        if weight_in is not None:
+            w_in = _floats(weight_in, (batch, cache.n_kv_heads, width), "weight_in", index)
     elif weight_in is not None:
         _fail("weight_in without weight_out")
-    w_shape = (batch, cache.n_kv_heads, width)
-    a = AttnC(q.data_ptr(), out.data_ptr(), DTYPE_CODES[dtype], heads, q_stride,
-              _heads(out, shape, dtype, "out", index), _ints(lens, batch, "lens", index),
-              plan.max_len, window, dim ** -0.5 if scale is None else scale,
-              _floats(lse, (batch, heads), "lse", index),
-              _floats(weight_in, w_shape, "weight_in", index),
-              _floats(weight_out, w_shape, "weight_out", index), width)
-    _call(lib().qg_paged_attn, index, cache._ref, ctypes.byref(a), plan.workspace.data_ptr(),
-          _handle(stream, index))
+    a = AttnC(q.data_ptr(), out.data_ptr(), DTYPE_CODES[dtype], heads, q_stride, out_stride,
+              _ints(lens, batch, "lens", index), plan.max_len, window,
+              dim ** -0.5 if scale is None else scale, None if lse is None else lse.data_ptr(),
+              w_in, w_out, width)
+    _call(lib().qg_paged_attn, index, cache._ref, _byref(a), plan.workspace_at,
+          _raw_stream(index) if stream is None else stream.cuda_stream)
     return out if lse is None else (out, lse)
 
 
@@ -283,9 +295,11 @@ def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: i
         to, pages = new_table.data_ptr(), new_table.shape[1]
         step = new_table.stride(0) if batch > 1 else pages
     shape = (batch, kv, width)
-    e = EvictC(_ints(lens, batch, "lens", index), _ints(lens_out, batch, "lens_out", index),
-               _floats(weight, shape, "weight", index), _floats(weight_out, shape, "weight_out", index),
+    weight_at, lens_at = _floats(weight, shape, "weight", index), _ints(lens, batch, "lens", index)
+    e = EvictC(lens_at, lens_at if lens_out is lens else _ints(lens_out, batch, "lens_out", index),
+               weight_at, weight_at if weight_out is weight else _floats(weight_out, shape, "weight_out", index),
                width, width, budget, sink, recent, _ints(kept, batch * kv * budget, "kept", index),
                to, pages, step)
-    _call(lib().qg_kv_evict, index, cache._ref, ctypes.byref(e), _handle(stream, index))
+    _call(lib().qg_kv_evict, index, cache._ref, _byref(e),
+          _raw_stream(index) if stream is None else stream.cuda_stream)
     return kept, lens_out
