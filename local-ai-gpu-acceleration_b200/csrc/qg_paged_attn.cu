@@ -105,6 +105,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// True in one lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0u;
+}
+
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -188,7 +199,7 @@ struct AttnShape {
   static constexpr int kCtasPerSm = 2;
   // What a segment costs beside its blocks, in blocks: queries in, sums out (about 3 us, a
   // block of 64 KB at an SM's half of the memory's rate).
-  static constexpr uint32_t kHeader = DP == 64 ? 2 : 1;
+  static constexpr uint32_t kHeader = DP == 64 ? 2 : DP == 128 ? 3 : 1;
   static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
 
@@ -210,7 +221,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   __shared__ uint32_t is_last;
   __shared__ float share[kHeads][64];
 
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t4 = lane & 3u;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
+  const uint32_t warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in every lane, and known to be
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* const ring = smem + warp * (kUnits * kUnit);
   const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(smem + Shape::kRing);
@@ -363,19 +375,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     if (!is_v && at_tile == tiles) next_set();
     if (at_tile == tiles) return;  // the range is fetched
     const uint32_t to = ring_at + u * kUnit, bar = smem_addr(&full[warp][u]);
-    if (lane == 0u) mbar_arrive_expect_tx(&full[warp][u], kUnit);
-    __syncwarp();
     const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+    const bool leads = elect_one();
+    if (leads) mbar_arrive_expect_tx(&full[warp][u], kUnit);
+    for (uint32_t i = 0; i < boxes; ++i) {  // one lane asks: a copy takes warp-uniform operands
+      const uint32_t from = ((at_tile << a.log_boxes) + i) & 31u;
+      const int32_t pg = __shfl_sync(0xffffffffu, page, from), pl = __shfl_sync(0xffffffffu, place, from);
+      if (leads) {
 #pragma unroll
-    for (uint32_t p = 0; p < kPanels; p += (kPanels == 1u ? 1u : 2u)) {
-      // lanes: boxes of one panel, or of two where both fit a warp
-      const uint32_t sub = kPanels == 1u ? lane : lane >> 1, panel = kPanels == 1u ? 0u : p + (lane & 1u);
-      constexpr uint32_t kOnce = kPanels == 1u ? 32u : 16u;
-      for (uint32_t s0 = 0; s0 < boxes; s0 += kOnce) {
-        const uint32_t from = ((at_tile << a.log_boxes) + s0 + sub) & 31u;
-        const int32_t pg = __shfl_sync(0xffffffffu, page, from), pl = __shfl_sync(0xffffffffu, place, from);
-        if (s0 + sub < boxes) {
-          tma_load_4d(to + panel * kPanel + ((s0 + sub) << log_box) * 128u, map, static_cast<int32_t>(panel * 64u),
+        for (uint32_t p = 0; p < kPanels; ++p) {
+          tma_load_4d(to + p * kPanel + (i << log_box) * 128u, map, static_cast<int32_t>(p * 64u),
                       a.heads_inside ? head : pl, a.heads_inside ? pl : head, pg, bar, policy);
         }
       }

@@ -71,6 +71,13 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
   auto cluster = cooperative_groups::this_cluster();
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t kv = blockIdx.y, b = blockIdx.z, rank = blockIdx.x, ctas = gridDim.x;
+  auto sync_all = [&]() {
+    if (ctas == 1u) {
+      __syncthreads();
+    } else {
+      cluster.sync();
+    }
+  };
   pdl_wait();
   pdl_trigger();
   const uint32_t n = paged_len(a.lens[b], min(a.max_len, c.capacity));
@@ -103,11 +110,12 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     zeros = __reduce_add_sync(0xffffffffu, zeros);
     if (lane == 0u && zeros != 0u) atomicAdd(&bins[zero_bin], zeros);
     zeros = 0u;
-    cluster.sync();
+    sync_all();
     // thread t holds bins 2 t and 2 t + 1; upto: keys in them and in higher bins
     uint32_t b0 = 0, b1 = 0;
     for (uint32_t r = 0; r < ctas; ++r) {
-      const uint2 x = reinterpret_cast<const uint2*>(cluster.map_shared_rank(bins, r))[tid];
+      const uint32_t* of = ctas == 1u ? bins : cluster.map_shared_rank(bins, r);
+      const uint2 x = reinterpret_cast<const uint2*>(of)[tid];
       b0 += x.x;
       b1 += x.y;
     }
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     } else if (above0 < left && left <= above0 + b0) {
       found_bin = 2u * tid, found_left = left - above0;
     }
-    cluster.sync();  // every CTA has read the bins
+    sync_all();  // every CTA has read the bins
     left = found_left;
   };
   auto clear_bins = [&]() {
@@ -188,7 +196,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
   }
   more = __reduce_add_sync(0xffffffffu, lane < warp ? in_a : 0u);
   ties = __reduce_add_sync(0xffffffffu, lane < warp ? in_b : 0u);
-  cluster.sync();
+  sync_all();
   for (uint32_t r = 0; r < rank; ++r) {
     const uint32_t* t = cluster.map_shared_rank(totals, r);
     more += t[0];
@@ -206,7 +214,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     more += __popc(mb);
     ties += __popc(tb);
   }
-  cluster.sync();  // no CTA leaves while another may read its totals
+  sync_all();  // no CTA leaves while another may read its totals
 }
 
 constexpr uint32_t kMoveThreads = 256;
@@ -221,7 +229,7 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, uint32_t from) {
 // ORDERED: one CTA walks all rows of a column slice of LANES pieces, a chunk at a time.
 // Otherwise LANES lanes hold a whole row and blockIdx.x is the chunk.
 template <bool ORDERED, int LANES>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedView c, const EvictArgs a) {
+__global__ void __launch_bounds__(kMoveThreads, 3) evict_move_kernel(const PagedView c, const EvictArgs a) {
   static_assert(!ORDERED || LANES == kMoveDepth, "an ordered chunk is read whole before it is written");
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t kv = blockIdx.y, b = blockIdx.z;
