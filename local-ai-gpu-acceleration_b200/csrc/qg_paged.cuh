@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "qg_common.cuh"
 #include "qg_host.h"
 
@@ -82,6 +84,37 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
 inline uint32_t dtype_bytes(int dtype) { return dtype == QG_F32 ? 4u : 2u; }
 inline bool dtype_ok(int dtype) { return dtype == QG_F32 || dtype == QG_F16 || dtype == QG_BF16; }
+
+constexpr int kMaxDevices = 64;  // whose attributes are remembered
+
+// Raises a kernel's dynamic shared memory limit, once a device.  (No locks or containers:
+// nothing at a C entry point may throw, and setting it twice does no harm.)
+struct SmemAttr {
+  std::atomic<bool> done[kMaxDevices] = {};
+  cudaError_t set(const void* kernel, uint32_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool known = dev >= 0 && dev < kMaxDevices;
+    if (known && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess && known) done[dev].store(true, std::memory_order_release);
+    return e;
+  }
+};
+
+// SMs of the current device, asked for once a device.
+inline int paged_sm_count() {
+  static std::atomic<int> count[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return device_sm_count();
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = device_sm_count();
+    count[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 // Checks the cache description and fills the kernels' view; false for one that the
 // operators refuse.

@@ -14,19 +14,27 @@
 // tcgen05 with its trip through tensor memory has nothing to win here.
 //
 // Work.  The unit is a block of 128 slots (64 at head size 256) of one (sequence, kv head, head
-// tile); all blocks of
-// the batch, whatever the lengths, form one line that is cut into equal ranges, one a CTA
-// (two CTAs an SM).  In a range, warp w owns a quarter, a tile, of every block and runs
-// on its own: it fetches its K and V tiles in turn through its own ring and keeps its own
-// (m, l, o).  Tiles arrive as TMA boxes of gcd(tile, page_size) slots x 64 values, swizzled for
-// ldmatrix, so no box crosses a page, whatever the page size, and values past head_dim, slots
-// of no page and slots past the sequence's last box are the tensor map's zeros; page ids are
-// read 32 boxes at a time, ahead of their use.  Only rows that share a box with the sequence's ends can hold what is
-// not the sequence's: their V rows are cleared in shared memory, their scores are masked.
-// Where a (sequence, head) ends inside the range the four warps join through
-// shared memory; where it was cut by the range, the CTA leaves a record.  The CTA
-// that arrives last joins a head's records (more than 48 in groups of 16 first, each by its
-// last CTA), always in CTA order, so results do not depend on timing.
+// tile).  All blocks of the batch, whatever the lengths, form one line that is cut into equal
+// ranges, one a CTA, two CTAs an SM; a segment of the line (one sequence, head and tile) counts
+// kHeader blocks more than it has, because its queries and sums cost about that.  In a range,
+// warp w owns a quarter of every block, a tile, and runs on its own: it fetches its K and V
+// tiles in turn through its own ring and keeps its own (m, l, o).  Tiles arrive as TMA boxes of
+// gcd(tile, page_size) slots x 64 values, swizzled for ldmatrix, so no box crosses a page,
+// whatever the page size, and values past head_dim, slots of no page and slots past the
+// sequence's last box are the tensor map's zeros; page ids are read 32 boxes at a time, ahead of
+// their use.  Only rows that share a box with the sequence's ends can hold what is not the
+// sequence's: their V rows are cleared in shared memory, their scores are masked.  Where a
+// segment ends inside the range the four warps join through shared memory; where the range cuts
+// it, the CTA leaves a record.  The CTA that arrives last joins a head's records (more than 48
+// in groups of 16 first, each by its last CTA), always in CTA order, so results do not depend
+// on timing.
+//
+// Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
+// at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 335 us (floor 332); 1 x 131072: 92 us
+// (83; the join of 37 records a head is 7 of them); 32 x 1..8191 bf16 with weights: 36 us (21);
+// 64 x ..4097, 16/16 heads x 64, window 2000, pages of 24: 84 us (70); 1 x 511: 10 us, all
+// latency.  Per-lane asynchronous copies in the place of TMA boxes took 439 us for the first,
+// one 16-slot tile at a time 384 us.
 //
 // Matrix fragments.  Rows of the A operand are query heads.  Eight heads fill rows 0-7 and
 // the rounding errors of their values rows 8-15: q = hi + lo in the cache's type, so one mma
@@ -43,8 +51,6 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <mutex>
-#include <set>
 #include <type_traits>
 
 #include "qg_paged.cuh"
@@ -197,8 +203,9 @@ struct AttnShape {
   static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
   static constexpr uint32_t kRecord = kHeads * (DP + 2u);   // m[], l[], o[][]
   static constexpr int kCtasPerSm = 2;
-  // What a segment costs beside its blocks, in blocks: queries in, sums out (about 3 us, a
-  // block of 64 KB at an SM's half of the memory's rate).
+  // What a segment costs beside its blocks, in blocks: queries in, sums out, joins.  Measured
+  // at 1, 2 and 3: 32 x ..8191 (head size 128) 38.5, 36.4 and 35.3 us, 62 x ..752 (256) 53, 58
+  // and 62 us; head size 64 at 2, 3 and 4: 88.8, 90.0 and 90.5 us.
   static constexpr uint32_t kHeader = DP == 64 ? 2 : DP == 128 ? 3 : 1;
   static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
@@ -450,7 +457,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         int power = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // top in [2^power, 2^(power + 1))
-        power = top == 0.f ? 0 : max(-100, min(100, power));
+        power = top == 0.f ? 0 : max(-126, min(126, power));  // both factors are normal numbers
         const float down = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
         if (lane == 0u) q_mult[r] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
 #pragma unroll
@@ -887,17 +894,6 @@ bool plan_attn(const PagedView& c, uint32_t n_q, uint32_t max_len, bool weights,
   return true;
 }
 
-int sm_count() {
-  static std::mutex mu;
-  static int cache[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lock(mu);
-  if (dev < 0 || dev >= 64) return device_sm_count();
-  if (cache[dev] == 0) cache[dev] = device_sm_count();
-  return cache[dev];
-}
-
 // cuTensorMapEncodeTiled from the driver (looked up once; no link-time dependency on libcuda).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
@@ -948,22 +944,12 @@ template <typename T, int DP, int MT, bool EXTRA>
 cudaError_t launch_attn(const PagedView& c, const AttnArgs& a, const AttnMaps& maps, cudaStream_t stream) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
   const auto kernel = paged_attn_kernel<T, DP, MT, EXTRA>;
-  {
-    static std::mutex mu;
-    static std::set<int> done;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    if (done.count(dev) == 0u) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
-      if (e != cudaSuccess) return e;
-      done.insert(dev);
-    }
-  }
+  static SmemAttr attr;
+  const cudaError_t e = attr.set(reinterpret_cast<const void*>(kernel), Shape::kSmem);
+  if (e != cudaSuccess) return e;
   const uint64_t blocks = static_cast<uint64_t>(c.batch) * c.n_kv * a.tiles *
                           ((std::min(a.max_len, c.capacity) + Shape::kBlock - 1u) / Shape::kBlock);
-  const uint64_t fit = static_cast<uint64_t>(sm_count()) * Shape::kCtasPerSm;
+  const uint64_t fit = static_cast<uint64_t>(paged_sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
   if (blocks / grid >= (1ull << 29)) return cudaErrorInvalidValue;  // a CTA counts its units in 32 bits
   return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);

@@ -241,6 +241,8 @@ def attend(plan: AttentionPlan, q: torch.Tensor, lens: torch.Tensor, *, window: 
     batch, heads, dim = shape
     if dtype not in DTYPE_CODES:
         _fail("q: float32, float16 or bfloat16 is needed")
+    if window < 0:
+        _fail("window is a number of slots, 0 for all")
     q_stride = _heads(q, shape, dtype, "q", index)
     if out is None:
         out, out_stride = _like(q, stream), heads * dim

@@ -212,6 +212,37 @@ def test_attend_small_large_and_infinite_values(cuda, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attend_queries_near_the_largest_fp32(cuda, dtype):
+    rng = np.random.default_rng(15)
+    c = make_cache(rng, 2, 10, 16, 2, 128, DTYPES[dtype])
+    q = queries(rng, 2, 4, 128, torch.float32) * 2e37  # up to about 2^126
+    out, lse = paged.attend(paged.AttentionPlan(c, 4), q, int32([160, 33]), scale=4e-39, return_lse=True)
+    assert torch.isfinite(out).all()
+    check(c, q, [160, 33], out, lse, scale=4e-39)
+
+
+@pytest.mark.gpu
+def test_attend_front_end_refuses(cuda):
+    rng = np.random.default_rng(16)
+    c = make_cache(rng, 2, 2, 16, 2, 64, torch.float16)
+    q, plan, lens = queries(rng, 2, 4, 64, torch.float16), paged.AttentionPlan(c, 4), int32([3, 4])
+    w = torch.zeros(2, 2, 32, device="cuda")
+    for bad in (dict(window=-1), dict(weight_in=w), dict(weight_out=w), dict(out=q[:1]), dict(lse=w)):
+        with pytest.raises(ValueError):
+            paged.attend(plan, q, lens, **bad)
+    for bad_q in (q[:1], q.double(), q.cpu(), q.transpose(0, 1), q.repeat(1, 1, 2)[..., ::2]):
+        with pytest.raises(ValueError):
+            paged.attend(plan, bad_q, lens)
+    for bad_lens in (lens.long(), lens.cpu(), lens[:1], int32([1, 2, 3, 4])[::2]):
+        with pytest.raises(ValueError):
+            paged.attend(plan, q, bad_lens)
+    with pytest.raises(qgemv_b200.CudaError):
+        paged.AttentionPlan(c, 3)
+    assert paged.attend(plan, q, lens).shape == (2, 4, 64) and ops.get_error() == 0
+
+
+@pytest.mark.gpu
 def test_attend_strides_streams_and_lengths_past_the_table(cuda):
     rng = np.random.default_rng(6)
     c = make_cache(rng, 3, 4, 16, 2, 64, torch.float16, pad=8)
