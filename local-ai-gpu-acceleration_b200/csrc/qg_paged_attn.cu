@@ -15,7 +15,7 @@
 //
 // Work.  The unit is a block of 128 slots (64 at head size 256) of one (sequence, kv head, head
 // tile).  All blocks of the batch, whatever the lengths, form one line that is cut into equal
-// ranges, one a CTA, two CTAs an SM; a segment of the line (one sequence, head and tile) counts
+// ranges, one a CTA, two or three CTAs an SM; a segment of the line (one sequence, head and tile) counts
 // kHeader blocks more than it has, because its queries and sums cost about that.  In a range,
 // warp w owns a quarter of every block, a tile, and runs on its own: it fetches its K and V
 // tiles in turn through its own ring and keeps its own (m, l, o).  Tiles arrive as TMA boxes of
@@ -32,7 +32,7 @@
 // Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
 // at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 335 us (floor 332); 1 x 131072: 92 us
 // (83; the join of 37 records a head is 7 of them); 32 x 1..8191 bf16 with weights: 36 us (21);
-// 64 x ..4097, 16/16 heads x 64, window 2000, pages of 24: 84 us (70); 1 x 511: 10 us, all
+// 64 x ..4097, 16/16 heads x 64, window 2000, pages of 24: 79 us (70); 1 x 511: 10 us, all
 // latency.  Per-lane asynchronous copies in the place of TMA boxes took 439 us for the first,
 // one 16-slot tile at a time 384 us.
 //
@@ -195,14 +195,18 @@ struct AttnShape {
   static constexpr uint32_t kBlock = block_slots(DP);
   static constexpr uint32_t kHeads = 8u * MT;
   static constexpr uint32_t kUnit = kTile * DP * 2u;        // a warp's K or V tile
-  static constexpr uint32_t kUnits = DP == 64 ? 6 : 3;      // of its ring
+  // CTAs an SM.  Small heads do the most work a byte and fit three in registers: 64 x ..4097
+  // (16/16 heads x 64) 84 us with two, 79 with three.  At 128 three CTAs of 168 registers are
+  // 2-7% faster where many segments run (256 x 300: 65 and 60 us) and 5-15% slower where few
+  // do (1 x 8192: 17.7 and 20.3, 1 x 131072: 92.6 and 97.1 us), so it keeps two.
+  static constexpr int kCtasPerSm = DP == 64 && MT == 1 ? 3 : 2;
+  static constexpr uint32_t kUnits = DP != 64 ? 3 : kCtasPerSm == 3 ? 4 : 6;  // of its ring
   static constexpr uint32_t kRing = kWarps * kUnits * kUnit;
   static constexpr uint32_t kQRows = MT * (EXTRA ? 24u : 16u);
   static constexpr uint32_t kQBytes = kQRows * DP * 2u;
   static constexpr uint32_t kSmem = kRing + kQBytes + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
   static constexpr uint32_t kRecord = kHeads * (DP + 2u);   // m[], l[], o[][]
-  static constexpr int kCtasPerSm = 2;
   // What a segment costs beside its blocks, in blocks: queries in, sums out, joins.  Measured
   // at 1, 2 and 3: 32 x ..8191 (head size 128) 38.5, 36.4 and 35.3 us, 62 x ..752 (256) 53, 58
   // and 62 us; head size 64 at 2, 3 and 4: 88.8, 90.0 and 90.5 us.
