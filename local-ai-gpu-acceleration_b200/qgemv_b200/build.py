@@ -22,7 +22,7 @@ def nvcc_command(out: Path, extra: list[str] | None = None) -> list[str]:
     return [
         NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-rdc=true",
         "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
-        "-shared", "-o", str(out), *[str(CSRC / s) for s in SOURCES],
+        "--threads", "0", "-shared", "-o", str(out), *[str(CSRC / s) for s in SOURCES],
         "-lnccl",
         *(extra or []),
     ]
