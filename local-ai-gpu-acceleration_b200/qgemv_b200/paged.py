@@ -87,16 +87,16 @@ def _call(fn, index: int, *args) -> None:
         raise CudaError(fn.__name__, code)
 
 
-def _new(shape: tuple, dtype, device, stream) -> torch.Tensor:
-    """A new tensor on the stream that will write it."""
+def _new_ints(shape: tuple, like: torch.Tensor, stream) -> torch.Tensor:
+    """The same of another shape."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape)
 
 
 def _like(t: torch.Tensor, stream) -> torch.Tensor:
-    """The same for a tensor like t (half the time of _new)."""
+    """A new tensor like t, on the stream that will write it."""
     if stream is None:
         return _empty_like(t)
     with torch.cuda.stream(stream):
@@ -277,30 +277,43 @@ def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: i
     """qg_kv_evict: keep `budget` slots per kv head of every longer sequence -- the first `sink`,
     the last `recent`, and the heaviest between them by weight [sequences, kv heads, >= longest
     length].  Rows move to the front of the same pages, lens and weight are updated; or, with
-    new_table [sequences, pages], to those pages, lens and weight left as they are.  Returns
-    (kept [sequences, kv heads, budget], new lens); the new weights are in weight_out."""
+    new_table [sequences, pages], to those pages, the new weights to weight_out (needed then; it
+    may be weight) and lens left as it is.  Returns (kept [sequences, kv heads, budget], new lens)."""
     index, batch, kv = cache.index, cache.batch, cache.n_kv_heads
     if weight.dim() != 3:
         _fail("weight: [sequences, kv heads, slots] is needed")
     width = weight.shape[2]
-    if lens_out is None:
-        lens_out = lens if new_table is None else _like(lens, stream)
-    if weight_out is None:
-        weight_out = weight if new_table is None else _like(weight, stream)
-    if kept is None:
-        kept = _new((batch, kv, budget), torch.int32, cache.device, stream)
-    to, pages, step = None, 0, 0
-    if new_table is not None:
-        if (new_table.dtype is not torch.int32 or new_table.dim() != 2 or new_table.shape[0] != batch
-                or new_table.get_device() != index or (new_table.shape[1] > 1 and new_table.stride(1) != 1)):
-            _fail("new_table: an int32 tensor [sequences, pages per sequence] is needed")
-        to, pages = new_table.data_ptr(), new_table.shape[1]
-        step = new_table.stride(0) if batch > 1 else pages
     shape = (batch, kv, width)
     weight_at, lens_at = _floats(weight, shape, "weight", index), _ints(lens, batch, "lens", index)
-    e = EvictC(lens_at, lens_at if lens_out is lens else _ints(lens_out, batch, "lens_out", index),
-               weight_at, weight_at if weight_out is weight else _floats(weight_out, shape, "weight_out", index),
-               width, width, budget, sink, recent, _ints(kept, batch * kv * budget, "kept", index),
+    to, pages, step, elsewhere = None, 0, 0, new_table is not None
+    if elsewhere:
+        if (new_table.dtype is not _I32 or new_table.dim() != 2 or new_table.get_device() != index
+                or new_table.shape[0] != batch):
+            _fail("new_table: an int32 tensor [sequences, pages per sequence] is needed")
+        pages = new_table.shape[1]
+        step, one = new_table.stride()
+        if one != 1 and pages > 1:
+            _fail("new_table: a sequence's pages must be contiguous")
+        to, step = new_table.data_ptr(), step if batch > 1 else pages
+    if lens_out is None and elsewhere:
+        lens_out = _like(lens, stream)
+        lens_out_at = lens_out.data_ptr()
+    elif lens_out is None or lens_out is lens:
+        lens_out, lens_out_at = lens, lens_at
+    else:
+        lens_out_at = _ints(lens_out, batch, "lens_out", index)
+    if weight_out is None and elsewhere:
+        _fail("new_table needs weight_out: a tensor for the new weights, or weight itself")
+    if weight_out is None or weight_out is weight:
+        weight_out_at = weight_at
+    else:
+        weight_out_at = _floats(weight_out, shape, "weight_out", index)
+    if kept is None:
+        kept = _new_ints((batch, kv, budget), lens, stream)
+        kept_at = kept.data_ptr()
+    else:
+        kept_at = _ints(kept, batch * kv * budget, "kept", index)
+    e = EvictC(lens_at, lens_out_at, weight_at, weight_out_at, width, width, budget, sink, recent, kept_at,
                to, pages, step)
     _call(lib().qg_kv_evict, index, cache._ref, _byref(e),
           _raw_stream(index) if stream is None else stream.cuda_stream)

@@ -180,6 +180,26 @@ def test_append_data_outside_the_cache_is_dropped(cuda):
 
 
 @pytest.mark.gpu
+def test_append_front_end_refuses(cuda):
+    rng = np.random.default_rng(9)
+    c = make_cache(rng, 2, 2, 16, 2, 64, torch.float16)
+    q, k, v = new_rows(rng, 2, 4, 2, 64, torch.float16)
+    pos, rope = torch.zeros(2, dtype=torch.int32, device="cuda"), paged.rope_table(8, 64)
+    good = dict(q=q, k=k, v=v, rope=rope, positions=pos)
+    before = c.k.clone()
+    for bad in (dict(q=q.double()), dict(q=q.view(2, -1)), dict(k=k.float()), dict(k=k[:1]), dict(v=v.cpu()),
+                dict(v=v.repeat(1, 1, 2)[..., ::2]), dict(positions=pos.long()), dict(positions=pos[:1]),
+                dict(slots=pos.cpu()), dict(seqs=pos.repeat(2)[::2]), dict(rope=rope.half()), dict(pairs="both"),
+                dict(q_norm=rope[0].half()), dict(k_norm=rope[0, :32]), dict(q_out=q.float())):
+        with pytest.raises(ValueError):
+            paged.qk_norm_rope_append(c, **(good | bad))
+    for bad in (dict(rope=paged.rope_table(8, 24)), dict(rope=paged.rope_table(8, 80))):
+        with pytest.raises(qgemv_b200.CudaError):
+            paged.qk_norm_rope_append(c, **(good | bad))
+    assert torch.equal(c.k, before) and ops.get_error() == 0
+
+
+@pytest.mark.gpu
 def test_append_offsets_past_32_bits(cuda):
     """Pools of more than 2^32 bytes: the last page's rows lie past any 32-bit offset."""
     page, heads, dim = 64, 8, 128

@@ -179,6 +179,26 @@ def test_evict_data_outside_the_cache(cuda):
 
 
 @pytest.mark.gpu
+def test_evict_front_end_refuses(cuda):
+    rng = np.random.default_rng(3)
+    c = make_cache(rng, 2, 4, 16, 2, 64, torch.float16)
+    lens, w, table = int32([20, 30]), torch.zeros(2, 2, 64, device="cuda"), int32([[0], [1]])
+    for bad in (dict(new_table=table), dict(new_table=table.long(), weight_out=w), dict(new_table=table[:1], weight_out=w),
+                dict(lens_out=lens.long()), dict(weight_out=w[:, :1]), dict(kept=int32([1]))):
+        with pytest.raises(ValueError):
+            paged.evict(c, lens, w, 10, **bad)
+    for bad in (w[:, :, ::2], w.half(), w.cpu(), w[0]):
+        with pytest.raises(ValueError):
+            paged.evict(c, lens, bad, 10)
+    for bad in (dict(sink=8, recent=8), dict(sink=-1), dict(recent=11)):
+        with pytest.raises(qgemv_b200.CudaError):
+            paged.evict(c, lens, w, 10, **bad)
+    with pytest.raises(qgemv_b200.CudaError):  # 16 slots are not room for 17
+        paged.evict(c, lens, w, 17, new_table=table, weight_out=w.clone())
+    assert lens.tolist() == [20, 30] and ops.get_error() == 0
+
+
+@pytest.mark.gpu
 def test_evict_offsets_past_32_bits(cuda):
     page, heads, dim = 64, 8, 128
     n = 2 ** 32 // (page * heads * dim * 2) + 3
