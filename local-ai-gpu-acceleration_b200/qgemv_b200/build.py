@@ -1,4 +1,5 @@
-"""Build step for libqgemv_b200.so (the sm_100a kernels + C-ABI) -- run by
+"""Build step for libqgemv_b200.so (the sm_100a kernels + C-ABI) and the torch front end of
+the paged cache operators -- run by
 __graft_entry__.build() and, when the library is missing, by the package loader.
 nvcc cross-compiles for sm_100a without a GPU."""
 
@@ -53,6 +54,44 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     return LIB_PATH
 
 
+# The torch front end of the paged cache operators: a CPython module built with g++ against the
+# torch that is installed; it holds no device code.
+TORCH_PATH = PKG_DIR / "qgemv_paged_torch.so"
+TORCH_SOURCE = CSRC / "qg_paged_torch.cpp"
+
+
+def torch_command(out: Path) -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(NVCC).resolve().parents[1]
+    include = [*cpp_extension.include_paths(), str(cuda / "include"), sysconfig.get_paths()["include"]]
+    libs = Path(torch.__file__).parent / "lib"
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[f"-I{p}" for p in dict.fromkeys(include)], str(TORCH_SOURCE), "-o", str(out),
+            f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+
+
+def build_torch(force: bool = False) -> Path:
+    header = PKG_DIR.parent / "include" / "qgemv_b200.h"
+    newest = max(p.stat().st_mtime for p in (TORCH_SOURCE, header))
+    if not force and TORCH_PATH.exists() and TORCH_PATH.stat().st_mtime >= newest:
+        return TORCH_PATH
+    tmp = TORCH_PATH.with_suffix(".so.tmp")
+    cmd = torch_command(tmp)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        print(" ".join(cmd))
+        print(res.stderr[-20000:])
+        raise RuntimeError(f"g++ failed ({res.returncode}) building {TORCH_PATH.name}")
+    tmp.replace(TORCH_PATH)
+    return TORCH_PATH
+
+
 if __name__ == "__main__":
     import sys
     build(force=True, verbose=True, extra=sys.argv[1:])
+    build_torch(force=True)

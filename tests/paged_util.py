@@ -1,5 +1,8 @@
 """Paged caches for the tests: pools and page tables in any layout, their logical rows, and
-the unit roundoffs that the tolerances are made of."""
+the unit roundoffs that the tolerances are made of; the C-ABI's structures."""
+
+import ctypes
+from ctypes import c_float, c_int, c_uint32, c_uint64, c_void_p
 
 import numpy as np
 import torch
@@ -40,3 +43,37 @@ def logical(cache, pool, seq, n):
     """The first n slots of a sequence: [heads, n, dim] in float64 on the CPU."""
     page, place = row_index(cache, seq, torch.arange(n))
     return pool[page, :, place].double().cpu().transpose(0, 1)
+
+
+class KvPagesC(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int),
+                ("num_pages", c_uint32), ("page_size", c_uint32), ("n_kv_heads", c_uint32),
+                ("head_dim", c_uint32), ("page_stride", c_uint64), ("head_stride", c_uint64),
+                ("slot_stride", c_uint64), ("table", c_void_p), ("batch", c_uint32),
+                ("table_pages", c_uint32), ("table_stride", c_uint32)]
+
+
+class AppendC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p),
+                ("dtype", c_int), ("tokens", c_uint32), ("n_q_heads", c_uint32),
+                ("q_stride", c_uint64), ("k_stride", c_uint64), ("v_stride", c_uint64),
+                ("q_out_stride", c_uint64), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("eps", c_float), ("rope", c_void_p), ("rope_rows", c_uint32),
+                ("rot_dim", c_uint32), ("pairs", c_int), ("positions", c_void_p),
+                ("slots", c_void_p), ("seqs", c_void_p)]
+
+
+class AttnC(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("dtype", c_int), ("n_q_heads", c_uint32),
+                ("q_stride", c_uint64), ("out_stride", c_uint64), ("lens", c_void_p),
+                ("max_len", c_uint32), ("window", c_uint32), ("scale", c_float),
+                ("lse", c_void_p), ("weight_in", c_void_p), ("weight_out", c_void_p),
+                ("weight_stride", c_uint32)]
+
+
+class EvictC(ctypes.Structure):
+    _fields_ = [("lens", c_void_p), ("lens_out", c_void_p), ("weight", c_void_p),
+                ("weight_out", c_void_p), ("max_len", c_uint32), ("weight_stride", c_uint32),
+                ("budget", c_uint32), ("sink", c_uint32), ("recent", c_uint32),
+                ("kept", c_void_p), ("new_table", c_void_p), ("new_table_pages", c_uint32),
+                ("new_table_stride", c_uint32)]

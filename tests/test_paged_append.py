@@ -13,7 +13,7 @@ import pytest
 import torch
 
 import qgemv_b200
-from paged_util import DTYPES, INVALID_VALUE, TINY, UNIT, make_cache, row_index
+from paged_util import AppendC, DTYPES, INVALID_VALUE, KvPagesC, make_cache, row_index, TINY, UNIT
 from qgemv_b200 import ops, paged
 
 
@@ -216,8 +216,8 @@ def test_append_offsets_past_32_bits(cuda):
 
 
 def _args():
-    c = paged.KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
-    a = paged.AppendC(64, 64, 64, 64, 1, 2, 4, 256, 128, 128, 256, None, None, 1e-5, 64, 8, 64, 0, 64, None, None)
+    c = KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
+    a = AppendC(64, 64, 64, 64, 1, 2, 4, 256, 128, 128, 256, None, None, 1e-5, 64, 8, 64, 0, 64, None, None)
     return c, a
 
 

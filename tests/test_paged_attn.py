@@ -16,7 +16,7 @@ import pytest
 import torch
 
 import qgemv_b200
-from paged_util import DTYPES, INVALID_VALUE, TINY, UNIT, logical, make_cache, row_index
+from paged_util import AttnC, DTYPES, INVALID_VALUE, KvPagesC, logical, make_cache, row_index, TINY, UNIT
 from qgemv_b200 import ops, paged
 
 
@@ -317,8 +317,8 @@ def test_attend_in_a_graph_follows_the_lengths(cuda):
 
 
 def _args():
-    c = paged.KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
-    a = paged.AttnC(64, 64, 1, 4, 256, 256, 64, 32, 0, 1.0, None, None, None, 0)
+    c = KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
+    a = AttnC(64, 64, 1, 4, 256, 256, 64, 32, 0, 1.0, None, None, None, 0)
     return c, a
 
 

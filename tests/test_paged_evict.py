@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import qgemv_b200
-from paged_util import DTYPES, INVALID_VALUE, make_cache, row_index
+from paged_util import DTYPES, EvictC, INVALID_VALUE, KvPagesC, make_cache, row_index
 from qgemv_b200 import ops, paged
 
 
@@ -213,8 +213,8 @@ def test_evict_offsets_past_32_bits(cuda):
 
 
 def _args():
-    c = paged.KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
-    return c, paged.EvictC(64, 64, 64, 64, 32, 32, 16, 4, 4, 64, 64, 1, 1)
+    c = KvPagesC(64, 64, 1, 4, 16, 2, 64, 2048, 1024, 64, 64, 2, 2, 2)
+    return c, EvictC(64, 64, 64, 64, 32, 32, 16, 4, 4, 64, 64, 1, 1)
 
 
 @pytest.mark.parametrize("what,field,value", [
