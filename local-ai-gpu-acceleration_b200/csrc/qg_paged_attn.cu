@@ -27,7 +27,11 @@
 // segment ends inside the range the four warps join through shared memory; where the range cuts
 // it, the CTA leaves a record.  The CTA that arrives last joins a head's records (more than 48
 // in groups of 16 first, each by its last CTA), always in CTA order, so results do not depend
-// on timing.
+// on timing.  Where segments are many and short (the rule is in the kernel, on the lengths) a CTA
+// would spend its time between them, 4.4 us each; there every warp takes whole segments alone,
+// with no barrier and no record.  98 sequences of 16/16 heads x 112 that see one slot: 26 us by
+// CTAs, 14 by warps; 256 x 300 slots, 32/8 heads x 128: 65 and 61 us; 89 x 1..2 slots, 40/8 heads x
+// 112: 17 and 9 us.
 //
 // Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
 // at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 335 us (floor 332); 1 x 131072: 92 us
@@ -164,26 +168,25 @@ __device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N
   }
 }
 
-// One (sequence, kv head x head tile) of the line: its seen slots [start, len) are blocks
-// [j0, j1); j is the next one.
-template <uint32_t kBlock>
+// The power p with top in [2^p, 2^(p + 1)), kept where both 2^p and 2^-p are normal numbers.
+__device__ __forceinline__ int power_of(float top) {
+  return top == 0.f ? 0 : max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+}
+__device__ __forceinline__ float power_of_two(int power) {
+  return __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+}
+
+// One (sequence, kv head x head tile) of the line: its seen slots [start, len) are steps
+// [j0, j1) of 2^log slots; j is the next one.
 struct Segment {
   uint32_t b, h, j, j0, j1, start, len;
 
-  __device__ __forceinline__ void bounds(const PagedView& c, const AttnArgs& a) {
+  __device__ __forceinline__ void bounds(const PagedView& c, const AttnArgs& a, uint32_t log) {
     len = paged_len(a.lens[b], min(a.max_len, c.capacity));
     start = a.window != 0u && len > a.window ? len - a.window : 0u;
-    j0 = start / kBlock;
-    j1 = max((len + kBlock - 1u) / kBlock, j0 + 1u);  // an empty sequence has one empty block
-  }
-  // The one after it, if `more` blocks of the range are left.
-  __device__ __forceinline__ void next(const PagedView& c, const AttnArgs& a, bool more) {
-    if (++h == c.n_kv * a.tiles) {
-      h = 0;
-      ++b;
-      if (more) bounds(c, a);
-    }
-    j = j0;
+    j0 = start >> log;
+    j1 = max(((len - 1u) >> log) + 1u, j0 + 1u);  // an empty sequence has one empty step
+    if (len == 0u) j1 = j0 + 1u;
   }
 };
 
@@ -211,6 +214,9 @@ struct AttnShape {
   // at 1, 2 and 3: 32 x ..8191 (head size 128) 38.5, 36.4 and 35.3 us, 62 x ..752 (256) 53, 58
   // and 62 us; head size 64 at 2, 3 and 4: 88.8, 90.0 and 90.5 us.
   static constexpr uint32_t kHeader = DP == 64 ? 2 : DP == 128 ? 3 : 1;
+  // Whether a lone warp may take whole segments (below): where its queries fit beside the rest.
+  // At head size 256 and with two tiles of heads the code for it cost the others 5-10%.
+  static constexpr bool kSolo = DP <= 128 && MT == 1;
   static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
 
@@ -218,8 +224,8 @@ template <typename T, int DP, int MT, bool EXTRA>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCtasPerSm)
     paged_attn_kernel(const PagedView c, const AttnArgs a, const __grid_constant__ AttnMaps maps) {
   using Shape = AttnShape<T, DP, MT, EXTRA>;
-  using Seg = Segment<Shape::kBlock>;
-  constexpr uint32_t kTile = Shape::kTile, kBlock = Shape::kBlock, kLogTile = log_tile(DP);
+  constexpr uint32_t kTile = Shape::kTile, kLogTile = log_tile(DP), kLogBlock = kLogTile + 2u;
+  static_assert(kWarps == 4u, "a block is four tiles");
   constexpr uint32_t kUnits = Shape::kUnits, kUnit = Shape::kUnit, kHeads = Shape::kHeads;
   constexpr int kTerms = EXTRA ? 3 : 2;
   constexpr int kSteps = kTile / 16;    // 16-slot steps of a product over slots
@@ -228,6 +234,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   __shared__ float join_m[kWarps][kHeads], join_l[kWarps][kHeads], q_mult[kHeads];
   __shared__ __align__(8) uint64_t full[kWarps][kUnits];
   __shared__ uint64_t sum64[kWarps];
+  __shared__ uint32_t most_of[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
   __shared__ float share[kHeads][64];
@@ -248,17 +255,21 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's range [r0, r1) of the line of units (blocks, and headers before each segment's)
+  // ---- this CTA's range [r0, r1) of the line of units (blocks, and headers before each
+  // segment's), or, where segments are short and many, a whole segment for every warp
   const uint32_t lines = c.n_kv * a.tiles;
-  auto blocks_of = [&](uint32_t b) {
-    Seg s;
+  auto blocks_of = [&](uint32_t b, uint32_t& most) {
+    Segment s;
     s.b = b;
-    s.bounds(c, a);
+    s.bounds(c, a, kLogTile);
+    most = max(most, s.j1 - s.j0);
+    s.bounds(c, a, kLogBlock);
     return s.j1 - s.j0;
   };
-  uint64_t total = 0;  // blocks of one line of every sequence, then of all lines
+  uint64_t total = 0;  // blocks of one line of every sequence, then units of all lines
+  uint32_t most = 0;   // tiles of the longest
   if (c.batch > kAttnThreads) {
-    for (uint32_t b = tid; b < c.batch; b += kAttnThreads) total += blocks_of(b);
+    for (uint32_t b = tid; b < c.batch; b += kAttnThreads) total += blocks_of(b, most);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
     if (lane == 0u) sum64[warp] = total;
@@ -268,18 +279,21 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     for (uint32_t w = 0; w < kWarps; ++w) total += sum64[w];
   }
   uint64_t ctas = 0, r0 = 0, r1 = 0;
+  const uint32_t segments = c.batch * lines;  // below 2^32: both are below 2^16
+  bool solo_now = false;
   uint32_t header = 0;  // units of a segment that stand for its cost beside its blocks
   for (uint64_t base = 0, b0 = 0; b0 < c.batch; b0 += kAttnThreads) {
     const uint32_t b = static_cast<uint32_t>(b0) + tid;
-    const uint64_t n = b < c.batch ? blocks_of(b) : 0u;
+    const uint64_t n = b < c.batch ? blocks_of(b, most) : 0u;
     uint64_t upto = n;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint64_t o = __shfl_up_sync(0xffffffffu, upto, off);
       if (lane >= static_cast<uint32_t>(off)) upto += o;
     }
+    most = __reduce_max_sync(0xffffffffu, most);
     __syncthreads();
-    if (lane == 31u) sum64[warp] = upto;
+    if (lane == 31u) sum64[warp] = upto, most_of[warp] = most;
     __syncthreads();
     uint64_t all = 0;
 #pragma unroll
@@ -289,9 +303,21 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     }
     if (b0 == 0u) {
       if (c.batch <= kAttnThreads) total = all;
+#pragma unroll
+      for (uint32_t w = 0; w < kWarps; ++w) most = max(most, most_of[w]);
+      const uint64_t blocks = total * lines;
+      if constexpr (Shape::kSolo) {
+        // Time in fifths of a microsecond: a tile takes 12 in a warp, a block 12 in a CTA, a
+        // segment 5 more in a warp and 10 in a CTA.  With every segment taken for the longest, a
+        // segment a warp has to be the faster way.
+        const uint64_t busy = min(static_cast<uint64_t>(gridDim.x), blocks);
+        const uint64_t rounds = (segments + gridDim.x * kWarps - 1u) / (gridDim.x * kWarps);
+        solo_now = rounds * (most * 12ull + 5u) * busy <= blocks * 12u + segments * 10ull;
+        if (solo_now) break;
+      }
       // fewer blocks than CTAs: a block each; otherwise segments cost more than their blocks
-      if (total * lines > gridDim.x) header = Shape::kHeader;
-      total = (total + static_cast<uint64_t>(header) * c.batch) * lines;
+      if (blocks > gridDim.x) header = Shape::kHeader;
+      total = blocks + static_cast<uint64_t>(header) * segments;
       ctas = min(static_cast<uint64_t>(gridDim.x), total);
       if (blockIdx.x >= ctas) return;
       r0 = blockIdx.x * total / ctas;
@@ -309,19 +335,52 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     if ((base + static_cast<uint64_t>(header) * (b0 + kAttnThreads)) * lines > r0) break;
   }
   __syncthreads();
-  Seg use;
-  use.b = first_at[0];
-  use.h = first_at[1];
-  use.bounds(c, a);
-  uint32_t left = static_cast<uint32_t>(r1 - r0);  // units of the range from use.j on (below 2^31)
+  const bool solo = Shape::kSolo && solo_now;
+  const uint32_t log_step = solo ? kLogTile : kLogBlock, warp_slot = solo ? 0u : warp * kTile;
+  Segment use;
+  uint32_t use_index = 0, left = 0;  // left: units of the range, or steps of the segment, from use.j on
   auto skip_header = [&](uint32_t& units, uint32_t done) { units -= min(units, header - min(done, header)); };
-  skip_header(left, first_at[2]);
-  use.j = use.j0 + (first_at[2] - min(first_at[2], header));
+  // segment `index` of the line for a lone warp
+  auto take = [&](Segment& s, uint32_t index, uint32_t& steps) {
+    steps = 0u;
+    if (index >= segments) return;
+    s.b = index / lines;
+    s.h = index - s.b * lines;
+    s.bounds(c, a, log_step);
+    s.j = s.j0;
+    steps = s.j1 - s.j0;
+  };
+  // the segment after one that is done
+  auto advance = [&](Segment& s, uint32_t& index, uint32_t& steps) {
+    if (solo) {
+      index += gridDim.x * kWarps;
+      take(s, index, steps);
+    } else {
+      skip_header(steps, 0u);
+      if (++s.h == lines) {
+        s.h = 0;
+        ++s.b;
+        if (steps != 0u) s.bounds(c, a, log_step);
+      }
+      s.j = s.j0;
+    }
+  };
+  if (solo) {
+    use_index = warp * gridDim.x + blockIdx.x;
+    take(use, use_index, left);
+  } else {
+    use.b = first_at[0];
+    use.h = first_at[1];
+    use.bounds(c, a, log_step);
+    left = static_cast<uint32_t>(r1 - r0);  // below 2^31
+    skip_header(left, first_at[2]);
+    use.j = use.j0 + (first_at[2] - min(first_at[2], header));
+  }
 
-  // a segment's queries as this lane splits them: rows warp, warp + 4, .. of its head tile
+  // A segment's queries as this lane of a CTA splits them: rows warp, warp + 4, .. of its head tile
   constexpr uint32_t kPer = DP / 32, kQRowsPerWarp = kHeads / kWarps;
   uint32_t q_raw[kQRowsPerWarp][kPer];  // fp32 words, or pairs of 16-bit values in the first half
-  auto load_queries = [&](const Seg& s) {
+  auto load_queries = [&](const Segment& s) {
     const uint32_t kv = s.h / a.tiles, ht = s.h - kv * a.tiles;
     const uint32_t heads = a.group - ht * kHeads;  // or more than the tile has
     const uint32_t bytes = a.dtype == QG_F32 ? 4u : 2u;
@@ -339,21 +398,22 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
       }
     }
   };
-  if (left != 0u) load_queries(use);
+  if (!solo && left != 0u) load_queries(use);
 
   // ---- fetching.  A set of page ids covers the next 32 boxes of this warp's tiles, a box a
   // lane; the set after it is read while this one is used.
   const uint64_t policy = l2_evict_first_policy();
   const uint32_t boxes = 1u << a.log_boxes, log_box = kLogTile - a.log_boxes;
-  Seg ahead = use;
-  uint32_t ahead_left = left;
+  Segment ahead = use;
+  uint32_t ahead_index = use_index, ahead_left = left;
   int32_t page = 0, place = 0, head = 0, next_page = 0, next_place = 0, next_head = 0;
   uint32_t at_tile = 0, tiles = 0, next_tiles = 0;  // of the set
   auto look_up = [&]() {
+    next_tiles = 0u;
+    if (ahead_left == 0u) return;
     next_tiles = min(min(32u >> a.log_boxes, ahead.j1 - ahead.j), ahead_left);
-    if (next_tiles == 0u) return;
     const uint32_t t = lane >> a.log_boxes;
-    const uint32_t slot = (ahead.j + t) * kBlock + warp * kTile + ((lane & (boxes - 1u)) << log_box);
+    const uint32_t slot = ((ahead.j + t) << log_step) + warp_slot + ((lane & (boxes - 1u)) << log_box);
     const uint32_t at = div_by(slot, c.page);
     next_page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
     next_place = static_cast<int32_t>(slot - at * c.page.d);
@@ -368,10 +428,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     }
     ahead.j += next_tiles;
     ahead_left -= next_tiles;
-    if (ahead.j == ahead.j1) {
-      skip_header(ahead_left, 0u);
-      ahead.next(c, a, ahead_left != 0u);
-    }
+    if (ahead.j == ahead.j1) advance(ahead, ahead_index, ahead_left);
   };
   auto next_set = [&]() {
     page = next_page;
@@ -438,8 +495,59 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     const uint32_t heads = min(kHeads, a.group - ht * kHeads);
     const uint32_t head0 = kv * a.group + ht * kHeads;
     const uint32_t from_j = use.j, to_j = min(use.j1, use.j + left);
+    // log-sum-exp of a finished head
+    auto put_stats = [&](uint32_t h, float top, float sum) {
+      const size_t at = static_cast<size_t>(use.b) * a.n_q + h;
+      const float full_sum = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
+      if (a.lse != nullptr) a.lse[at] = full_sum * 0.69314718055994530942f;
+      if (a.norm != nullptr) a.norm[at] = full_sum;
+    };
 
-    {  // ---- the queries
+    // ---- the queries
+    if (solo) {
+      // A lone warp takes them as the A operand does: this lane has values 16 k + 2 t4, + 1, + 8
+      // and + 9 of head g of every tile of 8.
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        constexpr uint32_t kK = DP / 16;
+        const uint64_t at = use.b * a.q_stride + static_cast<uint64_t>(head0 + i * 8u + g) * c.dim + 2u * t4;
+        float2 x[kK][2];
+        float top = 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < kK; ++k) {
+#pragma unroll
+          for (uint32_t e = 0; e < 2; ++e) {
+            const uint32_t d = 16u * k + 8u * e;
+            x[k][e] = make_float2(0.f, 0.f);
+            if (i * 8u + g < heads && d < c.dim) {
+              if (a.dtype == QG_F32) {
+                x[k][e] = *reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + at + d);
+              } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + at + d);
+                x[k][e] = a.dtype == QG_F16 ? unpack2(w, __half()) : unpack2(w, __nv_bfloat16());
+              }
+            }
+            top = fmaxf(top, fmaxf(fabsf(x[k][e].x), fabsf(x[k][e].y)));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int power = power_of(top);
+        const float down = power_of_two(-power);
+        mult[i] = a.scale_log2 * power_of_two(power);
+#pragma unroll
+        for (uint32_t k = 0; k < kK; ++k) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t term[kTerms];
+            split_terms<T>(x[k][e].x * down, x[k][e].y * down, term);
+            qa[i][k][2 * e] = term[0];
+            qa[i][k][2 * e + 1] = term[1];
+            if constexpr (EXTRA) qx[i][k][e] = term[2];
+          }
+        }
+      }
+    } else {
 #pragma unroll
       for (uint32_t row = 0; row < kQRowsPerWarp; ++row) {
         const uint32_t r = warp + row * kWarps;
@@ -460,10 +568,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         for (uint32_t e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        int power = static_cast<int>(__float_as_uint(top) >> 23) - 127;  // top in [2^power, 2^(power + 1))
-        power = top == 0.f ? 0 : max(-126, min(126, power));  // both factors are normal numbers
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
-        if (lane == 0u) q_mult[r] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+        const int power = power_of(top);
+        const float down = power_of_two(-power);
+        if (lane == 0u) q_mult[r] = a.scale_log2 * power_of_two(power);
 #pragma unroll
         for (uint32_t e = 0; e < kPer; e += 2) {
           uint32_t term[kTerms];
@@ -495,15 +602,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
           }
         }
         mult[i] = q_mult[i * 8 + g];
-        m[i] = -CUDART_INF_F;
-        l[i] = 0.f;
-#pragma unroll
-        for (uint32_t n = 0; n < DP / 8; ++n) o[i][n][0] = o[i][n][1] = 0.f;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      m[i] = -CUDART_INF_F;
+      l[i] = 0.f;
+#pragma unroll
+      for (uint32_t n = 0; n < DP / 8; ++n) o[i][n][0] = o[i][n][1] = 0.f;
     }
 
     for (; use.j < to_j; ++use.j) {
-      const uint32_t slot0 = use.j * kBlock + warp * kTile;
+      const uint32_t slot0 = (use.j << log_step) + warp_slot;
       const bool whole = slot0 >= use.start && slot0 + kTile <= use.len;
       const bool seen = slot0 < use.len && slot0 + kTile > use.start;
       // ---- scores
@@ -632,14 +742,34 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     left -= to_j - from_j;
 
     // ---- the end of the segment, or of the range inside it
-    Seg after = use;
+    Segment after = use;
     const uint64_t here = r1 - left;  // the unit after this segment's part
-    if (use.j == use.j1) {
-      skip_header(left, 0u);
-      after.next(c, a, left != 0u);
-    }
-    if (left != 0u) load_queries(after);  // on their way while this segment joins
-    {
+    if (use.j == use.j1) advance(after, use_index, left);
+    if (!solo && left != 0u) load_queries(after);  // on their way while this segment joins
+    if (solo) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint32_t h = i * 8u + g;
+        float sum = l[i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (h >= heads) continue;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const size_t at = use.b * a.out_stride + static_cast<size_t>(head0 + h) * c.dim + 2u * t4;
+#pragma unroll
+        for (uint32_t n = 0; n < DP / 8; ++n) {
+          if (n * 8u >= c.dim) break;
+          const float u = o[i][n][0] * inv, v = o[i][n][1] * inv;
+          if (a.dtype == QG_F32) {
+            *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at + n * 8u) = make_float2(u, v);
+          } else {
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at + n * 8u) =
+                a.dtype == QG_F16 ? pack2(u, v, __half()) : pack2(u, v, __nv_bfloat16());
+          }
+        }
+        if (t4 == 0u) put_stats(head0 + h, m[i], sum);
+      }
+    } else {
       const bool mine = from_j == use.j0 && to_j == use.j1;
       // each warp's sums into the unit it has just used, float4 pieces swizzled by head
 #pragma unroll
@@ -674,12 +804,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
                 make_uint2(pack2(v.x, v.y, __nv_bfloat16()), pack2(v.z, v.w, __nv_bfloat16()));
           }
         }
-        if (ch == 0u) {
-          const size_t hi = static_cast<size_t>(use.b) * a.n_q + head0 + h;
-          const float full_sum = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
-          if (a.lse != nullptr) a.lse[hi] = full_sum * 0.69314718055994530942f;
-          if (a.norm != nullptr) a.norm[hi] = full_sum;
-        }
+        if (ch == 0u) put_stats(head0 + h, top, sum);
       };
       for (uint32_t i = tid; i < heads * (DP / 4u); i += kAttnThreads) {
         const uint32_t h = i / (DP / 4u), ch = i % (DP / 4u);

@@ -169,6 +169,35 @@ def test_attend_long_sequences_and_many_of_them(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_type,cache_type", [("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page,longest,window", [
+    (4, 2, 128, 16, 64, 0),   # every warp with whole segments, more of them than warps
+    (16, 2, 112, 5, 31, 0),
+    (3, 3, 64, 24, 65, 40),   # three tiles, the window cutting into the first
+    (8, 1, 80, 32, 1, 0),
+])
+def test_attend_many_short_sequences(cuda, q_type, cache_type, q_heads, kv_heads, dim, page, longest, window):
+    rng = np.random.default_rng(dim + longest)
+    batch = 700
+    lens = [int(n) for n in rng.integers(0, longest + 1, batch)]
+    lens[0], lens[1], lens[-1] = longest, 0, longest
+    c = make_cache(rng, batch, longest // page + 1, page, kv_heads, dim, DTYPES[cache_type])
+    poison(c, lens, float("nan"))
+    q = queries(rng, batch, q_heads, dim, DTYPES[q_type])
+    plan = paged.AttentionPlan(c, q_heads, weights=True)
+    before = torch.rand(batch, kv_heads, plan.max_len, device="cuda")
+    weight = before.clone()
+    out, lse = paged.attend(plan, q, int32(lens), window=window, return_lse=True, weight_in=weight, weight_out=weight)
+    check(c, q, lens, out, lse, window=window, weight=weight, before=before)
+    lens = [longest] * batch  # as long as the pages reach: the same bits twice
+    c2 = make_cache(rng, batch, longest // page + 1, page, kv_heads, dim, DTYPES[cache_type], "shd")
+    plan = paged.AttentionPlan(c2, q_heads)
+    out = paged.attend(plan, q, int32(lens), window=window)
+    check(c2, q, lens, out, window=window)
+    assert torch.equal(out, paged.attend(plan, q, int32(lens), window=window)) and ops.get_error() == 0
+
+
+@pytest.mark.gpu
 def test_attend_equal_scores_over_a_long_context(cuda):
     """Every probability alike and tiny, next to one that dominates: their sum must not drown
     in the 16-bit split of the probabilities."""
