@@ -34,7 +34,7 @@
 // 112: 17 and 9 us.
 //
 // Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
-// at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 335 us (floor 332); 1 x 131072: 92 us
+// at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 336 us (floor 332); 1 x 131072: 93 us
 // (83; the join of 37 records a head is 7 of them); 32 x 1..8191 bf16 with weights: 36 us (21);
 // 64 x ..4097, 16/16 heads x 64, window 2000, pages of 24: 79 us (70); 1 x 511: 10 us, all
 // latency.  Per-lane asynchronous copies in the place of TMA boxes took 439 us for the first,
@@ -214,9 +214,10 @@ struct AttnShape {
   // at 1, 2 and 3: 32 x ..8191 (head size 128) 38.5, 36.4 and 35.3 us, 62 x ..752 (256) 53, 58
   // and 62 us; head size 64 at 2, 3 and 4: 88.8, 90.0 and 90.5 us.
   static constexpr uint32_t kHeader = DP == 64 ? 2 : DP == 128 ? 3 : 1;
-  // Whether a lone warp may take whole segments (below): where its queries fit beside the rest.
-  // At head size 256 and with two tiles of heads the code for it cost the others 5-10%.
-  static constexpr bool kSolo = DP <= 128 && MT == 1;
+  // Whether a lone warp may take whole segments (below): where the code for it costs the rest
+  // little (1%).  At head size 256 and with two tiles of heads it cost 5-10%, at 64, whose three
+  // CTAs an SM change segments faster, 2-4% (64 x ..4097: 79.2 and 81.1 us).
+  static constexpr bool kSolo = DP == 128 && MT == 1;
   static_assert(kHeads * DP * 4u <= kUnit, "a warp's sums join in a free unit");
 };
 
