@@ -566,9 +566,10 @@ cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
  * smaller at least head_dim, one a multiple of the other, page_stride a multiple of both and
  * below 2^39 (strides of a dimension of one entry are not looked at).  q, out:
  * [batch][n_q_heads][head_dim] with sequence strides in elements (multiples of 16 bytes);
- * 16-B aligned.  `workspace`: 256-B aligned, qg_paged_attn_workspace_bytes long, its
- * first QG_PAGED_ATTN_ZEROED bytes zero before its first use (every call leaves them
- * zero); calls that overlap need one each. */
+ * 16-B aligned.  `workspace`: 256-B aligned, qg_paged_attn_workspace_bytes long (of the same
+ * cache, heads and max_len; weights != 0 where weight_out is given), its first
+ * QG_PAGED_ATTN_ZEROED bytes zero before its first use (every call leaves them zero); calls
+ * that overlap need one each. */
 #define QG_PAGED_ATTN_ZEROED 4096u
 typedef struct qg_attn {
   const void* q;

@@ -15,23 +15,23 @@
 //
 // Work.  The unit is a block of 128 slots (64 at head size 256) of one (sequence, kv head, head
 // tile).  All blocks of the batch, whatever the lengths, form one line that is cut into equal
-// ranges, one a CTA, two or three CTAs an SM; a segment of the line (one sequence, head and tile) counts
-// kHeader blocks more than it has, because its queries and sums cost about that.  In a range,
-// warp w owns a quarter of every block, a tile, and runs on its own: it fetches its K and V
-// tiles in turn through its own ring and keeps its own (m, l, o).  Tiles arrive as TMA boxes of
-// gcd(tile, page_size) slots x 64 values, swizzled for ldmatrix, so no box crosses a page,
-// whatever the page size, and values past head_dim, slots of no page and slots past the
+// ranges, one a CTA, two or three CTAs an SM; a segment of the line (one sequence, head and
+// tile) counts kHeader blocks more than it has, because its queries and sums cost about that.
+// In a range, warp w owns a quarter of every block, a tile, and runs on its own: it fetches its K
+// and V tiles in turn through its own ring and keeps its own (m, l, o).  Tiles arrive as TMA
+// boxes of gcd(tile, page_size) slots x 64 values, swizzled for ldmatrix, so no box crosses a
+// page, whatever the page size, and values past head_dim, slots of no page and slots past the
 // sequence's last box are the tensor map's zeros; page ids are read 32 boxes at a time, ahead of
 // their use.  Only rows that share a box with the sequence's ends can hold what is not the
 // sequence's: their V rows are cleared in shared memory, their scores are masked.  Where a
 // segment ends inside the range the four warps join through shared memory; where the range cuts
-// it, the CTA leaves a record.  The CTA that arrives last joins a head's records (more than 48
-// in groups of 16 first, each by its last CTA), always in CTA order, so results do not depend
-// on timing.  Where segments are many and short (the rule is in the kernel, on the lengths) a CTA
+// it, the CTA leaves a record.  The CTA that arrives last joins a head's records (more than 48 in
+// groups of 16 first, each by its last CTA), always in CTA order, so results do not depend on
+// timing.  Where segments are many and short (the rule is in the kernel, on the lengths) a CTA
 // would spend its time between them, 4.4 us each; there every warp takes whole segments alone,
 // with no barrier and no record.  98 sequences of 16/16 heads x 112 that see one slot: 26 us by
-// CTAs, 14 by warps; 256 x 300 slots, 32/8 heads x 128: 65 and 61 us; 89 x 1..2 slots, 40/8 heads x
-// 112: 17 and 9 us.
+// CTAs, 14 by warps; 256 x 300 slots, 32/8 heads x 128: 65 and 61 us; 89 x 1..2 slots, 40/8 heads
+// x 112: 17 and 9 us.
 //
 // Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
 // at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 336 us (floor 332); 1 x 131072: 93 us
@@ -48,8 +48,8 @@
 // accumulators are laid out like the A operand of the next product, so probabilities go back
 // in without a shuffle, again as hi + lo; they carry a factor 2^14 (removed with l), which
 // keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
-// Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: the
-// matrix pipe truncates when it accumulates, and o lives for thousands of tiles.
+// Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: o lives for
+// thousands of tiles, and how the matrix pipe rounds a running sum is not specified.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math_constants.h>
