@@ -31,8 +31,10 @@
 namespace qg {
 namespace {
 
-constexpr uint32_t kSelectThreads = 1024;
-constexpr uint32_t kSelectWarps = kSelectThreads / 32;
+// Threads of a selecting CTA: few for short sequences, so that four CTAs share an SM and a
+// barrier waits for 8 warps; the rule is in qg_kv_evict.
+constexpr uint32_t kManyThreads = 1024, kFewThreads = 256;
+constexpr uint32_t kShort = 1024;              // slots: below this a sequence is short
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kCachedKeys = 48u * 1024u;  // keys that fit in a CTA's shared memory (192 KB)
 constexpr uint32_t kMaxCluster = 8;            // CTAs of a cluster on every device
@@ -60,13 +62,14 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr uint32_t kZeroKey = 0x80000000u;     // of weight 0, the one that many slots share
 
 // blockIdx.x: rank in the cluster.  A CTA's stretch is a multiple of 32 slots a warp.
-__host__ __device__ constexpr uint32_t stretch(uint32_t n, uint32_t ctas) {
-  const uint32_t unit = kSelectWarps * 32u;
-  return ((n + ctas - 1u) / ctas + unit - 1u) / unit * unit;
+__host__ __device__ constexpr uint32_t stretch(uint32_t n, uint32_t ctas, uint32_t threads) {
+  return ((n + ctas - 1u) / ctas + threads - 1u) / threads * threads;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const PagedView c, const EvictArgs a,
-                                                                      bool cached) {
+template <uint32_t kSelectThreads>
+__global__ void __launch_bounds__(kSelectThreads, kManyThreads / kSelectThreads)
+    evict_select_kernel(const PagedView c, const EvictArgs a, bool cached) {
+  constexpr uint32_t kSelectWarps = kSelectThreads / 32, kMine = kBins / kSelectThreads;
   extern __shared__ uint32_t keys[];  // cached: the keys of this CTA's stretch
   __shared__ uint32_t bins[kBins];
   __shared__ uint32_t warp_a[kSelectWarps], warp_b[kSelectWarps];
@@ -93,7 +96,8 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     return;
   }
   const uint32_t lo = a.sink, hi = n - a.recent;  // the slots that are chosen from
-  const uint32_t s0 = min(rank * stretch(n, ctas), n), s1 = min(s0 + stretch(n, ctas), n);
+  const uint32_t share = stretch(n, ctas, kSelectThreads);
+  const uint32_t s0 = min(rank * share, n), s1 = min(s0 + share, n);
   auto slot_key = [&](uint32_t i) { return i < lo || i >= hi ? kStays : weight_key(w[i]); };
   auto key_at = [&](uint32_t i) { return cached ? keys[i - s0] : slot_key(i); };
 
@@ -114,15 +118,20 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     if (lane == 0u && zeros != 0u) atomicAdd(&bins[zero_bin], zeros);
     zeros = 0u;
     sync_all();
-    // thread t holds bins 2 t and 2 t + 1; upto: keys in them and in higher bins
-    uint32_t b0 = 0, b1 = 0;
+    // thread t holds bins kMine t and on; upto: keys in them and in higher bins
+    uint32_t bin[kMine] = {};
     for (uint32_t r = 0; r < ctas; ++r) {
       const uint32_t* of = ctas == 1u ? bins : cluster.map_shared_rank(bins, r);
-      const uint2 x = reinterpret_cast<const uint2*>(of)[tid];
-      b0 += x.x;
-      b1 += x.y;
+#pragma unroll
+      for (uint32_t i = 0; i < kMine; i += 2u) {
+        const uint2 x = *reinterpret_cast<const uint2*>(of + kMine * tid + i);
+        bin[i] += x.x;
+        bin[i + 1u] += x.y;
+      }
     }
-    uint32_t upto = b0 + b1;
+    uint32_t upto = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) upto += bin[i];
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint32_t o = __shfl_down_sync(0xffffffffu, upto, off);
@@ -130,18 +139,19 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
     }
     if (lane == 0u) warp_a[warp] = upto;
     __syncthreads();
-    upto += __reduce_add_sync(0xffffffffu, lane > warp ? warp_a[lane] : 0u);
-    const uint32_t above1 = upto - b0 - b1, above0 = upto - b0;
-    if (above1 < left && left <= above1 + b1) {
-      found_bin = 2u * tid + 1u, found_left = left - above1;
-    } else if (above0 < left && left <= above0 + b0) {
-      found_bin = 2u * tid, found_left = left - above0;
+    upto += __reduce_add_sync(0xffffffffu, lane > warp && lane < kSelectWarps ? warp_a[lane] : 0u);
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) {
+      const uint32_t above = upto - bin[i];  // keys in higher bins
+      if (above < left && left <= upto) found_bin = kMine * tid + i, found_left = left - above;
+      if (i + 1u < kMine) upto = upto - bin[i];
     }
     sync_all();  // every CTA has read the bins
     left = found_left;
   };
   auto clear_bins = [&]() {
-    reinterpret_cast<uint2*>(bins)[tid] = make_uint2(0u, 0u);
+#pragma unroll
+    for (uint32_t i = 0; i < kMine; ++i) bins[i * kSelectThreads + tid] = 0u;
     __syncthreads();
   };
 
@@ -180,7 +190,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
   }
 
   // ---- the kept slots in ascending order: larger keys, and the first `left` equal ones
-  const uint32_t per = stretch(n, ctas) / kSelectWarps;
+  const uint32_t per = share / kSelectWarps;
   const uint32_t from = min(s0 + warp * per, s1), to = min(from + per, s1);
   uint32_t more = 0, ties = 0;
   for (uint32_t i = from + lane; i < to; i += 32u) {
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Page
   ties = __reduce_add_sync(0xffffffffu, ties);
   if (lane == 0u) warp_a[warp] = more, warp_b[warp] = ties;
   __syncthreads();
-  const uint32_t in_a = warp_a[lane], in_b = warp_b[lane];
+  const uint32_t in_a = lane < kSelectWarps ? warp_a[lane] : 0u, in_b = lane < kSelectWarps ? warp_b[lane] : 0u;
   if (warp == 0u) {
     const uint32_t all_a = __reduce_add_sync(0xffffffffu, in_a), all_b = __reduce_add_sync(0xffffffffu, in_b);
     if (lane == 0u) totals[0] = all_a, totals[1] = all_b;
@@ -353,17 +363,25 @@ extern "C" cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, 
   a.slices = ordered ? (c.dim + kSliceLanes * 8u - 1u) / (kSliceLanes * 8u) : 1u;
   a.parts = ordered ? 1u : (most + kMoveRows - 1u) / kMoveRows;
   static SmemAttr select_attr;
-  cudaError_t err = select_attr.set(reinterpret_cast<const void*>(evict_select_kernel), kCachedKeys * 4u);
+  cudaError_t err =
+      select_attr.set(reinterpret_cast<const void*>(evict_select_kernel<kManyThreads>), kCachedKeys * 4u);
   if (err != cudaSuccess) return err;
+  const uint64_t lines = static_cast<uint64_t>(c.n_kv) * c.batch, sms = static_cast<uint64_t>(paged_sm_count());
+  // Few threads for short lines, and up to twice that where the lines do not fit on the SMs at
+  // once.  Whole call with 1024 and 256 threads, head size 128 (112 in the first), us: 37 x 26..45
+  // slots of 16 heads 27.8 and 11.7, of 8 heads: 16 x 1000 20.7 and 15.4, 64 x 2048 75.2 and 61.1,
+  // 1 x 1000 11.5 and 11.8.  Past the rule: 1 x 2000 12.5 and 17.0, 20 x 3096..4096 35 and 39,
+  // 40 x 100..8000 44 and 61; only where all are long and many it would gain (64 x 4096 82 and 70).
+  const bool few = e->max_len < kShort || (e->max_len <= 2u * kShort && lines > sms);
+  const uint32_t threads = few ? kFewThreads : kManyThreads;
   // CTAs of a selection: while SMs are free and a stretch keeps two slots a thread
   uint32_t ctas = 1;
-  const uint64_t lines = static_cast<uint64_t>(c.n_kv) * c.batch, sms = static_cast<uint64_t>(paged_sm_count());
-  while (ctas < kMaxCluster && lines * ctas * 2u <= sms && e->max_len >= ctas * 2u * 2u * kSelectThreads) ctas *= 2u;
-  const uint32_t slots = stretch(e->max_len, ctas);
+  while (ctas < kMaxCluster && lines * ctas * 2u <= sms && e->max_len >= ctas * 2u * 2u * threads) ctas *= 2u;
+  const uint32_t slots = stretch(e->max_len, ctas, threads);
   const bool cached = slots <= kCachedKeys;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, c.n_kv, c.batch);
-  cfg.blockDim = kSelectThreads;
+  cfg.blockDim = threads;
   cfg.dynamicSmemBytes = cached ? slots * 4u : 0u;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -374,7 +392,8 @@ extern "C" cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  err = cudaLaunchKernelEx(&cfg, evict_select_kernel, c, a, cached);
+  err = few ? cudaLaunchKernelEx(&cfg, evict_select_kernel<kFewThreads>, c, a, cached)
+            : cudaLaunchKernelEx(&cfg, evict_select_kernel<kManyThreads>, c, a, cached);
   if (err != cudaSuccess) return err;
   const dim3 grid(a.slices * a.parts, c.n_kv, c.batch);
   if (ordered) return launch_k(evict_move_kernel<true, kSliceLanes>, grid, kMoveThreads, 0, stream, c, a);
