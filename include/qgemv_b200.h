@@ -554,10 +554,11 @@ cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
  * `window` slots are seen.  For query head h of kv head h / (n_q_heads / n_kv_heads):
  *   s_j = scale * q . k_j,  m = max_j s_j,  l = sum_j exp(s_j - m)
  *   out = sum_j exp(s_j - m) v_j / l,  lse = m + ln(l)    (lse may be NULL)
- * over the seen slots; with none (length 0) out is 0 and lse -inf.  Slots past the length
- * are never read as numbers, whatever they hold; an infinite or NaN value in a seen V row
- * makes that column of the output infinite or NaN.  With weight_out each seen slot's share
- * is summed over the query heads of its kv head:
+ * over the seen slots; with none (length 0), or where every seen score is -inf, out is 0 and
+ * lse -inf, and the head adds nothing to the weights below.  Slots past the length are never
+ * read as numbers, whatever they hold; an infinite or NaN value in a seen V row makes that
+ * column of the output infinite or NaN.  With weight_out each seen slot's share is summed
+ * over the query heads of its kv head:
  *   weight_out[b][kv][j] = weight_in[b][kv][j] + sum_h exp(s_hj - m_h) / l_h
  * for every j < lens[b] (unseen slots: weight_in alone), rows of weight_stride floats;
  * weight_in may be weight_out, or NULL for zero; slots at or past lens[b] are left alone.

@@ -981,7 +981,8 @@ __global__ void __launch_bounds__(kWeightThreads) attn_weight_kernel(const Paged
   }
 #pragma unroll 2
   for (uint32_t h = 0; h < a.group; ++h) {
-    const float full = a.norm[head + h];
+    // minus infinity: no seen score of the head is above it, so its output is zero and so are its shares
+    const float norm = a.norm[head + h], full = norm == -CUDART_INF_F ? 0.f : norm;
     const float* scores = a.scores + (head + h) * a.score_stride;
 #pragma unroll
     for (uint32_t u = 0; u < kWeightSlots; ++u) {

@@ -252,6 +252,39 @@ def test_attend_queries_near_the_largest_fp32(cuda, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cache_type,q_type", [("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attend_weights_of_rows_without_a_finite_score(cuda, cache_type, q_type, dim):
+    """A head all of whose scores are minus infinity adds nothing to its kv head's weights: the
+    other heads' shares arrive alone, and where every head is such a row the weights stay."""
+    rng = np.random.default_rng(dim)
+    lens = [150, 1, 31, 0]
+    c = make_cache(rng, 4, 10, 16, 1, dim, DTYPES[cache_type])
+    poison(c, lens, float("nan"))
+    for b in (0, 2):  # positive against the one head's minus infinity
+        page, place = row_index(c, b, torch.arange(lens[b]))
+        c.k[page, :, place, 0] = c.k[page, :, place, 0].abs() + 0.125
+    page, place = row_index(c, 1, [0])
+    c.k[page, :, place] = 0
+    c.k[page, :, place, 0] = float("inf")
+    q = queries(rng, 4, 4, dim, DTYPES[q_type])
+    q[:, 2] = 0
+    q[:, 2, 0] = -float("inf")
+    q[1] = 1
+    q[1, :, 0] = -1
+    plan = paged.AttentionPlan(c, 4, weights=True)
+    before = torch.rand(4, 1, plan.max_len, device="cuda")
+    weight = before.clone()
+    out, lse = paged.attend(plan, q, int32(lens), return_lse=True, weight_in=weight, weight_out=weight)
+    assert torch.count_nonzero(out[:, 2]) == 0 and (lse[:, 2] == -np.inf).all()
+    assert torch.count_nonzero(out[1]) == 0 and (lse[1] == -np.inf).all()
+    assert torch.equal(weight[1], before[1]) and torch.equal(weight[3], before[3])
+    live = [0, 1, 3]
+    lens[1] = 0  # nothing seen, as its output has it
+    check(c, q[:, live], lens, out[:, live], lse[:, live], weight=weight, before=before)
+
+
+@pytest.mark.gpu
 def test_attend_front_end_refuses(cuda):
     rng = np.random.default_rng(16)
     c = make_cache(rng, 2, 2, 16, 2, 64, torch.float16)
