@@ -25,16 +25,20 @@ struct Entries {
   decltype(&qg_kv_evict) evict = nullptr;
 } g_entries;
 
-// What a PagedCache and an AttentionPlan hold.
+// What a PagedCache and an AttentionPlan hold: addresses, and the storages that they lie in, so
+// that no memory goes back to the allocator while a description of it lives, whatever becomes of
+// the caller's tensors.
 struct Cache {
   qg_kv_pages pages;
   int index;  // device
+  c10::Storage k, v, table;
 };
 struct Plan {
-  const Cache* cache;
+  Cache cache;
   uint32_t n_q, max_len;
   bool weights;
   void* workspace;
+  c10::Storage space;
 };
 constexpr char kCacheName[] = "qgemv_b200.paged.cache", kPlanName[] = "qgemv_b200.paged.plan";
 
@@ -201,6 +205,9 @@ PyObject* py_cache(PyObject*, PyObject* const* args, Py_ssize_t n) {
     c.pages.batch = static_cast<uint32_t>(table.size(0));
     c.pages.table_pages = static_cast<uint32_t>(table.size(1));
     c.pages.table_stride = static_cast<uint32_t>(table.size(0) > 1 ? table.stride(0) : table.size(1));
+    c.k = k.storage();
+    c.v = v.storage();
+    c.table = table.storage();
     PyObject* capsule = hold(c, kCacheName);
     if (capsule == nullptr) return nullptr;
     PyObject* at = PyLong_FromVoidPtr(&held<Cache>(capsule, kCacheName)->pages);
@@ -216,12 +223,15 @@ PyObject* py_cache(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 5, [&]() -> PyObject* {
     Plan p{};
-    p.cache = held<Cache>(args[0], kCacheName);
-    if (p.cache == nullptr) throw Refused();
+    const Cache* cache = held<Cache>(args[0], kCacheName);
+    if (cache == nullptr) throw Refused();
+    p.cache = *cache;
     p.n_q = count_of(args[1]);
     p.max_len = count_of(args[2]);
     p.weights = args[3] == Py_True;
-    p.workspace = tensor_of(args[4], "workspace").data_ptr();
+    const at::Tensor& workspace = tensor_of(args[4], "workspace");
+    p.workspace = workspace.data_ptr();
+    p.space = workspace.storage();
     return hold(p, kPlanName);
   });
 }
@@ -276,7 +286,7 @@ PyObject* py_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 11, [&]() -> PyObject* {
     const Plan* p = held<Plan>(args[0], kPlanName);
     if (p == nullptr) throw Refused();
-    const Cache* c = p->cache;
+    const Cache* c = &p->cache;
     const at::Tensor& q = tensor_of(args[1], "q");
     const int64_t batch = c->pages.batch, heads = p->n_q, dim = c->pages.head_dim, kv = c->pages.n_kv_heads;
     const at::ScalarType type = q.scalar_type();

@@ -49,10 +49,23 @@ def _calls():
     return _CALLS
 
 
-class PagedCache:
+class _MadeOnce:
+    """What the library was told when an object was made holds for its calls: an attribute of the
+    constructor's can be read, not replaced."""
+
+    _replaceable: tuple[str, ...] = ()
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__ and name not in self._replaceable:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: calls use what the object was made of")
+        object.__setattr__(self, name, value)
+
+
+class PagedCache(_MadeOnce):
     """Pools `k` and `v` [pages, kv heads, page size, head dim] (fp16 or bf16, any strides
     with contiguous dims, the same for both) and `table` [sequences, pages per sequence]
-    (int32).  The caller owns them: it hands out pages by writing the table."""
+    (int32).  The caller shares them: it hands out pages by writing into the table, and replaces
+    or resizes none of the three.  Their memory stays while the cache, or a plan for it, does."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
         self.calls = _calls()
@@ -98,9 +111,12 @@ def qk_norm_rope_append(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: 
     return q_out
 
 
-class AttentionPlan:
+class AttentionPlan(_MadeOnce):
     """The workspace of `attend` for a cache, a number of query heads and lengths up to
-    max_len (default: all that a table row names).  Calls that may overlap need a plan each."""
+    max_len (default: all that a table row names).  Calls that may overlap need a plan each.
+    `scale` is the scale of calls that name none."""
+
+    _replaceable = ("scale",)
 
     def __init__(self, cache: PagedCache, n_q_heads: int, max_len: int | None = None,
                  weights: bool = False):
