@@ -46,8 +46,9 @@
 // cache takes a third term, 24 bits, in a second mma.)  q is first scaled by a power of two
 // per head to a largest value in [1, 2), so neither term leaves fp16's range.  The scores'
 // accumulators are laid out like the A operand of the next product, so probabilities go back
-// in without a shuffle, again as hi + lo; they carry a factor 2^14 (removed with l), which
-// keeps probabilities down to 2^-38 exact enough in fp16 when a million slots share the sum.
+// in without a shuffle, again as hi + lo; in fp16 they carry a factor 2^14 (removed with l), which
+// keeps probabilities down to 2^-38 exact enough when a million slots share the sum.  bf16 has
+// fp32's exponents: it needs no factor, and values above 2^114 could not bear one.
 // Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: o lives for
 // thousands of tiles, and how the matrix pipe rounds a running sum is not specified.
 #include <cuda.h>
@@ -73,7 +74,9 @@ constexpr uint32_t kJoin = 16;                // records of a group where there 
 constexpr uint32_t kInFlight = 16;            // records whose sums are asked for together
 static_assert(2u * kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "two counters per CTA");
 static_assert(kMaxCtas / kJoin <= 64u && kJoinAll <= 64u, "two records a lane");
-constexpr float kShareBits = 14.f;            // log2 of the factor that probabilities carry
+// log2 of the factor that probabilities carry in the cache's type
+template <typename T>
+constexpr float kShareBits = std::is_same<T, __half>::value ? 14.f : 0.f;
 
 struct AttnArgs {
   const void* q;
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
     // log-sum-exp of a finished head
     auto put_stats = [&](uint32_t h, float top, float sum) {
       const size_t at = static_cast<size_t>(use.b) * a.n_q + h;
-      const float full_sum = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits;
+      const float full_sum = sum == 0.f ? -CUDART_INF_F : top + log2f(sum) - kShareBits<T>;
       if (a.lse != nullptr) a.lse[at] = full_sum * 0.69314718055994530942f;
       if (a.norm != nullptr) a.norm[at] = full_sum;
     };
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
           const float from = now == -CUDART_INF_F ? 0.f : now;
           fade[i] = exp2_fast(m[i] - from);
           m[i] = now;
-          const float base = kShareBits - from;
+          const float base = kShareBits<T> - from;
           float sum = 0.f;
 #pragma unroll
           for (int n = 0; n < 2 * kSteps; ++n) {

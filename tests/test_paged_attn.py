@@ -285,6 +285,22 @@ def test_attend_weights_of_rows_without_a_finite_score(cuda, cache_type, q_type,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_type", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,heads", [(64, 4), (64, 16), (128, 4), (256, 4)])
+def test_attend_values_near_the_largest_bf16(cuda, q_type, dim, heads):
+    """Values of up to about 2^116: their weighted sum is far from overflowing."""
+    rng = np.random.default_rng(dim + heads)
+    lens = [700, 0, 1, 33, 160]
+    c = make_cache(rng, len(lens), 44, 16, 1, dim, torch.bfloat16)
+    c.v.mul_(2.0 ** 114)
+    poison(c, lens, float("nan"))
+    q = queries(rng, len(lens), heads, dim, DTYPES[q_type])
+    out, lse = paged.attend(paged.AttentionPlan(c, heads), q, int32(lens), return_lse=True)
+    assert torch.isfinite(out).all()
+    check(c, q, lens, out, lse)
+
+
+@pytest.mark.gpu
 def test_attend_front_end_refuses(cuda):
     rng = np.random.default_rng(16)
     c = make_cache(rng, 2, 2, 16, 2, 64, torch.float16)
