@@ -44,7 +44,8 @@
 // the rounding errors of their values rows 8-15: q = hi + lo in the cache's type, so one mma
 // gives (hi + lo) . k, fp16 pairs carrying 22 bits and bf16 pairs 16.  (A fp32 q with a bf16
 // cache takes a third term, 24 bits, in a second mma.)  q is first scaled by a power of two
-// per head to a largest value in [1, 2), so neither term leaves fp16's range.  The scores'
+// per head to a largest value in [1, 2), so neither term leaves fp16's range, or in
+// [2^-10, 2^-9) over bf16, so 256 products with its largest keys stay within fp32's.  The scores'
 // accumulators are laid out like the A operand of the next product, so probabilities go back
 // in without a shuffle, again as hi + lo; in fp16 they carry a factor 2^14 (removed with l), which
 // keeps probabilities down to 2^-38 exact enough when a million slots share the sum.  bf16 has
@@ -171,9 +172,13 @@ __device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N
   }
 }
 
-// The power p with top in [2^p, 2^(p + 1)), kept where both 2^p and 2^-p are normal numbers.
+// The power p with top in [2^p, 2^(p + 1)), kept where both 2^p and 2^-p are normal numbers.  For
+// bf16 it is 10 more, less where that would pass 116 (the scale times 2^p has to stay finite).
+template <typename T>
 __device__ __forceinline__ int power_of(float top) {
-  return top == 0.f ? 0 : max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+  constexpr int kRoom = std::is_same<T, __half>::value ? 0 : 10;
+  const int p = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+  return top == 0.f ? 0 : min(p + kRoom, max(p, 126 - kRoom));
 }
 __device__ __forceinline__ float power_of_two(int power) {
   return __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
@@ -536,7 +541,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int power = power_of(top);
+        const int power = power_of<T>(top);
         const float down = power_of_two(-power);
         mult[i] = a.scale_log2 * power_of_two(power);
 #pragma unroll
@@ -572,7 +577,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<T, DP, MT, EXTRA>::kCt
         for (uint32_t e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[e]));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const int power = power_of(top);
+        const int power = power_of<T>(top);
         const float down = power_of_two(-power);
         if (lane == 0u) q_mult[r] = a.scale_log2 * power_of_two(power);
 #pragma unroll

@@ -301,6 +301,23 @@ def test_attend_values_near_the_largest_bf16(cuda, q_type, dim, heads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("power", [125, -120])
+@pytest.mark.parametrize("dim,heads", [(64, 4), (64, 16), (128, 4), (256, 4)])
+def test_attend_keys_near_the_ends_of_bf16(cuda, dim, heads, power):
+    """Keys near bf16's largest and near its smallest normal values, with queries that make
+    ordinary scores of them."""
+    rng = np.random.default_rng(dim + heads + power % 1000)
+    lens = [700, 0, 1, 33, 160]
+    c = make_cache(rng, len(lens), 44, 16, 1, dim, torch.bfloat16)
+    c.k.mul_(2.0 ** power)
+    poison(c, lens, float("nan"))
+    q = queries(rng, len(lens), heads, dim, torch.float32) * 2.0 ** -power
+    out, lse = paged.attend(paged.AttentionPlan(c, heads), q, int32(lens), return_lse=True)
+    assert torch.isfinite(out).all()
+    check(c, q, lens, out, lse)
+
+
+@pytest.mark.gpu
 def test_attend_front_end_refuses(cuda):
     rng = np.random.default_rng(16)
     c = make_cache(rng, 2, 2, 16, 2, 64, torch.float16)
