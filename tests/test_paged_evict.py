@@ -138,6 +138,33 @@ def test_evict_ties_and_special_weights(cuda, kind, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lens,width,budget", [
+    ([50000, 49999, 7, 0, 3000] * 8, 50000, 2500),  # a line a CTA: more lines than SMs, rows wider than it keeps
+    ([400000], 400003, 100000),                     # a cluster of 8 with more than it keeps
+])
+def test_evict_keys_past_shared_memory(cuda, lens, width, budget, in_place):
+    """Selections whose keys do not stay in shared memory read the weights again in every pass."""
+    rng = np.random.default_rng(width)
+    page, heads, dim = 100, 2, 8
+    pages, to = -(-max(lens) // page), -(-budget // page)
+    both = make_cache(rng, len(lens), pages + to, page, heads, dim, torch.float16)
+    c, table = paged.PagedCache(both.k, both.v, both.table[:, :pages]), both.table[:, pages:]
+    old = {"k": c.k.clone(), "v": c.v.clone()}
+    w = weights(rng, (len(lens), heads, width), lens)
+    w0, ln = w.clone(), int32(lens)
+    if in_place:
+        kept, new = paged.evict(c, ln, w, budget, sink=3, recent=201)
+        check(c, old, c.table, kept, w0, w, lens, new, budget, 3, 201)
+    else:
+        w1 = torch.full_like(w, 3.0)
+        kept, new = paged.evict(c, ln, w, budget, sink=3, recent=201, new_table=table, weight_out=w1)
+        check(c, old, table, kept, w0, w1, lens, new, budget, 3, 201)
+        assert torch.equal(w, w0) and ln.tolist() == lens
+    assert ops.get_error() == 0
+
+
+@pytest.mark.gpu
 def test_evict_twice_and_on_a_stream(cuda):
     """A second call at the same budget changes nothing; eviction, growth and eviction again."""
     rng = np.random.default_rng(1)
