@@ -38,10 +38,16 @@ def up_to_date(out: Path = LIB_PATH) -> bool:
     return out.stat().st_mtime >= newest
 
 
+def scratch(out: Path) -> Path:
+    """Where this process builds `out` before it takes its place: processes that build at the same
+    time do not share it."""
+    return out.with_name(f"{out.name}.{os.getpid()}.tmp")
+
+
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> Path:
     if not force and up_to_date():
         return LIB_PATH
-    tmp = LIB_PATH.with_suffix(".so.tmp")
+    tmp = scratch(LIB_PATH)
     cmd = nvcc_command(tmp, extra)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
@@ -49,6 +55,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         print(res.stdout[-20000:])
         print(res.stderr[-20000:])
     if res.returncode != 0:
+        tmp.unlink(missing_ok=True)
         raise RuntimeError(f"nvcc failed ({res.returncode}) building {LIB_PATH.name}")
     tmp.replace(LIB_PATH)
     return LIB_PATH
@@ -56,8 +63,17 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
 
 # The torch front end of the paged cache operators: a CPython module built with g++ against the
 # torch that is installed; it holds no device code.
-TORCH_PATH = PKG_DIR / "qgemv_paged_torch.so"
 TORCH_SOURCE = CSRC / "qg_paged_torch.cpp"
+
+
+def torch_path() -> Path:
+    """The module of the installed torch and Python, by name: one that was compiled against the
+    headers of another is never loaded."""
+    import sysconfig
+
+    import torch
+
+    return PKG_DIR / f"qgemv_paged_torch.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
 
 
 def torch_command(out: Path) -> list[str]:
@@ -78,17 +94,19 @@ def torch_command(out: Path) -> list[str]:
 def build_torch(force: bool = False) -> Path:
     header = PKG_DIR.parent / "include" / "qgemv_b200.h"
     newest = max(p.stat().st_mtime for p in (TORCH_SOURCE, header))
-    if not force and TORCH_PATH.exists() and TORCH_PATH.stat().st_mtime >= newest:
-        return TORCH_PATH
-    tmp = TORCH_PATH.with_suffix(".so.tmp")
+    out = torch_path()
+    if not force and out.exists() and out.stat().st_mtime >= newest:
+        return out
+    tmp = scratch(out)
     cmd = torch_command(tmp)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         print(" ".join(cmd))
         print(res.stderr[-20000:])
-        raise RuntimeError(f"g++ failed ({res.returncode}) building {TORCH_PATH.name}")
-    tmp.replace(TORCH_PATH)
-    return TORCH_PATH
+        tmp.unlink(missing_ok=True)
+        raise RuntimeError(f"g++ failed ({res.returncode}) building {out.name}")
+    tmp.replace(out)
+    return out
 
 
 if __name__ == "__main__":
