@@ -525,8 +525,8 @@ typedef struct qg_kv_pages {
  * rope unused) or a multiple of 16 up to head_dim.  All in fp32, rounded once: queries
  * to q_out (same type as q; may be q itself), keys and values to slot slots[t] (NULL: the
  * position) of sequence seqs[t] (NULL: t).  positions[t] < 0 marks a padding row: its
- * q_out is zero, nothing is appended, slots[t] and seqs[t] are not read.  slots[t] < 0
- * appends nothing.  A position past the table sets QG_ERR_POSITION and gives a padding
+ * q_out is zero, nothing is appended, whatever slots[t] and seqs[t] are (every array has an
+ * entry for every token).  slots[t] < 0 appends nothing.  A position past the table sets QG_ERR_POSITION and gives a padding
  * row.  Two tokens of one call must not name the same slot.
  * n_q_heads + 2 * n_kv_heads is at most 65535.
  * q, k, v: heads of a token are contiguous, token t starts at t * {q,k,v}_stride elements
@@ -562,8 +562,10 @@ cudaError_t qg_qk_norm_rope_append(const qg_kv_pages* cache, const qg_append* a,
  *   weight_out[b][kv][j] = weight_in[b][kv][j] + sum_h exp(s_hj - m_h) / l_h
  * for every j < lens[b] (unseen slots: weight_in alone), rows of weight_stride floats;
  * weight_in may be weight_out, or NULL for zero; slots at or past lens[b] are left alone.
- * Scores, statistics and sums are fp32; results are deterministic.  The cache's strides
- * have to nest, as they do in every dense or padded layout: slot_stride and head_stride, the
+ * Scores, statistics and sums are fp32; results are deterministic.  Queries enter the products
+ * as sums of two 16-bit terms of the cache's type (22 bits over fp16, 16 over bf16), fp32
+ * queries over bf16 as three (24 bits), and probabilities alike.  The cache's strides
+ * have to nest, as they do in every dense layout: slot_stride and head_stride, the
  * smaller at least head_dim, one a multiple of the other, page_stride a multiple of both and
  * below 2^39 (strides of a dimension of one entry are not looked at).  q, out:
  * [batch][n_q_heads][head_dim] with sequence strides in elements (multiples of 16 bytes);
@@ -605,7 +607,8 @@ cudaError_t qg_paged_attn(const qg_kv_pages* cache, const qg_attn* a, void* work
  * distinct from every page that the call reads.  NULL moves within the old pages (the
  * freed pages are the tail of each row); no page may then belong to two sequences.
  * weight_out may be weight, lens_out lens.
- * lens[b] at most max_len; weight rows of weight_stride floats. */
+ * lens[b] at most max_len, for which the work is sized: one near the longest length is the
+ * fastest; weight rows of weight_stride floats. */
 typedef struct qg_evict {
   const int32_t* lens;
   int32_t* lens_out;

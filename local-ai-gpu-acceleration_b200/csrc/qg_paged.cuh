@@ -15,7 +15,8 @@ namespace qg {
 
 constexpr uint32_t kMaxPagedDim = 256;
 
-// n / d for n < 2^31, d >= 1: q = (umulhi(n, mul) + n) >> shift.
+// n / d for n < 2^31, d >= 1, by a multiplication (Granlund and Montgomery, Division by Invariant
+// Integers using Multiplication, 1994): q = (umulhi(n, mul) + n) >> shift.
 struct FastDiv {
   uint32_t d, mul, shift;
 };

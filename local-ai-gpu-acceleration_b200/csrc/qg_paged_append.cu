@@ -11,7 +11,7 @@
 // Bound by memory: a value is read once and written once for ~7 flops.  A warp's task is one
 // batch of query, key or value rows of one token; it asks for all of it before it looks up
 // where the token goes, so 2 KB are in flight behind one latency and no warp waits for another.
-// 16384 tokens of 64/8 heads x 128 bf16: 131 us, 5.1 TB/s of the bytes that have to move, 80%
+// 16384 tokens of 64/8 heads x 128 bf16: 132 us, 5.1 TB/s of the bytes that have to move, 80%
 // of a plain copy's rate; issue and latency share the rest (24 warps an SM).
 #include "qg_paged.cuh"
 

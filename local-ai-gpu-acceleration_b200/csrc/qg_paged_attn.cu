@@ -6,8 +6,9 @@
 //   m' = max(m, s),  l' = l 2^(m - m') + 2^(s - m'),  o' = o 2^(m - m') + 2^(s - m') v;
 // two passes over disjoint slots join by the same rule, so a sequence is cut anywhere.
 //
-// Bound by memory: a slot's K and V rows are read once for all query heads of their kv head,
-// at 1 to 16 multiply-adds a byte.  The dot products still go to the matrix pipe, because on
+// Bound by memory: a slot's K and V rows are read once for every 8 or 16 query heads of their kv
+// head (16 where more than 8 share it: at head size 64, and at 128 but for fp32 queries over
+// bf16), at half a multiply-add a byte for one query head, 8 for 16.  The dot products still go to the matrix pipe, because on
 // the CUDA cores a group of 8 heads would need 8 fp32 FMAs and conversions for every 2 bytes.
 // mma.sync (m16n8k16) keeps scores, probabilities and sums in the registers of the warp that
 // loads the slots; its rate is far above the few per cent that the memory can feed, so
@@ -34,7 +35,7 @@
 // x 112: 17 and 9 us.
 //
 // Measured (B200, 6.46 TB/s for a plain copy; time on the GPU, floor = bytes that have to move
-// at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 336 us (floor 332); 1 x 131072: 93 us
+// at that rate): 16 x 32768 slots, 64/8 heads x 128 fp16: 338 us (floor 332); 1 x 131072: 94 us
 // (83; the join of 37 records a head is 7 of them); 32 x 1..8191 bf16 with weights: 36 us (21);
 // 64 x ..4097, 16/16 heads x 64, window 2000, pages of 24: 79 us (70); 1 x 511: 10 us, all
 // latency.  Per-lane asynchronous copies in the place of TMA boxes took 439 us for the first,
@@ -209,7 +210,10 @@ struct AttnShape {
   // CTAs an SM.  Small heads do the most work a byte and fit three in registers: 64 x ..4097
   // (16/16 heads x 64) 84 us with two, 79 with three.  At 128 three CTAs of 168 registers are
   // 2-7% faster where many segments run (256 x 300: 65 and 60 us) and 5-15% slower where few
-  // do (1 x 8192: 17.7 and 20.3, 1 x 131072: 92.6 and 97.1 us), so it keeps two.
+  // do (1 x 8192: 17.7 and 20.3, 1 x 131072: 92.6 and 97.1 us), so it keeps two.  Both sizes then
+  // hold a head tile without spills.  The wider forms do spill, bytes of stores: two tiles at 128
+  // 364; 256 104; fp32 over bf16 64 (64), two tiles at 64 216, 128 180, 256 482.  8 x 16384 slots,
+  // us (floor): 64/4 heads x 128 64 (42), 32/4 x 256 fp16 98 (83), fp32 over bf16 108 (83).
   static constexpr int kCtasPerSm = DP == 64 && MT == 1 ? 3 : 2;
   static constexpr uint32_t kUnits = DP != 64 ? 3 : kCtasPerSm == 3 ? 4 : 6;  // of its ring
   static constexpr uint32_t kRing = kWarps * kUnits * kUnit;
@@ -218,9 +222,14 @@ struct AttnShape {
   static constexpr uint32_t kSmem = kRing + kQBytes + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kPanels = DP / 64u;             // 128-byte column panels of a row
   static constexpr uint32_t kRecord = kHeads * (DP + 2u);   // m[], l[], o[][]
-  // What a segment costs beside its blocks, in blocks: queries in, sums out, joins.  Measured
-  // at 1, 2 and 3: 32 x ..8191 (head size 128) 38.5, 36.4 and 35.3 us, 62 x ..752 (256) 53, 58
-  // and 62 us; head size 64 at 2, 3 and 4: 88.8, 90.0 and 90.5 us.
+  // What a segment costs beside its blocks, in blocks: queries in, sums out, joins.  No value is
+  // the best for all lengths; us at
+  //   head size 64, 1 to 4: 64 x ..4097 (16/16 heads, window 2000) 78.9, 79.5, 80.8 and 78.2;
+  //     100 x 10..2000 (32/8) 27.0, 26.7, 27.5 and 28.4; 32 x 100..8191 34.3, 33.6, 32.5 and 31.3;
+  //   128, 1 to 4: 32 x ..8191 (32/8) 35.3, 33.2, 32.0 and 32.3; 100 x 10..2000 38.4, 39.7, 42.9
+  //     and 46.0; 48 x 200..6000 (40/8) 64.6, 64.4, 64.1 and 63.9;
+  //   256, 0 to 3: 62 x ..752 (16/4) 21.0, 19.1, 20.0 and 19.3; 32 x ..8191 (16/2) 33.3, 28.3, 27.5
+  //     and 26.7; 100 x 10..2000 (8/2) 30.8, 26.6, 25.5 and 25.0.
   static constexpr uint32_t kHeader = DP == 64 ? 2 : DP == 128 ? 3 : 1;
   // Whether a lone warp may take whole segments (below): where the code for it costs the rest
   // little (1%).  At head size 256 and with two tiles of heads it cost 5-10%, at 64, whose three

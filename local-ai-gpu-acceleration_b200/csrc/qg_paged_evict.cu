@@ -18,10 +18,12 @@
 //    such order: whole rows, split over CTAs.  Bound by memory: the kept rows once in and
 //    once out.
 //
-// Measured (B200, time on the GPU, floor = weights in, kept rows in and out at 6.46 TB/s):
-// 8 x 32768 slots to 8192, 8 heads x 128 fp16: 113 us (floor 86; selection 22, move 90);
-// 16 x 700..9001 to 1500, 8 heads x 80 bf16: 41 us (18; selection 18, latency of its 12 barriers);
-// 1 x 2500 to 2048: 13 us.
+// Measured (B200, time on the GPU, floor = weights in, kept rows in and out at 6.46 TB/s), into
+// other pages and in place:
+// 8 x 32768 slots to 8192, 8 heads x 128 fp16: 113 and 147 us (floor 86; selection 22, move 90);
+// 16 x 700..9001 to 1500, 8 heads x 80 bf16: 42 and 43 us (18; selection 18, latency of its 12
+// barriers); 1 x 2500 to 2048: 12.5 and 21 us; 1 x 131072 to 65536, 8 heads x 128: 119 and 506 us
+// (85): in place it is 32 CTAs, one for each head and 64-byte slice, whatever the length.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -367,11 +369,14 @@ extern "C" cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, 
       select_attr.set(reinterpret_cast<const void*>(evict_select_kernel<kManyThreads>), kCachedKeys * 4u);
   if (err != cudaSuccess) return err;
   const uint64_t lines = static_cast<uint64_t>(c.n_kv) * c.batch, sms = static_cast<uint64_t>(paged_sm_count());
-  // Few threads for short lines, and up to twice that where the lines do not fit on the SMs at
-  // once.  Whole call with 1024 and 256 threads, head size 128 (112 in the first), us: 37 x 26..45
+  // The lengths are on the device, so max_len stands for them.  Few threads for short lines, and up
+  // to twice that where the lines do not fit on the SMs at once.  Whole call with 1024 and 256
+  // threads, max_len the longest length, head size 128 (112 in the first), us: 37 x 26..45
   // slots of 16 heads 27.8 and 11.7, of 8 heads: 16 x 1000 20.7 and 15.4, 64 x 2048 75.2 and 61.1,
   // 1 x 1000 11.5 and 11.8.  Past the rule: 1 x 2000 12.5 and 17.0, 20 x 3096..4096 35 and 39,
   // 40 x 100..8000 44 and 61; only where all are long and many it would gain (64 x 4096 82 and 70).
+  // A max_len far above the lengths costs the form for long lines and their tail of zeros: in
+  // place with 131072 in the place of the longest, 64 x 576 to 512 130 us (59), 1 x 2500 37 (21).
   const bool few = e->max_len < kShort || (e->max_len <= 2u * kShort && lines > sms);
   const uint32_t threads = few ? kFewThreads : kManyThreads;
   // CTAs of a selection: while SMs are free and a stretch keeps two slots a thread

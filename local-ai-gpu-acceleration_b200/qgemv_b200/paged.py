@@ -8,7 +8,8 @@
 * `AttentionPlan`, `attend` -- one new token per sequence attends to its sequence's slots.
 * `evict` -- sequences are cut back to a budget of slots by the weight that `attend` summed.
 
-Device memory and streams only; every computation happens in the library.  Every call takes
+Device memory and streams only; every computation happens in the library.  Inference only: no
+call records a gradient, whatever its tensors require.  Every call takes
 `stream` (default: the current one) and allocates what it returns on that stream, unless the
 caller passes the output; tensors of other streams are the caller's to order.  Tensors that do
 not fit raise ValueError (they are checked in csrc/qg_paged_torch.cpp: on small batches a call
@@ -154,7 +155,9 @@ def evict(cache: PagedCache, lens: torch.Tensor, weight: torch.Tensor, budget: i
     the last `recent`, and the heaviest between them by weight [sequences, kv heads, >= longest
     length].  Rows move to the front of the same pages, lens and weight are updated; or, with
     new_table [sequences, pages], to those pages, the new weights to weight_out (needed then; it
-    may be weight) and lens left as it is.  Returns (kept [sequences, kv heads, budget], new lens)."""
+    may be weight) and lens left as it is.  The work is sized for the rows of weight, so rows not
+    much wider than the longest length are the fastest; into other pages takes less time than in
+    place.  Returns (kept [sequences, kv heads, budget], new lens)."""
     code, kept, lens_out = cache.calls.evict(cache.held, lens, weight, budget, sink, recent, new_table, lens_out,
                                              weight_out, kept, None if stream is None else stream.cuda_stream)
     if code != 0:
