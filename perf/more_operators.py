@@ -299,10 +299,10 @@ def _places(table, at, page):
 # --------------------------------------------------------------------------- plain form
 
 def _power(top):
-    """The least power of two, of 2^-90 at least, whose product with e4m3's largest value is `top` or more."""
+    """The least power of two, between 2^-60 and 2^60, whose product with e4m3's largest value is `top` or more."""
     part, exponent = torch.frexp(top)
     e = torch.where(part <= 0.875, exponent - 9, exponent - 8)
-    e = torch.where(top > 0, e.clamp(-90, 120), -90)
+    e = torch.where(top > 0, e.clamp(-60, 60), -60)
     return ((e.int() + 127) << 23).view(torch.float32)
 
 
@@ -528,7 +528,7 @@ def _exact_append(case, st):
                 fill = min(block - at % block, p + n - slot)
                 x, base = rows[row: row + fill].transpose(0, 1), at // block * block
                 need = torch.exp2(torch.ceil(torch.log2(x.abs().amax((1, 2)) / TOP)))
-                need = need.clamp(2.0 ** -90, 2.0 ** 120)
+                need = need.clamp(2.0 ** -60, 2.0 ** 60)
                 if at % block:
                     need = torch.maximum(need, scale[id_, :, at // block])
                     held = pool[id_, :, base: base + block] * (scale[id_, :, at // block] / need)[:, None, None]
