@@ -450,9 +450,12 @@ def _cache(st):
 
 def _own_append(st):
     paged8, cache = _cache(st)
+    if "q_out" not in st:  # rows of no sequence are left as they are
+        st["q_out"] = torch.zeros_like(st["q_new"], memory_format=torch.contiguous_format)
     q = paged8.qk_norm_rope_append(
         cache, st["q_new"], st["k_new"], st["v_new"], st["rope"], st["positions"], st["lens"],
-        offsets=st["offsets"], q_norm=st["q_norm"], k_norm=st["k_norm"], eps=EPS, pairs=st["case"]["pairs"])
+        offsets=st["offsets"], q_norm=st["q_norm"], k_norm=st["k_norm"], eps=EPS, pairs=st["case"]["pairs"],
+        q_out=st["q_out"])
     return {"q": q, "k": st["k"], "v": st["v"], "k_scale": st["k_scale"], "v_scale": st["v_scale"]}
 
 
