@@ -53,14 +53,11 @@
 // fp32's exponents: it needs no factor, and values above 2^114 could not bear one.
 // Each tile's P V is accumulated from zero and added to o in fp32 on the CUDA cores: o lives for
 // thousands of tiles, and how the matrix pipe rounds a running sum is not specified.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <math_constants.h>
 
 #include <algorithm>
-#include <type_traits>
 
-#include "qg_paged.cuh"
+#include "qg_mma.cuh"
 
 namespace qg {
 namespace {
@@ -104,75 +101,6 @@ struct AttnMaps {
   CUtensorMap k, v;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// One box of a pool's tensor map (a kernel parameter) into shared memory, completing on `bar`.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
-                                            int32_t page, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(page), "r"(bar), "l"(policy)
-      : "memory");
-}
-
-// True in one lane of the (whole) warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(is));
-  return is != 0u;
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
-               : "memory");
-}
-
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1, __half) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                    uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// (x, y) as TERMS pairs of the 16-bit type whose sum is (x, y) to 11 (8) bits a term.
-template <typename T, int N>
-__device__ __forceinline__ void split_terms(float x, float y, uint32_t (&term)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    term[i] = pack2(x, y, T());
-    const float2 f = unpack2(term[i], T());
-    x -= f.x;
-    y -= f.y;
-  }
-}
-
 // The power p with top in [2^p, 2^(p + 1)), kept where both 2^p and 2^-p are normal numbers.  For
 // bf16 it is 10 more, less where that would pass 116 (the scale times 2^p has to stay finite).
 template <typename T>
@@ -181,10 +109,6 @@ __device__ __forceinline__ int power_of(float top) {
   const int p = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
   return top == 0.f ? 0 : min(p + kRoom, max(p, 126 - kRoom));
 }
-__device__ __forceinline__ float power_of_two(int power) {
-  return __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
-}
-
 // One (sequence, kv head x head tile) of the line: its seen slots [start, len) are steps
 // [j0, j1) of 2^log slots; j is the next one.
 struct Segment {
@@ -1040,19 +964,6 @@ bool plan_attn(const PagedView& c, uint32_t n_q, uint32_t max_len, bool weights,
   p->norm_at = round_up(p->scores_at + (weights ? static_cast<size_t>(c.batch) * n_q * stride * 4u : 0u));
   p->bytes = round_up(p->norm_at + (weights ? static_cast<size_t>(c.batch) * n_q * 4u : 0u));
   return true;
-}
-
-// cuTensorMapEncodeTiled from the driver (looked up once; no link-time dependency on libcuda).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    const bool found = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
-                                                        &q) == cudaSuccess &&
-                       q == cudaDriverEntryPointSuccess;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(found ? p : nullptr);
-  }();
-  return fn;
 }
 
 // Strides of a tensor map nest: each is a multiple of the one inside it (a dimension of one
