@@ -622,6 +622,116 @@ typedef struct qg_evict {
 cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged key-value cache in 8 bits.  Keys and values are e4m3 codes (1 sign, 4 exponent, 3
+ * mantissa bits, largest value 448, no infinities); every block of `block` consecutive slots of
+ * a page has one fp32 scale per kv head for its keys and one for its values, and a code c stands
+ * for c times its block's scale.  Half the bytes of the 16-bit cache.  Three operators:
+ *   qg_qk_norm_rope_append8  the 16-bit append's norm and rotation, keys and values quantised
+ *                            into their blocks;
+ *   qg_kv_read8              rows of the cache as the values that they stand for;
+ *   qg_paged_attn8           the new tokens of every sequence, one or many, attend to its slots.
+ *
+ * Pools, pages and the table are those of qg_kv_pages, strides in bytes (= codes) and multiples
+ * of 16; head_dim a multiple of 16 up to 256; `block` is 16, 32, 64 or 128 and divides page_size.
+ * The scale of (page, head, block i of the page) is at page * scale_page_stride +
+ * head * scale_head_stride + i of k_scale and v_scale.  Scales of blocks that hold slots of a
+ * sequence lie between 2^-60 and 2^60, so the cache holds magnitudes up to 5e20 in steps down to
+ * 1.7e-21; the append's are powers of two, the readers take any (qg_paged_attn8 takes a scale of
+ * values outside that range as its end).
+ *
+ * New rows.  A call has `tokens` rows, sequence after sequence: rows offsets[b] to
+ * offsets[b + 1] - 1 ([batch + 1], ascending) are the new tokens of sequence b, rows before
+ * offsets[0] and from offsets[batch] on belong to none and are left alone, in and out.  NULL: one row a sequence, row
+ * b of sequence b (tokens at most batch).  lens[b] counts the sequence's slots with its new
+ * tokens, which are the last of them: with n rows, row i has slot lens[b] - n + i.  A sequence
+ * with lens[b] <= 0 is padding.  Data that does not fit (an offset outside [0, tokens] or below
+ * the one before it, more new tokens than slots, a length past the table, a page id outside the
+ * pool) sets QG_ERR_PAGE and never leads to an access outside.
+ * ------------------------------------------------------------------------- */
+typedef struct qg_kv_pages8 {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  uint32_t num_pages, page_size, n_kv_heads, head_dim, block;
+  uint64_t page_stride, head_stride, slot_stride;
+  uint64_t scale_page_stride, scale_head_stride;
+  const int32_t* table;      /* [batch][table_stride] page ids */
+  uint32_t batch, table_pages, table_stride;
+} qg_kv_pages8;
+
+/* Norm and rotation of qg_qk_norm_rope_append (same formulas, tables and pairs, fp32), queries
+ * rounded once to q_out.  Then, for each block that receives rows and each kv head, K and V apart:
+ *   a = max |x| over the finite new values x,  e = the least integer with a <= 448 * 2^e, within
+ *   [-60, 60];  s = max(2^e, the block's scale) where the block holds earlier slots of the
+ *   sequence, 2^e where its first slot is new;
+ *   new codes e4m3(x / s), to nearest even, at most +-448 (infinities too; NaN stays
+ *   NaN);
+ *   where the scale grew, the block's other codes become e4m3(c * old scale / s): what they stand
+ *   for stays.
+ * Growth by a power of two is exact but for codes that leave e4m3's normal range, so a sequence
+ * appended token by token holds what one call would have written, to within 2^-8 s, 2e-5 of
+ * the block's largest value.
+ * positions[t] < 0 (of padding), or past the table (QG_ERR_POSITION): the row's q_out is zero, and
+ * its key and value, where it has a slot, are zeros.  No two sequences may write to one page. */
+typedef struct qg_append8 {
+  const void *q, *k, *v;
+  void* q_out;
+  int dtype;                 /* of q, k, v and q_out: QG_F32, QG_F16 or QG_BF16 */
+  uint32_t tokens, n_q_heads;
+  uint64_t q_stride, k_stride, v_stride, q_out_stride;
+  const float *q_norm, *k_norm;
+  float eps;
+  const float* rope;
+  uint32_t rope_rows, rot_dim;
+  int pairs;
+  const int32_t *positions, *lens, *offsets;
+} qg_append8;
+cudaError_t qg_qk_norm_rope_append8(const qg_kv_pages8* cache, const qg_append8* a, cudaStream_t stream);
+
+/* Rows of the cache as values: row offsets[b] + i of k_out and v_out ([tokens][n_kv_heads]
+ * [head_dim], dtype) receives slot starts[b] + i of sequence b, code times scale in fp32, rounded
+ * once.  offsets as above, never NULL; rows of no sequence are left alone; a slot outside the table or
+ * in a page outside the pool gives a zero row and QG_ERR_PAGE.  Strides from row to row in
+ * elements, multiples of 16 bytes; 16-B aligned. */
+typedef struct qg_read8 {
+  const int32_t *starts, *offsets;
+  uint32_t tokens;
+  void *k_out, *v_out;
+  int dtype;
+  uint64_t k_stride, v_stride;
+} qg_read8;
+cudaError_t qg_kv_read8(const qg_kv_pages8* cache, const qg_read8* r, cudaStream_t stream);
+
+/* Attention of new tokens over the cache that already holds them.  The token of slot p sees the
+ * slots j <= p of its sequence with window == 0, j > p - window or j < sink: all before it, or the
+ * last `window` and the first `sink`.  For query head h of kv head h / (n_q_heads / n_kv_heads)
+ * out = softmax over the seen slots of (scale * q . k_j) times v_j, lse the log of the softmax's
+ * sum, as in qg_paged_attn; out 0 and lse -inf where nothing is seen (rows of an empty sequence).
+ * What a token does not see never reaches its row, whatever the codes and scales there; a NaN
+ * code among the seen makes the row (key) or the column (value) NaN.
+ * q, out: [tokens][n_q_heads][head_dim] with row strides in elements (multiples of 16 bytes),
+ * 16-B aligned; lse [tokens][n_q_heads] or NULL; rows of no sequence are left alone.
+ * fp32 queries enter the products as sums of two fp16 terms (22 bits) and so do probabilities; 16-bit
+ * queries exactly, or as far as 2^-25 of their row's largest value, and probabilities, where a call has
+ * more than 8 rows for a kv head, in fp16 (11 bits).  Statistics and sums are fp32; results are
+ * deterministic.  The pools' strides nest as in qg_paged_attn.  `workspace` as there:
+ * qg_paged_attn8_workspace_bytes long for the same cache, heads and at least as many tokens, its
+ * first QG_PAGED_ATTN_ZEROED bytes zero before its first use; calls that overlap need one each. */
+typedef struct qg_attn8 {
+  const void* q;
+  void* out;
+  int dtype;                 /* of q and out */
+  uint32_t tokens, n_q_heads;
+  uint64_t q_stride, out_stride;
+  const int32_t *lens, *offsets;
+  uint32_t window, sink;
+  float scale;
+  float* lse;
+} qg_attn8;
+cudaError_t qg_paged_attn8_workspace_bytes(const qg_kv_pages8* cache, uint32_t n_q_heads, uint32_t tokens,
+                                           size_t* bytes);
+cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8* a, void* workspace, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * GGUF ingest (host code; the reference's reader is runtime/apps/gguf_probe/main.cpp:124-631):
  * header, metadata (general.alignment, general.architecture), tensor infos, the data
  * section offset, tensor spans and the probe's validation (supported ggml type, block-

@@ -95,6 +95,10 @@ SIGNATURES: dict[str, list] = {
     "qg_paged_attn_workspace_bytes": [P, U32, U32, c_int, P],
     "qg_paged_attn": [P, P, P, P],
     "qg_kv_evict": [P, P, P],
+    "qg_qk_norm_rope_append8": [P, P, P],
+    "qg_kv_read8": [P, P, P],
+    "qg_paged_attn8_workspace_bytes": [P, U32, U32, P],
+    "qg_paged_attn8": [P, P, P, P],
     "qg_gguf_open": [ctypes.c_char_p, P],
     "qg_gguf_summary": [P, P],
     "qg_gguf_tensor": [P, U64, P],

@@ -46,6 +46,8 @@ def _calls():
         handle = lib()
         module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             handle.qg_qk_norm_rope_append, handle.qg_paged_attn, handle.qg_kv_evict)))
+        module.bind8(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            handle.qg_qk_norm_rope_append8, handle.qg_kv_read8, handle.qg_paged_attn8)))
         _CALLS = module
     return _CALLS
 
