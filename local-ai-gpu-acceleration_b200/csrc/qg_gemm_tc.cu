@@ -57,6 +57,7 @@
 
 #include "qg_formats.cuh"
 #include "qg_host.h"
+#include "qg_umma.cuh"
 
 namespace qg {
 namespace {
@@ -84,7 +85,6 @@ constexpr uint32_t kSmemLimit = 232448;  // 227 KB: the opt-in maximum per block
 constexpr uint32_t kMaxRawStages = 8;
 constexpr uint32_t kMaxTcPolls = 4000;   // bounded waits: suspended polls of up to kPollNs
 constexpr uint32_t kMaxSpinPolls = 1u << 26;  // bounded spin of the MMA thread (~1 s)
-constexpr uint32_t kPollNs = 500000;
 
 template <int FMT>
 struct TcFmt;
@@ -136,7 +136,7 @@ struct TcLayout {
 };
 
 // ---------------------------------------------------------------------------
-// tcgen05 / UMMA primitives (PTX ISA 8.7, sm_100a).
+// Operand descriptors.
 
 // Shared-memory matrix descriptor, K-major without swizzle: core matrices of 8 rows x
 // 16 bytes stored contiguously; the two core matrices along K (one K=16 step) are
@@ -153,76 +153,6 @@ __host__ __device__ constexpr uint32_t umma_idesc() {
   return (1u << 4) | ((NB >> 3) << 17) | ((kTileM >> 4) << 24);
 }
 
-// D (tensor memory) (+)= A (shared-memory descriptor) x B (shared-memory descriptor).
-__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
-      : "memory");
-}
-
-// D (tensor memory) (+)= A (tensor memory: row m = lane m, fp16 element k in column
-// k/2) x B (shared-memory descriptor).
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u),
-      "r"(0u)
-      : "memory");
-}
-
-// Arrive on `bar` once every tcgen05 operation this thread issued so far has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-// 32 lanes x 16 consecutive 32-bit columns: thread i of the warp gets its lane's 16.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Thread i of the warp writes 16 consecutive 32-bit columns of its lane.
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&w)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
-      "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
 // 2-D tiled tensor copy global -> shared of the box at (x, y) of `tmap` (a kernel
 // parameter), completing on `bar`; plain form, the source is this GPU's memory.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tmap, int32_t x, int32_t y,
@@ -232,20 +162,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tmap, 
       " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(smem_addr(bar)), "l"(policy)
       : "memory");
-}
-
-// try_wait that suspends the thread (up to kPollNs) until the phase completes, so
-// waiting warps do not take issue slots from the working ones.
-__device__ __forceinline__ bool mbar_try_wait_sleep(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity), "r"(kPollNs)
-      : "memory");
-  return ok != 0u;
 }
 
 // Bounded wait of at most kMaxTcPolls suspended polls; gives up early once another
@@ -265,18 +181,6 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
 // cost hundreds under load (measured on B200: Q4_K 28672x8192 at batch 16 takes 79.5 us
 // with this spin, 88 us with suspending try_waits).  Up to three phases at once (b1 may
 // be null): the polls are independent, so their latencies overlap.
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return ok != 0u;
-}
-
 __device__ __forceinline__ bool tc_spin3(uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2, uint64_t* b3,
                                          uint32_t p3, volatile uint32_t* abort) {
   bool ok1 = b1 == nullptr, ok2 = false, ok3 = false;
@@ -649,11 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
     fence_mbar_init();
   }
   if (warp == 1u) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(tmem_slot)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc_all(tmem_slot);
   }
   if constexpr (F::window) {
     if (warp >= kDequantWarp0) build_tables<FMT>(sT, tid - 64u, kThreads - 64u);
@@ -921,8 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
   __syncthreads();
   if (warp == 1u) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols)
-                 : "memory");
+    tmem_free_all(tmem);
   }
 }
 

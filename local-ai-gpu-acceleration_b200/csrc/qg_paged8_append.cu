@@ -186,9 +186,11 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
       float ss = (s.x + s.y) + (z.x + z.y);
 #pragma unroll
       for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off, LPR);
-      // one Newton step on the fast root: an error here moves every code of the row near a border
+      // one Newton step on the fast root: an error here moves every code of the row near a border.
+      // (Its step is below 2^-20; the bound keeps roots of 0 and infinity.)
       const float mean = fmaf(ss, a.inv_dim, a.eps), fast = rsqrtf(mean);
-      const float inv = fmaf(0.5f * fast, fmaf(-mean * fast, fast, 1.f), fast);
+      const float step = fmaxf(fminf(fmaf(-mean * fast, fast, 1.f), 0x1p-20f), -0x1p-20f);
+      const float inv = fmaf(0.5f * fast, step, fast);
       const F2 by = f2(inv, inv);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {

@@ -118,21 +118,16 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   // the segment (s.item, s.line); `fresh`: the item is another one than before
   auto make = [&](Segment8& s, bool fresh) {
     if (ragged) {
-      if (fresh) {
-        const uint4 it = a.items[s.item];
-        s.b = it.x, s.token = it.y, s.p0 = static_cast<int32_t>(it.z);
-        s.sub = it.w & 0xffffu, s.rows = it.w >> 16;
-      }
-      s.kv = s.line;
-    } else {
-      if (fresh) {
-        s.b = s.token = s.item;
-        s.p0 = static_cast<int32_t>(paged_len(a.lens[s.b], c.capacity)) - 1;
-      }
-      s.kv = s.line / a.tiles;
-      s.sub = (s.line - s.kv * a.tiles) * kRows;
-      s.rows = min(kRows, a.group.d - s.sub);
+      take_item8(a, s, fresh, kLogBlock);
+      return;
     }
+    if (fresh) {
+      s.b = s.token = s.item;
+      s.p0 = static_cast<int32_t>(paged_len(a.lens[s.b], c.capacity)) - 1;
+    }
+    s.kv = s.line / a.tiles;
+    s.sub = (s.line - s.kv * a.tiles) * kRows;
+    s.rows = min(kRows, a.group.d - s.sub);
     s.bounds(a, kLogBlock);
     s.j = 0u;
   };
@@ -156,19 +151,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   if (ragged) {
     const uint32_t n = *a.item_count;
     if (n == 0u || !cut(a.item_blocks[n] * lines, static_cast<uint64_t>(n) * lines)) return;
-    auto before = [&](uint32_t i) { return (a.item_blocks[i] + static_cast<uint64_t>(header) * i) * lines; };
-    uint32_t lo = 0, hi = n;  // the item lies in [lo, hi)
-    while (hi - lo > 1u) {
-      const uint32_t step = (hi - lo + 31u) / 32u, at = lo + lane * step;
-      const uint32_t ok = __ballot_sync(0xffffffffu, at < hi && before(at) <= r0);
-      lo += (31u - __clz(ok)) * step;
-      hi = min(hi, lo + step);
-    }
-    const uint64_t in = r0 - before(lo);
-    const uint64_t units = (before(lo + 1u) - before(lo)) / lines;
-    use.item = lo;
-    use.line = static_cast<uint32_t>(in / units);
-    in_segment = static_cast<uint32_t>(in % units);
+    find_unit8(a, n, lines, header, r0, use.item, use.line, in_segment);
   } else {
     auto blocks_of = [&](uint32_t b) {
       Segment8 s;
@@ -886,7 +869,7 @@ constexpr size_t round_up8(size_t v) { return (v + 255u) & ~static_cast<size_t>(
 
 struct Plan8 {
   uint32_t dp, rs;
-  size_t records_at, count_at, items_at, blocks_at, seqs_at, bytes;
+  size_t records_at, count_at, items_at, blocks_at, seqs_at, prompt_at, bytes;
   uint32_t max_items;
 };
 
@@ -903,7 +886,8 @@ bool plan_attn8(const Paged8View& c, uint32_t n_q, uint32_t tokens, Plan8* p) {
   p->items_at = p->count_at + 256u;
   p->blocks_at = round_up8(p->items_at + items * 16u);
   p->seqs_at = round_up8(p->blocks_at + (items + 1u) * 8u);
-  p->bytes = round_up8(p->seqs_at + (c.c.batch + 1u) * 4u);
+  p->prompt_at = round_up8(p->seqs_at + (c.c.batch + 1u) * 4u);
+  p->bytes = p->prompt_at + (prompt8_fits(p->dp, tokens, c.c.batch, group) ? prompt8_bytes(p->dp) : 0u);
   return true;
 }
 
@@ -1030,6 +1014,10 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
   }
   a.log_boxes = kLogTile - log_box;
   a.heads_inside = strides.heads_inside;
+  if (p->offsets != nullptr && p->dtype != QG_F32 && prompt8_fits(plan.dp, p->tokens, cache->batch, a.group.d)) {
+    a.records = reinterpret_cast<float*>(ws + plan.prompt_at);
+    return launch_prompt8(c, a, plan.dp, stream);
+  }
   // rows of a kv head: a call of one row a sequence has its group
   const bool few = p->offsets == nullptr && a.group.d <= 8u;
   const bool wide = p->dtype == QG_F32;

@@ -70,9 +70,52 @@ __device__ __forceinline__ bool sees(const Attn8Args& a, int32_t p, uint32_t j) 
   return static_cast<int32_t>(j) <= p && (a.window == 0u || static_cast<uint32_t>(p) - j < a.window || j < a.sink);
 }
 
+// Where unit r0 of a ragged call's line lies: the line is the blocks of all segments, `header` units before
+// each segment's, `lines` segments a tile.  A whole warp takes part.
+__device__ __forceinline__ void find_unit8(const Attn8Args& a, uint32_t n, uint32_t lines, uint32_t header, uint64_t r0,
+                                           uint32_t& item, uint32_t& line, uint32_t& in_segment) {
+  auto before = [&](uint32_t i) { return (a.item_blocks[i] + static_cast<uint64_t>(header) * i) * lines; };
+  uint32_t lo = 0, hi = n;  // the tile lies in [lo, hi)
+  while (hi - lo > 1u) {
+    const uint32_t step = (hi - lo + 31u) / 32u, at = lo + (threadIdx.x & 31u) * step;
+    const uint32_t ok = __ballot_sync(0xffffffffu, at < hi && before(at) <= r0);
+    lo += (31u - __clz(ok)) * step;
+    hi = min(hi, lo + step);
+  }
+  const uint64_t in = r0 - before(lo), units = (before(lo + 1u) - before(lo)) / lines;
+  item = lo;
+  line = static_cast<uint32_t>(in / units);
+  in_segment = static_cast<uint32_t>(in % units);
+}
+// A tile of a ragged call and one of its kv heads.
+__device__ __forceinline__ void take_item8(const Attn8Args& a, Segment8& s, bool fresh, uint32_t log) {
+  if (fresh) {
+    const uint4 it = a.items[s.item];
+    s.b = it.x, s.token = it.y, s.p0 = static_cast<int32_t>(it.z);
+    s.sub = it.w & 0xffffu, s.rows = it.w >> 16;
+    s.bounds(a, log);
+  }
+  s.kv = s.line;
+  s.j = 0u;
+}
+
 // The tiles of `rows` rows of a ragged call, and how many blocks of 2^log slots each sees, before
 // the attention reads them.
 cudaError_t launch_plan8(const Paged8View& c, const Attn8Args& a, uint32_t rows, uint32_t log, cudaStream_t stream);
+
+// ---- the kernel for many rows (qg_paged8_prompt.cu)
+constexpr uint32_t kPromptRows = 256;
+constexpr uint32_t kMaxPromptCtas = 148;
+// bytes of its records
+constexpr size_t prompt8_bytes(uint32_t dp) {
+  return static_cast<size_t>(kMaxPromptCtas) * 2u * kPromptRows * (dp + 2u) * 4u;
+}
+// 16-bit queries and heads up to 128 wide, where a sequence has `kPromptFrom` rows or more for a kv head on average.
+constexpr uint32_t kPromptFrom = 64;
+inline bool prompt8_fits(uint32_t dp, uint64_t tokens, uint32_t batch, uint32_t group) {
+  return dp <= 128u && tokens * group >= static_cast<uint64_t>(kPromptFrom) * (tokens < batch ? tokens : batch);
+}
+cudaError_t launch_prompt8(const Paged8View& c, const Attn8Args& a, uint32_t dp, cudaStream_t stream);
 
 // Largest number of tiles of `rows` rows: every sequence's last may be ragged.
 inline uint64_t most_tiles(uint64_t tokens, uint32_t batch, uint32_t group, uint32_t rows) {

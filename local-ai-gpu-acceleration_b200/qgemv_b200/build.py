@@ -15,7 +15,7 @@ LIB_PATH = PKG_DIR / "libqgemv_b200.so"
 SOURCES = ["qg_gemv.cu", "qg_aux.cu", "qg_abi.cu", "qg_slice.cu", "qg_attn.cu", "qg_decode.cu",
            "qg_noalloc.cu", "qg_gemm_tc.cu", "qg_gguf.cu", "qg_gemv_batch.cu", "qg_paged_append.cu",
            "qg_paged_attn.cu", "qg_paged_evict.cu", "qg_paged8_append.cu", "qg_paged8_read.cu",
-           "qg_paged8_attn.cu"]
+           "qg_paged8_attn.cu", "qg_paged8_prompt.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

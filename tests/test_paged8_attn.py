@@ -154,6 +154,24 @@ def test_ragged_rows(cuda, q_heads, kv_heads, dim, page, block, order, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page,block,order", SHAPES)
+def test_drafted_tokens(cuda, q_heads, kv_heads, dim, page, block, order, dtype):
+    """A few rows of every sequence."""
+    rng = np.random.default_rng(q_heads * 7 + dim + 2)
+    counts = [int(n) for n in rng.integers(0, 5 if q_heads // kv_heads < 12 else 3, 24)]
+    lens = [n + int(m) for n, m in zip(counts, rng.integers(0, 600, 24))]
+    c = make_cache(rng, 24, 640 // page + 1, page, block, kv_heads, dim, order)
+    poison(c, lens)
+    q = queries(rng, sum(counts), q_heads, dim, DTYPES[dtype])
+    plan = paged8.AttentionPlan8(c, q_heads, max_tokens=sum(counts))
+    for window, sink in ((0, 0), (2, 0), (100, 4), (64, 500)):
+        out, lse = paged8.attend(plan, q, int32(lens), offsets=offsets(counts), window=window, sink=sink, return_lse=True)
+        check(c, q, lens, counts, out, lse, window, sink)
+    assert ops.get_error() == 0 and torch.count_nonzero(plan.workspace[:4096]) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_nan_reaches_only_rows_that_see_it(cuda, dim, dtype):
