@@ -5,8 +5,8 @@
 // A tile is 256 rows (query heads of a kv head, token after token) in two halves of 128, the lanes of
 // tensor memory; a step is 128 slots.  For each half
 //   S = Q C_k^T    both operands fp16 in shared memory, 128 x 128 fp32 in tensor memory
-//   P = 2^(y - M)  one thread a row: it reads its row of S twice (maximum, then powers), writes P as
-//                  fp16 over S
+//   P = 2^(y - M)  one thread a row: it reads its row of S twice (maximum, then powers) and writes P
+//                  as fp16 over S
 //   O += P C_v     P from tensor memory, fp32 sums in tensor memory
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
@@ -40,6 +40,7 @@ constexpr uint32_t kPromptThreads = (kIssueWarp + 1u) * 32u;
 constexpr uint32_t kScaleRing = 4;
 constexpr uint32_t kMaxPolls = 4000;             // of up to kPollNs each
 constexpr float kCarry = 7.f, kSlack = 8.f;      // log2: the factor of powers, the growth of M that is let pass
+constexpr float kLeastFactor = 1e-30f;           // of scores: zero would turn minus infinity into NaN
 constexpr uint32_t kPromptHeader = 2;            // what a segment costs beside its blocks, in blocks
 static_assert(2u * 256u * 4u <= QG_PAGED_ATTN_ZEROED && kMaxPromptCtas <= 256u, "a counter per CTA and half");
 static_assert(kPromptRows == 2u * kHalf, "two halves");
@@ -224,37 +225,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         const int32_t lo = a.window == 0u || hi < 0 || a.window > static_cast<uint32_t>(hi)
                                ? INT32_MIN : hi - static_cast<int32_t>(a.window) + 1;
         const int32_t first = a.sink > slot0 ? static_cast<int32_t>(min(a.sink - slot0, kHalf)) : 0;
-        auto seen = [&](int32_t e) { return e <= hi && (e >= lo || e < first); };
         wait(&s_full[half], steps & 1u);
         wait(&scale_full[ring], (kt / kScaleRing) & 1u);  // long done: S needed the step's codes
         tc_fence_after();
-        // ---- the largest y
-        float top = -CUDART_INF_F;
+        // S comes 32 columns at a time, the next ones while these are worked on; columns that the row does
+        // not see become minus infinity
         uint32_t s[2][32];
-        tmem_ld32(s_at, s[0]);
+        auto mask = [&](uint32_t (&x)[32], int32_t at) {
+          auto low = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // bits [0, n)
+          const uint32_t bits = low(hi + 1 - at) & (low(first - at) | ~(lo <= at ? 0u : low(lo - at)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          tmem_wait_ld();
-          if (i < 3) tmem_ld32(s_at + 32u * (i + 1), s[(i + 1) & 1]);
+          for (int e = 0; e < 32; ++e) {
+            if ((bits >> e & 1u) == 0u) x[e] = 0xff800000u;
+          }
+        };
+        auto over = [&](auto work) {
+          tmem_ld32(s_at, s[0]);
+#pragma unroll 1
+          for (int i = 0; i < 4; i += 2) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 sc = scale[2 * i + g];
-            const float by = mult * sc.x;
-            auto x = [&](int e) { return __uint_as_float(s[i & 1][16 * g + e]); };
-            if (whole) {
-              float u = max3(x(0), x(1), x(2)), v = max3(x(3), x(4), x(5));
-              u = max3(u, x(6), x(7)), v = max3(v, x(8), x(9));
-              u = max3(u, x(10), x(11)), v = max3(v, x(12), x(13));
-              u = max3(u, x(14), x(15));
-              top = fmaxf(top, fmaf(fmaxf(u, v), by, sc.y));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if (seen(32 * i + 16 * g + e)) top = fmaxf(top, fmaf(x(e), by, sc.y));
-              }
+            for (int k = 0; k < 2; ++k) {
+              tmem_wait_ld();
+              if (k == 0 || i == 0) tmem_ld32(s_at + 32u * (i + k + 1), s[k ^ 1]);
+              if (!whole) mask(s[k], 32 * (i + k));
+              work(i + k, s[k]);
             }
           }
-        }
+        };
+        // ---- the largest y
+        float top = -CUDART_INF_F;
+        over([&](int i, const uint32_t (&raw)[32]) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            auto x = [&](int e) { return __uint_as_float(raw[16 * g + e]); };
+            float u = max3(x(0), x(1), x(2)), v = max3(x(3), x(4), x(5));
+            u = max3(u, x(6), x(7)), v = max3(v, x(8), x(9));
+            u = max3(u, x(10), x(11)), v = max3(v, x(12), x(13));
+            u = max3(u, x(14), x(15));
+            const float4 sc = scale[2 * i + g];
+            top = fmaxf(top, fmaf(fmaxf(u, v), fmaxf(mult * sc.x, kLeastFactor), sc.y));
+          }
+        });
         // ---- M moves at the first step, and when it has grown by more than the slack
         const float now = fmaxf(m, top);
         if (j == from_j) {
@@ -264,36 +275,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           const float fade = exp2_fast(m - (now == -CUDART_INF_F ? 0.f : now));
           m = now;
           l *= fade;
-#pragma unroll
-          for (uint32_t i = 0; i < DP / 32u; ++i) {
-            tmem_ld32(o_at + 32u * i, s[0]);
+#pragma unroll 1
+          for (uint32_t i = 0; i < DP / 16u; ++i) {
+            float v[16];
+            uint32_t raw[16];
+            tmem_ld16(o_at + 16u * i, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * fade);
-            tmem_st32(o_at + 32u * i, s[0]);
+            for (int e = 0; e < 16; ++e) raw[e] = __float_as_uint(v[e] * fade);
+            tmem_st16(o_at + 16u * i, raw);
           }
         }
-        const float base = kCarry - (m == -CUDART_INF_F ? 0.f : m);
         // ---- powers, over S
-        tmem_ld32(s_at, s[0]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          tmem_wait_ld();
-          if (i < 3) tmem_ld32(s_at + 32u * (i + 1), s[(i + 1) & 1]);
+        const float base = kCarry - (m == -CUDART_INF_F ? 0.f : m);
+        over([&](int i, const uint32_t (&raw)[32]) {
           uint32_t out[16];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const float4 sc = scale[2 * i + g];
-            const float by = mult * sc.x, plus = sc.y + base;
+            const float by = fmaxf(mult * sc.x, kLeastFactor), plus = sc.y + base;
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              float x = exp2_fast(fmaf(__uint_as_float(s[i & 1][16 * g + e]), by, plus));
-              float y = exp2_fast(fmaf(__uint_as_float(s[i & 1][16 * g + e + 1]), by, plus));
-              if (!whole) {
-                if (!seen(32 * i + 16 * g + e)) x = 0.f;
-                if (!seen(32 * i + 16 * g + e + 1)) y = 0.f;
-              }
+              const float x = exp2_fast(fmaf(__uint_as_float(raw[16 * g + e]), by, plus));
+              const float y = exp2_fast(fmaf(__uint_as_float(raw[16 * g + e + 1]), by, plus));
               sum[0] += x;
               sum[1] += y;
               out[8 * g + e / 2] = pack2(x, y, __half());
@@ -301,14 +306,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
             l = fmaf(sum[0] + sum[1], sc.z, l);
           }
           tmem_st16(s_at + 16u * i, out);
-        }
+        });
         if (!whole) {  // a NaN value that some rows see and some do not was taken out of the codes
           wait(&v_full[kt & 1u], (kt >> 1) & 1u);
           for (uint32_t w = 0; w < kCodeWarps; ++w) {
             if (nan_flag[kt & 1u][w] == 0u) continue;
             for (uint32_t e = w * 32u; e < w * 32u + 32u; ++e) {
               const uint4 bits = reinterpret_cast<const uint4*>(smem + Shape::nan_bits)[(kt & 1u) * kHalf + e];
-              if ((bits.x | bits.y | bits.z | bits.w) == 0u || !seen(static_cast<int32_t>(e))) continue;
+              if ((bits.x | bits.y | bits.z | bits.w) == 0u || !sees(a, p, slot0 + e)) continue;
               uint4 mine = *row_nan;
               mine.x |= bits.x, mine.y |= bits.y, mine.z |= bits.z, mine.w |= bits.w;
               *row_nan = mine;
@@ -543,14 +548,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           for (uint32_t h = 0; h < 2u; ++h) {  // both halves of a row's 128 columns
             uint32_t bits = 0;
             if (h < kMine && (now_flags >> (4u + i) & 1u) == 0u) {
-              uint32_t word[4] = {vw[i][h % kMine].x, vw[i][h % kMine].y, vw[i][h % kMine].z, vw[i][h % kMine].w};
-#pragma unroll
-              for (uint32_t e = 0; e < 16u; ++e) {
-                if ((word[e / 4u] >> (8u * (e % 4u)) & 0x7fu) != 0x7fu) continue;
-                bits |= 1u << e;
-                word[e / 4u] &= ~(0xffu << (8u * (e % 4u)));
-              }
-              vw[i][h % kMine] = make_uint4(word[0], word[1], word[2], word[3]);
+              auto clean = [&](uint32_t& word, uint32_t e) {
+                const uint32_t is = (((word & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+                word &= ~(is * 0xffu);
+                bits |= (is * 0x01020408u >> 24 & 15u) << (4u * e);
+              };
+              clean(vw[i][h % kMine].x, 0u), clean(vw[i][h % kMine].y, 1u);
+              clean(vw[i][h % kMine].z, 2u), clean(vw[i][h % kMine].w, 3u);
             }
             reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(buf * kHalf + (4u * w + i) * 8u + r) * 8u + pq + 4u * h] =
                 static_cast<uint16_t>(bits);
@@ -562,7 +566,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       if (lane == 0u) mbar_arrive(&v_full[buf]);
       if (next) load(c.v, vw);
     }
-  } else if (lane == 0u) {
+  } else if (elect_one()) {
     // ================= the products, by one thread
     uint32_t parts[2] = {0u, 0u}, steps[2] = {0u, 0u};
     const uint32_t base = smem_addr(smem);
