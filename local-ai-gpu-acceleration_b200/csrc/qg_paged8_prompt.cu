@@ -3,21 +3,22 @@
 // qg_paged8_attn.cu).
 //
 // A tile is 256 rows (query heads of a kv head, token after token) in two halves of 128, the lanes of
-// tensor memory; a step is 128 slots.  For each half
-//   S = Q C_k^T    both operands fp16 in shared memory, 128 x 128 fp32 in tensor memory
-//   P = 2^(y - M)  one thread a row: it reads its row of S twice (maximum, then powers) and writes P
-//                  as fp16 over S
+// tensor memory; a step is 64 slots.  For each half
+//   S = Q C_k^T    both operands fp16 in shared memory, 128 x 64 fp32 in tensor memory, two of them
+//   P = 2^(y - M)  one thread a row: it takes its 64 scores into registers, finds the largest y and
+//                  writes P as fp16 over S
 //   O += P C_v     P from tensor memory, fp32 sums in tensor memory
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
 //
 // Codes become fp16 once for 256 rows: four warps load a step's codes into registers a step ahead,
-// convert them and write them as core matrices of 8 slots x 16 bytes, stored [16-byte chunk of dims][8 slots].
-// This one layout is a K-major operand over dims (for K, slots are N) and an MN-major one over slots
-// (for V, dims are N); no byte is transposed.
-//
-// Warps: 0-3 and 4-7 the rows of the halves, 8-11 codes, 12 issues the products.  The halves take turns
-// on the tensor pipe: while one waits for its S, the other's powers are computed.
+// convert them and write them as core matrices of 8 slots x 16 bytes, the two of a product's 16-deep step
+// side by side: over dims for K, a K-major operand whose N are slots, over slots for V, an MN-major
+// one whose N are dims, so no byte is transposed.
+// Warps: 0-3 and 4-7 the rows of the halves, 8-11 codes, 12 issues the products.  With two S of a half
+// the scores of the next step are there before the powers of this one are written, so the rows never
+// wait for a product.  The four roles' loops have to stay small: unrolled further they left the
+// instruction cache and took twice the time.
 //
 // Work.  Segments, blocks, equal ranges for one CTA an SM, records and joins as in
 // qg_paged8_attn.cu.  Every wait is bounded; after one has run out (QG_ERR_WAIT_TIMEOUT) no wait
@@ -28,45 +29,50 @@
 
 #include "qg_mma.cuh"
 #include "qg_paged8_attn.cuh"
+#include "qg_rows.cuh"
 #include "qg_umma.cuh"
 
 namespace qg {
 namespace {
 
-constexpr uint32_t kHalf = 128;                  // rows of a half, and slots of a step
-constexpr uint32_t kLogStep = 7;
+constexpr uint32_t kHalf = 128;                  // rows of a half
+constexpr uint32_t kLogStep = 6, kStep = 1u << kLogStep;  // slots of a step
+constexpr uint32_t kStages = 3;                  // steps of codes in fp16, for K and for V
+constexpr uint32_t kGroups = kStep / 16u;        // 16-slot groups of a step, one scale each
+static_assert(kGroups == 4u, "a code warp each");
 constexpr uint32_t kRowWarps = 8, kCodeWarp0 = 8, kCodeWarps = 4, kIssueWarp = 12;
-constexpr uint32_t kPromptThreads = (kIssueWarp + 1u) * 32u;
+constexpr uint32_t kPromptThreads = (kIssueWarp + 1u) * 32u;  // four warps a scheduler: 128 registers a thread
 constexpr uint32_t kScaleRing = 4;
 constexpr uint32_t kMaxPolls = 4000;             // of up to kPollNs each
 constexpr float kCarry = 7.f, kSlack = 8.f;      // log2: the factor of powers, the growth of M that is let pass
 constexpr float kLeastFactor = 1e-30f;           // of scores: zero would turn minus infinity into NaN
-constexpr uint32_t kPromptHeader = 2;            // what a segment costs beside its blocks, in blocks
+constexpr uint32_t kPromptHeader = 4;            // what a segment costs beside its blocks, in blocks
 static_assert(2u * 256u * 4u <= QG_PAGED_ATTN_ZEROED && kMaxPromptCtas <= 256u, "a counter per CTA and half");
 static_assert(kPromptRows == 2u * kHalf, "two halves");
 
 template <int DP>
 struct PromptShape {
-  static constexpr uint32_t kChunks = DP / 8u;             // 16-byte chunks of a row in fp16
-  static constexpr uint32_t kTileBytes = kHalf * DP * 2u;  // 128 rows or slots
-  static constexpr uint32_t q_at = 0, k_at = 2u * kTileBytes, v_at = 4u * kTileBytes, end = 6u * kTileBytes;
-  static constexpr uint32_t scales = end;                              // [ring][8] {key scale, log2 value scale, reciprocal}
-  static constexpr uint32_t nan_bits = scales + kScaleRing * 8u * 16u;  // [2][128 slots][8 pieces] 16 columns each
-  static constexpr uint32_t row_nan = nan_bits + 2u * kHalf * 16u;      // [256 rows] the columns that are NaN
+  static constexpr uint32_t kChunks = DP / 8u;               // 16-byte chunks of a row in fp16
+  static constexpr uint32_t kQBytes = kHalf * DP * 2u, kCodeBytes = kStep * DP * 2u;
+  static constexpr uint32_t q_at = 0, k_at = 2u * kQBytes, v_at = k_at + kStages * kCodeBytes;
+  static constexpr uint32_t scales = v_at + kStages * kCodeBytes;  // [ring][group] {key scale, log2 value scale, reciprocal}
+  static constexpr uint32_t nan_bits = scales + kScaleRing * kGroups * 16u;  // [stage][slot][8 pieces] 16 columns each
+  static constexpr uint32_t row_nan = nan_bits + kStages * kStep * 16u;      // [256 rows] the columns that are NaN
   static constexpr uint32_t kSmem = row_nan + kPromptRows * 16u + 1024u;
-  static constexpr uint32_t kRecord = kHalf * (DP + 2u);   // of a half: m[], l[], o[DP / 4][row] float4
+  static constexpr uint32_t kRecord = kHalf * (DP + 2u);     // of a half: m[], l[], o[DP / 4][row] float4
 };
 
-// Descriptor of an operand stored as core matrices of 8 x 16 bytes, consecutive ones of a chunk 128 bytes
-// apart, chunks 2048 bytes; no swizzle, version 1.
-template <uint32_t LEADING, uint32_t STRIDE>
+// Descriptor of an operand stored as core matrices of 8 x 16 bytes, the two of a 16-deep step 128 bytes
+// apart, those of the next 8 rows (columns) 256; no swizzle, version 1.
 __device__ __forceinline__ uint64_t core_desc(uint32_t at) {
-  return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(LEADING >> 4) << 16) |
-         (static_cast<uint64_t>(STRIDE >> 4) << 32) | (1ull << 46);
+  return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 16) |
+         (static_cast<uint64_t>(256u >> 4) << 32) | (1ull << 46);
 }
-constexpr uint32_t kChunkBytes = kHalf * 16u;
+constexpr uint32_t kQDepth = kHalf * 32u, kKDepth = kStep * 32u;  // bytes of a 16-deep step of Q, of K
+template <int DP>
+constexpr uint32_t kVDepth = DP * 32u;                            // of V
 // fp16 operands, fp32 sums, M = 128
-constexpr uint32_t score_idesc() { return (1u << 4) | ((kHalf >> 3) << 17) | ((kHalf >> 4) << 24); }
+constexpr uint32_t score_idesc() { return (1u << 4) | ((kStep >> 3) << 17) | ((kHalf >> 4) << 24); }
 template <int DP>
 constexpr uint32_t value_idesc() {  // B MN-major
   return (1u << 4) | (1u << 16) | ((DP >> 3) << 17) | ((kHalf >> 4) << 24);
@@ -83,10 +89,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
   using Shape = PromptShape<DP>;
   const PagedView& c = cache.c;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kScaleRing], drained;
+  __shared__ __align__(8) uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_full[2][2], k_full[kStages], k_empty[kStages],
+      v_full[kStages], v_empty[kStages], scale_full[kScaleRing], drained;
   __shared__ uint32_t tmem_slot, abort_flag, last_flag[2];
-  __shared__ uint32_t nan_flag[2][kCodeWarps];
+  __shared__ uint32_t nan_flag[kStages][kCodeWarps];
   const uint32_t tid = threadIdx.x, lane = tid & 31u;
   const uint32_t warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -94,15 +100,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
   if (tid == 0u) {
     for (uint32_t i = 0; i < 2u; ++i) {
       mbar_init(&q_full[i], kHalf);
-      mbar_init(&s_full[i], 1u);
-      mbar_init(&p_full[i], kHalf);
-      mbar_init(&o_full[i], 1u);
+      for (uint32_t k = 0; k < 2u; ++k) {
+        mbar_init(&s_full[i][k], 1u);
+        mbar_init(&p_full[i][k], kHalf);
+        mbar_init(&pv_full[i][k], 1u);
+      }
+    }
+    for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], kCodeWarps);
       mbar_init(&k_empty[i], 1u);
       mbar_init(&v_full[i], kCodeWarps);
       mbar_init(&v_empty[i], 1u);
     }
-    for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 1u);
+    for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], kCodeWarps);
     mbar_init(&drained, 1u);
     abort_flag = 0u;
     fence_mbar_init();
@@ -118,6 +128,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
 
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return;
+#pragma unroll 1
     for (uint32_t i = 0; i < kMaxPolls; ++i) {
       if (*abort != 0u) return;
       if (mbar_try_wait_sleep(bar, parity)) return;
@@ -164,7 +175,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
     const uint32_t half = warp / 4u, row = tid % kHalf;      // of the half
     const uint32_t s_at = tmem + half * kHalf + ((warp & 3u) << 21), o_at = s_at + 2u * kHalf;
     uint4* const row_nan = reinterpret_cast<uint4*>(smem + Shape::row_nan) + half * kHalf + row;
-    uint32_t parts = 0, steps = 0;                           // of this half
+    uint32_t steps = 0;                                      // of this half
     for (; left != 0u; advance(use, left)) {
       const uint32_t from_j = use.j, to_j = min(use.j1, use.j + left);
       left -= to_j - from_j;
@@ -180,98 +191,92 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       // ---- the query, scaled to a largest value in [1, 2); the scale's sign goes with it
       float mult = fabsf(a.scale_log2);
       {
-        uint4 w[Shape::kChunks];
-        float top = 0.f;
         const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + token * a.q_stride +
                                                            static_cast<uint64_t>(head) * c.dim);
         auto two = [&](uint32_t u) { return a.dtype == QG_F16 ? unpack2(u, __half()) : unpack2(u, __nv_bfloat16()); };
+        constexpr uint32_t kBatch = 4;  // pieces in flight
+        auto each = [&](auto work) {
+#pragma unroll 1
+          for (uint32_t i = 0; i < Shape::kChunks; i += kBatch) {
+            uint4 w[kBatch];
 #pragma unroll
-        for (uint32_t i = 0; i < Shape::kChunks; ++i) {
-          w[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (has && i * 8u < c.dim) w[i] = from[i];
-        }
+            for (uint32_t k = 0; k < kBatch; ++k) {
+              w[k] = make_uint4(0u, 0u, 0u, 0u);
+              if (has && (i + k) * 8u < c.dim) w[k] = from[i + k];
+            }
 #pragma unroll
-        for (uint32_t i = 0; i < Shape::kChunks; ++i) {
-          const float2 x = two(w[i].x), y = two(w[i].y), z = two(w[i].z), u = two(w[i].w);
-          top = max3(top, fabsf(x.x), fabsf(x.y));
-          top = max3(top, fabsf(y.x), fabsf(y.y));
-          top = max3(top, fabsf(z.x), fabsf(z.y));
-          top = max3(top, fabsf(u.x), fabsf(u.y));
-        }
+            for (uint32_t k = 0; k < kBatch; ++k) work(i + k, w[k]);
+          }
+        };
+        float top = 0.f;
+        each([&](uint32_t, uint4 w) {
+          const float2 x = two(w.x), y = two(w.y), z = two(w.z), u = two(w.w);
+          top = max3(top, max3(fabsf(x.x), fabsf(x.y), fabsf(y.x)), fabsf(y.y));
+          top = max3(top, max3(fabsf(z.x), fabsf(z.y), fabsf(u.x)), fabsf(u.y));
+        });
         const int power = top == 0.f ? 0 : max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
         const float by = a.scale_log2 < 0.f ? -power_of_two(-power) : power_of_two(-power);
         mult *= power_of_two(power);
-        uint8_t* const to = smem + Shape::q_at + half * Shape::kTileBytes + (row >> 3) * 128u + (row & 7u) * 16u;
-#pragma unroll
-        for (uint32_t i = 0; i < Shape::kChunks; ++i) {
+        uint8_t* const to = smem + Shape::q_at + half * Shape::kQBytes + (row >> 3) * 256u + (row & 7u) * 16u;
+        each([&](uint32_t i, uint4 w) {
           auto half2 = [&](uint32_t u) {
             const float2 x = two(u);
             return pack2(x.x * by, x.y * by, __half());
           };
-          *reinterpret_cast<uint4*>(to + i * kChunkBytes) =
-              make_uint4(half2(w[i].x), half2(w[i].y), half2(w[i].z), half2(w[i].w));
-        }
+          *reinterpret_cast<uint4*>(to + (i >> 1) * kQDepth + (i & 1u) * 128u) = make_uint4(half2(w.x), half2(w.y), half2(w.z), half2(w.w));
+        });
         fence_proxy_async_smem();
         mbar_arrive(&q_full[half]);
       }
       float m = -CUDART_INF_F, l = 0.f;
       bool any_nan = false;  // columns of the row are NaN
       for (uint32_t j = from_j; j < to_j; ++j, ++kt, ++steps) {
-        const uint32_t slot0 = use.block(j) << kLogStep, ring = kt % kScaleRing;
-        const bool whole = use.all_see(a, slot0, kHalf);
-        const float4* const scale = reinterpret_cast<const float4*>(smem + Shape::scales) + ring * 8u;
-        // the row's slots of the step: up to hi, from lo on or before `first`
-        const int32_t hi = p - static_cast<int32_t>(slot0);
-        const int32_t lo = a.window == 0u || hi < 0 || a.window > static_cast<uint32_t>(hi)
-                               ? INT32_MIN : hi - static_cast<int32_t>(a.window) + 1;
-        const int32_t first = a.sink > slot0 ? static_cast<int32_t>(min(a.sink - slot0, kHalf)) : 0;
-        wait(&s_full[half], steps & 1u);
+        const uint32_t slot0 = use.block(j) << kLogStep, ring = kt % kScaleRing, s_now = s_at + (steps & 1u) * kStep;
+        const bool whole = use.all_see(a, slot0, kStep);
+        const float4* const scale = reinterpret_cast<const float4*>(smem + Shape::scales) + ring * kGroups;
+        wait(&s_full[half][steps & 1u], (steps >> 1) & 1u);
         wait(&scale_full[ring], (kt / kScaleRing) & 1u);  // long done: S needed the step's codes
         tc_fence_after();
-        // S comes 32 columns at a time, the next ones while these are worked on; columns that the row does
-        // not see become minus infinity
         uint32_t s[2][32];
-        auto mask = [&](uint32_t (&x)[32], int32_t at) {
+        tmem_ld32(s_now, s[0]);
+        tmem_ld32(s_now + 32u, s[1]);
+        tmem_wait_ld();
+        if (!whole) {  // columns that the row does not see become minus infinity
+          // the row's slots of the step: up to hi, from lo on or before `first`
+          const int32_t hi = p - static_cast<int32_t>(slot0);
+          const int32_t lo = a.window == 0u || hi < 0 || a.window > static_cast<uint32_t>(hi)
+                                 ? INT32_MIN : hi - static_cast<int32_t>(a.window) + 1;
+          const int32_t first = a.sink > slot0 ? static_cast<int32_t>(min(a.sink - slot0, kStep)) : 0;
           auto low = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // bits [0, n)
-          const uint32_t bits = low(hi + 1 - at) & (low(first - at) | ~(lo <= at ? 0u : low(lo - at)));
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if ((bits >> e & 1u) == 0u) x[e] = 0xff800000u;
-          }
-        };
-        auto over = [&](auto work) {
-          tmem_ld32(s_at, s[0]);
-#pragma unroll 1
-          for (int i = 0; i < 4; i += 2) {
+          for (int i = 0; i < 2; ++i) {
+            const int32_t at = 32 * i;
+            const uint32_t bits = low(hi + 1 - at) & (low(first - at) | ~(lo <= at ? 0u : low(lo - at)));
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              tmem_wait_ld();
-              if (k == 0 || i == 0) tmem_ld32(s_at + 32u * (i + k + 1), s[k ^ 1]);
-              if (!whole) mask(s[k], 32 * (i + k));
-              work(i + k, s[k]);
+            for (int e = 0; e < 32; ++e) {
+              if ((bits >> e & 1u) == 0u) s[i][e] = 0xff800000u;
             }
           }
-        };
+        }
         // ---- the largest y
         float top = -CUDART_INF_F;
-        over([&](int i, const uint32_t (&raw)[32]) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            auto x = [&](int e) { return __uint_as_float(raw[16 * g + e]); };
-            float u = max3(x(0), x(1), x(2)), v = max3(x(3), x(4), x(5));
-            u = max3(u, x(6), x(7)), v = max3(v, x(8), x(9));
-            u = max3(u, x(10), x(11)), v = max3(v, x(12), x(13));
-            u = max3(u, x(14), x(15));
-            const float4 sc = scale[2 * i + g];
-            top = fmaxf(top, fmaf(fmaxf(u, v), fmaxf(mult * sc.x, kLeastFactor), sc.y));
-          }
-        });
+        for (uint32_t g = 0; g < kGroups; ++g) {
+          const float4 sc = scale[g];
+          auto x = [&](int e) { return __uint_as_float(s[g / 2u][16 * (g & 1u) + e]); };
+          float u = max3(x(0), x(1), x(2)), v = max3(x(3), x(4), x(5));
+          u = max3(u, x(6), x(7)), v = max3(v, x(8), x(9));
+          u = max3(u, x(10), x(11)), v = max3(v, x(12), x(13));
+          u = max3(u, x(14), x(15));
+          top = fmaxf(top, fmaf(fmaxf(u, v), fmaxf(mult * sc.x, kLeastFactor), sc.y));
+        }
         // ---- M moves at the first step, and when it has grown by more than the slack
         const float now = fmaxf(m, top);
         if (j == from_j) {
           m = now;
         } else if (__any_sync(0xffffffffu, now > m + kSlack)) {
-          // the products before are done: they were issued before S was, and it is complete
+          wait(&pv_full[half][(steps - 1u) & 1u], ((steps - 1u) >> 1) & 1u);  // the sums of the step before are in O
+          tc_fence_after();
           const float fade = exp2_fast(m - (now == -CUDART_INF_F ? 0.f : now));
           m = now;
           l *= fade;
@@ -288,31 +293,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         }
         // ---- powers, over S
         const float base = kCarry - (m == -CUDART_INF_F ? 0.f : m);
-        over([&](int i, const uint32_t (&raw)[32]) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; ++i) {
           uint32_t out[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 sc = scale[2 * i + g];
+          for (uint32_t h = 0; h < 2u; ++h) {
+            const uint32_t g = 2u * i + h;
+            const float4 sc = scale[g];
             const float by = fmaxf(mult * sc.x, kLeastFactor), plus = sc.y + base;
-            float sum[2] = {0.f, 0.f};
+            const F2 by2 = f2(by, by), plus2 = f2(plus, plus);
+            F2 sum = f2(0.f, 0.f);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float x = exp2_fast(fmaf(__uint_as_float(raw[16 * g + e]), by, plus));
-              const float y = exp2_fast(fmaf(__uint_as_float(raw[16 * g + e + 1]), by, plus));
-              sum[0] += x;
-              sum[1] += y;
-              out[8 * g + e / 2] = pack2(x, y, __half());
+            for (uint32_t e = 0; e < 16u; e += 2u) {
+              const float2 y = split(fma(f2(__uint_as_float(s[i][16u * h + e]), __uint_as_float(s[i][16u * h + e + 1u])), by2, plus2));
+              const float2 x = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+              sum = sum + f2(x.x, x.y);
+              out[8u * h + e / 2u] = pack2(x.x, x.y, __half());
             }
-            l = fmaf(sum[0] + sum[1], sc.z, l);
+            const float2 z = split(sum);
+            l = fmaf(z.x + z.y, sc.z, l);
           }
-          tmem_st16(s_at + 16u * i, out);
-        });
+          tmem_st16(s_now + 16u * i, out);
+        }
         if (!whole) {  // a NaN value that some rows see and some do not was taken out of the codes
-          wait(&v_full[kt & 1u], (kt >> 1) & 1u);
-          for (uint32_t w = 0; w < kCodeWarps; ++w) {
-            if (nan_flag[kt & 1u][w] == 0u) continue;
-            for (uint32_t e = w * 32u; e < w * 32u + 32u; ++e) {
-              const uint4 bits = reinterpret_cast<const uint4*>(smem + Shape::nan_bits)[(kt & 1u) * kHalf + e];
+          const uint32_t stage = kt % kStages;
+          wait(&v_full[stage], (kt / kStages) & 1u);
+#pragma unroll 1
+          for (uint32_t e = 0; e < kStep; ++e) {
+            if (nan_flag[stage][e / 16u] == 0u) {
+              e |= 15u;
+              continue;
+            }
+            {
+              const uint4 bits = reinterpret_cast<const uint4*>(smem + Shape::nan_bits)[stage * kStep + e];
               if ((bits.x | bits.y | bits.z | bits.w) == 0u || !sees(a, p, slot0 + e)) continue;
               uint4 mine = *row_nan;
               mine.x |= bits.x, mine.y |= bits.y, mine.z |= bits.z, mine.w |= bits.w;
@@ -323,7 +336,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[half]);
+        mbar_arrive(&p_full[half][steps & 1u]);
       }
 
       // ---- the end of the segment, or of the range inside it
@@ -341,11 +354,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
               sum == 0.f ? -CUDART_INF_F : (top + log2f(sum) - kCarry) * 0.69314718055994530942f;
         }
       };
-      wait(&o_full[half], parts & 1u);
-      ++parts;
+      wait(&pv_full[half][(steps - 1u) & 1u], ((steps - 1u) >> 1) & 1u);
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+#pragma unroll 1
       for (uint32_t i = 0; i < DP / 32u; ++i) {
         uint32_t raw[32];
         tmem_ld32(o_at + 32u * i, raw);
@@ -402,8 +414,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
             all = fmaf(__ldcg(record_of(i) + kHalf + row), exp2_fast(__ldcg(record_of(i) + row) - from), all);
           }
           const float by = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll 1
           for (uint32_t i0 = 0; i0 < DP / 16u; ++i0) {  // 16 columns at a time
             float x[16] = {};
+#pragma unroll 2
             for (uint32_t i = 0; i < count; ++i) {
               const float f = exp2_fast(__ldcg(record_of(i) + row) - from);
               const float4* rec = reinterpret_cast<const float4*>(record_of(i) + 2u * kHalf) + (4u * i0) * kHalf + row;
@@ -422,132 +436,128 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       }
     }
   } else if (warp < kIssueWarp) {
-    // ================= codes to fp16: this thread has place r of the 8-slot groups 4 w to 4 w + 3 and every
-    // fourth 16-code piece, so 8 lanes write 128 consecutive bytes and a group's lanes read 64 of a row
+    // ================= codes to fp16: warp w has the step's 16-slot group w, this thread places r and 8 + r of
+    // it and every fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
     constexpr uint32_t kMine = DP / 64u;                     // pieces of a row
-    const uint32_t w = warp - kCodeWarp0, r = lane & 7u, pq = lane >> 3, thread = tid - kCodeWarp0 * 32u;
+    const uint32_t w = warp - kCodeWarp0, r = lane & 7u, pq = lane >> 3;
     Segment8 s = use;
     uint32_t rem = left;
-    uint32_t id[4] = {}, scale_id = 0, flags = 0;            // flags: row i is seen by some, bit 4 + i: by all
+    uint32_t id = 0, flags = 0;                              // flags: row i is seen by some, bit 2 + i: by all
     float ks = 0.f, vs = 1.f;
-    uint64_t off[4] = {};
-    uint4 kw[4][kMine], vw[4][kMine];
-    auto slot_of = [&](uint32_t i) { return (s.block(s.j) << kLogStep) + (4u * w + i) * 8u + r; };
-    auto look = [&]() {  // page ids of the step's rows
-      const int32_t* list = c.table + static_cast<size_t>(s.b) * c.table_stride;
-#pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
-        id[i] = 0xffffffffu;
-        if (s.some_see(slot_of(i), 1u)) id[i] = static_cast<uint32_t>(list[div_by(slot_of(i), c.page)]);
-      }
-      if (thread < 8u) {
-        const uint32_t slot = (s.block(s.j) << kLogStep) + thread * 16u;
-        scale_id = 0xffffffffu;
-        if (s.some_see(slot, 16u)) scale_id = static_cast<uint32_t>(list[div_by(slot, c.page)]);
+    uint64_t off = 0;
+    uint4 kw[2][kMine], vw[2][kMine];
+    auto group = [&]() { return (s.block(s.j) << kLogStep) + 16u * w; };  // its first slot
+    auto look = [&]() {  // the group's page
+      id = 0xffffffffu;
+      if (s.some_see(group(), 16u)) {
+        id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + div_by(group(), c.page)]);
       }
     };
     auto place = [&]() {  // where the rows lie, and the scales
+      const uint32_t slot = group(), at = div_by(slot, c.page), on = slot - at * c.page.d;
       flags = 0u;
-#pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
-        const uint32_t slot = slot_of(i), at = div_by(slot, c.page);
-        if (!s.some_see(slot, 1u)) continue;
-        if (s.all_see(a, slot, 1u)) flags |= 16u << i;
-        if (id[i] >= c.num_pages) {
-          atomicOr(&g_error_word, QG_ERR_PAGE);
-          continue;
-        }
-        flags |= 1u << i;
-        off[i] = id[i] * c.page_bytes + s.kv * c.head_bytes + (slot - at * c.page.d) * c.slot_bytes;
-      }
       ks = 0.f;
       vs = 1.f;
-      if (thread < 8u && scale_id < c.num_pages) {
-        const uint32_t slot = (s.block(s.j) << kLogStep) + thread * 16u, at = div_by(slot, c.page);
-        const uint64_t in = scale_id * cache.scale_page + s.kv * cache.scale_head + ((slot - at * c.page.d) >> cache.log_block);
-        ks = cache.ks[in];
-        vs = cache.vs[in];
+      if (!s.some_see(slot, 16u)) return;
+      if (id >= c.num_pages) {
+        atomicOr(&g_error_word, QG_ERR_PAGE);
+        return;
+      }
+      off = id * c.page_bytes + s.kv * c.head_bytes + (on + r) * c.slot_bytes + pq * 16u;
+      const uint64_t in = id * cache.scale_page + s.kv * cache.scale_head + (on >> cache.log_block);
+      ks = cache.ks[in];
+      vs = cache.vs[in];
+      if (s.all_see(a, slot, 16u)) {
+        flags = 15u;
+        return;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+        if (s.some_see(slot + 8u * i + r, 1u)) flags |= 1u << i;
+        if (s.all_see(a, slot + 8u * i + r, 1u)) flags |= 4u << i;
       }
     };
-    auto load = [&](const uint8_t* pool, uint4 (&to)[4][kMine]) {
+    auto load = [&](const uint8_t* pool, uint4 (&to)[2][kMine]) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
+      for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
         for (uint32_t h = 0; h < kMine; ++h) {
           to[i][h] = make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t piece = pq + 4u * h;
-          if ((flags >> i & 1u) != 0u && piece * 16u < c.dim) {
-            to[i][h] = *reinterpret_cast<const uint4*>(pool + off[i] + piece * 16u);
+          if ((flags >> i & 1u) != 0u && (pq + 4u * h) * 16u < c.dim) {
+            to[i][h] = *reinterpret_cast<const uint4*>(pool + off + i * 8u * c.slot_bytes + h * 64u);
           }
         }
       }
     };
-    auto store = [&](uint32_t at, const uint4 (&from)[4][kMine]) {
+    // piece p, 8-slot group 2 w + i: of K in step p at that group, of V in step w at chunks 2 p and 2 p + 1
+    uint8_t* const k_mem = smem + Shape::k_at + pq * kKDepth + 2u * w * 256u + r * 16u;
+    uint8_t* const v_mem = smem + Shape::v_at + w * kVDepth<DP> + 2u * pq * 256u + r * 16u;
+    auto store = [&](uint8_t* at, uint32_t per_i, uint32_t per_h, uint32_t beside, const uint4 (&from)[2][kMine]) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) {
+      for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
         for (uint32_t h = 0; h < kMine; ++h) {
-          uint8_t* const to = smem + at + 2u * (pq + 4u * h) * kChunkBytes + (4u * w + i) * 128u + r * 16u;
+          uint8_t* const to = at + h * per_h + i * per_i;
           uint4 x, y;
           codes_to_half(from[i][h].x, x.x, x.y);
           codes_to_half(from[i][h].y, x.z, x.w);
           codes_to_half(from[i][h].z, y.x, y.y);
           codes_to_half(from[i][h].w, y.z, y.w);
           *reinterpret_cast<uint4*>(to) = x;
-          *reinterpret_cast<uint4*>(to + kChunkBytes) = y;
+          *reinterpret_cast<uint4*>(to + beside) = y;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
-    bool next = rem != 0u;
-    if (next) {
-      look();
-      place();
-      load(c.k, kw);
-      load(c.v, vw);
-    }
-    for (; next; ++kt) {
-      const uint32_t buf = kt & 1u, ring = kt % kScaleRing, now_flags = flags;
+    uint32_t stage = 0, round = 0;                           // kt = round * kStages + stage
+    if (rem != 0u) look();
+    for (bool first = true; rem != 0u; first = false) {      // a step's codes are stored once the next one's are asked for
+      if (first) {
+        place();
+        load(c.k, kw);
+        load(c.v, vw);
+      }
+      const uint32_t ring = kt % kScaleRing, now_flags = flags;
       const float now_ks = ks, now_vs = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
       ++s.j;
       --rem;
       if (s.j == s.j1) advance(s, rem);
-      next = rem != 0u;
-      if (next) look();
-      if (kt >= 2u) wait(&k_empty[buf], ((kt >> 1) - 1u) & 1u);
-      if (thread < 8u) {
-        reinterpret_cast<float4*>(smem + Shape::scales)[ring * 8u + thread] = make_float4(now_ks, log2f(now_vs), 1.f / now_vs, 0.f);
+      if (rem != 0u) look();
+      if (round != 0u) wait(&k_empty[stage], (round - 1u) & 1u);
+      if (lane == 0u) {
+        reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + w] = make_float4(now_ks, log2f(now_vs), 1.f / now_vs, 0.f);
       }
-      store(Shape::k_at + buf * Shape::kTileBytes, kw);
-      if (lane == 0u) mbar_arrive(&k_full[buf]);
-      if (thread == 0u) mbar_arrive(&scale_full[ring]);
-      if (next) {
+      store(k_mem + stage * Shape::kCodeBytes, 256u, 4u * kKDepth, 128u, kw);
+      if (lane == 0u) {
+        mbar_arrive(&k_full[stage]);
+        mbar_arrive(&scale_full[ring]);
+      }
+      if (rem != 0u) {
         place();
         load(c.k, kw);
       }
       // NaN codes of rows that not all see: out of the codes, noted by column
       uint32_t odd = 0;
-      if ((now_flags >> 4) != (now_flags & 15u)) {
+      if (now_flags != 15u) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
+        for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < kMine; ++h) {
-            if ((now_flags >> (4u + i) & 1u) != 0u) continue;
             auto nan = [](uint32_t u) { return ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-            odd |= nan(vw[i][h].x) | nan(vw[i][h].y) | nan(vw[i][h].z) | nan(vw[i][h].w);
+            if ((now_flags >> (2u + i) & 1u) == 0u) odd |= nan(vw[i][h].x) | nan(vw[i][h].y) | nan(vw[i][h].z) | nan(vw[i][h].w);
           }
         }
       }
       const bool flagged = __any_sync(0xffffffffu, odd != 0u);
-      if (kt >= 2u) wait(&v_empty[buf], ((kt >> 1) - 1u) & 1u);
+      if (round != 0u) wait(&v_empty[stage], (round - 1u) & 1u);
       if (flagged) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
+        for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < 2u; ++h) {  // both halves of a row's 128 columns
             uint32_t bits = 0;
-            if (h < kMine && (now_flags >> (4u + i) & 1u) == 0u) {
+            if (h < kMine && (now_flags >> (2u + i) & 1u) == 0u) {
               auto clean = [&](uint32_t& word, uint32_t e) {
                 const uint32_t is = (((word & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
                 word &= ~(is * 0xffu);
@@ -556,71 +566,72 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
               clean(vw[i][h % kMine].x, 0u), clean(vw[i][h % kMine].y, 1u);
               clean(vw[i][h % kMine].z, 2u), clean(vw[i][h % kMine].w, 3u);
             }
-            reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(buf * kHalf + (4u * w + i) * 8u + r) * 8u + pq + 4u * h] =
+            reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(stage * kStep + 16u * w + 8u * i + r) * 8u + pq + 4u * h] =
                 static_cast<uint16_t>(bits);
           }
         }
       }
-      if (lane == 0u) nan_flag[buf][w] = flagged ? 1u : 0u;
-      store(Shape::v_at + buf * Shape::kTileBytes, vw);
-      if (lane == 0u) mbar_arrive(&v_full[buf]);
-      if (next) load(c.v, vw);
+      if (lane == 0u) nan_flag[stage][w] = flagged ? 1u : 0u;
+      store(v_mem + stage * Shape::kCodeBytes, 128u, 8u * 256u, 256u, vw);
+      if (lane == 0u) mbar_arrive(&v_full[stage]);
+      if (rem != 0u) load(c.v, vw);
+      ++kt;
+      if (++stage == kStages) stage = 0u, ++round;
     }
-  } else if (elect_one()) {
+  } else if (warp == kIssueWarp && elect_one()) {
     // ================= the products, by one thread
     uint32_t parts[2] = {0u, 0u}, steps[2] = {0u, 0u};
+    uint32_t k_stage = 0, k_round = 0, v_stage = 0, v_round = 0;
     const uint32_t base = smem_addr(smem);
-    auto scores = [&](uint32_t half, uint32_t buf) {
+    const uint64_t q0 = core_desc(base + Shape::q_at), k0 = core_desc(base + Shape::k_at), v0 = core_desc(base + Shape::v_at);
+    auto scores = [&](uint32_t half, uint32_t buffer) {  // of the K stage
+      const uint64_t q = q0 + half * (Shape::kQBytes / 16u), k = k0 + k_stage * (Shape::kCodeBytes / 16u);
+      const uint32_t s = tmem + half * kHalf + buffer * kStep;
       if (*abort != 0u) return;
-      const uint32_t q = base + Shape::q_at + half * Shape::kTileBytes, k = base + Shape::k_at + buf * Shape::kTileBytes;
 #pragma unroll
-      for (uint32_t i = 0; i < DP / 16u; ++i) {
-        umma_ss(tmem + half * kHalf, core_desc<kChunkBytes, 128u>(q + i * 2u * kChunkBytes),
-                core_desc<kChunkBytes, 128u>(k + i * 2u * kChunkBytes), score_idesc(), i != 0u ? 1u : 0u);
-      }
+      for (uint32_t i = 0; i < DP / 16u; ++i) umma_ss(s, q + i * (kQDepth / 16u), k + i * (kKDepth / 16u), score_idesc(), i);
     };
-    auto values = [&](uint32_t half, uint32_t buf, bool more) {
+    auto values = [&](uint32_t half, uint32_t buffer, uint32_t more) {  // of the V stage
+      const uint64_t v = v0 + v_stage * (Shape::kCodeBytes / 16u);
+      const uint32_t p = tmem + half * kHalf + buffer * kStep, o = tmem + 2u * kHalf + half * kHalf;
       if (*abort != 0u) return;
-      const uint32_t v = base + Shape::v_at + buf * Shape::kTileBytes;
 #pragma unroll
-      for (uint32_t i = 0; i < kHalf / 16u; ++i) {
-        umma_ts(tmem + (2u + half) * kHalf, tmem + half * kHalf + 8u * i, core_desc<128u, kChunkBytes>(v + i * 256u),
-                value_idesc<DP>(), more || i != 0u ? 1u : 0u);
-      }
+      for (uint32_t i = 0; i < kStep / 16u; ++i) umma_ts(o, p + 8u * i, v + i * (kVDepth<DP> / 16u), value_idesc<DP>(), more | i);
     };
     for (; left != 0u; advance(use, left)) {
       const uint32_t count = min(use.j1 - use.j, left), halves = use.rows > kHalf ? 2u : 1u;
       left -= count;
       for (uint32_t h = 0; h < halves; ++h) wait(&q_full[h], parts[h]++ & 1u);
-      wait(&k_full[kt & 1u], (kt >> 1) & 1u);
-      tc_fence_after();
-      for (uint32_t h = 0; h < halves; ++h) {
-        scores(h, kt & 1u);
-        umma_commit(&s_full[h]);
-      }
-      umma_commit(&k_empty[kt & 1u]);
-      for (uint32_t i = 0; i < count; ++i, ++kt) {
-        const uint32_t buf = kt & 1u;
-        const bool more = i + 1u < count;
+      // step i's scores two ahead of its sums: S(i) is free once the sums of step i - 2 have been issued
+#pragma unroll 1
+      for (uint32_t i = 0; i < count + 2u; ++i) {
+        if (i >= 2u) wait(&v_full[v_stage], v_round & 1u);
+        if (i < count) wait(&k_full[k_stage], k_round & 1u);
+#pragma unroll 1
         for (uint32_t h = 0; h < halves; ++h) {
-          wait(&p_full[h], steps[h]++ & 1u);
-          if (h == 0u) wait(&v_full[buf], (kt >> 1) & 1u);
-          tc_fence_after();
-          values(h, buf, i != 0u);
-          if (h + 1u == halves) umma_commit(&v_empty[buf]);
-          if (!more) {
-            umma_commit(&o_full[h]);
-            continue;
-          }
-          if (h == 0u) {
-            wait(&k_full[buf ^ 1u], ((kt + 1u) >> 1) & 1u);
+          const uint32_t step = steps[h] + i;
+          if (i >= 2u) {
+            wait(&p_full[h][step & 1u], ((step - 2u) >> 1) & 1u);
             tc_fence_after();
+            values(h, step & 1u, i - 2u);
+            umma_commit(&pv_full[h][step & 1u]);
           }
-          scores(h, buf ^ 1u);
-          umma_commit(&s_full[h]);
-          if (h + 1u == halves) umma_commit(&k_empty[buf ^ 1u]);
+          if (i < count) {
+            tc_fence_after();
+            scores(h, step & 1u);
+            umma_commit(&s_full[h][step & 1u]);
+          }
+        }
+        if (i >= 2u) {
+          umma_commit(&v_empty[v_stage]);
+          if (++v_stage == kStages) v_stage = 0u, ++v_round;
+        }
+        if (i < count) {
+          umma_commit(&k_empty[k_stage]);
+          if (++k_stage == kStages) k_stage = 0u, ++k_round;
         }
       }
+      for (uint32_t h = 0; h < halves; ++h) steps[h] += count;
     }
     // what was issued ends before the CTA's memory goes, also after a wait that ran out
     umma_commit(&drained);
