@@ -12,9 +12,10 @@
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
 //
 // Codes become fp16 once for 256 rows: four warps load a step's codes into registers a step ahead,
-// convert them and write them as core matrices of 8 slots x 16 bytes, the two of a product's 16-deep step
-// side by side: over dims for K, a K-major operand whose N are slots, over slots for V, an MN-major
-// one whose N are dims, so no byte is transposed.
+// convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
+// K-major operand over dims (for K, whose N are slots) and an MN-major one over slots (for V, whose N
+// are dims), so no byte is transposed.
+//
 // Warps: 0-3 and 4-7 the rows of the halves, 8-11 codes, 12 issues the products.  With two S of a half
 // the scores of the next step are there before the powers of this one are written, so the rows never
 // wait for a product.  The four roles' loops have to stay small: unrolled further they left the
@@ -62,15 +63,15 @@ struct PromptShape {
   static constexpr uint32_t kRecord = kHalf * (DP + 2u);     // of a half: m[], l[], o[DP / 4][row] float4
 };
 
-// Descriptor of an operand stored as core matrices of 8 x 16 bytes, the two of a 16-deep step 128 bytes
-// apart, those of the next 8 rows (columns) 256; no swizzle, version 1.
-__device__ __forceinline__ uint64_t core_desc(uint32_t at) {
-  return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 16) |
-         (static_cast<uint64_t>(256u >> 4) << 32) | (1ull << 46);
+// Descriptor of an operand in panels of rows of 64 values (128 bytes, swizzled in groups of 8 rows, 1024
+// bytes): `panel` the bytes from panel to panel, used where columns are M or N; version 1, 128-byte swizzle.
+__device__ __forceinline__ uint64_t panel_desc(uint32_t at, uint32_t panel) {
+  return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | (static_cast<uint64_t>(panel >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-constexpr uint32_t kQDepth = kHalf * 32u, kKDepth = kStep * 32u;  // bytes of a 16-deep step of Q, of K
-template <int DP>
-constexpr uint32_t kVDepth = DP * 32u;                            // of V
+// the 16-byte piece of row r and values 8 c to 8 c + 7 of a panel
+__device__ __forceinline__ uint32_t in_panel(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
+constexpr uint32_t kQPanel = kHalf * 128u, kCodePanel = kStep * 128u;
 // fp16 operands, fp32 sums, M = 128
 constexpr uint32_t score_idesc() { return (1u << 4) | ((kStep >> 3) << 17) | ((kHalf >> 4) << 24); }
 template <int DP>
@@ -217,13 +218,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         const int power = top == 0.f ? 0 : max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
         const float by = a.scale_log2 < 0.f ? -power_of_two(-power) : power_of_two(-power);
         mult *= power_of_two(power);
-        uint8_t* const to = smem + Shape::q_at + half * Shape::kQBytes + (row >> 3) * 256u + (row & 7u) * 16u;
+        uint8_t* const to = smem + Shape::q_at + half * Shape::kQBytes;
         each([&](uint32_t i, uint4 w) {
           auto half2 = [&](uint32_t u) {
             const float2 x = two(u);
             return pack2(x.x * by, x.y * by, __half());
           };
-          *reinterpret_cast<uint4*>(to + (i >> 1) * kQDepth + (i & 1u) * 128u) = make_uint4(half2(w.x), half2(w.y), half2(w.z), half2(w.w));
+          *reinterpret_cast<uint4*>(to + (i >> 3) * kQPanel + in_panel(row, i & 7u)) = make_uint4(half2(w.x), half2(w.y), half2(w.z), half2(w.w));
         });
         fence_proxy_async_smem();
         mbar_arrive(&q_full[half]);
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         tmem_ld32(s_now, s[0]);
         tmem_ld32(s_now + 32u, s[1]);
         tmem_wait_ld();
-        if (!whole) {  // columns that the row does not see become minus infinity
+        if (__builtin_expect(!whole, 0)) {  // columns that the row does not see become minus infinity
           // the row's slots of the step: up to hi, from lo on or before `first`
           const int32_t hi = p - static_cast<int32_t>(slot0);
           const int32_t lo = a.window == 0u || hi < 0 || a.window > static_cast<uint32_t>(hi)
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         const float now = fmaxf(m, top);
         if (j == from_j) {
           m = now;
-        } else if (__any_sync(0xffffffffu, now > m + kSlack)) {
+        } else if (__builtin_expect(__any_sync(0xffffffffu, now > m + kSlack), 0)) {
           wait(&pv_full[half][(steps - 1u) & 1u], ((steps - 1u) >> 1) & 1u);  // the sums of the step before are in O
           tc_fence_after();
           const float fade = exp2_fast(m - (now == -CUDART_INF_F ? 0.f : now));
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           }
           tmem_st16(s_now + 16u * i, out);
         }
-        if (!whole) {  // a NaN value that some rows see and some do not was taken out of the codes
+        if (__builtin_expect(!whole, 0)) {  // a NaN value that some rows see and some do not was taken out of the codes
           const uint32_t stage = kt % kStages;
           wait(&v_full[stage], (kt / kStages) & 1u);
 #pragma unroll 1
@@ -442,40 +443,49 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
     const uint32_t w = warp - kCodeWarp0, r = lane & 7u, pq = lane >> 3;
     Segment8 s = use;
     uint32_t rem = left;
-    uint32_t id = 0, flags = 0;                              // flags: row i is seen by some, bit 2 + i: by all
+    // Of a step ahead: its group's page, first place on it, kv head and flags (row i is seen by some; bit 2 + i:
+    // by all), then where this thread's rows lie, and the scales.
+    uint32_t id = 0, on = 0, kv = 0, seen = 0, flags = 0;
     float ks = 0.f, vs = 1.f;
     uint64_t off = 0;
     uint4 kw[2][kMine], vw[2][kMine];
-    auto group = [&]() { return (s.block(s.j) << kLogStep) + 16u * w; };  // its first slot
-    auto look = [&]() {  // the group's page
-      id = 0xffffffffu;
-      if (s.some_see(group(), 16u)) {
-        id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + div_by(group(), c.page)]);
+    auto look = [&]() {  // at the step of s; goes on to the next
+      const uint32_t slot = (s.block(s.j) << kLogStep) + 16u * w, at = div_by(slot, c.page);
+      on = slot - at * c.page.d;
+      kv = s.kv;
+      seen = 0u;
+      if (s.all_see(a, slot, 16u)) {
+        seen = 15u;
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u; ++i) {
+          if (s.some_see(slot + 8u * i + r, 1u)) seen |= 1u << i;
+          if (s.all_see(a, slot + 8u * i + r, 1u)) seen |= 4u << i;
+        }
       }
+      // 16 slots of a page that some row sees have an id (rows of it may still be unseen)
+      id = c.num_pages;
+      if (s.some_see(slot, 16u)) {
+        id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + at]);
+        seen |= 16u;
+      }
+      ++s.j;
+      --rem;
+      if (s.j == s.j1) advance(s, rem);
     };
-    auto place = [&]() {  // where the rows lie, and the scales
-      const uint32_t slot = group(), at = div_by(slot, c.page), on = slot - at * c.page.d;
-      flags = 0u;
+    auto place = [&]() {  // of the step looked up last
+      flags = seen & 15u;
       ks = 0.f;
       vs = 1.f;
-      if (!s.some_see(slot, 16u)) return;
       if (id >= c.num_pages) {
-        atomicOr(&g_error_word, QG_ERR_PAGE);
+        flags = 0u;
+        if (seen > 15u) atomicOr(&g_error_word, QG_ERR_PAGE);
         return;
       }
-      off = id * c.page_bytes + s.kv * c.head_bytes + (on + r) * c.slot_bytes + pq * 16u;
-      const uint64_t in = id * cache.scale_page + s.kv * cache.scale_head + (on >> cache.log_block);
+      off = id * c.page_bytes + kv * c.head_bytes + (on + r) * c.slot_bytes + pq * 16u;
+      const uint64_t in = id * cache.scale_page + kv * cache.scale_head + (on >> cache.log_block);
       ks = cache.ks[in];
       vs = cache.vs[in];
-      if (s.all_see(a, slot, 16u)) {
-        flags = 15u;
-        return;
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {
-        if (s.some_see(slot + 8u * i + r, 1u)) flags |= 1u << i;
-        if (s.all_see(a, slot + 8u * i + r, 1u)) flags |= 4u << i;
-      }
     };
     auto load = [&](const uint8_t* pool, uint4 (&to)[2][kMine]) {
 #pragma unroll
@@ -489,54 +499,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         }
       }
     };
-    // piece p, 8-slot group 2 w + i: of K in step p at that group, of V in step w at chunks 2 p and 2 p + 1
-    uint8_t* const k_mem = smem + Shape::k_at + pq * kKDepth + 2u * w * 256u + r * 16u;
-    uint8_t* const v_mem = smem + Shape::v_at + w * kVDepth<DP> + 2u * pq * 256u + r * 16u;
-    auto store = [&](uint8_t* at, uint32_t per_i, uint32_t per_h, uint32_t beside, const uint4 (&from)[2][kMine]) {
+    // piece pq + 4 h is chunks 2 pq and 2 pq + 1 of panel h
+    const uint32_t store_at = (16u * w) * 128u, chunk0 = in_panel(r, 2u * pq), chunk1 = in_panel(r, 2u * pq + 1u);
+    auto store = [&](uint32_t at, const uint4 (&from)[2][kMine]) {
 #pragma unroll
       for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
         for (uint32_t h = 0; h < kMine; ++h) {
-          uint8_t* const to = at + h * per_h + i * per_i;
+          uint8_t* const to = smem + at + store_at + h * kCodePanel + i * 1024u;
           uint4 x, y;
           codes_to_half(from[i][h].x, x.x, x.y);
           codes_to_half(from[i][h].y, x.z, x.w);
           codes_to_half(from[i][h].z, y.x, y.y);
           codes_to_half(from[i][h].w, y.z, y.w);
-          *reinterpret_cast<uint4*>(to) = x;
-          *reinterpret_cast<uint4*>(to + beside) = y;
+          *reinterpret_cast<uint4*>(to + chunk0) = x;
+          *reinterpret_cast<uint4*>(to + chunk1) = y;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
     uint32_t stage = 0, round = 0;                           // kt = round * kStages + stage
-    if (rem != 0u) look();
-    for (bool first = true; rem != 0u; first = false) {      // a step's codes are stored once the next one's are asked for
-      if (first) {
-        place();
-        load(c.k, kw);
-        load(c.v, vw);
-      }
+    uint32_t more = rem != 0u ? 1u : 0u, after = 0u;         // there is a step; one after it
+    if (more != 0u) {
+      look();
+      place();
+      load(c.k, kw);
+      load(c.v, vw);
+      after = rem != 0u ? 1u : 0u;
+      if (after != 0u) look();
+    }
+    // A step's codes are stored while the next one's are loaded and the page of the one after is looked up.
+#pragma unroll 1
+    while (more != 0u) {
       const uint32_t ring = kt % kScaleRing, now_flags = flags;
       const float now_ks = ks, now_vs = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
-      ++s.j;
-      --rem;
-      if (s.j == s.j1) advance(s, rem);
-      if (rem != 0u) look();
+      more = after;
+      if (more != 0u) {
+        place();
+        after = rem != 0u ? 1u : 0u;
+        if (after != 0u) look();
+      }
       if (round != 0u) wait(&k_empty[stage], (round - 1u) & 1u);
       if (lane == 0u) {
         reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + w] = make_float4(now_ks, log2f(now_vs), 1.f / now_vs, 0.f);
       }
-      store(k_mem + stage * Shape::kCodeBytes, 256u, 4u * kKDepth, 128u, kw);
+      store(Shape::k_at + stage * Shape::kCodeBytes, kw);
       if (lane == 0u) {
         mbar_arrive(&k_full[stage]);
         mbar_arrive(&scale_full[ring]);
       }
-      if (rem != 0u) {
-        place();
-        load(c.k, kw);
-      }
+      if (more != 0u) load(c.k, kw);
       // NaN codes of rows that not all see: out of the codes, noted by column
       uint32_t odd = 0;
       if (now_flags != 15u) {
@@ -551,7 +564,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       }
       const bool flagged = __any_sync(0xffffffffu, odd != 0u);
       if (round != 0u) wait(&v_empty[stage], (round - 1u) & 1u);
-      if (flagged) {
+      if (__builtin_expect(flagged, 0)) {
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
@@ -572,9 +585,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         }
       }
       if (lane == 0u) nan_flag[stage][w] = flagged ? 1u : 0u;
-      store(v_mem + stage * Shape::kCodeBytes, 128u, 8u * 256u, 256u, vw);
+      store(Shape::v_at + stage * Shape::kCodeBytes, vw);
       if (lane == 0u) mbar_arrive(&v_full[stage]);
-      if (rem != 0u) load(c.v, vw);
+      if (more != 0u) load(c.v, vw);
       ++kt;
       if (++stage == kStages) stage = 0u, ++round;
     }
@@ -583,55 +596,65 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
     uint32_t parts[2] = {0u, 0u}, steps[2] = {0u, 0u};
     uint32_t k_stage = 0, k_round = 0, v_stage = 0, v_round = 0;
     const uint32_t base = smem_addr(smem);
-    const uint64_t q0 = core_desc(base + Shape::q_at), k0 = core_desc(base + Shape::k_at), v0 = core_desc(base + Shape::v_at);
+    const uint64_t q0 = panel_desc(base + Shape::q_at, kQPanel), k0 = panel_desc(base + Shape::k_at, kCodePanel);
+    const uint64_t v0 = panel_desc(base + Shape::v_at, kCodePanel);
     auto scores = [&](uint32_t half, uint32_t buffer) {  // of the K stage
       const uint64_t q = q0 + half * (Shape::kQBytes / 16u), k = k0 + k_stage * (Shape::kCodeBytes / 16u);
       const uint32_t s = tmem + half * kHalf + buffer * kStep;
-      if (*abort != 0u) return;
 #pragma unroll
-      for (uint32_t i = 0; i < DP / 16u; ++i) umma_ss(s, q + i * (kQDepth / 16u), k + i * (kKDepth / 16u), score_idesc(), i);
+      for (uint32_t i = 0; i < DP / 16u; ++i) {  // 32 bytes of the rows of panel i / 4
+        umma_ss(s, q + (i / 4u * kQPanel + i % 4u * 32u) / 16u, k + (i / 4u * kCodePanel + i % 4u * 32u) / 16u, score_idesc(), i);
+      }
     };
     auto values = [&](uint32_t half, uint32_t buffer, uint32_t more) {  // of the V stage
       const uint64_t v = v0 + v_stage * (Shape::kCodeBytes / 16u);
       const uint32_t p = tmem + half * kHalf + buffer * kStep, o = tmem + 2u * kHalf + half * kHalf;
-      if (*abort != 0u) return;
 #pragma unroll
-      for (uint32_t i = 0; i < kStep / 16u; ++i) umma_ts(o, p + 8u * i, v + i * (kVDepth<DP> / 16u), value_idesc<DP>(), more | i);
+      for (uint32_t i = 0; i < kStep / 16u; ++i) umma_ts(o, p + 8u * i, v + i * (2048u / 16u), value_idesc<DP>(), more | i);
     };
     for (; left != 0u; advance(use, left)) {
       const uint32_t count = min(use.j1 - use.j, left), halves = use.rows > kHalf ? 2u : 1u;
       left -= count;
-      for (uint32_t h = 0; h < halves; ++h) wait(&q_full[h], parts[h]++ & 1u);
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        if (h < halves) wait(&q_full[h], parts[h]++ & 1u);
+      }
       // step i's scores two ahead of its sums: S(i) is free once the sums of step i - 2 have been issued
 #pragma unroll 1
       for (uint32_t i = 0; i < count + 2u; ++i) {
-        if (i >= 2u) wait(&v_full[v_stage], v_round & 1u);
-        if (i < count) wait(&k_full[k_stage], k_round & 1u);
-#pragma unroll 1
-        for (uint32_t h = 0; h < halves; ++h) {
-          const uint32_t step = steps[h] + i;
-          if (i >= 2u) {
-            wait(&p_full[h][step & 1u], ((step - 2u) >> 1) & 1u);
+        const bool sums = i >= 2u, more = i < count;
+        if (sums) wait(&v_full[v_stage], v_round & 1u);
+        if (more) wait(&k_full[k_stage], k_round & 1u);
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+          if (h >= halves) break;
+          const uint32_t buffer = steps[h] & 1u;
+          if (sums) {
+            wait(&p_full[h][buffer], ((steps[h] - 2u) >> 1) & 1u);
             tc_fence_after();
-            values(h, step & 1u, i - 2u);
-            umma_commit(&pv_full[h][step & 1u]);
+            values(h, buffer, i - 2u);
+            umma_commit(&pv_full[h][buffer]);
           }
-          if (i < count) {
+          if (more) {
             tc_fence_after();
-            scores(h, step & 1u);
-            umma_commit(&s_full[h][step & 1u]);
+            scores(h, buffer);
+            umma_commit(&s_full[h][buffer]);
           }
+          ++steps[h];
         }
-        if (i >= 2u) {
+        if (sums) {
           umma_commit(&v_empty[v_stage]);
           if (++v_stage == kStages) v_stage = 0u, ++v_round;
         }
-        if (i < count) {
+        if (more) {
           umma_commit(&k_empty[k_stage]);
           if (++k_stage == kStages) k_stage = 0u, ++k_round;
         }
       }
-      for (uint32_t h = 0; h < halves; ++h) steps[h] += count;
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        if (h < halves) steps[h] -= 2u;
+      }
     }
     // what was issued ends before the CTA's memory goes, also after a wait that ran out
     umma_commit(&drained);
