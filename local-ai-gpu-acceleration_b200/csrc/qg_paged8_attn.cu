@@ -18,7 +18,7 @@
 // ldmatrix as 16-bit pairs, they are two slots x two dims; one byte permutation makes them pairs
 // of slots of even and of odd dims, and a lane's sums become four dims in a row.
 //
-// Work.  Segments, blocks of 128 slots, ranges of equal length for every CTA, four tiles of a
+// Work.  Segments, blocks of 256 slots (128 at head size 256), ranges of equal length for every CTA, four tiles of a
 // block for the four warps, records and joins as in qg_paged_attn.cu; a tile's rows may be several
 // tokens', with a mask for each where the tile touches the end of what any row sees.  A ragged
 // call's tiles are listed by a small kernel before (one CTA; it costs 2 to 3 us), a call of one row
@@ -39,13 +39,16 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kAttnThreads = kWarps * 32;
-constexpr uint32_t kLogTile = 5, kTile = 1u << kLogTile;    // slots of one warp's tile
-constexpr uint32_t kLogBlock = kLogTile + 2u;
+// Slots of one warp's tile: as many as 255 registers hold.  At head size 128 tiles of 32 slots took 236 us for
+// 16 x 32768 (TILE64 with 64): a tile's scores, sums and bookkeeping cost the same whatever its slots.
+constexpr uint32_t log_tile8(uint32_t dp, uint32_t rs, uint32_t terms) {
+  return dp == 256u || (dp == 128u && rs * terms == 4u) ? 5u : 6u;
+}
 constexpr uint32_t kMaxCtas = 512;
 constexpr uint32_t kJoinAll = 48;             // records of a tile that are joined at once
 constexpr uint32_t kJoin = 16;                // records of a group where there are more
 constexpr uint32_t kInFlight = 16;            // records whose sums are asked for together
-constexpr uint32_t kQueue = 64;               // tiles whose scales a warp keeps
+constexpr uint32_t kSet = 16, kQueue = 2u * kSet;  // tiles looked up together; whose scales a warp keeps
 static_assert(2u * kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "two counters per CTA");
 static_assert(kMaxCtas / kJoin <= 64u && kJoinAll <= 64u, "two records a lane");
 constexpr float kShare = 14.f;                // log2 of the factor that fp16 probabilities carry
@@ -65,9 +68,10 @@ template <int DP, int RS, int TERMS>
 struct Attn8Shape {
   static_assert(TERMS == 2 || RS == 2, "one term: 16 rows");
   static constexpr uint32_t kRows = 8u * RS;
+  static constexpr uint32_t kLogTile = log_tile8(DP, RS, TERMS), kTile = 1u << kLogTile, kLogBlock = kLogTile + 2u;
   static constexpr uint32_t kUnit = kTile * DP;             // a warp's K or V tile
   static constexpr int kCtasPerSm = DP == 64 && RS == 1 ? 3 : 2;
-  static constexpr uint32_t kUnits = DP == 256 ? 3 : DP == 128 ? 6 : kCtasPerSm == 3 ? 8 : 10;  // of its ring
+  static constexpr uint32_t kUnits = (kCtasPerSm == 3 ? 64u : 96u) * 1024u / (kWarps * kUnit);  // of its ring
   static constexpr uint32_t kSmem = kWarps * kUnits * kUnit + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kRowBytes = DP == 64 ? 64u : 128u;        // of a box
   static constexpr uint32_t kPanels = DP / kRowBytes;
@@ -82,6 +86,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
     paged_attn8_kernel(const Paged8View cache, const Attn8Args a, const __grid_constant__ AttnMaps8 maps) {
   using Shape = Attn8Shape<DP, RS, TERMS>;
   constexpr uint32_t kUnits = Shape::kUnits, kUnit = Shape::kUnit, kRows = Shape::kRows;
+  constexpr uint32_t kLogTile = Shape::kLogTile, kTile = Shape::kTile, kLogBlock = Shape::kLogBlock;
   constexpr uint32_t kRowBytes = Shape::kRowBytes, kPanels = Shape::kPanels, kPanel = kTile * kRowBytes;
   constexpr uint32_t kPieces = kRowBytes / 16u;             // 16-byte pieces of a row of a panel
   constexpr int kMma = TERMS == 2 ? RS : 1;                 // products for a tile
@@ -91,8 +96,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   extern __shared__ uint8_t smem_raw[];
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
   __shared__ __align__(8) uint64_t full[kWarps][kUnits];
-  __shared__ float2 k_queue[kWarps][kQueue];                // key scales of a tile's steps
-  __shared__ float4 v_queue[kWarps][kQueue];                // log2 of the value scales, their reciprocals
+  // of a tile's steps: key scales, log2 of the value scales, their reciprocals
+  __shared__ __align__(16) float ks_queue[kWarps][kQueue][kSteps], lg_queue[kWarps][kQueue][kSteps],
+      inv_queue[kWarps][kQueue][kSteps];
   __shared__ uint64_t sum64[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   auto look_up = [&]() {
     next_tiles = 0u;
     if (ahead_left == 0u) return;
-    next_tiles = min(min(32u >> a.log_boxes, ahead.j1 - ahead.j), ahead_left);
+    next_tiles = min(min(min(32u >> a.log_boxes, kSet), ahead.j1 - ahead.j), ahead_left);
     const uint32_t t = lane >> a.log_boxes;
     const uint32_t slot = (ahead.block(ahead.j + min(t, next_tiles - 1u)) << kLogBlock) + warp * kTile +
                           ((lane & (boxes - 1u)) << log_box);
@@ -263,14 +269,12 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
     const uint32_t t = lane >> a.log_boxes, to = (queued + t) % kQueue;
     if (t < wait_tiles) {
       const float vs = fminf(fmaxf(wait_vs, 0x1p-60f), 0x1p60f), lg = log2f(vs), inv = 1.f / vs;
-      if (boxes == 1u) {
-        k_queue[warp][to] = make_float2(wait_ks, wait_ks);
-        v_queue[warp][to] = make_float4(lg, lg, inv, inv);
-      } else {
-        const uint32_t e = lane & 1u;
-        reinterpret_cast<float*>(&k_queue[warp][to])[e] = wait_ks;
-        reinterpret_cast<float*>(&v_queue[warp][to])[e] = lg;
-        reinterpret_cast<float*>(&v_queue[warp][to])[2u + e] = inv;
+      const uint32_t per = kSteps >> a.log_boxes;  // steps of a box
+      for (uint32_t e = 0; e < per; ++e) {
+        const uint32_t at = (lane & (boxes - 1u)) * per + e;
+        ks_queue[warp][to][at] = wait_ks;
+        lg_queue[warp][to][at] = lg;
+        inv_queue[warp][to][at] = inv;
       }
     }
     queued += wait_tiles;
@@ -405,9 +409,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
       const bool whole = use.all_see(a, slot0, kTile);
       const bool seen = use.some_see(slot0, kTile);
       if (used == queued) flush();
-      const float2 ks = k_queue[warp][used % kQueue];
-      const float4 vs = v_queue[warp][used % kQueue];
-      ++used;
+      const uint32_t scales = used++ % kQueue;
       // ---- scores
       uint32_t p[kMma][kSteps][2][2];  // probabilities: [16-slot step][8-slot half][term or row]
       float fade[RS];
@@ -444,8 +446,13 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
         // ---- probabilities: this lane's slots are 8 n + 2 t4 and one more
 #pragma unroll
         for (int i = 0; i < RS; ++i) {
-          const float by[kSteps] = {mult[i] * ks.x, mult[i] * ks.y}, lg[kSteps] = {vs.x, vs.y};
-          const float inv[kSteps] = {vs.z, vs.w};
+          float by[kSteps], lg[kSteps], inv[kSteps];
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            by[st] = mult[i] * ks_queue[warp][scales][st];
+            lg[st] = lg_queue[warp][scales][st];
+            inv[st] = inv_queue[warp][scales][st];
+          }
           float x[2 * kSteps][2];
           float top = -CUDART_INF_F;
 #pragma unroll
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
           fade[i] = exp2_fast(m[i] - from);
           m[i] = now;
           const float base = kShare - from;
-          float sum[kSteps] = {0.f, 0.f};
+          float sum[kSteps] = {}, all = 0.f;
 #pragma unroll
           for (int n = 0; n < 2 * kSteps; ++n) {
             x[n][0] = exp2_fast(x[n][0] + base);
@@ -477,7 +484,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
               p[0][n / 2][n % 2][i] = pack2(x[n][0], x[n][1], __half());
             }
           }
-          l[i] = fmaf(l[i], fade[i], fmaf(sum[0], inv[0], sum[1] * inv[1]));
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) all = fmaf(sum[st], inv[st], all);
+          l[i] = fmaf(l[i], fade[i], all);
         }
       }
       if (RS == 2 && ends) {  // the sums of rows 8 to 15 join here
@@ -934,12 +943,12 @@ cudaError_t launch_attn8(const Paged8View& c, const Attn8Args& args, const AttnM
   a.tiles = (a.group.d + Shape::kRows - 1u) / Shape::kRows;
   const uint64_t tiles = a.offsets != nullptr ? most_tiles(a.tokens, c.c.batch, a.group.d, Shape::kRows)
                                               : static_cast<uint64_t>(a.tokens) * a.tiles;
-  const uint64_t blocks = tiles * c.c.n_kv * ((c.c.capacity + (1u << kLogBlock) - 1u) >> kLogBlock);
+  const uint64_t blocks = tiles * c.c.n_kv * ((c.c.capacity + (1u << Shape::kLogBlock) - 1u) >> Shape::kLogBlock);
   const uint64_t fit = static_cast<uint64_t>(paged_sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
   if (blocks / grid >= (1ull << 29)) return cudaErrorInvalidValue;  // a CTA counts its units in 32 bits
   if (a.offsets != nullptr) {
-    e = launch_plan8(c, a, Shape::kRows, kLogBlock, stream);
+    e = launch_plan8(c, a, Shape::kRows, Shape::kLogBlock, stream);
     if (e != cudaSuccess) return e;
   }
   return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);
@@ -980,8 +989,13 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
   }
   PoolStrides8 strides;
   if (!pool_strides8(cache, &strides)) return cudaErrorInvalidValue;
+  // rows of a kv head: a call of one row a sequence has its group
+  const uint32_t group = p->n_q_heads / c.c.n_kv;
+  const bool few = p->offsets == nullptr && group <= 8u, wide = p->dtype == QG_F32;
+  const uint32_t rs = few || (wide && plan.dp == 256u) ? 1u : 2u, terms = few || wide ? 2u : 1u;
   // a box is part of one tile, page and scale block
-  const uint32_t log_box = std::min<uint32_t>(kLogTile, __builtin_ctz(cache->block));
+  const uint32_t log_tile = log_tile8(plan.dp, rs, terms);
+  const uint32_t log_box = std::min<uint32_t>(log_tile, __builtin_ctz(cache->block));
   AttnMaps8 maps;
   if (!encode_pool8(&maps.k, cache->k, cache, strides, 1u << log_box, plan.dp) ||
       !encode_pool8(&maps.v, cache->v, cache, strides, 1u << log_box, plan.dp)) {
@@ -1000,7 +1014,7 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
   a.window = p->window;
   a.sink = p->sink;
   a.n_q = p->n_q_heads;
-  a.group = fast_div(p->n_q_heads / c.c.n_kv);
+  a.group = fast_div(group);
   a.scale_log2 = p->scale * 1.44269504088896340736f;
   a.lse = p->lse;
   a.arrived = reinterpret_cast<uint32_t*>(ws);
@@ -1012,23 +1026,19 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
     a.seq_tiles = reinterpret_cast<uint32_t*>(ws + plan.seqs_at);
     a.max_items = plan.max_items;
   }
-  a.log_boxes = kLogTile - log_box;
+  a.log_boxes = log_tile - log_box;
   a.heads_inside = strides.heads_inside;
   if (p->offsets != nullptr && p->dtype != QG_F32 && prompt8_fits(plan.dp, p->tokens, cache->batch, a.group.d)) {
     a.records = reinterpret_cast<float*>(ws + plan.prompt_at);
     return launch_prompt8(c, a, plan.dp, stream);
   }
-  // rows of a kv head: a call of one row a sequence has its group
-  const bool few = p->offsets == nullptr && a.group.d <= 8u;
-  const bool wide = p->dtype == QG_F32;
   if (plan.dp == 64u) {
-    if (few) return launch_attn8<64, 1, 2>(c, a, maps, stream);
-    return wide ? launch_attn8<64, 2, 2>(c, a, maps, stream) : launch_attn8<64, 2, 1>(c, a, maps, stream);
+    if (rs == 1u) return launch_attn8<64, 1, 2>(c, a, maps, stream);
+    return terms == 2u ? launch_attn8<64, 2, 2>(c, a, maps, stream) : launch_attn8<64, 2, 1>(c, a, maps, stream);
   }
   if (plan.dp == 128u) {
-    if (few) return launch_attn8<128, 1, 2>(c, a, maps, stream);
-    return wide ? launch_attn8<128, 2, 2>(c, a, maps, stream) : launch_attn8<128, 2, 1>(c, a, maps, stream);
+    if (rs == 1u) return launch_attn8<128, 1, 2>(c, a, maps, stream);
+    return terms == 2u ? launch_attn8<128, 2, 2>(c, a, maps, stream) : launch_attn8<128, 2, 1>(c, a, maps, stream);
   }
-  if (few || wide) return launch_attn8<256, 1, 2>(c, a, maps, stream);
-  return launch_attn8<256, 2, 1>(c, a, maps, stream);
+  return rs == 1u ? launch_attn8<256, 1, 2>(c, a, maps, stream) : launch_attn8<256, 2, 1>(c, a, maps, stream);
 }
