@@ -48,7 +48,7 @@ constexpr uint32_t kMaxCtas = 512;
 constexpr uint32_t kJoinAll = 48;             // records of a tile that are joined at once
 constexpr uint32_t kJoin = 16;                // records of a group where there are more
 constexpr uint32_t kInFlight = 16;            // records whose sums are asked for together
-constexpr uint32_t kSet = 16, kQueue = 2u * kSet;  // tiles looked up together; whose scales a warp keeps
+constexpr uint32_t kEntries = 64;             // 16-slot steps whose places and scales a warp keeps
 static_assert(2u * kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "two counters per CTA");
 static_assert(kMaxCtas / kJoin <= 64u && kJoinAll <= 64u, "two records a lane");
 constexpr float kShare = 14.f;                // log2 of the factor that fp16 probabilities carry
@@ -62,6 +62,13 @@ __device__ __forceinline__ int power_of8(float top) {
   return top == 0.f ? 0 : max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
 }
 
+// As mma() without `volatile`: the products of a tile may be put in any order, between the loads.
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // DP: head_dim rounded up to 64, 128 or 256.  RS: rows of a lane (8 RS rows a tile).  TERMS: fp16
 // terms of a query and of a probability.
 template <int DP, int RS, int TERMS>
@@ -71,13 +78,15 @@ struct Attn8Shape {
   static constexpr uint32_t kLogTile = log_tile8(DP, RS, TERMS), kTile = 1u << kLogTile, kLogBlock = kLogTile + 2u;
   static constexpr uint32_t kUnit = kTile * DP;             // a warp's K or V tile
   static constexpr int kCtasPerSm = DP == 64 && RS == 1 ? 3 : 2;
-  static constexpr uint32_t kUnits = (kCtasPerSm == 3 ? 64u : 96u) * 1024u / (kWarps * kUnit);  // of its ring
-  static constexpr uint32_t kSmem = kWarps * kUnits * kUnit + 1024u;  // the ring starts on 1024 bytes
+  // K and V tiles of a warp's ring: V of the tile in work, K of the next one too, more where they fit
+  static constexpr uint32_t kUnits = (kCtasPerSm == 3 ? 64u : 96u) * 1024u / (kWarps * kUnit);
+  static constexpr uint32_t kK = kUnits >= 6u ? 4u : 2u, kV = kUnits >= 4u ? 2u : 1u;
+  static constexpr uint32_t kSmem = kWarps * (kK + kV) * kUnit + 1024u;  // the ring starts on 1024 bytes
   static constexpr uint32_t kRowBytes = DP == 64 ? 64u : 128u;        // of a box
   static constexpr uint32_t kPanels = DP / kRowBytes;
   static constexpr uint32_t kRecord = kRows * (DP + 2u);    // m[], l[], o[][]
   // what a segment costs beside its blocks, in blocks
-  static constexpr uint32_t kHeader = 3;
+  static constexpr uint32_t kHeader = 2;
   static_assert(8u * DP * 4u <= kUnit, "the sums of eight rows join in a free unit");
 };
 
@@ -85,21 +94,23 @@ template <int DP, int RS, int TERMS>
 __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtasPerSm)
     paged_attn8_kernel(const Paged8View cache, const Attn8Args a, const __grid_constant__ AttnMaps8 maps) {
   using Shape = Attn8Shape<DP, RS, TERMS>;
-  constexpr uint32_t kUnits = Shape::kUnits, kUnit = Shape::kUnit, kRows = Shape::kRows;
+  constexpr uint32_t kUnit = Shape::kUnit, kRows = Shape::kRows, kK = Shape::kK, kV = Shape::kV;
   constexpr uint32_t kLogTile = Shape::kLogTile, kTile = Shape::kTile, kLogBlock = Shape::kLogBlock;
   constexpr uint32_t kRowBytes = Shape::kRowBytes, kPanels = Shape::kPanels, kPanel = kTile * kRowBytes;
   constexpr uint32_t kPieces = kRowBytes / 16u;             // 16-byte pieces of a row of a panel
   constexpr int kMma = TERMS == 2 ? RS : 1;                 // products for a tile
   constexpr int kSteps = kTile / 16;                        // 16-slot steps
   constexpr uint32_t kChunks = DP / 16;                     // 16-dim chunks
+  constexpr uint32_t kSet = 32u / kSteps, kTiles = kEntries / kSteps;  // tiles looked up together; that are kept
   const PagedView& c = cache.c;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
-  __shared__ __align__(8) uint64_t full[kWarps][kUnits];
-  // of a tile's steps: key scales, log2 of the value scales, their reciprocals
-  __shared__ __align__(16) float ks_queue[kWarps][kQueue][kSteps], lg_queue[kWarps][kQueue][kSteps],
-      inv_queue[kWarps][kQueue][kSteps];
+  __shared__ __align__(8) uint64_t full_k[kWarps][kK], full_v[kWarps][kV];
+  // of the steps of a warp's next tiles: {page, place, head}; key scale, log2 of the value scale, its reciprocal
+  __shared__ int4 where[kWarps][kEntries];
+  __shared__ __align__(16) float ks_of[kWarps][kEntries], lg_of[kWarps][kEntries], inv_of[kWarps][kEntries];
   __shared__ uint64_t sum64[kWarps];
+  __shared__ uint32_t most_of[kWarps];
   __shared__ uint32_t first_at[3];
   __shared__ uint32_t is_last;
   __shared__ float share[kRows][64];
@@ -107,10 +118,11 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   const uint32_t tid = threadIdx.x, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
   const uint32_t warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  uint8_t* const ring = smem + warp * (kUnits * kUnit);
+  uint8_t* const ring = smem + warp * ((kK + kV) * kUnit);   // kK tiles of K, kV of V
   const uint32_t ring_at = smem_addr(ring);
   if (lane == 0u) {
-    for (uint32_t i = 0; i < kUnits; ++i) mbar_init(&full[warp][i], 1u);
+    for (uint32_t i = 0; i < kK; ++i) mbar_init(&full_k[warp][i], 1u);
+    for (uint32_t i = 0; i < kV; ++i) mbar_init(&full_v[warp][i], 1u);
     fence_mbar_init();
   }
   if (tid < 2u) {
@@ -121,10 +133,10 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
 
   const bool ragged = a.items != nullptr;
   const uint32_t lines = ragged ? c.n_kv : c.n_kv * a.tiles;  // segments of an item (a tile, a sequence)
-  // the segment (s.item, s.line); `fresh`: the item is another one than before
-  auto make = [&](Segment8& s, bool fresh) {
+  // the segment (s.item, s.line) in steps of 2^log slots; `fresh`: the item is another one than before
+  auto make = [&](Segment8& s, bool fresh, uint32_t log) {
     if (ragged) {
-      take_item8(a, s, fresh, kLogBlock);
+      take_item8(a, s, fresh, log);
       return;
     }
     if (fresh) {
@@ -134,15 +146,22 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
     s.kv = s.line / a.tiles;
     s.sub = (s.line - s.kv * a.tiles) * kRows;
     s.rows = min(kRows, a.group.d - s.sub);
-    s.bounds(a, kLogBlock);
+    s.bounds(a, log);
     s.j = 0u;
   };
 
   // ---- this CTA's range [r0, r1) of the line of units: the blocks of all segments, and headers
-  // before each segment's
+  // before each segment's; or, where segments are short and many, whole segments for every warp
   uint64_t total = 0, ctas = 0, r0 = 0, r1 = 0;
   uint32_t header = 0;
-  auto cut = [&](uint64_t blocks, uint64_t segments) {  // false where nothing is left for this CTA
+  bool solo = false;
+  auto cut = [&](uint64_t blocks, uint64_t segments, uint32_t most) {  // false where nothing is left for this CTA
+    // Time in 1500 cycles: a tile (a block of a CTA) takes 3, a segment 4 in a warp and 5 in a CTA.  With every
+    // segment taken for the longest, a segment a warp has to be the faster way.
+    const uint64_t busy = min(static_cast<uint64_t>(gridDim.x), blocks);
+    const uint64_t rounds = (segments + gridDim.x * kWarps - 1u) / (gridDim.x * kWarps);
+    solo = rounds * (most * 3ull + 4u) * busy <= blocks * 3u + segments * 5u;
+    if (solo) return true;
     // fewer blocks than CTAs: a block each; otherwise segments cost more than their blocks
     if (blocks > gridDim.x) header = Shape::kHeader;
     total = blocks + header * segments;
@@ -153,31 +172,41 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
     return true;
   };
   Segment8 use;
-  uint32_t in_segment = 0;  // units of the first segment before the range
+  uint32_t in_segment = 0, segments = 0;  // units of the first segment before the range
   if (ragged) {
-    const uint32_t n = *a.item_count;
-    if (n == 0u || !cut(a.item_blocks[n] * lines, static_cast<uint64_t>(n) * lines)) return;
-    find_unit8(a, n, lines, header, r0, use.item, use.line, in_segment);
+    const uint32_t n = a.item_count[0];
+    if (n == 0u) return;
+    segments = n * lines;
+    if (!cut(a.item_blocks[n] * lines, segments, a.item_count[1])) return;
+    if (!solo) find_unit8(a, n, lines, header, r0, use.item, use.line, in_segment);
   } else {
+    uint32_t most = 0;
     auto blocks_of = [&](uint32_t b) {
       Segment8 s;
       s.item = b;
       s.line = 0u;
-      make(s, true);
+      make(s, true, kLogTile);
+      most = max(most, s.j1);
+      s.bounds(a, kLogBlock);
       return s.j1;
     };
     uint64_t blocks = 0;  // of one line of every sequence
-    for (uint32_t b = tid; b < c.batch && b < a.tokens; b += kAttnThreads) blocks += blocks_of(b);
+    for (uint32_t b = tid; b < a.tokens; b += kAttnThreads) blocks += blocks_of(b);
     const uint64_t mine = blocks;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) blocks += __shfl_xor_sync(0xffffffffu, blocks, off);
-    if (lane == 0u) sum64[warp] = blocks;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0u) sum64[warp] = blocks, most_of[warp] = most;
     __syncthreads();
     blocks = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) blocks += sum64[w];
-    if (!cut(blocks * lines, static_cast<uint64_t>(a.tokens) * lines)) return;
-    for (uint64_t base = 0, b0 = 0; b0 < a.tokens; b0 += kAttnThreads) {
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      blocks += sum64[w];
+      most = max(most, most_of[w]);
+    }
+    segments = a.tokens * lines;
+    if (!cut(blocks * lines, segments, most)) return;
+    for (uint64_t base = 0, b0 = 0; !solo && b0 < a.tokens; b0 += kAttnThreads) {
       const uint32_t b = static_cast<uint32_t>(b0) + tid;
       const uint64_t n = b < a.tokens ? (a.tokens <= kAttnThreads ? mine : blocks_of(b)) : 0u;
       uint64_t upto = n;
@@ -207,116 +236,141 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
       if ((base + static_cast<uint64_t>(header) * (b0 + kAttnThreads)) * lines > r0) break;
     }
     __syncthreads();
-    use.item = first_at[0];
-    use.line = first_at[1];
-    in_segment = first_at[2];
+    if (!solo) {
+      use.item = first_at[0];
+      use.line = first_at[1];
+      in_segment = first_at[2];
+    }
   }
-  make(use, true);
-  uint32_t left = static_cast<uint32_t>(r1 - r0);  // units of the range from use.j on (below 2^31)
+  const uint32_t log_step = solo ? kLogTile : kLogBlock, warp_slot = solo ? 0u : warp * kTile;
+  uint32_t left;  // units of the range, or steps of the segment, from use.j on (below 2^31)
+  uint32_t index = warp * gridDim.x + blockIdx.x;  // of a lone warp's segment
   auto skip_header = [&](uint32_t& units, uint32_t done) { units -= min(units, header - min(done, header)); };
-  skip_header(left, in_segment);
-  use.j = in_segment - min(in_segment, header);
+  // segment `at` of the line for a lone warp
+  auto take = [&](Segment8& s, uint32_t at, uint32_t& units) {
+    units = 0u;
+    if (at >= segments) return;
+    s.item = at / lines;
+    s.line = at - s.item * lines;
+    make(s, true, kLogTile);
+    units = s.j1;
+  };
   // the segment after one that is done
-  auto advance = [&](Segment8& s, uint32_t& units) {
+  auto advance = [&](Segment8& s, uint32_t& at, uint32_t& units) {
+    if (solo) {
+      at += gridDim.x * kWarps;
+      take(s, at, units);
+      return;
+    }
     skip_header(units, 0u);
     if (units == 0u) return;
     const bool fresh = ++s.line == lines;
     if (fresh) s.line = 0u, ++s.item;
-    make(s, fresh);
+    make(s, fresh, kLogBlock);
   };
+  if (solo) {
+    take(use, index, left);
+  } else {
+    make(use, true, kLogBlock);
+    left = static_cast<uint32_t>(r1 - r0);
+    skip_header(left, in_segment);
+    use.j = in_segment - min(in_segment, header);
+  }
 
-  // ---- fetching.  A set of page ids and scales covers the next 32 boxes of this warp's tiles, a
-  // box a lane; the set after it is read while this one is used.  Scales go through a queue in
-  // shared memory, a set behind the ids, because they are found through them.
+  // ---- fetching.  The page ids of the next 32 steps of this warp's tiles are asked for a set ahead, a step
+  // a lane; a set that is settled has its places in `where` and asks for its scales, which go to
+  // shared memory with the next set, or when the first of its tiles needs them.
   const uint64_t policy = l2_evict_first_policy();
-  const uint32_t boxes = 1u << a.log_boxes, log_box = kLogTile - a.log_boxes;
+  const uint32_t boxes = 1u << a.log_boxes;
   Segment8 ahead = use;
-  uint32_t ahead_left = left;
-  int32_t page = 0, place = 0, head = 0, next_page = 0, next_place = 0, next_head = 0;
-  uint32_t at_tile = 0, tiles = 0, next_tiles = 0;     // of the set
-  float next_ks = 0.f, next_vs = 0.f, wait_ks = 0.f, wait_vs = 0.f;
-  uint32_t wait_tiles = 0, queued = 0, used = 0;       // tiles of the range: in wait_*, in the queue, worked on
-  auto look_up = [&]() {
-    next_tiles = 0u;
+  uint32_t ahead_left = left, ahead_index = index;
+  int32_t ask_page = 0, ask_place = 0, ask_head = 0;
+  bool ask_scales = false;
+  uint32_t ask_tiles = 0, settled = 0, scaled = 0;          // tiles asked for; with places; with scales
+  float wait_ks = 0.f, wait_vs = 1.f;                        // of tiles [scaled, settled)
+  auto ask = [&]() {
+    ask_tiles = 0u;
     if (ahead_left == 0u) return;
-    next_tiles = min(min(min(32u >> a.log_boxes, kSet), ahead.j1 - ahead.j), ahead_left);
-    const uint32_t t = lane >> a.log_boxes;
-    const uint32_t slot = (ahead.block(ahead.j + min(t, next_tiles - 1u)) << kLogBlock) + warp * kTile +
-                          ((lane & (boxes - 1u)) << log_box);
-    const uint32_t at = div_by(slot, c.page);
-    next_page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
-    next_place = static_cast<int32_t>(slot - at * c.page.d);
-    next_head = static_cast<int32_t>(ahead.kv);
-    next_ks = 0.f;
-    next_vs = 1.f;
-    if (t < next_tiles && ahead.some_see(slot, 1u << log_box)) {
+    ask_tiles = min(min(kSet, ahead.j1 - ahead.j), ahead_left);
+    const uint32_t step = min(lane / kSteps, ask_tiles - 1u);
+    const uint32_t slot = (ahead.block(ahead.j + step) << log_step) + warp_slot + lane % kSteps * 16u;
+    const uint32_t at = div_by(slot, c.page), box = kTile >> a.log_boxes;
+    ask_page = static_cast<int32_t>(c.num_pages);  // past the pool: a box of zeros
+    ask_place = static_cast<int32_t>(slot - at * c.page.d);
+    ask_head = static_cast<int32_t>(ahead.kv);
+    ask_scales = false;
+    if (ahead.some_see(slot & ~(box - 1u), box)) {
       const uint32_t id = static_cast<uint32_t>(c.table[static_cast<size_t>(ahead.b) * c.table_stride + at]);
       if (id < c.num_pages) {
-        next_page = static_cast<int32_t>(id);
-        const uint64_t s = id * cache.scale_page + ahead.kv * cache.scale_head +
-                           (static_cast<uint32_t>(next_place) >> cache.log_block);
-        next_ks = cache.ks[s];
-        next_vs = cache.vs[s];
+        ask_page = static_cast<int32_t>(id);
+        ask_scales = ahead.some_see(slot, 16u);
       } else {
         atomicOr(&g_error_word, QG_ERR_PAGE);
       }
     }
-    ahead.j += next_tiles;
-    ahead_left -= next_tiles;
-    if (ahead.j == ahead.j1) advance(ahead, ahead_left);
+    ahead.j += ask_tiles;
+    ahead_left -= ask_tiles;
+    if (ahead.j == ahead.j1) advance(ahead, ahead_index, ahead_left);
   };
-  auto flush = [&]() {  // the waiting scales into the queue
-    const uint32_t t = lane >> a.log_boxes, to = (queued + t) % kQueue;
-    if (t < wait_tiles) {
-      const float vs = fminf(fmaxf(wait_vs, 0x1p-60f), 0x1p60f), lg = log2f(vs), inv = 1.f / vs;
-      const uint32_t per = kSteps >> a.log_boxes;  // steps of a box
-      for (uint32_t e = 0; e < per; ++e) {
-        const uint32_t at = (lane & (boxes - 1u)) * per + e;
-        ks_queue[warp][to][at] = wait_ks;
-        lg_queue[warp][to][at] = lg;
-        inv_queue[warp][to][at] = inv;
-      }
+  auto flush = [&]() {  // the scales that have been waited for
+    if (lane / kSteps < settled - scaled) {
+      const uint32_t at = (scaled * kSteps + lane) % kEntries;
+      const float vs = fminf(fmaxf(wait_vs, 0x1p-60f), 0x1p60f);
+      ks_of[warp][at] = wait_ks;
+      lg_of[warp][at] = log2f(vs);
+      inv_of[warp][at] = 1.f / vs;
     }
-    queued += wait_tiles;
-    wait_tiles = 0u;
+    scaled = settled;
     __syncwarp();
   };
-  auto next_set = [&]() {
+  auto settle = [&]() {
     flush();
-    page = next_page;
-    place = next_place;
-    head = next_head;
-    tiles = wait_tiles = next_tiles;
-    wait_ks = next_ks;
-    wait_vs = next_vs;
-    at_tile = 0;
-    look_up();
+    if (lane / kSteps < ask_tiles) {
+      where[warp][(settled * kSteps + lane) % kEntries] = make_int4(ask_page, ask_place, ask_head, 0);
+      wait_ks = 0.f;
+      wait_vs = 1.f;
+      if (ask_scales) {
+        const uint64_t s = static_cast<uint32_t>(ask_page) * cache.scale_page + static_cast<uint32_t>(ask_head) * cache.scale_head +
+                           (static_cast<uint32_t>(ask_place) >> cache.log_block);
+        wait_ks = cache.ks[s];
+        wait_vs = cache.vs[s];
+      }
+    }
+    settled += ask_tiles;
+    __syncwarp();
+    ask();
   };
-  // the K (before its V) or V tile of the next block into unit u
-  auto fetch = [&](uint32_t u, bool is_v) {
-    if (!is_v && at_tile == tiles) next_set();
-    if (at_tile == tiles) return;  // the range is fetched
-    const uint32_t to = ring_at + u * kUnit, bar = smem_addr(&full[warp][u]);
-    const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+  auto fetch = [&](const CUtensorMap* map, uint64_t* bar, uint32_t to, uint32_t tile) {
     const bool leads = elect_one();
-    if (leads) mbar_arrive_expect_tx(&full[warp][u], kUnit);
-    for (uint32_t i = 0; i < boxes; ++i) {  // one lane asks: a copy takes warp-uniform operands
-      const uint32_t from = ((at_tile << a.log_boxes) + i) & 31u;
-      const int32_t pg = __shfl_sync(0xffffffffu, page, from), pl = __shfl_sync(0xffffffffu, place, from);
+    if (leads) mbar_arrive_expect_tx(bar, kUnit);
+#pragma unroll 1
+    for (uint32_t i = 0; i < boxes; ++i) {
+      const int4 at = where[warp][(tile * kSteps + (i * kSteps >> a.log_boxes)) % kEntries];
       if (leads) {
 #pragma unroll
         for (uint32_t p = 0; p < kPanels; ++p) {
-          tma_load_4d(to + p * kPanel + (i << log_box) * kRowBytes, map, static_cast<int32_t>(p * kRowBytes),
-                      a.heads_inside ? head : pl, a.heads_inside ? pl : head, pg, bar, policy);
+          tma_load_4d(to + p * kPanel + (i * kTile >> a.log_boxes) * kRowBytes, map, static_cast<int32_t>(p * kRowBytes),
+                      a.heads_inside ? at.z : at.y, a.heads_inside ? at.y : at.z, at.x, smem_addr(bar), policy);
         }
       }
     }
-    if (is_v) ++at_tile;
   };
-  look_up();
-#pragma unroll
-  for (uint32_t u = 0; u < kUnits; ++u) fetch(u, (u & 1u) != 0u);
-  bool fetch_v = (kUnits & 1u) != 0u;  // what the next free unit receives
+  uint32_t tile = 0, next_k = 0, next_v = 0;                 // this warp's tile in work; the next ones to fetch
+  auto refill = [&]() {  // what tile `tile` and the ring leave room for
+    while (next_k < tile + kK) {
+      if (next_k == settled) {
+        if (ask_tiles == 0u) break;
+        settle();
+      }
+      fetch(&maps.k, &full_k[warp][next_k % kK], ring_at + next_k % kK * kUnit, next_k);
+      ++next_k;
+    }
+    while (next_v < min(tile + kV, settled)) {
+      fetch(&maps.v, &full_v[warp][next_v % kV], ring_at + (kK + next_v % kV) * kUnit, next_v);
+      ++next_v;
+    }
+  };
+  ask();
 
   // ldmatrix rows and 16-byte pieces of this lane (K: 8 slots x 2 pieces x 2; V, transposed:
   // 16 slots x 2 pieces); pieces 2 n and 2 n + 1 of a panel are at lane_at ^ (n << 5)
@@ -330,27 +384,22 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   uint32_t qa[kMma][kChunks][4];
   float o[RS][DP / 8][2], m[RS], l[RS], mult[RS];
   int32_t p_row[RS];                                        // slot of the row's token
-  uint32_t unit = 0, parity = 0;
-  bool arrives = true;
-  auto await_unit = [&]() {
-    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[warp][unit], parity))) {
-      arrives = arrives && __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][unit], parity));
-    }
-  };
-  auto refill = [&](uint32_t u, bool written) {
-    if (written) fence_proxy_async_smem();
-    __syncwarp();
-    if (arrives) fetch(u, fetch_v);
-    fetch_v = !fetch_v;
-  };
-  auto next_unit = [&]() {
-    if (++unit == kUnits) {
-      unit = 0;
-      parity ^= 1u;
+  bool arrives = true, written = false;  // written: by this warp, where a tile will land
+  auto await = [&](uint64_t* bar, uint32_t parity) {
+    if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+      arrives = arrives && __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
     }
   };
 
+  auto go_on = [&]() {  // what has been used is fetched into
+    if (written) fence_proxy_async_smem();
+    __syncwarp();
+    written = false;
+    if (arrives) refill();
+  };
+
   while (left != 0u) {
+    go_on();
     const uint32_t from_j = use.j, to_j = min(use.j1, use.j + left);
     // ---- the queries, as the A operand takes them: of chunk k this lane has dims 16 k + 4 t4 to
     // + 3 of its rows
@@ -402,18 +451,17 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
       for (uint32_t n = 0; n < DP / 8; ++n) o[i][n][0] = o[i][n][1] = 0.f;
     }
 
-    uint32_t k_unit = 0;
-    for (; use.j < to_j; ++use.j) {
-      const bool ends = use.j + 1u == to_j;
-      const uint32_t slot0 = (use.block(use.j) << kLogBlock) + warp * kTile;
+
+    while (true) {
+      const uint32_t slot0 = (use.block(use.j) << log_step) + warp_slot;
       const bool whole = use.all_see(a, slot0, kTile);
       const bool seen = use.some_see(slot0, kTile);
-      if (used == queued) flush();
-      const uint32_t scales = used++ % kQueue;
+      if (tile == scaled) flush();
+      const uint32_t scales = tile * kSteps % kEntries;
       // ---- scores
       uint32_t p[kMma][kSteps][2][2];  // probabilities: [16-slot step][8-slot half][term or row]
       float fade[RS];
-      await_unit();
+      await(&full_k[warp][tile % kK], tile / kK & 1u);
       if (seen && arrives) {
         float s[kMma][2 * kSteps][4];
 #pragma unroll
@@ -424,21 +472,28 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
             for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
           }
         }
-        const uint32_t k_at = ring_at + unit * kUnit;
-#pragma unroll
-        for (uint32_t kk = 0; kk < kChunks / 2u; ++kk) {
+        const uint32_t k_at = ring_at + tile % kK * kUnit;
+        uint32_t kb[2][kSteps][4];  // the next pair of chunks is loaded while this one is multiplied
+        auto load_k = [&](uint32_t kk) {
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) {
-            uint32_t kb[4];
-            ldsm_x4(kb, k_at + (k_lane ^ ((kk % kPairs) << 5)) + kk / kPairs * kPanel + st * 16u * kRowBytes);
+            ldsm_x4(kb[kk & 1u][st], k_at + (k_lane ^ ((kk % kPairs) << 5)) + kk / kPairs * kPanel + st * 16u * kRowBytes);
+          }
+        };
+        load_k(0u);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // slots 8 (e / 2), chunk 2 kk + e % 2
-              uint32_t lo, hi;
-              codes_to_half(kb[e], lo, hi);
+        for (uint32_t kk = 0; kk < kChunks / 2u; ++kk) {
+          if (kk + 1u < kChunks / 2u) load_k(kk + 1u);
 #pragma unroll
-              for (int i = 0; i < kMma; ++i) {
-                const uint32_t* q = qa[i][2 * kk + e % 2];
-                mma(s[i][2 * st + e / 2], q[0], q[1], q[2], q[3], lo, hi, __half());
+          for (int f = 0; f < 2; ++f) {          // chunk 2 kk + f
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {      // slots 8 e of the step
+                uint32_t lo, hi;
+                codes_to_half(kb[kk & 1u][st][2 * e + f], lo, hi);
+#pragma unroll
+                for (int i = 0; i < kMma; ++i) mma8(s[i][2 * st + e], qa[i][2 * kk + f], lo, hi);
               }
             }
           }
@@ -449,9 +504,9 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
           float by[kSteps], lg[kSteps], inv[kSteps];
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) {
-            by[st] = mult[i] * ks_queue[warp][scales][st];
-            lg[st] = lg_queue[warp][scales][st];
-            inv[st] = inv_queue[warp][scales][st];
+            by[st] = mult[i] * ks_of[warp][scales + st];
+            lg[st] = lg_of[warp][scales + st];
+            inv[st] = inv_of[warp][scales + st];
           }
           float x[2 * kSteps][2];
           float top = -CUDART_INF_F;
@@ -489,19 +544,11 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
           l[i] = fmaf(l[i], fade[i], all);
         }
       }
-      if (RS == 2 && ends) {  // the sums of rows 8 to 15 join here
-        __syncwarp();
-        k_unit = unit;
-      } else {
-        refill(unit, false);
-      }
-      next_unit();
 
       // ---- weighted values
-      await_unit();
-      bool written = false;  // by this warp, where the next box will land
+      await(&full_v[warp][tile % kV], tile / kV & 1u);
       if (seen && arrives) {
-        uint8_t* const v_mem = ring + unit * kUnit;
+        uint8_t* const v_mem = ring + (kK + tile % kV) * kUnit;
         if (!whole) {  // 0 x NaN must not reach the sums: what no row sees is cleared
           written = true;
           bool odd = false;  // a NaN that some rows see and some do not
@@ -543,13 +590,21 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
             __syncwarp();
           }
         }
-        const uint32_t v_at = ring_at + unit * kUnit;
-#pragma unroll
-        for (uint32_t n = 0; n < kChunks / 2u; ++n) {
-          uint32_t vb[kSteps][4];
+        const uint32_t v_at = ring_at + (kK + tile % kV) * kUnit;
+        uint32_t vw[2][kSteps][4];
+        auto load_v = [&](uint32_t n) {
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) {
-            ldsm_x4_trans(vb[st], v_at + (v_lane ^ ((n % kPairs) << 5)) + n / kPairs * kPanel + st * 16u * kRowBytes);
+            ldsm_x4_trans(vw[n & 1u][st], v_at + (v_lane ^ ((n % kPairs) << 5)) + n / kPairs * kPanel + st * 16u * kRowBytes);
+          }
+        };
+        load_v(0u);
+#pragma unroll
+        for (uint32_t n = 0; n < kChunks / 2u; ++n) {
+          if (n + 1u < kChunks / 2u) load_v(n + 1u);
+          uint32_t (&vb)[kSteps][4] = vw[n & 1u];
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) vb[st][e] = __byte_perm(vb[st][e], 0u, 0x3120u);
           }
@@ -568,8 +623,8 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < kSteps; ++st) {
-                  const auto& ps = p[i][st];
-                  mma(d, ps[0][0], ps[0][1], ps[1][0], ps[1][1], b[st][f][0], b[st][f][1], __half());
+                  const uint32_t ps[4] = {p[i][st][0][0], p[i][st][0][1], p[i][st][1][0], p[i][st][1][1]};
+                  mma8(d, ps, b[st][f][0], b[st][f][1]);
                 }
                 const uint32_t at = 2u * (2u * n + e) + f;
                 if constexpr (TERMS == 2) {
@@ -587,16 +642,16 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
         }
       }
       __syncwarp();
-      if (!ends) {  // the last one is where the warp joins
-        refill(unit, written);
-        next_unit();
-      }
+      if (++use.j == to_j) break;
+      ++tile;
+      go_on();
     }
     left -= to_j - from_j;
 
     // ---- the end of the segment, or of the range inside it
-    const bool mine = from_j == 0u && to_j == use.j1;
-    // each warp's sums into the units it has just used, float4 pieces swizzled by row
+    const bool mine = solo || (from_j == 0u && to_j == use.j1);
+    // each warp's sums over the tile it has just used, rows 0-7 over V, 8-15 over K, pieces swizzled by row
+    const uint32_t at0 = (kK + tile % kV) * kUnit, at1 = tile % kK * kUnit;
 #pragma unroll
     for (int i = 0; i < RS; ++i) {
       float sum = l[i];
@@ -606,15 +661,21 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
         join_m[warp][i * 8 + g] = m[i];
         join_l[warp][i * 8 + g] = sum;
       }
-      float4* to = reinterpret_cast<float4*>(ring + (i == 0 ? unit : k_unit) * kUnit) + g * (DP / 4u);
+      float4* to = reinterpret_cast<float4*>(ring + (i == 0 ? at0 : at1)) + g * (DP / 4u);
 #pragma unroll
       for (uint32_t k = 0; k < kChunks; ++k) {
         to[(k * 4u + t4) ^ ((g & 1u) << 2)] = make_float4(o[i][2 * k][0], o[i][2 * k + 1][0], o[i][2 * k][1], o[i][2 * k + 1][1]);
       }
     }
-    // where the other warps' sums lie: every warp has gone the same number of units
-    const uint32_t at0 = unit * kUnit, at1 = k_unit * kUnit;
-    __syncthreads();
+    written = true;
+    ++tile;
+    // a lone warp joins nothing but its own; the others' lie where its own do, they have gone as many tiles
+    const uint32_t w0 = solo ? warp : 0u, w1 = solo ? warp + 1u : kWarps;
+    if (solo) {
+      __syncwarp();
+    } else {
+      __syncthreads();
+    }
     float* record = a.records + (static_cast<size_t>(blockIdx.x) * 2u + (from_j == 0u ? 1u : 0u)) * Shape::kRecord;
     auto finish = [&](uint32_t r, uint32_t ch, float top, float sum, float4 v) {
       const uint32_t at = use.sub + r, down = div_by(at, a.group);
@@ -638,18 +699,17 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
             sum == 0.f ? -CUDART_INF_F : (top + log2f(sum) - kShare) * 0.69314718055994530942f;
       }
     };
-    for (uint32_t i = tid; i < use.rows * (DP / 4u); i += kAttnThreads) {
+#pragma unroll 1
+    for (uint32_t i = solo ? lane : tid; i < use.rows * (DP / 4u); i += solo ? 32u : kAttnThreads) {
       const uint32_t r = i / (DP / 4u), ch = i % (DP / 4u);
-      float top = join_m[0][r];
-#pragma unroll
-      for (uint32_t w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w][r]);
+      float top = -CUDART_INF_F;
+      for (uint32_t w = w0; w < w1; ++w) top = fmaxf(top, join_m[w][r]);
       const float from = top == -CUDART_INF_F ? 0.f : top;
       float sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (uint32_t w = 0; w < kWarps; ++w) {
+      for (uint32_t w = w0; w < w1; ++w) {
         const float f = exp2_fast(join_m[w][r] - from);
-        const float4 x = reinterpret_cast<const float4*>(smem + w * (kUnits * kUnit) + (r < 8u ? at0 : at1))
+        const float4 x = reinterpret_cast<const float4*>(smem + w * ((kK + kV) * kUnit) + (r < 8u ? at0 : at1))
             [(r & 7u) * (DP / 4u) + (ch ^ ((r & 1u) << 2))];
         sum = fmaf(join_l[w][r], f, sum);
         v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y);
@@ -776,17 +836,17 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
         }
       }
     }
-    __syncthreads();  // the units and the joins are free again
-    if (use.j == use.j1) advance(use, left);
-    if constexpr (RS == 2) refill(k_unit, true);
-    refill(unit, true);
-    next_unit();
+    // the units and the joins are free again
+    if (solo) {
+      __syncwarp();
+    } else {
+      __syncthreads();
+    }
+    if (use.j == use.j1) advance(use, index, left);
   }
   if (!arrives) {  // a wait ran out (QG_ERR_WAIT_TIMEOUT is set): let what is in flight land
-    for (uint32_t i = 0; i < kUnits; ++i) {
-      const uint32_t u = unit + i < kUnits ? unit + i : unit + i - kUnits;
-      mbar_wait_bounded(&full[warp][u], unit + i < kUnits ? parity : parity ^ 1u);
-    }
+    for (uint32_t i = next_k > kK ? next_k - kK : 0u; i < next_k; ++i) mbar_wait_bounded(&full_k[warp][i % kK], i / kK & 1u);
+    for (uint32_t i = next_v > kV ? next_v - kV : 0u; i < next_v; ++i) mbar_wait_bounded(&full_v[warp][i % kV], i / kV & 1u);
   }
 }
 
@@ -816,8 +876,10 @@ __device__ __forceinline__ uint64_t plan_scan(uint64_t v, uint64_t& all) {
   return before + upto - v;
 }
 
+// log: of a block; log_tile: of the steps of a lone warp
 __global__ void __launch_bounds__(kPlanThreads) plan8_kernel(const Paged8View cache, const Attn8Args a, uint32_t rows,
-                                                             uint32_t log) {
+                                                             uint32_t log, uint32_t log_tile) {
+  __shared__ uint32_t longest;
   pdl_wait();
   pdl_trigger();
   const PagedView& c = cache.c;
@@ -835,7 +897,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan8_kernel(const Paged8View ca
   const uint32_t items = static_cast<uint32_t>(min(tiles, static_cast<uint64_t>(a.max_items)));
   if (tid == 0u) {
     a.seq_tiles[c.batch] = items;
-    *a.item_count = items;
+    a.item_count[0] = items;
+    longest = 0u;
     if (items < tiles) atomicOr(&g_error_word, QG_ERR_PAGE);
   }
   __syncthreads();
@@ -861,6 +924,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan8_kernel(const Paged8View ca
       s.rows = static_cast<uint32_t>(min(static_cast<uint64_t>(rows), most - row));
       // no slots: rows of a sequence that holds nothing, or does not fit
       s.p0 = r.len == 0u ? INT32_MIN / 2 : static_cast<int32_t>(r.len - r.n + down);
+      s.bounds(a, log_tile);
+      atomicMax(&longest, s.j1);
       s.bounds(a, log);
       n = s.j1;
       a.items[i] = make_uint4(lo, r.first + down, static_cast<uint32_t>(s.p0), s.sub | (s.rows << 16));
@@ -869,7 +934,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan8_kernel(const Paged8View ca
     blocks += all;
     if (i < items) a.item_blocks[i] = at;
   }
-  if (tid == 0u) a.item_blocks[items] = blocks;
+  __syncthreads();
+  if (tid == 0u) {
+    a.item_blocks[items] = blocks;
+    a.item_count[1] = longest;
+  }
 }
 
 // ---- host side
@@ -946,9 +1015,10 @@ cudaError_t launch_attn8(const Paged8View& c, const Attn8Args& args, const AttnM
   const uint64_t blocks = tiles * c.c.n_kv * ((c.c.capacity + (1u << Shape::kLogBlock) - 1u) >> Shape::kLogBlock);
   const uint64_t fit = static_cast<uint64_t>(paged_sm_count()) * Shape::kCtasPerSm;
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(std::min<uint64_t>(blocks, fit), kMaxCtas));
-  if (blocks / grid >= (1ull << 29)) return cudaErrorInvalidValue;  // a CTA counts its units in 32 bits
+  // a CTA counts its units in 32 bits, segments are numbered in 32
+  if (blocks / grid >= (1ull << 29) || tiles * c.c.n_kv >= (1ull << 32)) return cudaErrorInvalidValue;
   if (a.offsets != nullptr) {
-    e = launch_plan8(c, a, Shape::kRows, Shape::kLogBlock, stream);
+    e = launch_plan8(c, a, Shape::kRows, Shape::kLogBlock, Shape::kLogTile, stream);
     if (e != cudaSuccess) return e;
   }
   return launch_k(kernel, grid, kAttnThreads, Shape::kSmem, stream, c, a, maps);
@@ -956,8 +1026,9 @@ cudaError_t launch_attn8(const Paged8View& c, const Attn8Args& args, const AttnM
 
 }  // namespace
 
-cudaError_t launch_plan8(const Paged8View& c, const Attn8Args& a, uint32_t rows, uint32_t log, cudaStream_t stream) {
-  return launch_k(plan8_kernel, 1u, kPlanThreads, 0, stream, c, a, rows, log);
+cudaError_t launch_plan8(const Paged8View& c, const Attn8Args& a, uint32_t rows, uint32_t log, uint32_t log_tile,
+                         cudaStream_t stream) {
+  return launch_k(plan8_kernel, 1u, kPlanThreads, 0, stream, c, a, rows, log, log_tile);
 }
 
 }  // namespace qg
@@ -993,9 +1064,9 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
   const uint32_t group = p->n_q_heads / c.c.n_kv;
   const bool few = p->offsets == nullptr && group <= 8u, wide = p->dtype == QG_F32;
   const uint32_t rs = few || (wide && plan.dp == 256u) ? 1u : 2u, terms = few || wide ? 2u : 1u;
-  // a box is part of one tile, page and scale block
+  // a box is part of one tile and page
   const uint32_t log_tile = log_tile8(plan.dp, rs, terms);
-  const uint32_t log_box = std::min<uint32_t>(log_tile, __builtin_ctz(cache->block));
+  const uint32_t log_box = std::min<uint32_t>(log_tile, __builtin_ctz(cache->page_size));
   AttnMaps8 maps;
   if (!encode_pool8(&maps.k, cache->k, cache, strides, 1u << log_box, plan.dp) ||
       !encode_pool8(&maps.v, cache->v, cache, strides, 1u << log_box, plan.dp)) {

@@ -25,7 +25,7 @@ struct Attn8Args {
   uint32_t* arrived;              // counters, zero between calls
   float* records;                 // partial results
   // of a ragged call
-  uint32_t* item_count;           // tiles
+  uint32_t* item_count;           // [0] tiles, [1] steps of the longest
   uint4* items;                   // [tile] {sequence, first token's row, its slot, first row's head | rows << 16}
   uint64_t* item_blocks;          // [tile + 1] blocks of all tiles before
   uint32_t* seq_tiles;            // [batch + 1] tiles of all sequences before
@@ -99,9 +99,10 @@ __device__ __forceinline__ void take_item8(const Attn8Args& a, Segment8& s, bool
   s.j = 0u;
 }
 
-// The tiles of `rows` rows of a ragged call, and how many blocks of 2^log slots each sees, before
-// the attention reads them.
-cudaError_t launch_plan8(const Paged8View& c, const Attn8Args& a, uint32_t rows, uint32_t log, cudaStream_t stream);
+// The tiles of `rows` rows of a ragged call, how many blocks of 2^log slots each sees, and how many of
+// 2^log_tile the longest, before the attention reads them.
+cudaError_t launch_plan8(const Paged8View& c, const Attn8Args& a, uint32_t rows, uint32_t log, uint32_t log_tile,
+                         cudaStream_t stream);
 
 // ---- the kernel for many rows (qg_paged8_prompt.cu)
 constexpr uint32_t kPromptRows = 256;

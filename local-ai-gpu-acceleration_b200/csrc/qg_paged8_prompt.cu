@@ -682,7 +682,7 @@ cudaError_t launch_prompt8(const Paged8View& c, const Attn8Args& a, cudaStream_t
   const uint32_t fit = std::min<uint32_t>(static_cast<uint32_t>(paged_sm_count()), kMaxPromptCtas);
   const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(blocks, fit));
   if (blocks / grid >= (1ull << 29)) return cudaErrorInvalidValue;  // a CTA counts its units in 32 bits
-  e = launch_plan8(c, a, kPromptRows, kLogStep, stream);
+  e = launch_plan8(c, a, kPromptRows, kLogStep, kLogStep, stream);
   if (e != cudaSuccess) return e;
   return launch_k(kernel, grid, kPromptThreads, Shape::kSmem, stream, c, a);
 }
