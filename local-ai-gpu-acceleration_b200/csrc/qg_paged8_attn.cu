@@ -40,7 +40,7 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kAttnThreads = kWarps * 32;
 // Slots of one warp's tile: as many as 255 registers hold.  At head size 128 tiles of 32 slots took 236 us for
-// 16 x 32768 (TILE64 with 64): a tile's scores, sums and bookkeeping cost the same whatever its slots.
+// 16 x 32768, of 64 208: a tile's sums and bookkeeping cost the same whatever its slots.
 constexpr uint32_t log_tile8(uint32_t dp, uint32_t rs, uint32_t terms) {
   return dp == 256u || (dp == 128u && rs * terms == 4u) ? 5u : 6u;
 }
@@ -85,7 +85,9 @@ struct Attn8Shape {
   static constexpr uint32_t kRowBytes = DP == 64 ? 64u : 128u;        // of a box
   static constexpr uint32_t kPanels = DP / kRowBytes;
   static constexpr uint32_t kRecord = kRows * (DP + 2u);    // m[], l[], o[][]
-  // what a segment costs beside its blocks, in blocks
+  // What a segment costs beside its blocks, in blocks; us with 0, 1, 2 and 4: head size 64, 100 x 10..2000 (16/16
+  // heads) 66, 56, 55 and 61; 128, the same of 32/8 64, 55, 51 and 57, 2 x 30000 49, 45, 43 and 43; 256, 32 x
+  // ..8191 (8/2) 43, 43, 37 and 37.
   static constexpr uint32_t kHeader = 2;
   static_assert(8u * DP * 4u <= kUnit, "the sums of eight rows join in a free unit");
 };
@@ -996,8 +998,13 @@ bool encode_pool8(CUtensorMap* map, void* pool, const qg_kv_pages8* cache, const
   const cuuint64_t strides[3] = {s.inner, s.outer, s.page};
   const cuuint32_t box[4] = {dp == 64u ? 64u : 128u, s.heads_inside ? 1u : box_slots, s.heads_inside ? box_slots : 1u, 1u};
   const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+  // Where a row's neighbours in memory are other heads' rows, no more than the row is brought to L2: 16 x 32768 in
+  // that order 287 us with 256 bytes a request, 217 with 128; 64 x ..4097 of 64-byte rows 115 and, with 64, 100 us.
+  const auto promotion = !s.heads_inside ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                         : dp == 64u     ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
+                                         : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                dp == 64u ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                dp == 64u ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, promotion,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

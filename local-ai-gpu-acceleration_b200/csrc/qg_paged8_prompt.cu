@@ -16,7 +16,7 @@
 // K-major operand over dims (for K, whose N are slots) and an MN-major one over slots (for V, whose N
 // are dims), so no byte is transposed.
 //
-// Warps: 0-3 and 4-7 the rows of the halves, 8-11 codes, 12 issues the products.  With two S of a half
+// Warps: 0 issues the products, 1-4 codes, 5-8 and 9-12 the rows of the halves.  With two S of a half
 // the scores of the next step are there before the powers of this one are written, so the rows never
 // wait for a product.  The four roles' loops have to stay small: unrolled further they left the
 // instruction cache and took twice the time.
@@ -41,8 +41,8 @@ constexpr uint32_t kLogStep = 6, kStep = 1u << kLogStep;  // slots of a step
 constexpr uint32_t kStages = 3;                  // steps of codes in fp16, for K and for V
 constexpr uint32_t kGroups = kStep / 16u;        // 16-slot groups of a step, one scale each
 static_assert(kGroups == 4u, "a code warp each");
-constexpr uint32_t kRowWarps = 8, kCodeWarp0 = 8, kCodeWarps = 4, kIssueWarp = 12;
-constexpr uint32_t kPromptThreads = (kIssueWarp + 1u) * 32u;  // four warps a scheduler: 128 registers a thread
+constexpr uint32_t kIssueWarp = 0, kCodeWarp0 = 1, kCodeWarps = 4, kRowWarp0 = 5, kRowWarps = 8;
+constexpr uint32_t kPromptThreads = (kRowWarp0 + kRowWarps) * 32u;  // four warps a scheduler: 128 registers a thread
 constexpr uint32_t kScaleRing = 4;
 constexpr uint32_t kMaxPolls = 4000;             // of up to kPollNs each
 constexpr float kCarry = 7.f, kSlack = 8.f;      // log2: the factor of powers, the growth of M that is let pass
@@ -171,9 +171,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
 
   uint32_t kt = 0;  // steps of the range
 
-  if (warp < kRowWarps) {
+  if (warp >= kRowWarp0) {
     // ================= the rows of a half: a thread has one
-    const uint32_t half = warp / 4u, row = tid % kHalf;      // of the half
+    const uint32_t half = (warp - kRowWarp0) / 4u, row = (warp & 3u) * 32u + lane;  // of the half: a lane of tensor memory
     const uint32_t s_at = tmem + half * kHalf + ((warp & 3u) << 21), o_at = s_at + 2u * kHalf;
     uint4* const row_nan = reinterpret_cast<uint4*>(smem + Shape::row_nan) + half * kHalf + row;
     uint32_t steps = 0;                                      // of this half
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         half_sync();  // the flag is free again
       }
     }
-  } else if (warp < kIssueWarp) {
+  } else if (warp >= kCodeWarp0) {
     // ================= codes to fp16: warp w has the step's 16-slot group w, this thread places r and 8 + r of
     // it and every fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
     constexpr uint32_t kMine = DP / 64u;                     // pieces of a row
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       ++kt;
       if (++stage == kStages) stage = 0u, ++round;
     }
-  } else if (warp == kIssueWarp && elect_one()) {
+  } else if (elect_one()) {
     // ================= the products, by one thread
     uint32_t parts[2] = {0u, 0u}, steps[2] = {0u, 0u};
     uint32_t k_stage = 0, k_round = 0, v_stage = 0, v_round = 0;
