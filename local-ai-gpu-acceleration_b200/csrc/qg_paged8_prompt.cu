@@ -11,12 +11,12 @@
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
 //
-// Codes become fp16 once for 256 rows: four warps load a step's codes into registers a step ahead,
-// convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
+// Codes become fp16 once for 256 rows: seven warps take turns at 16 slots
+// of K or of V, load the codes into registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
 // K-major operand over dims (for K, whose N are slots) and an MN-major one over slots (for V, whose N
 // are dims), so no byte is transposed.
 //
-// Warps: 0 issues the products, 1-4 codes, 5-8 and 9-12 the rows of the halves.  With two S of a half
+// Warps: 0 issues the products, 1-7 codes, 8-11 and 12-15 the rows of the halves.  With two S of a half
 // the scores of the next step are there before the powers of this one are written, so the rows never
 // wait for a product.  The four roles' loops have to stay small: unrolled further they left the
 // instruction cache and took twice the time.
@@ -40,10 +40,10 @@ constexpr uint32_t kHalf = 128;                  // rows of a half
 constexpr uint32_t kLogStep = 6, kStep = 1u << kLogStep;  // slots of a step
 constexpr uint32_t kStages = 3;                  // steps of codes in fp16, for K and for V
 constexpr uint32_t kGroups = kStep / 16u;        // 16-slot groups of a step, one scale each
-static_assert(kGroups == 4u, "a code warp each");
-constexpr uint32_t kIssueWarp = 0, kCodeWarp0 = 1, kCodeWarps = 4, kRowWarp0 = 5, kRowWarps = 8;
+constexpr uint32_t kTurns = 2u * kGroups;        // of a step: its groups of K, then of V
+constexpr uint32_t kIssueWarp = 0, kCodeWarp0 = 1, kCodeWarps = 7, kRowWarp0 = 8, kRowWarps = 8;
 constexpr uint32_t kPromptThreads = (kRowWarp0 + kRowWarps) * 32u;  // four warps a scheduler: 128 registers a thread
-constexpr uint32_t kScaleRing = 4;
+constexpr uint32_t kScaleRing = 8;               // steps whose scales are kept: rows are up to 5 behind the K that is stored
 constexpr uint32_t kMaxPolls = 4000;             // of up to kPollNs each
 constexpr float kCarry = 7.f, kSlack = 8.f;      // log2: the factor of powers, the growth of M that is let pass
 constexpr float kLeastFactor = 1e-30f;           // of scores: zero would turn minus infinity into NaN
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
   __shared__ __align__(8) uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_full[2][2], k_full[kStages], k_empty[kStages],
       v_full[kStages], v_empty[kStages], scale_full[kScaleRing], drained;
   __shared__ uint32_t tmem_slot, abort_flag, last_flag[2];
-  __shared__ uint32_t nan_flag[kStages][kCodeWarps];
+  __shared__ uint32_t nan_flag[kStages][kGroups];
   const uint32_t tid = threadIdx.x, lane = tid & 31u;
   const uint32_t warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint8_t* const smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -108,12 +108,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       }
     }
     for (uint32_t i = 0; i < kStages; ++i) {
-      mbar_init(&k_full[i], kCodeWarps);
+      mbar_init(&k_full[i], kGroups);
       mbar_init(&k_empty[i], 1u);
-      mbar_init(&v_full[i], kCodeWarps);
+      mbar_init(&v_full[i], kGroups);
       mbar_init(&v_empty[i], 1u);
     }
-    for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], kCodeWarps);
+    for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], kGroups);
     mbar_init(&drained, 1u);
     abort_flag = 0u;
     fence_mbar_init();
@@ -437,22 +437,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       }
     }
   } else if (warp >= kCodeWarp0) {
-    // ================= codes to fp16: warp w has the step's 16-slot group w, this thread places r and 8 + r of
-    // it and every fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
+    // ================= codes to fp16, in turns: of 16 slots of K or V this thread has places r and 8 + r and every
+    // fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
     constexpr uint32_t kMine = DP / 64u;                     // pieces of a row
-    const uint32_t w = warp - kCodeWarp0, r = lane & 7u, pq = lane >> 3;
+    const uint32_t r = lane & 7u, pq = lane >> 3;
     Segment8 s = use;
-    uint32_t rem = left;
-    // Of a step ahead: its group's page, first place on it, kv head and flags (row i is seen by some; bit 2 + i:
-    // by all), then where this thread's rows lie, and the scales.
-    uint32_t id = 0, on = 0, kv = 0, seen = 0, flags = 0;
-    float ks = 0.f, vs = 1.f;
-    uint64_t off = 0;
-    uint4 kw[2][kMine], vw[2][kMine];
-    auto look = [&]() {  // at the step of s; goes on to the next
-      const uint32_t slot = (s.block(s.j) << kLogStep) + 16u * w, at = div_by(slot, c.page);
+    uint32_t rem = left;                                     // steps from s.j on
+    uint32_t turn = warp - kCodeWarp0;                       // of the step of s: groups of K, then of V
+    // Of a turn ahead: the group's page, first place on it, kv head, flags (row i is seen by some; bit 2 + i: by
+    // all; bit 4: any) and turn, then its codes and scales.
+    uint32_t id = 0, on = 0, kv = 0, seen = 0, at_turn = 0;
+    bool ahead = false;                                      // there is a turn looked up
+    auto look = [&]() {  // at a turn of the step of s; goes on to this warp's next
+      ahead = rem != 0u;
+      if (!ahead) return;
+      const uint32_t slot = (s.block(s.j) << kLogStep) + 16u * (turn % kGroups), at = div_by(slot, c.page);
       on = slot - at * c.page.d;
       kv = s.kv;
+      at_turn = turn;
       seen = 0u;
       if (s.all_see(a, slot, 16u)) {
         seen = 15u;
@@ -463,133 +465,139 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           if (s.all_see(a, slot + 8u * i + r, 1u)) seen |= 4u << i;
         }
       }
-      // 16 slots of a page that some row sees have an id (rows of it may still be unseen)
       id = c.num_pages;
       if (s.some_see(slot, 16u)) {
         id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + at]);
         seen |= 16u;
       }
-      ++s.j;
-      --rem;
-      if (s.j == s.j1) advance(s, rem);
+      turn += kCodeWarps;
+      if (turn >= kTurns) {
+        turn -= kTurns;
+        ++s.j;
+        --rem;
+        if (s.j == s.j1) advance(s, rem);
+      }
     };
-    auto place = [&]() {  // of the step looked up last
+    uint32_t flags = 0, now_turn = 0;
+    float ks = 0.f, vs = 1.f;
+    uint4 codes[2][kMine];
+    auto load = [&]() {  // the turn looked up last
       flags = seen & 15u;
+      now_turn = at_turn;
       ks = 0.f;
       vs = 1.f;
       if (id >= c.num_pages) {
         flags = 0u;
         if (seen > 15u) atomicOr(&g_error_word, QG_ERR_PAGE);
-        return;
+      } else if (now_turn < kGroups) {  // the scales go with K
+        const uint64_t in = id * cache.scale_page + kv * cache.scale_head + (on >> cache.log_block);
+        ks = cache.ks[in];
+        vs = cache.vs[in];
       }
-      off = id * c.page_bytes + kv * c.head_bytes + (on + r) * c.slot_bytes + pq * 16u;
-      const uint64_t in = id * cache.scale_page + kv * cache.scale_head + (on >> cache.log_block);
-      ks = cache.ks[in];
-      vs = cache.vs[in];
-    };
-    auto load = [&](const uint8_t* pool, uint4 (&to)[2][kMine]) {
+      const uint8_t* const from = (now_turn < kGroups ? c.k : c.v) + id * c.page_bytes + kv * c.head_bytes +
+                                  (on + r) * c.slot_bytes + pq * 16u;
 #pragma unroll
       for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
         for (uint32_t h = 0; h < kMine; ++h) {
-          to[i][h] = make_uint4(0u, 0u, 0u, 0u);
+          codes[i][h] = make_uint4(0u, 0u, 0u, 0u);
           if ((flags >> i & 1u) != 0u && (pq + 4u * h) * 16u < c.dim) {
-            to[i][h] = *reinterpret_cast<const uint4*>(pool + off + i * 8u * c.slot_bytes + h * 64u);
+            codes[i][h] = *reinterpret_cast<const uint4*>(from + i * 8u * c.slot_bytes + h * 64u);
           }
         }
       }
     };
     // piece pq + 4 h is chunks 2 pq and 2 pq + 1 of panel h
-    const uint32_t store_at = (16u * w) * 128u, chunk0 = in_panel(r, 2u * pq), chunk1 = in_panel(r, 2u * pq + 1u);
-    auto store = [&](uint32_t at, const uint4 (&from)[2][kMine]) {
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {
-#pragma unroll
-        for (uint32_t h = 0; h < kMine; ++h) {
-          uint8_t* const to = smem + at + store_at + h * kCodePanel + i * 1024u;
-          uint4 x, y;
-          codes_to_half(from[i][h].x, x.x, x.y);
-          codes_to_half(from[i][h].y, x.z, x.w);
-          codes_to_half(from[i][h].z, y.x, y.y);
-          codes_to_half(from[i][h].w, y.z, y.w);
-          *reinterpret_cast<uint4*>(to + chunk0) = x;
-          *reinterpret_cast<uint4*>(to + chunk1) = y;
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
-    uint32_t stage = 0, round = 0;                           // kt = round * kStages + stage
-    uint32_t more = rem != 0u ? 1u : 0u, after = 0u;         // there is a step; one after it
-    if (more != 0u) {
+    const uint32_t chunk0 = in_panel(r, 2u * pq), chunk1 = in_panel(r, 2u * pq + 1u);
+    uint32_t stage = 0, round = 0, ring = 0;                 // of the turn whose codes are in registers
+    look();
+    bool more = ahead;
+    if (more) {
+      load();
       look();
-      place();
-      load(c.k, kw);
-      load(c.v, vw);
-      after = rem != 0u ? 1u : 0u;
-      if (after != 0u) look();
     }
-    // A step's codes are stored while the next one's are loaded and the page of the one after is looked up.
+    // A turn's codes are stored once the next one's page is known, and the next one's loaded then.
 #pragma unroll 1
-    while (more != 0u) {
-      const uint32_t ring = kt % kScaleRing, now_flags = flags;
-      const float now_ks = ks, now_vs = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
-      more = after;
-      if (more != 0u) {
-        place();
-        after = rem != 0u ? 1u : 0u;
-        if (after != 0u) look();
-      }
-      if (round != 0u) wait(&k_empty[stage], (round - 1u) & 1u);
-      if (lane == 0u) {
-        reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + w] = make_float4(now_ks, log2f(now_vs), 1.f / now_vs, 0.f);
-      }
-      store(Shape::k_at + stage * Shape::kCodeBytes, kw);
-      if (lane == 0u) {
-        mbar_arrive(&k_full[stage]);
-        mbar_arrive(&scale_full[ring]);
-      }
-      if (more != 0u) load(c.k, kw);
-      // NaN codes of rows that not all see: out of the codes, noted by column
-      uint32_t odd = 0;
-      if (now_flags != 15u) {
+    while (more) {
+      const bool is_k = now_turn < kGroups;
+      const uint32_t group = now_turn % kGroups;
+      const uint32_t tile = (is_k ? Shape::k_at : Shape::v_at) + stage * Shape::kCodeBytes;
+      // NaN codes of V that not all rows see: out of the codes, noted by column
+      bool flagged = false;
+      if (__builtin_expect(!is_k && flags != 15u, 0)) {
+        uint32_t odd = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < kMine; ++h) {
             auto nan = [](uint32_t u) { return ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-            if ((now_flags >> (2u + i) & 1u) == 0u) odd |= nan(vw[i][h].x) | nan(vw[i][h].y) | nan(vw[i][h].z) | nan(vw[i][h].w);
+            if ((flags >> (2u + i) & 1u) == 0u) {
+              odd |= nan(codes[i][h].x) | nan(codes[i][h].y) | nan(codes[i][h].z) | nan(codes[i][h].w);
+            }
           }
         }
+        flagged = odd != 0u;
       }
-      const bool flagged = __any_sync(0xffffffffu, odd != 0u);
-      if (round != 0u) wait(&v_empty[stage], (round - 1u) & 1u);
+      flagged = __any_sync(0xffffffffu, flagged);
+      if (round != 0u) wait(is_k ? &k_empty[stage] : &v_empty[stage], (round - 1u) & 1u);
       if (__builtin_expect(flagged, 0)) {
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < 2u; ++h) {  // both halves of a row's 128 columns
             uint32_t bits = 0;
-            if (h < kMine && (now_flags >> (2u + i) & 1u) == 0u) {
+            if (h < kMine && (flags >> (2u + i) & 1u) == 0u) {
               auto clean = [&](uint32_t& word, uint32_t e) {
                 const uint32_t is = (((word & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
                 word &= ~(is * 0xffu);
                 bits |= (is * 0x01020408u >> 24 & 15u) << (4u * e);
               };
-              clean(vw[i][h % kMine].x, 0u), clean(vw[i][h % kMine].y, 1u);
-              clean(vw[i][h % kMine].z, 2u), clean(vw[i][h % kMine].w, 3u);
+              uint4& w = codes[i][h % kMine];
+              clean(w.x, 0u), clean(w.y, 1u), clean(w.z, 2u), clean(w.w, 3u);
             }
-            reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(stage * kStep + 16u * w + 8u * i + r) * 8u + pq + 4u * h] =
+            reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(stage * kStep + 16u * group + 8u * i + r) * 8u + pq + 4u * h] =
                 static_cast<uint16_t>(bits);
           }
         }
       }
-      if (lane == 0u) nan_flag[stage][w] = flagged ? 1u : 0u;
-      store(Shape::v_at + stage * Shape::kCodeBytes, vw);
-      if (lane == 0u) mbar_arrive(&v_full[stage]);
-      if (more != 0u) load(c.v, vw);
-      ++kt;
-      if (++stage == kStages) stage = 0u, ++round;
+      if (lane == 0u) {
+        if (is_k) {
+          const float to = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
+          reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + group] = make_float4(ks, log2f(to), 1.f / to, 0.f);
+        } else {
+          nan_flag[stage][group] = flagged ? 1u : 0u;
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+#pragma unroll
+        for (uint32_t h = 0; h < kMine; ++h) {
+          uint8_t* const to = smem + tile + group * 2048u + h * kCodePanel + i * 1024u;
+          uint4 x, y;
+          codes_to_half(codes[i][h].x, x.x, x.y);
+          codes_to_half(codes[i][h].y, x.z, x.w);
+          codes_to_half(codes[i][h].z, y.x, y.y);
+          codes_to_half(codes[i][h].w, y.z, y.w);
+          *reinterpret_cast<uint4*>(to + chunk0) = x;
+          *reinterpret_cast<uint4*>(to + chunk1) = y;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0u) {
+        mbar_arrive(is_k ? &k_full[stage] : &v_full[stage]);
+        if (is_k) mbar_arrive(&scale_full[ring]);
+      }
+      more = ahead;
+      if (more) {
+        const uint32_t before = now_turn;
+        load();
+        if (now_turn < before) {  // the next step
+          ring = (ring + 1u) % kScaleRing;
+          if (++stage == kStages) stage = 0u, ++round;
+        }
+        look();
+      }
     }
   } else if (elect_one()) {
     // ================= the products, by one thread
