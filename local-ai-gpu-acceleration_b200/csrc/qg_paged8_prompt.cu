@@ -11,8 +11,8 @@
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
 //
-// Codes become fp16 once for 256 rows: seven warps take turns at 16 slots
-// of K or of V, load the codes into registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
+// Codes become fp16 once for 256 rows: seven warps take turns at 16 slots,
+// load their codes into registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
 // K-major operand over dims (for K, whose N are slots) and an MN-major one over slots (for V, whose N
 // are dims), so no byte is transposed.
 //
@@ -40,7 +40,6 @@ constexpr uint32_t kHalf = 128;                  // rows of a half
 constexpr uint32_t kLogStep = 6, kStep = 1u << kLogStep;  // slots of a step
 constexpr uint32_t kStages = 3;                  // steps of codes in fp16, for K and for V
 constexpr uint32_t kGroups = kStep / 16u;        // 16-slot groups of a step, one scale each
-constexpr uint32_t kTurns = 2u * kGroups;        // of a step: its groups of K, then of V
 constexpr uint32_t kIssueWarp = 0, kCodeWarp0 = 1, kCodeWarps = 7, kRowWarp0 = 8, kRowWarps = 8;
 constexpr uint32_t kPromptThreads = (kRowWarp0 + kRowWarps) * 32u;  // four warps a scheduler: 128 registers a thread
 constexpr uint32_t kScaleRing = 8;               // steps whose scales are kept: rows are up to 5 behind the K that is stored
@@ -85,6 +84,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// A wait that does not end at once, as a call: the roles' loops have to fit the instruction cache together.
+__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kMaxPolls; ++i) {
+    if (*abort != 0u) return;
+    if (mbar_try_wait_sleep(bar, parity)) return;
+  }
+  atomicOr(&g_error_word, QG_ERR_WAIT_TIMEOUT);
+  *abort = 1u;
+}
+
 template <int DP>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8View cache, const Attn8Args a) {
   using Shape = PromptShape<DP>;
@@ -100,10 +110,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
   volatile uint32_t* const abort = &abort_flag;
   if (tid == 0u) {
     for (uint32_t i = 0; i < 2u; ++i) {
-      mbar_init(&q_full[i], kHalf);
+      mbar_init(&q_full[i], kHalf / 32u);
       for (uint32_t k = 0; k < 2u; ++k) {
         mbar_init(&s_full[i][k], 1u);
-        mbar_init(&p_full[i][k], kHalf);
+        mbar_init(&p_full[i][k], kHalf / 32u);
         mbar_init(&pv_full[i][k], 1u);
       }
     }
@@ -128,14 +138,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
   pdl_trigger();
 
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return;
-#pragma unroll 1
-    for (uint32_t i = 0; i < kMaxPolls; ++i) {
-      if (*abort != 0u) return;
-      if (mbar_try_wait_sleep(bar, parity)) return;
-    }
-    atomicOr(&g_error_word, QG_ERR_WAIT_TIMEOUT);
-    *abort = 1u;
+    if (__builtin_expect(!mbar_try_wait(bar, parity), 0)) wait_long(bar, parity, abort);
   };
 
   // ---- this CTA's range [r0, r1) of the line of units; every warp finds it
@@ -227,7 +230,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           *reinterpret_cast<uint4*>(to + (i >> 3) * kQPanel + in_panel(row, i & 7u)) = make_uint4(half2(w.x), half2(w.y), half2(w.z), half2(w.w));
         });
         fence_proxy_async_smem();
-        mbar_arrive(&q_full[half]);
+        __syncwarp();
+        if (lane == 0u) mbar_arrive(&q_full[half]);
       }
       float m = -CUDART_INF_F, l = 0.f;
       bool any_nan = false;  // columns of the row are NaN
@@ -337,7 +341,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[half][steps & 1u]);
+        __syncwarp();
+        if (lane == 0u) mbar_arrive(&p_full[half][steps & 1u]);
       }
 
       // ---- the end of the segment, or of the range inside it
@@ -437,122 +442,159 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       }
     }
   } else if (warp >= kCodeWarp0) {
-    // ================= codes to fp16, in turns: of 16 slots of K or V this thread has places r and 8 + r and every
-    // fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
+    // ================= codes to fp16, in turns: of a step's 16-slot group this thread has places r and 8 + r and
+    // every fourth 16-code piece, so 8 lanes write 128 consecutive bytes and read 64 of a row
     constexpr uint32_t kMine = DP / 64u;                     // pieces of a row
     const uint32_t r = lane & 7u, pq = lane >> 3;
     Segment8 s = use;
     uint32_t rem = left;                                     // steps from s.j on
-    uint32_t turn = warp - kCodeWarp0;                       // of the step of s: groups of K, then of V
+    uint32_t turn = warp - kCodeWarp0;                       // this warp's next, in groups from the step of s on
+    uint32_t step = 0;                                       // of the range, where s is
     // Of a turn ahead: the group's page, first place on it, kv head, flags (row i is seen by some; bit 2 + i: by
-    // all; bit 4: any) and turn, then its codes and scales.
-    uint32_t id = 0, on = 0, kv = 0, seen = 0, at_turn = 0;
+    // all; bit 4: any), step and group.
+    uint32_t id = 0, on = 0, kv = 0, seen = 0, at_step = 0, at_group = 0;
     bool ahead = false;                                      // there is a turn looked up
-    auto look = [&]() {  // at a turn of the step of s; goes on to this warp's next
+    auto look = [&]() {
+#pragma unroll 1
+      while (turn >= kGroups && rem != 0u) {
+        turn -= kGroups;
+        ++step;
+        ++s.j;
+        --rem;
+        if (s.j == s.j1) advance(s, rem);
+      }
       ahead = rem != 0u;
       if (!ahead) return;
-      const uint32_t slot = (s.block(s.j) << kLogStep) + 16u * (turn % kGroups), at = div_by(slot, c.page);
+      const uint32_t slot = (s.block(s.j) << kLogStep) + 16u * turn, at = div_by(slot, c.page);
       on = slot - at * c.page.d;
       kv = s.kv;
-      at_turn = turn;
-      seen = 0u;
+      at_step = step;
+      at_group = turn;
+      id = c.num_pages;
       if (s.all_see(a, slot, 16u)) {
-        seen = 15u;
+        seen = 31u;
       } else {
+        seen = s.some_see(slot, 16u) ? 16u : 0u;
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
           if (s.some_see(slot + 8u * i + r, 1u)) seen |= 1u << i;
           if (s.all_see(a, slot + 8u * i + r, 1u)) seen |= 4u << i;
         }
       }
-      id = c.num_pages;
-      if (s.some_see(slot, 16u)) {
-        id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + at]);
-        seen |= 16u;
-      }
+      if (seen > 15u) id = static_cast<uint32_t>(c.table[static_cast<size_t>(s.b) * c.table_stride + at]);
       turn += kCodeWarps;
-      if (turn >= kTurns) {
-        turn -= kTurns;
-        ++s.j;
-        --rem;
-        if (s.j == s.j1) advance(s, rem);
-      }
     };
-    uint32_t flags = 0, now_turn = 0;
+    uint32_t flags = 0, now_step = 0, now_group = 0;
     float ks = 0.f, vs = 1.f;
-    uint4 codes[2][kMine];
-    auto load = [&]() {  // the turn looked up last
+    uint64_t off = 0;
+    uint4 kw[2][kMine], vw[2][kMine];
+    auto place = [&]() {  // of the turn looked up last
       flags = seen & 15u;
-      now_turn = at_turn;
+      now_step = at_step;
+      now_group = at_group;
       ks = 0.f;
       vs = 1.f;
       if (id >= c.num_pages) {
         flags = 0u;
         if (seen > 15u) atomicOr(&g_error_word, QG_ERR_PAGE);
-      } else if (now_turn < kGroups) {  // the scales go with K
-        const uint64_t in = id * cache.scale_page + kv * cache.scale_head + (on >> cache.log_block);
-        ks = cache.ks[in];
-        vs = cache.vs[in];
+        return;
       }
-      const uint8_t* const from = (now_turn < kGroups ? c.k : c.v) + id * c.page_bytes + kv * c.head_bytes +
-                                  (on + r) * c.slot_bytes + pq * 16u;
+      off = id * c.page_bytes + kv * c.head_bytes + (on + r) * c.slot_bytes + pq * 16u;
+      const uint64_t in = id * cache.scale_page + kv * cache.scale_head + (on >> cache.log_block);
+      ks = cache.ks[in];
+      vs = cache.vs[in];
+    };
+    auto load = [&](const uint8_t* pool, uint4 (&to)[2][kMine]) {
 #pragma unroll
       for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
         for (uint32_t h = 0; h < kMine; ++h) {
-          codes[i][h] = make_uint4(0u, 0u, 0u, 0u);
+          to[i][h] = make_uint4(0u, 0u, 0u, 0u);
           if ((flags >> i & 1u) != 0u && (pq + 4u * h) * 16u < c.dim) {
-            codes[i][h] = *reinterpret_cast<const uint4*>(from + i * 8u * c.slot_bytes + h * 64u);
+            to[i][h] = *reinterpret_cast<const uint4*>(pool + off + i * 8u * c.slot_bytes + h * 64u);
           }
         }
       }
     };
     // piece pq + 4 h is chunks 2 pq and 2 pq + 1 of panel h
     const uint32_t chunk0 = in_panel(r, 2u * pq), chunk1 = in_panel(r, 2u * pq + 1u);
-    uint32_t stage = 0, round = 0, ring = 0;                 // of the turn whose codes are in registers
+    auto store = [&](uint8_t* at, const uint4 (&from)[2][kMine]) {
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+#pragma unroll
+        for (uint32_t h = 0; h < kMine; ++h) {
+          uint8_t* const to = at + h * kCodePanel + i * 1024u;
+          uint4 x, y;
+          codes_to_half(from[i][h].x, x.x, x.y);
+          codes_to_half(from[i][h].y, x.z, x.w);
+          codes_to_half(from[i][h].z, y.x, y.y);
+          codes_to_half(from[i][h].w, y.z, y.w);
+          *reinterpret_cast<uint4*>(to + chunk0) = x;
+          *reinterpret_cast<uint4*>(to + chunk1) = y;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
     look();
     bool more = ahead;
     if (more) {
-      load();
+      place();
+      load(c.k, kw);
+      load(c.v, vw);
       look();
     }
-    // A turn's codes are stored once the next one's page is known, and the next one's loaded then.
+    // A turn's codes are stored while the next one's are loaded and the page of the one after is looked up.
 #pragma unroll 1
     while (more) {
-      const bool is_k = now_turn < kGroups;
-      const uint32_t group = now_turn % kGroups;
-      const uint32_t tile = (is_k ? Shape::k_at : Shape::v_at) + stage * Shape::kCodeBytes;
-      // NaN codes of V that not all rows see: out of the codes, noted by column
+      const uint32_t round = now_step / kStages, stage = now_step - round * kStages, ring = now_step % kScaleRing;
+      const uint32_t group = now_group, now_flags = flags;
+      uint8_t* const tile = smem + Shape::k_at + stage * Shape::kCodeBytes + group * 2048u;
+      if (round != 0u) wait(&k_empty[stage], (round - 1u) & 1u);
+      if (lane == 0u) {
+        const float to = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
+        reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + group] = make_float4(ks, log2f(to), 1.f / to, 0.f);
+      }
+      store(tile, kw);
+      if (lane == 0u) {
+        mbar_arrive(&k_full[stage]);
+        mbar_arrive(&scale_full[ring]);
+      }
+      more = ahead;
+      if (more) {
+        place();
+        load(c.k, kw);
+        look();
+      }
+      // NaN codes of rows that not all see: out of the codes, noted by column
       bool flagged = false;
-      if (__builtin_expect(!is_k && flags != 15u, 0)) {
+      if (__builtin_expect(now_flags != 15u, 0)) {
         uint32_t odd = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < kMine; ++h) {
             auto nan = [](uint32_t u) { return ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-            if ((flags >> (2u + i) & 1u) == 0u) {
-              odd |= nan(codes[i][h].x) | nan(codes[i][h].y) | nan(codes[i][h].z) | nan(codes[i][h].w);
-            }
+            if ((now_flags >> (2u + i) & 1u) == 0u) odd |= nan(vw[i][h].x) | nan(vw[i][h].y) | nan(vw[i][h].z) | nan(vw[i][h].w);
           }
         }
         flagged = odd != 0u;
       }
       flagged = __any_sync(0xffffffffu, flagged);
-      if (round != 0u) wait(is_k ? &k_empty[stage] : &v_empty[stage], (round - 1u) & 1u);
+      if (round != 0u) wait(&v_empty[stage], (round - 1u) & 1u);
       if (__builtin_expect(flagged, 0)) {
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
 #pragma unroll
           for (uint32_t h = 0; h < 2u; ++h) {  // both halves of a row's 128 columns
             uint32_t bits = 0;
-            if (h < kMine && (flags >> (2u + i) & 1u) == 0u) {
+            if (h < kMine && (now_flags >> (2u + i) & 1u) == 0u) {
               auto clean = [&](uint32_t& word, uint32_t e) {
                 const uint32_t is = (((word & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
                 word &= ~(is * 0xffu);
                 bits |= (is * 0x01020408u >> 24 & 15u) << (4u * e);
               };
-              uint4& w = codes[i][h % kMine];
+              uint4& w = vw[i][h % kMine];
               clean(w.x, 0u), clean(w.y, 1u), clean(w.z, 2u), clean(w.w, 3u);
             }
             reinterpret_cast<uint16_t*>(smem + Shape::nan_bits)[(stage * kStep + 16u * group + 8u * i + r) * 8u + pq + 4u * h] =
@@ -560,44 +602,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           }
         }
       }
-      if (lane == 0u) {
-        if (is_k) {
-          const float to = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
-          reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + group] = make_float4(ks, log2f(to), 1.f / to, 0.f);
-        } else {
-          nan_flag[stage][group] = flagged ? 1u : 0u;
-        }
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 2u; ++i) {
-#pragma unroll
-        for (uint32_t h = 0; h < kMine; ++h) {
-          uint8_t* const to = smem + tile + group * 2048u + h * kCodePanel + i * 1024u;
-          uint4 x, y;
-          codes_to_half(codes[i][h].x, x.x, x.y);
-          codes_to_half(codes[i][h].y, x.z, x.w);
-          codes_to_half(codes[i][h].z, y.x, y.y);
-          codes_to_half(codes[i][h].w, y.z, y.w);
-          *reinterpret_cast<uint4*>(to + chunk0) = x;
-          *reinterpret_cast<uint4*>(to + chunk1) = y;
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0u) {
-        mbar_arrive(is_k ? &k_full[stage] : &v_full[stage]);
-        if (is_k) mbar_arrive(&scale_full[ring]);
-      }
-      more = ahead;
-      if (more) {
-        const uint32_t before = now_turn;
-        load();
-        if (now_turn < before) {  // the next step
-          ring = (ring + 1u) % kScaleRing;
-          if (++stage == kStages) stage = 0u, ++round;
-        }
-        look();
-      }
+      if (lane == 0u) nan_flag[stage][group] = flagged ? 1u : 0u;
+      store(tile + (Shape::v_at - Shape::k_at), vw);
+      if (lane == 0u) mbar_arrive(&v_full[stage]);
+      if (more) load(c.v, vw);
     }
   } else if (elect_one()) {
     // ================= the products, by one thread
