@@ -5,6 +5,7 @@
 //
 // A CPython module (qgemv_b200/paged.py and paged8.py are its only users).  It does not link the library: bind()
 // is given the addresses of its entry points.  No device code, no computation.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -121,14 +122,15 @@ float* floats_of(const at::Tensor& t, std::initializer_list<int64_t> shape, int 
 float* floats_or_null(PyObject* o, std::initializer_list<int64_t> shape, int index, const char* name) {
   return o == Py_None ? nullptr : floats_of(tensor_of(o, name), shape, index, name);
 }
-int dtype_of(const at::Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
+int dtype_code(at::ScalarType type, const char* name) {
+  switch (type) {
     case at::kFloat: return QG_F32;
     case at::kHalf: return QG_F16;
     case at::kBFloat16: return QG_BF16;
     default: refuse(name, "float32, float16 or bfloat16 is needed");
   }
 }
+int dtype_of(const at::Tensor& t, const char* name) { return dtype_code(t.scalar_type(), name); }
 // A number of slots, heads and the like; one that is none becomes the largest, which the
 // library refuses.
 uint32_t count_of(PyObject* o) {
@@ -541,8 +543,7 @@ PyObject* py_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// read8(cache, starts, offsets, tokens, like, k_out, v_out, stream) -> (cudaError_t, k_out, v_out);
-// `like` is an empty tensor of the type and device of the rows
+// read8(cache, starts, offsets, tokens, dtype, k_out, v_out, stream) -> (cudaError_t, k_out, v_out)
 PyObject* py_read8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 8, [&]() -> PyObject* {
     const Cache8* c = held<Cache8>(args[0], kCache8Name);
@@ -554,13 +555,15 @@ PyObject* py_read8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     r.tokens = count_of(args[3]);
     if (r.tokens > 0x7fffffffu) refuse("tokens", "a number of rows below 2^31 is needed");
     const int64_t tokens = r.tokens;
-    const at::Tensor& like = tensor_of(args[4], "dtype");
-    r.dtype = dtype_of(like, "dtype");
+    if (!THPDtype_Check(args[4])) refuse("dtype", "a torch.dtype is needed");
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    r.dtype = dtype_code(type, "dtype");
+    const auto options = at::TensorOptions().dtype(type).device(at::kCUDA, static_cast<c10::DeviceIndex>(c->index));
     const Call call(c->index, args[7]);
-    const at::Tensor k = args[5] == Py_None ? at::empty({tokens, kv, dim}, like.options()) : tensor_of(args[5], "k_out");
-    const at::Tensor v = args[6] == Py_None ? at::empty({tokens, kv, dim}, like.options()) : tensor_of(args[6], "v_out");
-    r.k_stride = heads_of(k, tokens, kv, dim, like.scalar_type(), c->index, "k_out");
-    r.v_stride = heads_of(v, tokens, kv, dim, like.scalar_type(), c->index, "v_out");
+    const at::Tensor k = args[5] == Py_None ? at::empty({tokens, kv, dim}, options) : tensor_of(args[5], "k_out");
+    const at::Tensor v = args[6] == Py_None ? at::empty({tokens, kv, dim}, options) : tensor_of(args[6], "v_out");
+    r.k_stride = heads_of(k, tokens, kv, dim, type, c->index, "k_out");
+    r.v_stride = heads_of(v, tokens, kv, dim, type, c->index, "v_out");
     r.k_out = k.data_ptr();
     r.v_out = v.data_ptr();
     const cudaError_t e = g_entries.read8(&c->pages, &r, call.stream);

@@ -78,8 +78,7 @@ def read(cache: PagedCache8, starts: torch.Tensor, offsets: torch.Tensor, tokens
          v_out: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """qg_kv_read8: keys and values [tokens, kv heads, dim] of `dtype`; rows offsets[b] on are the
     slots from starts[b] [sequences] on of sequence b."""
-    like = torch.empty(0, dtype=dtype, device=cache.device)
-    code, k_out, v_out = cache.calls.read8(cache.held, starts, offsets, tokens, like, k_out, v_out,
+    code, k_out, v_out = cache.calls.read8(cache.held, starts, offsets, tokens, dtype, k_out, v_out,
                                            None if stream is None else stream.cuda_stream)
     if code != 0:
         raise CudaError("qg_kv_read8", code)
