@@ -14,6 +14,7 @@
 // A row lies in LPR lanes as in qg_paged_append.cu: pairs never leave a lane, the sum of
 // squares is log2(LPR) shuffles.
 #include <algorithm>
+#include <type_traits>
 
 #include "qg_paged8.cuh"
 #include "qg_rows.cuh"
@@ -25,9 +26,6 @@ constexpr uint32_t kWarps8 = 4;
 constexpr uint32_t kThreads8 = kWarps8 * 32u;
 template <typename T>
 constexpr uint32_t kBatch8 = 4 / sizeof(T);  // rows that a lane has in flight: 64 bytes
-
-// CTAs of queries from which they are a launch of their own, with more warps an SM than the blocks' registers allow.
-constexpr uint64_t kApartFrom = 8192;
 
 struct Append8Args {
   const void *q, *k, *v;
@@ -126,17 +124,15 @@ __device__ __forceinline__ float least_scale(uint32_t size) {
   return __uint_as_float(static_cast<uint32_t>(127 + max(kLeastPower, min(kMostPower, e))) << 23);
 }
 
-enum class Part8 { both, queries, blocks };
-
-template <typename T, int LPR, bool HALVES, Part8 PART>
-__global__ void __launch_bounds__(kThreads8, PART == Part8::queries ? 6 : 5) append8_kernel(const Paged8View c, const Append8Args a) {
+template <typename T, int LPR, bool HALVES>
+__global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View c, const Append8Args a) {
   constexpr uint32_t kSide = 32 / LPR;                 // rows side by side in a warp
   constexpr uint32_t kRows = kSide * kBatch8<T>;       // of a warp's pass
   extern __shared__ float4 kept[];                     // rows of passes after the first
   __shared__ uint32_t tops[kWarps8];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, chunk = lane % LPR;
-  const uint32_t block_ctas = PART == Part8::queries ? 0u : a.block_tasks * 2u * c.c.n_kv;
-  const bool is_q = PART == Part8::queries || (PART == Part8::both && blockIdx.x >= block_ctas);
+  const uint32_t block_ctas = a.block_tasks * 2u * c.c.n_kv;
+  const bool is_q = blockIdx.x >= block_ctas;
   uint32_t head0 = 0, heads = 0, t = 0;
   bool is_k = false;
   if (is_q) {
@@ -189,31 +185,30 @@ __global__ void __launch_bounds__(kThreads8, PART == Part8::queries ? 6 : 5) app
     float ss = (s.x + s.y) + (z.x + z.y);
 #pragma unroll
     for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off, LPR);
-    // One Newton step on the fast root: an error here moves every code of the row near a border.
-    // (Its step is below 2^-20; the bound keeps roots of 0 and infinity.)
-    const float mean = fmaf(ss, a.inv_dim, a.eps), fast = rsqrtf(mean);
-    const float step = fmaxf(fminf(fmaf(-mean * fast, fast, 1.f), 0x1p-20f), -0x1p-20f);
-    return fmaf(0.5f * fast, step, fast);
+    return rsqrtf(__fadd_rn(__fmul_rn(ss, a.inv_dim), a.eps));
   };
-  // norm and rotation of a lane's share of a key, in place; all lanes of the warp take part
-  auto finish = [&](float (&xa)[8], float (&xb)[8], const Turn& turn) {
+  // Norm and rotation of a lane's share of a row, in place; all lanes of the warp take part.  A key that lies near
+  // the border of two codes goes by its last bit, so keys take every product and sum rounded by itself, as the
+  // formula is written, queries the cheaper fused ones.
+  auto finish = [&](float (&xa)[8], float (&xb)[8], const Turn& turn, auto key) {
+    constexpr bool kKey = decltype(key)::value;
     Pairs p = pairs_of<HALVES>(xa, xb);
     if (norm != nullptr) {
       const float inv = root(p);
       const F2 by = f2(inv, inv);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        p.u[h] = p.u[h] * (by * weight.u[h]);
-        p.v[h] = p.v[h] * (by * weight.v[h]);
+        p.u[h] = kKey ? (p.u[h] * by) * weight.u[h] : p.u[h] * (by * weight.u[h]);
+        p.v[h] = kKey ? (p.v[h] * by) * weight.v[h] : p.v[h] * (by * weight.v[h]);
       }
     }
     if (!some_stay || turned) {
       const F2 minus = f2(-1.f, -1.f);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const F2 u = p.u[h], v = p.v[h];
-        p.u[h] = fma(u, turn.co[h], minus * (v * turn.si[h]));
-        p.v[h] = fma(v, turn.co[h], u * turn.si[h]);
+        const F2 u = p.u[h], v = p.v[h], down = minus * (v * turn.si[h]);
+        p.u[h] = kKey ? u * turn.co[h] + down : fma(u, turn.co[h], down);
+        p.v[h] = kKey ? u * turn.si[h] + v * turn.co[h] : fma(v, turn.co[h], u * turn.si[h]);
       }
     }
     values_of<HALVES>(p, xa, xb);
@@ -237,39 +232,13 @@ __global__ void __launch_bounds__(kThreads8, PART == Part8::queries ? 6 : 5) app
     const int32_t pos = place(t);
     Turn turn = {};
     if (turned && pos >= 0) turn.load(a.rope + static_cast<size_t>(pos) * a.rot + chunk * 8u, a.rot / 2u);
-    // u <- u uu + v uv, v <- v vv + u vu: the rotation with the weights in it, once for the token's heads
-    Pairs same = weight, other = weight;
-    if (turned) {
-      const F2 minus = f2(-1.f, -1.f);
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        same.u[h] = weight.u[h] * turn.co[h];
-        same.v[h] = weight.v[h] * turn.co[h];
-        other.u[h] = weight.v[h] * (minus * turn.si[h]);
-        other.v[h] = weight.u[h] * turn.si[h];
-      }
-    }
 #pragma unroll
     for (uint32_t i = 0; i < kBatch8<T>; ++i) {
       float xa[8] = {}, xb[8] = {};
       if (pos >= 0) {  // the same in all lanes
         raw[i][0].get(xa);
         raw[i][1].get(xb);
-        Pairs p = pairs_of<HALVES>(xa, xb);
-        const float inv = norm == nullptr ? 1.f : root(p);
-        const F2 by = f2(inv, inv);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const F2 u = by * p.u[h], v = by * p.v[h];
-          if (some_stay && !turned) {
-            p.u[h] = u * same.u[h];
-            p.v[h] = v * same.v[h];
-          } else {
-            p.u[h] = fma(u, same.u[h], v * other.u[h]);
-            p.v[h] = fma(v, same.v[h], u * other.v[h]);
-          }
-        }
-        values_of<HALVES>(p, xa, xb);
+        finish(xa, xb, turn, std::false_type());
       }
       const bool live = head0 + i * kSide < heads;
       if (live && has0) store8<T>(to + at0 + i * (kSide * c.c.dim), xa);
@@ -277,7 +246,6 @@ __global__ void __launch_bounds__(kThreads8, PART == Part8::queries ? 6 : 5) app
     }
     return;
   }
-  if constexpr (PART == Part8::queries) return;
 
   // ---- the rows of one block and kv head
   const Run run = find_run(c, a, blockIdx.x / (2u * c.c.n_kv));
@@ -319,7 +287,7 @@ __global__ void __launch_bounds__(kThreads8, PART == Part8::queries ? 6 : 5) app
       if (turned && pos[i] >= 0) turn.load(a.rope + static_cast<size_t>(pos[i]) * a.rot + chunk * 8u, a.rot / 2u);
       raw[i][0].get(xa[i]);
       raw[i][1].get(xb[i]);
-      if (is_k) finish(xa[i], xb[i], turn);
+      if (is_k) finish(xa[i], xb[i], turn, std::true_type());
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (pos[i] < 0) xa[i][e] = xb[i][e] = 0.f;
@@ -392,20 +360,15 @@ cudaError_t launch_append8(const Paged8View& c, const Append8Args& a, cudaStream
   const uint32_t longest = a.offsets == nullptr ? 1u : std::min(1u << c.log_block, a.tokens);
   const uint32_t passes = (longest + kRows * kWarps8 - 1u) / (kRows * kWarps8);
   const uint32_t smem = (passes - 1u) * kBatch8<T> * 64u * kThreads8;
-  const uint64_t block_ctas = static_cast<uint64_t>(a.block_tasks) * 2u * c.c.n_kv;
-  const uint64_t q_ctas = static_cast<uint64_t>((a.tokens + kWarps8 - 1u) / kWarps8) * w.q_parts;
-  if (block_ctas + q_ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+  static SmemAttr attr;
   constexpr uint32_t kMost = (128u / (kRows * kWarps8) - 1u) * kBatch8<T> * 64u * kThreads8;
-  auto launch = [&](auto kernel, SmemAttr& attr, uint64_t ctas) {
-    const cudaError_t e = attr.set(reinterpret_cast<const void*>(kernel), kMost);
-    if (e != cudaSuccess) return e;
-    return launch_k(kernel, static_cast<uint32_t>(ctas), kThreads8, smem, stream, c, w);
-  };
-  static SmemAttr both, blocks;
-  if (q_ctas < kApartFrom) return launch(append8_kernel<T, LPR, HALVES, Part8::both>, both, block_ctas + q_ctas);
-  const cudaError_t e = launch(append8_kernel<T, LPR, HALVES, Part8::blocks>, blocks, block_ctas);
+  const auto kernel = append8_kernel<T, LPR, HALVES>;
+  const cudaError_t e = attr.set(reinterpret_cast<const void*>(kernel), kMost);
   if (e != cudaSuccess) return e;
-  return launch_k(append8_kernel<T, LPR, HALVES, Part8::queries>, static_cast<uint32_t>(q_ctas), kThreads8, 0, stream, c, w);
+  const uint64_t ctas = static_cast<uint64_t>(a.block_tasks) * 2u * c.c.n_kv +
+                        static_cast<uint64_t>((a.tokens + kWarps8 - 1u) / kWarps8) * w.q_parts;
+  if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+  return launch_k(kernel, static_cast<uint32_t>(ctas), kThreads8, smem, stream, c, w);
 }
 
 template <typename T, int LPR>

@@ -289,6 +289,16 @@ def test_long_and_many(cuda, dtype):
     check(c, q[: sum(counts)], lens, counts, out, lse)
     out = paged8.attend(plan, q[:1500], int32(lens), window=40, sink=3)
     check(c, q[:1500], lens, [1] * 1500, out, None, 40, 3)
+    # many sequences of many rows each: more tiles than SMs, some cut between them
+    counts = [int(n) for n in rng.integers(0, 130, 120)]
+    lens = [n + int(m) for n, m in zip(counts, rng.integers(0, 500, 120))]
+    for dim, heads, kv in ((128, 8, 2), (48, 3, 1)):
+        c = make_cache(rng, 120, 20, 32, 16, kv, dim)
+        q = queries(rng, sum(counts), heads, dim, DTYPES[dtype])
+        plan = paged8.AttentionPlan8(c, heads, max_tokens=len(q))
+        for window, sink in ((0, 0), (90, 7)):
+            out, lse = paged8.attend(plan, q, int32(lens), offsets=offsets(counts), window=window, sink=sink, return_lse=True)
+            check(c, q, lens, counts, out, lse, window, sink)
     assert ops.get_error() == 0
 
 
