@@ -257,13 +257,10 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
   if (run.n == 0u) return;
   const uint32_t block_slots = 1u << c.log_block, block0 = run.slot & ~(block_slots - 1u);
   const int32_t* row = c.c.table + static_cast<size_t>(run.b) * c.c.table_stride;
-  const uint64_t base = paged_row(c.c, row, block0, head0);
-  if (base == kNoRow) return;
-  const uint32_t on_page = div_by(block0, c.c.page);
-  float* const scale_at = (is_k ? c.ks : c.vs) + static_cast<uint32_t>(row[on_page]) * c.scale_page +
-                          head0 * c.scale_head + ((block0 - on_page * c.c.page.d) >> c.log_block);
-  uint8_t* const codes = (is_k ? c.c.k : c.c.v) + base;
-  const float old = run.slot != block0 ? *scale_at : 0.f;
+  const uint32_t on_page = div_by(block0, c.c.page), place0 = block0 - on_page * c.c.page.d;
+  const uint32_t id = static_cast<uint32_t>(row[on_page]);  // looked at once the rows are on their way
+  float* scale_at = nullptr;
+  float old = 0.f;
   const T* src = static_cast<const T*>(is_k ? a.k : a.v) + head0 * c.c.dim;
   const uint64_t stride = is_k ? a.k_stride : a.v_stride;
   constexpr uint32_t kPass = kRows * kWarps8;
@@ -285,6 +282,14 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
         if (has1) raw[i][1].load(from + at1);
         pos[i] = place(run.token + r);
       }
+    }
+    if (p + 1u == passes) {
+      if (id >= c.c.num_pages) {  // the same for the whole CTA
+        if (tid == 0u) atomicOr(&g_error_word, QG_ERR_PAGE);
+        return;
+      }
+      scale_at = (is_k ? c.ks : c.vs) + id * c.scale_page + head0 * c.scale_head + (place0 >> c.log_block);
+      if (run.slot != block0) old = *scale_at;
     }
 #pragma unroll
     for (uint32_t i = 0; i < kBatch8<T>; ++i) {
@@ -314,6 +319,7 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
   for (uint32_t w = 0; w < kWarps8; ++w) top = max(top, tops[w]);
   const float scale = fmaxf(least_scale(top), old), by = 1.f / scale;
   if (tid == 0u) *scale_at = scale;
+  uint8_t* const codes = (is_k ? c.c.k : c.c.v) + id * c.c.page_bytes + head0 * c.c.head_bytes + place0 * c.c.slot_bytes;
   if (scale > old && run.slot != block0) {
     const float shrink = old / scale;
     const uint32_t pieces = c.c.dim / 16u;
