@@ -9,7 +9,10 @@
 // grows, the CTA also scales the block's other codes down, so that they stand for what they stood
 // for: scales are powers of two, so this moves exponents and rounds only what falls below e4m3's
 // normal range.  Query rows need no neighbour: a warp takes a batch of one token's heads.  Both
-// kinds of task are in one launch, the blocks first, because they wait the longest.
+// kinds of task are in one launch, the blocks first, because they wait the longest.  In a call with
+// one row a sequence (decoding) nothing but that row is new in a block, so its keys and values go
+// a batch of heads a warp too, without the CTA's barrier: 256 sequences of 64/8 heads x 128 bf16 are
+// 640 CTAs and 10 us on the GPU, against 4608 and 25 us with a CTA for each block.
 //
 // Measured (B200, floor = bytes at 6.56 TB/s): 16384 tokens of 64/8 heads x 128 bf16, blocks of 64: 149 us
 // (floor 98); launched apart the queries took 110 us, 63% of the issue slots, and the blocks 42, a chain of
@@ -40,24 +43,39 @@ struct Append8Args {
   const int32_t *positions, *lens, *offsets;
   float eps, inv_dim;
   uint32_t n_q, rot, rope_rows, tokens;
-  uint32_t block_tasks;  // of one kv head
-  uint32_t q_parts;      // tasks of a token's queries
+  uint32_t block_tasks;  // of one kv head, of a ragged call
+  uint32_t q_parts, kv_parts;  // tasks of a token's queries; of its keys, and values, of a call with a row a sequence
 };
+
+// A begun block's other codes, when its scale grows by 1 / shrink: those of all rows but [at, at + n).
+__device__ __forceinline__ void shrink_others(uint8_t* codes, uint64_t slot_bytes, uint32_t dim, uint32_t slots,
+                                              uint32_t at, uint32_t n, float shrink, uint32_t tid, uint32_t threads) {
+  const uint32_t pieces = dim / 16u;
+#pragma unroll 4
+  for (uint32_t i = tid; i < (slots - n) * pieces; i += threads) {
+    uint32_t r = i / pieces;
+    const uint32_t piece = i - r * pieces;
+    if (r >= at) r += n;
+    uint4* from = reinterpret_cast<uint4*>(codes + r * slot_bytes + piece * 16u);
+    uint4 w = *from;
+    auto less = [&](uint32_t u) {
+      float x[4];
+      codes_to_float(u, x);
+      return float_to_codes(x[0] * shrink, x[1] * shrink, x[2] * shrink, x[3] * shrink);
+    };
+    w.x = less(w.x), w.y = less(w.y), w.z = less(w.z), w.w = less(w.w);
+    *from = w;
+  }
+}
 
 // What a CTA writes to one block: rows [token, token + n) of the call to slots from `slot` on.
 struct Run {
   uint32_t b, token, slot, n;
 };
 
-// The run with index `want` among all sequences' (a sequence's runs are the blocks that its new
-// tokens touch); n 0 where there are fewer.  All threads of the CTA take part.
+// The run with index `want` among all sequences' of a ragged call (a sequence's runs are the blocks that
+// its new tokens touch); n 0 where there are fewer.  All threads of the CTA take part.
 __device__ __forceinline__ Run find_run(const Paged8View& c, const Append8Args& a, uint32_t want) {
-  Run run{0u, 0u, 0u, 0u};
-  if (a.offsets == nullptr) {  // one row a sequence
-    const Rows8 r = rows_of(c.c, a.lens, nullptr, a.tokens, want);
-    if (r.len != 0u) run = Run{want, want, r.len - 1u, 1u};
-    return run;
-  }
   __shared__ uint32_t sums[kWarps8];
   __shared__ Run found;
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
@@ -129,18 +147,32 @@ __device__ __forceinline__ float least_scale(uint32_t size) {
   return __uint_as_float(static_cast<uint32_t>(127 + max(kLeastPower, min(kMostPower, e))) << 23);
 }
 
-template <typename T, int LPR, bool HALVES>
+__device__ __forceinline__ void put8(uint8_t* to, const float (&x)[8], float by) {
+  *reinterpret_cast<uint2*>(to) = make_uint2(float_to_codes(x[0] * by, x[1] * by, x[2] * by, x[3] * by),
+                                             float_to_codes(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+}
+
+// ONE: a row a sequence (no offsets).
+template <typename T, int LPR, bool HALVES, bool ONE>
 __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View c, const Append8Args a) {
   constexpr uint32_t kSide = 32 / LPR;                 // rows side by side in a warp
   constexpr uint32_t kRows = kSide * kBatch8<T>;       // of a warp's pass
   extern __shared__ float4 kept[];                     // rows of passes after the first
   __shared__ uint32_t tops[kWarps8];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, chunk = lane % LPR;
-  const uint32_t block_ctas = a.block_tasks * 2u * c.c.n_kv;
-  const bool is_q = blockIdx.x >= block_ctas;
+  const uint32_t block_ctas = ONE ? 0u : a.block_tasks * 2u * c.c.n_kv;
+  bool is_q = blockIdx.x >= block_ctas, is_k = false;
   uint32_t head0 = 0, heads = 0, t = 0;
-  bool is_k = false;
-  if (is_q) {
+  if constexpr (ONE) {
+    const uint32_t task = blockIdx.x * kWarps8 + warp, parts = a.q_parts + 2u * a.kv_parts;
+    uint32_t part = task % parts;
+    t = task / parts;
+    is_q = part >= 2u * a.kv_parts;
+    is_k = part < a.kv_parts;
+    if (!is_k) part -= is_q ? 2u * a.kv_parts : a.kv_parts;
+    head0 = part * kRows + lane / LPR;
+    heads = is_q ? a.n_q : c.c.n_kv;
+  } else if (is_q) {
     const uint32_t task = blockIdx.x - block_ctas, part = task % a.q_parts;
     t = task / a.q_parts * kWarps8 + warp;
     head0 = part * kRows + lane / LPR;
@@ -221,7 +253,7 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
 
   if (is_q) {
     if (t >= a.tokens) return;
-    if (a.offsets != nullptr && (static_cast<int64_t>(t) < a.offsets[0] || static_cast<int64_t>(t) >= a.offsets[c.c.batch])) {
+    if (!ONE && (static_cast<int64_t>(t) < a.offsets[0] || static_cast<int64_t>(t) >= a.offsets[c.c.batch])) {
       return;  // a row of no sequence
     }
     const T* src = static_cast<const T*>(a.q) + t * a.q_stride + head0 * c.c.dim;
@@ -248,6 +280,73 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
       const bool live = head0 + i * kSide < heads;
       if (live && has0) store8<T>(to + at0 + i * (kSide * c.c.dim), xa);
       if (live && has1) store8<T>(to + at1 + i * (kSide * c.c.dim), xb);
+    }
+    return;
+  }
+
+  if constexpr (ONE) {  // ---- a warp's heads of one token's keys or values
+    if (t >= a.tokens) return;
+    const Rows8 rows = rows_of(c.c, a.lens, nullptr, a.tokens, t);
+    if (rows.len == 0u) return;
+    const T* src = static_cast<const T*>(is_k ? a.k : a.v) + t * (is_k ? a.k_stride : a.v_stride) + head0 * c.c.dim;
+    const uint32_t slot = rows.len - 1u, block_slots = 1u << c.log_block;
+    const uint32_t in_block = slot & (block_slots - 1u), block0 = slot - in_block;
+    const uint32_t on_page = div_by(block0, c.c.page), place0 = block0 - on_page * c.c.page.d;
+    const uint32_t id = static_cast<uint32_t>(c.c.table[static_cast<size_t>(t) * c.c.table_stride + on_page]);
+    Piece<T> raw[kBatch8<T>][2];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch8<T>; ++i) {
+      raw[i][0] = raw[i][1] = Piece<T>{};
+      const bool live = head0 + i * kSide < heads;
+      if (live && has0) raw[i][0].load(src + at0 + i * (kSide * c.c.dim));
+      if (live && has1) raw[i][1].load(src + at1 + i * (kSide * c.c.dim));
+    }
+    const int32_t pos = place(t);
+    Turn turn = {};
+    if (turned && pos >= 0) turn.load(a.rope + static_cast<size_t>(pos) * a.rot + chunk * 8u, a.rot / 2u);
+    if (id >= c.c.num_pages) {
+      if (lane == 0u) atomicOr(&g_error_word, QG_ERR_PAGE);
+      return;
+    }
+    float* const scales = (is_k ? c.ks : c.vs) + id * c.scale_page + (place0 >> c.log_block);
+    uint8_t* const codes = (is_k ? c.c.k : c.c.v) + id * c.c.page_bytes + place0 * c.c.slot_bytes;
+    float old[kBatch8<T>];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch8<T>; ++i) {
+      const uint32_t head = head0 + i * kSide;
+      old[i] = in_block != 0u && head < heads ? scales[head * c.scale_head] : 0.f;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch8<T>; ++i) {
+      const uint32_t head = head0 + i * kSide;
+      float xa[8] = {}, xb[8] = {};
+      if (pos >= 0) {  // the same in all lanes
+        raw[i][0].get(xa);
+        raw[i][1].get(xb);
+        if (is_k) finish(xa, xb, turn, std::true_type());
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, max(finite_size(xa[e]), finite_size(xb[e])));
+#pragma unroll
+      for (int off = LPR / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off, LPR));
+      const float scale = fmaxf(least_scale(top), old[i]), by = 1.f / scale;
+      __syncwarp();  // every lane has read the old scale
+      if (head < heads) {
+        if (chunk == 0u) scales[head * c.scale_head] = scale;
+        uint8_t* to = codes + head * c.c.head_bytes + in_block * c.c.slot_bytes;
+        if (has0) put8(to + at0, xa, by);
+        if (has1) put8(to + at1, xb, by);
+      }
+      // blocks whose scale grew, one after another with all lanes
+      uint32_t grown = __ballot_sync(0xffffffffu, chunk == 0u && head < heads && in_block != 0u && scale > old[i]);
+      while (grown != 0u) {
+        const int from = __ffs(static_cast<int>(grown)) - 1;
+        grown &= grown - 1u;
+        const float shrink = __shfl_sync(0xffffffffu, old[i] / scale, from);
+        shrink_others(codes + __shfl_sync(0xffffffffu, head, from) * c.c.head_bytes, c.c.slot_bytes, c.c.dim,
+                      block_slots, in_block, 1u, shrink, lane, 32u);
+      }
     }
     return;
   }
@@ -321,22 +420,7 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
   if (tid == 0u) *scale_at = scale;
   uint8_t* const codes = (is_k ? c.c.k : c.c.v) + id * c.c.page_bytes + head0 * c.c.head_bytes + place0 * c.c.slot_bytes;
   if (scale > old && run.slot != block0) {
-    const float shrink = old / scale;
-    const uint32_t pieces = c.c.dim / 16u;
-    for (uint32_t i = tid; i < (block_slots - run.n) * pieces; i += kThreads8) {
-      uint32_t r = i / pieces;  // of the block's rows but the new ones
-      const uint32_t piece = i - r * pieces;
-      if (r >= run.slot - block0) r += run.n;
-      uint4* at = reinterpret_cast<uint4*>(codes + r * c.c.slot_bytes + piece * 16u);
-      uint4 w = *at;
-      auto less = [&](uint32_t u) {
-        float x[4];
-        codes_to_float(u, x);
-        return float_to_codes(x[0] * shrink, x[1] * shrink, x[2] * shrink, x[3] * shrink);
-      };
-      w.x = less(w.x), w.y = less(w.y), w.z = less(w.z), w.w = less(w.w);
-      *at = w;
-    }
+    shrink_others(codes, c.c.slot_bytes, c.c.dim, block_slots, run.slot - block0, run.n, old / scale, tid, kThreads8);
   }
   for (uint32_t p = 0; p < passes; ++p) {
 #pragma unroll
@@ -352,13 +436,8 @@ __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View 
       const uint32_t r = p * kPass + warp * kRows + lane / LPR + i * kSide;
       if (r >= run.n) continue;
       uint8_t* to = codes + (run.slot - block0 + r) * c.c.slot_bytes;
-      auto put = [&](uint32_t at, const float (&x)[8]) {
-        *reinterpret_cast<uint2*>(to + at) =
-            make_uint2(float_to_codes(x[0] * by, x[1] * by, x[2] * by, x[3] * by),
-                       float_to_codes(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
-      };
-      if (has0) put(at0, xa[i]);
-      if (has1) put(at1, xb[i]);
+      if (has0) put8(to + at0, xa[i], by);
+      if (has1) put8(to + at1, xb[i], by);
     }
   }
 }
@@ -368,12 +447,19 @@ cudaError_t launch_append8(const Paged8View& c, const Append8Args& a, cudaStream
   constexpr uint32_t kRows = 32 / LPR * kBatch8<T>;
   Append8Args w = a;
   w.q_parts = (a.n_q + kRows - 1u) / kRows;
-  const uint32_t longest = a.offsets == nullptr ? 1u : std::min(1u << c.log_block, a.tokens);
+  w.kv_parts = (c.c.n_kv + kRows - 1u) / kRows;
+  if (a.offsets == nullptr) {
+    const uint64_t warps = static_cast<uint64_t>(a.tokens) * (w.q_parts + 2u * w.kv_parts);
+    if (warps > 0x7fffffffull) return cudaErrorInvalidValue;
+    return launch_k(append8_kernel<T, LPR, HALVES, true>, static_cast<uint32_t>((warps + kWarps8 - 1u) / kWarps8),
+                    kThreads8, 0u, stream, c, w);
+  }
+  const uint32_t longest = std::min(1u << c.log_block, a.tokens);
   const uint32_t passes = (longest + kRows * kWarps8 - 1u) / (kRows * kWarps8);
   const uint32_t smem = (passes - 1u) * kBatch8<T> * 64u * kThreads8;
   static SmemAttr attr;
   constexpr uint32_t kMost = (128u / (kRows * kWarps8) - 1u) * kBatch8<T> * 64u * kThreads8;
-  const auto kernel = append8_kernel<T, LPR, HALVES>;
+  const auto kernel = append8_kernel<T, LPR, HALVES, false>;
   const cudaError_t e = attr.set(reinterpret_cast<const void*>(kernel), kMost);
   if (e != cudaSuccess) return e;
   const uint64_t ctas = static_cast<uint64_t>(a.block_tasks) * 2u * c.c.n_kv +
@@ -440,11 +526,8 @@ extern "C" cudaError_t qg_qk_norm_rope_append8(const qg_kv_pages8* cache, const 
   a.rope_rows = p->rope_rows;
   a.tokens = p->tokens;
   // a sequence of n new tokens touches at most n / block + 2 blocks
-  a.block_tasks = p->tokens;
-  if (p->offsets != nullptr) {
-    const uint64_t most = (static_cast<uint64_t>(p->tokens) >> c.log_block) + 2ull * std::min(p->tokens, cache->batch);
-    a.block_tasks = static_cast<uint32_t>(std::min<uint64_t>(most, p->tokens));
-  }
+  const uint64_t most = (static_cast<uint64_t>(p->tokens) >> c.log_block) + 2ull * std::min(p->tokens, cache->batch);
+  a.block_tasks = static_cast<uint32_t>(std::min<uint64_t>(most, p->tokens));
   const bool halves = p->pairs == QG_PAIRS_HALVES;
   if (p->dtype == QG_F32) return launch_append8<float>(c, a, halves, stream);
   if (p->dtype == QG_F16) return launch_append8<__half>(c, a, halves, stream);

@@ -368,3 +368,31 @@ def test_append_of_nothing_does_nothing():
     assert qgemv_b200.call("qg_qk_norm_rope_append8", ctypes.byref(c), ctypes.byref(a), None) == 0
     assert qgemv_b200.call("qg_qk_norm_rope_append8", None, ctypes.byref(a), None) == INVALID_VALUE
     assert qgemv_b200.call("qg_qk_norm_rope_append8", ctypes.byref(c), None, None) == INVALID_VALUE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dim,rot,block,src,pairs", [
+    (9, 128, 128, 32, "f32", "halves"), (9, 128, 64, 16, "bf16", "adjacent"), (17, 48, 48, 64, "f16", "halves"),
+    (5, 256, 256, 128, "f16", "adjacent"), (1, 16, 0, 16, "f32", "adjacent"),
+])
+def test_append_one_row_a_sequence_equals_the_ragged_call(cuda, heads, dim, rot, block, src, pairs):
+    """Without offsets a row is a warp's, with them a block is a CTA's: the same bits, while scales grow, where
+    sequences are padding or have a bad page, and where a position is none."""
+    rng = np.random.default_rng(6)
+    one = make_cache(rng, 7, 2, 128, block, heads, dim)
+    one.table[3, 0] = one.num_pages
+    ragged = paged8.PagedCache8(*(codes(t).clone().view(torch.float8_e4m3fn) for t in (one.k, one.v)),
+                                one.k_scale.clone(), one.v_scale.clone(), one.table)
+    rope = paged.rope_table(60, rot) if rot else None
+    norm = 1 + 0.1 * torch.from_numpy(rng.standard_normal(dim)).float().cuda()
+    for i in range(block - 3, block + 40):
+        q, k, v = new_rows(rng, 7, heads + 2, heads, dim, DTYPES[src])
+        k, v = k * 2.0 ** (i % 23 - 12), v * 2.0 ** (i % 19 - 12)
+        lens, pos = int32([i, 1, 0, 5, i + 100, 3 * i, i]), int32([i % 60, 1, 2, 3, -1, 59, 60 if i % 2 else 0])
+        got = [paged8.qk_norm_rope_append(c, q, k, v, rope, pos, lens, offsets=at, q_norm=norm, pairs=pairs)
+               for c, at in ((one, None), (ragged, offsets([1] * 7)))]
+        assert torch.equal(*got)
+        for name in ("k", "v"):
+            assert torch.equal(codes(getattr(one, name)), codes(getattr(ragged, name)))
+            assert torch.equal(getattr(one, name + "_scale"), getattr(ragged, name + "_scale"))
+        assert ops.get_error() == paged.QG_ERR_PAGE | (paged.QG_ERR_POSITION if rot and i % 2 else 0)
