@@ -16,7 +16,7 @@
 //
 // Measured (B200, floor = bytes at 6.56 TB/s): 16384 tokens of 64/8 heads x 128 bf16, blocks of 64: 149 us
 // (floor 98); launched apart the queries took 110 us, 63% of the issue slots, and the blocks 42, a chain of
-// loads in CTAs of 3 to 4 us each.  32 tokens 4.0 us, 2047 of 32/8 x 80 17 us.  Several heads a CTA, one after
+// loads in CTAs of 3 to 4 us each.  32 tokens 2.9 us, 2047 of 32/8 x 80 17 us.  Several heads a CTA, one after
 // another, took 157 (2 heads) to 189 us (16).
 //
 // A row lies in LPR lanes as in qg_paged_append.cu: pairs never leave a lane, the sum of
@@ -152,7 +152,7 @@ __device__ __forceinline__ void put8(uint8_t* to, const float (&x)[8], float by)
                                              float_to_codes(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
 }
 
-// ONE: a row a sequence (no offsets).
+// ONE: a row a sequence (no offsets).  Five CTAs an SM: 16384 tokens took 155 us, 178 with four, 176 with six.
 template <typename T, int LPR, bool HALVES, bool ONE>
 __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View c, const Append8Args a) {
   constexpr uint32_t kSide = 32 / LPR;                 // rows side by side in a warp

@@ -28,8 +28,8 @@
 //
 // Measured (B200, 6.56 TB/s for a plain copy; time on the GPU, floor = bytes that have to move at that rate):
 // 16 x 32768 slots, 64/8 heads x 128: 179 us (floor 164); 1 x 131072: 56 us (41; 37 CTAs a head leave
-// records that are joined at the end); 64 x ..4097, 16/16 heads x 64, window 2000, rows 1024 bytes apart: 85 us (34); 256 x 300, 32/8
-// heads: 50 us (25); 1 x 511: 12.6 us, all latency.  Two warps a scheduler (255 registers) issue in 40% of the
+// records that are joined at the end); 64 x ..4097, 16/16 heads x 64, window 2000, rows 1024 bytes apart:
+// 85 us (34); 256 x 300, 32/8 heads: 50 us (25); 1 x 511: 12.6 us, all latency.  Two warps a scheduler (255 registers) issue in 40% of the
 // cycles; the rest is the latency of their chains.
 //
 // Rows.  fp32 queries, and any where a kv head has at most 8 rows: eight rows fill rows 0-7 of the A

@@ -11,10 +11,10 @@
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
 //
-// Codes become fp16 once for 256 rows: seven warps take turns at 16 slots,
-// load their codes into registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.  The one layout is a
-// K-major operand over dims (for K, whose N are slots) and an MN-major one over slots (for V, whose N
-// are dims), so no byte is transposed.
+// Codes become fp16 once for 256 rows: seven warps take turns at 16 slots, load their codes into
+// registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.
+// The one layout is a K-major operand over dims (for K, whose N are slots) and an MN-major one over
+// slots (for V, whose N are dims), so no byte is transposed.
 //
 // Warps: 0 issues the products, 1-7 codes, 8-11 and 12-15 the rows of the halves.  With two S of a half
 // the scores of the next step are there before the powers of this one are written, so the rows never
