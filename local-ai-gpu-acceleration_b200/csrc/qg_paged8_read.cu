@@ -3,10 +3,11 @@
 //
 // out = T(code * scale), one multiplication a value: bound by memory, 1 byte read and 2 or 4
 // written a value.  A thread takes 16 codes, a 16-byte piece, of a key row and of the value row
-// beside it, for kTake pieces a CTA's width apart, so that their loads are in flight together and a
-// warp writes whole lines.  Where a row comes from is looked up once a piece; the sequence of a
-// CTA's first row is found by all its threads at once, its later rows go on from there.
-// Measured (B200): 8 x 9000..30001 rows of 8 x 128 to fp16 155 us, 85% of a plain copy's rate; 700 rows 5.1 us.
+// beside it, and writes 32 bytes at a time, a whole sector, where the outputs' rows begin on 32 bytes.  Where
+// a row comes from is looked up once a piece; the sequence of a CTA's first row is found by all its
+// threads at once, its later rows go on from there.
+// Measured (B200; a plain copy's rate is 100%): 8 x 9000..30001 rows of 8 x 128 to fp16 141 us, 94%, and 8 x 20000 to
+// fp32 258 us, 97%; in stores of 16 bytes 147 and 367.  With 256 threads and two pieces each 158 us for the former.
 #include <algorithm>
 
 #include "qg_paged8.cuh"
@@ -14,8 +15,7 @@
 namespace qg {
 namespace {
 
-constexpr uint32_t kReadThreads = 256;
-constexpr uint32_t kTake = 2;  // pieces of a thread
+constexpr uint32_t kReadThreads = 128;
 
 struct Read8Args {
   const int32_t *starts, *offsets;
@@ -25,10 +25,32 @@ struct Read8Args {
   FastDiv row_pieces, head_pieces;  // 16-code pieces of a row (all heads), of a head
 };
 
-template <typename T>
+// 32 bytes at once
+__device__ __forceinline__ void put32(void* to, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// WIDE: rows begin on 32 bytes
+template <typename T, bool WIDE>
 __device__ __forceinline__ void put16(T* to, uint4 w, float scale) {
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
   uint32_t out[8];
+  if constexpr (WIDE && sizeof(T) == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[4];
+        codes_to_float(words[2 * h + i], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[4 * i + e] = __float_as_uint(x[e] * scale);
+      }
+      put32(to + 8 * h, out);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float x[4];
@@ -40,17 +62,19 @@ __device__ __forceinline__ void put16(T* to, uint4 w, float scale) {
       out[2 * i + 1] = pack2(x[2] * scale, x[3] * scale, T());
     }
   }
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (WIDE) {
+    put32(to, out);
+  } else if constexpr (sizeof(T) == 2) {
     reinterpret_cast<uint4*>(to)[0] = make_uint4(out[0], out[1], out[2], out[3]);
     reinterpret_cast<uint4*>(to)[1] = make_uint4(out[4], out[5], out[6], out[7]);
   }
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kReadThreads) read8_kernel(const Paged8View c, const Read8Args a) {
   pdl_wait();
   pdl_trigger();
-  const uint64_t piece0 = static_cast<uint64_t>(blockIdx.x) * (kReadThreads * kTake);
+  const uint64_t piece0 = static_cast<uint64_t>(blockIdx.x) * kReadThreads;
   const uint32_t row0 = static_cast<uint32_t>(piece0 / a.row_pieces.d);
   const uint32_t in0 = static_cast<uint32_t>(piece0 - static_cast<uint64_t>(row0) * a.row_pieces.d);
   // sequences that end at or before the CTA's first row
@@ -64,48 +88,34 @@ __global__ void __launch_bounds__(kReadThreads) read8_kernel(const Paged8View c,
   if (blockIdx.x == 0u && threadIdx.x == 0u && a.offsets[c.c.batch] > static_cast<int64_t>(a.tokens)) {
     atomicOr(&g_error_word, QG_ERR_PAGE);
   }
+  const uint32_t p = in0 + threadIdx.x, down = div_by(p, a.row_pieces);  // from the CTA's first row on
+  const uint32_t row = row0 + down, in = p - down * a.row_pieces.d;
   uint32_t b = before;
-  uint4 kw[kTake], vw[kTake];
-  float ks[kTake], vs[kTake];
-  uint32_t row[kTake], in[kTake];
-#pragma unroll
-  for (uint32_t i = 0; i < kTake; ++i) {
-    const uint32_t p = in0 + threadIdx.x + i * kReadThreads;  // from the CTA's first row on
-    const uint32_t down = div_by(p, a.row_pieces);
-    row[i] = row0 + down;
-    in[i] = p - down * a.row_pieces.d;
-    kw[i] = vw[i] = make_uint4(0u, 0u, 0u, 0u);
-    ks[i] = vs[i] = 0.f;
-    while (b < c.c.batch && a.offsets[b + 1u] <= static_cast<int64_t>(row[i])) ++b;
-    const int32_t first = b < c.c.batch ? a.offsets[b] : 0x7fffffff;
-    if (row[i] >= a.tokens || first > static_cast<int64_t>(row[i])) {
-      row[i] = 0xffffffffu;  // a row of no sequence
-      continue;
-    }
-    const int64_t slot = static_cast<int64_t>(a.starts[b]) + row[i] - first;
-    if (first < 0 || slot < 0 || slot >= c.c.capacity) {
-      atomicOr(&g_error_word, QG_ERR_PAGE);
-      continue;
-    }
-    const uint32_t s = static_cast<uint32_t>(slot), head = div_by(in[i], a.head_pieces);
+  while (b < c.c.batch && a.offsets[b + 1u] <= static_cast<int64_t>(row)) ++b;
+  const int32_t first = b < c.c.batch ? a.offsets[b] : 0x7fffffff;
+  if (row >= a.tokens || first > static_cast<int64_t>(row)) return;  // a row of no sequence
+  const int64_t slot = static_cast<int64_t>(a.starts[b]) + row - first;
+  uint4 kw = make_uint4(0u, 0u, 0u, 0u), vw = kw;
+  float ks = 0.f, vs = 0.f;
+  if (first < 0 || slot < 0 || slot >= c.c.capacity) {
+    atomicOr(&g_error_word, QG_ERR_PAGE);
+  } else {
+    const uint32_t s = static_cast<uint32_t>(slot), head = div_by(in, a.head_pieces);
     const int32_t* list = c.c.table + static_cast<size_t>(b) * c.c.table_stride;
     const uint64_t at = paged_row(c.c, list, s, head);
-    if (at == kNoRow) continue;
-    const uint64_t code = at + (in[i] - head * a.head_pieces.d) * 16u;
-    kw[i] = *reinterpret_cast<const uint4*>(c.c.k + code);
-    vw[i] = *reinterpret_cast<const uint4*>(c.c.v + code);
-    const uint32_t page = div_by(s, c.c.page);
-    const uint64_t scale = static_cast<uint32_t>(list[page]) * c.scale_page + head * c.scale_head +
-                           ((s - page * c.c.page.d) >> c.log_block);
-    ks[i] = c.ks[scale];
-    vs[i] = c.vs[scale];
+    if (at != kNoRow) {
+      const uint64_t code = at + (in - head * a.head_pieces.d) * 16u;
+      kw = *reinterpret_cast<const uint4*>(c.c.k + code);
+      vw = *reinterpret_cast<const uint4*>(c.c.v + code);
+      const uint32_t page = div_by(s, c.c.page);
+      const uint64_t scale = static_cast<uint32_t>(list[page]) * c.scale_page + head * c.scale_head +
+                             ((s - page * c.c.page.d) >> c.log_block);
+      ks = c.ks[scale];
+      vs = c.vs[scale];
+    }
   }
-#pragma unroll
-  for (uint32_t i = 0; i < kTake; ++i) {
-    if (row[i] == 0xffffffffu) continue;
-    put16(static_cast<T*>(a.k) + row[i] * a.k_stride + in[i] * 16u, kw[i], ks[i]);
-    put16(static_cast<T*>(a.v) + row[i] * a.v_stride + in[i] * 16u, vw[i], vs[i]);
-  }
+  put16<T, WIDE>(static_cast<T*>(a.k) + row * a.k_stride + in * 16u, kw, ks);
+  put16<T, WIDE>(static_cast<T*>(a.v) + row * a.v_stride + in * 16u, vw, vs);
 }
 
 }  // namespace
@@ -133,10 +143,18 @@ extern "C" cudaError_t qg_kv_read8(const qg_kv_pages8* cache, const qg_read8* p,
   a.head_pieces = fast_div(c.c.dim / 16u);
   a.row_pieces = fast_div(c.c.n_kv * (c.c.dim / 16u));
   const uint64_t pieces = static_cast<uint64_t>(p->tokens) * a.row_pieces.d;
-  const uint64_t ctas = (pieces + kReadThreads * kTake - 1u) / (kReadThreads * kTake);
+  const uint64_t ctas = (pieces + kReadThreads - 1u) / kReadThreads;
   if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
   const uint32_t grid = static_cast<uint32_t>(ctas);
-  if (p->dtype == QG_F32) return launch_k(read8_kernel<float>, grid, kReadThreads, 0, stream, c, a);
-  if (p->dtype == QG_F16) return launch_k(read8_kernel<__half>, grid, kReadThreads, 0, stream, c, a);
-  return launch_k(read8_kernel<__nv_bfloat16>, grid, kReadThreads, 0, stream, c, a);
+  const uint64_t bytes = dtype_bytes(p->dtype);
+  const bool wide = ((reinterpret_cast<uintptr_t>(p->k_out) | reinterpret_cast<uintptr_t>(p->v_out) | p->k_stride * bytes |
+                      p->v_stride * bytes) & 31u) == 0u;
+  auto launch = [&](auto t) {
+    using T = decltype(t);
+    return wide ? launch_k(read8_kernel<T, true>, grid, kReadThreads, 0, stream, c, a)
+                : launch_k(read8_kernel<T, false>, grid, kReadThreads, 0, stream, c, a);
+  };
+  if (p->dtype == QG_F32) return launch(0.f);
+  if (p->dtype == QG_F16) return launch(__half());
+  return launch(__nv_bfloat16());
 }

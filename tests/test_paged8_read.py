@@ -146,3 +146,23 @@ def test_read_refuses_bad_arguments(field, value):
     c, r = _args()
     setattr(r, field, value)
     assert qgemv_b200.call("qg_kv_read8", ctypes.byref(c), ctypes.byref(r), None) == INVALID_VALUE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_read_rows_that_begin_on_16_bytes(cuda, dtype):
+    """Outputs 16 bytes past a 32-byte boundary, or with such strides: the same bits, and nothing beside them."""
+    rng = np.random.default_rng(8)
+    c = make_cache(rng, 3, 4, 64, 32, 3, 80)
+    starts, ends = int32([7, 0, 100]), offsets([90, 64, 33])
+    dt = DTYPES[dtype]
+    want = paged8.read(c, starts, ends, 190, dtype=dt)
+    few = 16 // dt.itemsize
+    for lead, tail in ((few, 0), (0, few), (few, few)):
+        wide = [torch.full((190, 3 * 80 + lead + tail), 9.0, dtype=dt, device="cuda") for _ in range(2)]
+        outs = [w[:, lead: lead + 240].unflatten(1, (3, 80)) for w in wide]
+        paged8.read(c, starts, ends, 190, dtype=dt, k_out=outs[0], v_out=outs[1])
+        for w, out, x in zip(wide, outs, want):
+            assert torch.equal(out[:187], x[:187]) and (out[187:] == 9).all()
+            assert (w[:, :lead] == 9).all() and (w[:, lead + 240:] == 9).all()
+    assert ops.get_error() == 0
