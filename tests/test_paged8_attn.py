@@ -424,7 +424,7 @@ def _args():
     return pages_c(), Attn8C(64, 64, 1, 2, 4, 256, 256, 64, None, 0, 0, 1.0, None)
 
 
-@pytest.mark.parametrize("field,value", BAD_PAGES + [("head_stride", 1040), ("slot_stride", 48), ("page_stride", 3072)])
+@pytest.mark.parametrize("field,value", BAD_PAGES + [("head_stride", 1040), ("slot_stride", 48), ("page_stride", 5120)])
 def test_attend_refuses_bad_caches(field, value):
     c, a = _args()
     setattr(c, field, value)
