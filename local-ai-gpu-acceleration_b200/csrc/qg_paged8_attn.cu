@@ -7,8 +7,10 @@
 //   s = (q . c) * scale * ks * log2 e,  y = s + log2 vs,
 // the probability that multiplies the value's codes is 2^(y - M), M the running maximum of y:
 // the block's scale costs one addition a score and none a value.  The softmax's sum takes
-// 2^(y - M) / vs, one multiplication for 16 slots.  Scales between 2^-60 and 2^60 keep all of
-// this far inside fp32, and weigh probabilities in fp16 by what they add to the row.
+// 2^(y - M) / vs, one multiplication for 16 slots: probabilities in fp16 are weighed by what they add
+// to the row.  Two scales can lie 120 powers apart, and a slot of the smaller one weighs as much in the
+// sum as one of the larger, so fp32 does not hold the sum's terms as they are: small powers of slots
+// with small scales are raised (kRaise) for the sum, and a sum is scaled by the root of a factor, twice.
 //
 // Bound by memory for few rows: a slot's K and V codes are read once for all rows of a tile, and there
 // is half as much of them as in 16 bits, so a byte carries twice the arithmetic.  Codes become fp16
@@ -60,6 +62,12 @@ constexpr uint32_t kEntries = 64;             // 16-slot steps whose places and 
 static_assert(2u * kMaxCtas * 4u <= QG_PAGED_ATTN_ZEROED, "two counters per CTA");
 static_assert(kMaxCtas / kJoin <= 64u && kJoinAll <= 64u, "two records a lane");
 constexpr float kShare = 14.f;                // log2 of the factor that fp16 probabilities carry
+// exp2 gives zero below 2^-126.  Where a lane's four powers of a 16-slot step are all below 2^kRaiseBelow (zero in
+// fp16 either way) and the step's value scale below 2^kLowScale, they are computed 2^kRaise times as large.  So what a
+// sum loses has at most 2^(60 - kLowScale - 126) = 2^-42 of the heaviest slot's weight, or 2^-24 of that of one of
+// the four, or, raised, 2^(120 - 126 - kRaise).  Without raising it was 2^-20 (kShare counted): 65520 such slots
+// beside 16 of the largest scale came out 2^-8 too light.
+constexpr float kLowScale = -24.f, kRaiseBelow = -102.f, kRaise = 64.f, kLower = 0x1p-64f;
 
 struct AttnMaps8 {
   CUtensorMap k, v;
@@ -534,14 +542,23 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const float now = fmaxf(m[i], top);
           const float from = now == -CUDART_INF_F ? 0.f : now;
-          fade[i] = exp2_fast(m[i] - from);
+          const float root = exp2_fast(0.5f * (m[i] - from));
+          fade[i] = root * root;
           m[i] = now;
           const float base = kShare - from;
-          float sum[kSteps] = {}, all = 0.f;
+          float sum[kSteps] = {}, plus[kSteps], all = 0.f;
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            plus[st] = base;
+            if (__builtin_expect(lg[st] < kLowScale, 0)) {  // the same for the whole warp
+              const float most = fmaxf(fmaxf(x[2 * st][0], x[2 * st][1]), fmaxf(x[2 * st + 1][0], x[2 * st + 1][1]));
+              if (most + base < kRaiseBelow) plus[st] += kRaise, inv[st] *= kLower;
+            }
+          }
 #pragma unroll
           for (int n = 0; n < 2 * kSteps; ++n) {
-            x[n][0] = exp2_fast(x[n][0] + base);
-            x[n][1] = exp2_fast(x[n][1] + base);
+            x[n][0] = exp2_fast(x[n][0] + plus[n / 2]);
+            x[n][1] = exp2_fast(x[n][1] + plus[n / 2]);
             sum[n / 2] += x[n][0] + x[n][1];
             if constexpr (TERMS == 2) {
               split_terms<__half>(x[n][0], x[n][1], p[i][n / 2][n % 2]);
@@ -551,7 +568,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
           }
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) all = fmaf(sum[st], inv[st], all);
-          l[i] = fmaf(l[i], fade[i], all);
+          l[i] = fmaf(l[i] * root, root, all);
         }
       }
 
@@ -718,10 +735,10 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
       float sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (uint32_t w = w0; w < w1; ++w) {
-        const float f = exp2_fast(join_m[w][r] - from);
+        const float root = exp2_fast(0.5f * (join_m[w][r] - from)), f = root * root;
         const float4 x = reinterpret_cast<const float4*>(smem + w * ((kK + kV) * kUnit) + (r < 8u ? at0 : at1))
             [(r & 7u) * (DP / 4u) + (ch ^ ((r & 1u) << 2))];
-        sum = fmaf(join_l[w][r], f, sum);
+        sum = fmaf(join_l[w][r] * root, root, sum);
         v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y);
         v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
       }
@@ -796,12 +813,12 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
           const float from = top == -CUDART_INF_F ? 0.f : top;
-          const float f0 = exp2_fast(pm[i][0] - from), f1 = exp2_fast(pm[i][1] - from);
-          float all = fmaf(pl[i][0], f0, pl[i][1] * f1);
+          const float r0 = exp2_fast(0.5f * (pm[i][0] - from)), r1 = exp2_fast(0.5f * (pm[i][1] - from));
+          float all = fmaf(pl[i][0] * r0, r0, pl[i][1] * r1 * r1);
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-          share[r][lane] = f0;
-          share[r][lane + 32u] = f1;
+          share[r][lane] = r0 * r0;
+          share[r][lane + 32u] = r1 * r1;
           if (lane == 0u) join_m[0][r] = top, join_l[0][r] = all;
         }
         __syncthreads();

@@ -9,7 +9,9 @@
 //                  writes P as fp16 over S
 //   O += P C_v     P from tensor memory, fp32 sums in tensor memory
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
-// they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.
+// they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.  For the
+// softmax's sum they are 2^64 times as large (why is in qg_paged8_attn.cu); that costs 3% of the time.  A branch for
+// steps whose scales need it, in any of five forms, cost 5 to 13%.
 //
 // Codes become fp16 once for 256 rows: seven warps take turns at 16 slots, load their codes into
 // registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.
@@ -21,10 +23,10 @@
 // wait for a product.  The four roles' loops have to stay small: unrolled further they left the
 // instruction cache and took twice the time.
 //
-// Measured (B200): 4096 new tokens of 5600 slots, 64/8 heads x 128 bf16: 624 us, 764 TFLOP/s, 0.46 of what
+// Measured (B200): 4096 new tokens of 5600 slots, 64/8 heads x 128 bf16: 650 us, 733 TFLOP/s, 0.44 of what
 // cuBLAS reaches; a step takes about 3000 cycles, its products 1024.  Leaving out any one of the powers, the
 // products or the conversions saves under 8%: issuer, rows and codes each take about as long, by latency.
-// 4 ragged prompts of 288 to 2500 tokens, 32/8 heads x 64, window 1000: 119 us.
+// 4 ragged prompts of 288 to 2500 tokens, 32/8 heads x 64, window 1000: 120 us.
 //
 // Work.  Segments, blocks, equal ranges for one CTA an SM, records and joins as in
 // qg_paged8_attn.cu.  Every wait is bounded; after one has run out (QG_ERR_WAIT_TIMEOUT) no wait
@@ -50,6 +52,7 @@ constexpr uint32_t kPromptThreads = (kRowWarp0 + kRowWarps) * 32u;  // four warp
 constexpr uint32_t kScaleRing = 8;               // steps whose scales are kept: rows are up to 5 behind the K that is stored
 constexpr uint32_t kMaxPolls = 4000;             // of up to kPollNs each
 constexpr float kCarry = 7.f, kSlack = 8.f;      // log2: the factor of powers, the growth of M that is let pass
+constexpr float kRaise = 64.f, kLower = 0x1p-64f;  // log2 of what the summed powers carry more, and what takes it off
 constexpr float kLeastFactor = 1e-30f;           // of scores: zero would turn minus infinity into NaN
 constexpr uint32_t kPromptHeader = 4;            // what a segment costs beside its blocks, in blocks
 static_assert(2u * 256u * 4u <= QG_PAGED_ATTN_ZEROED && kMaxPromptCtas <= 256u, "a counter per CTA and half");
@@ -60,7 +63,7 @@ struct PromptShape {
   static constexpr uint32_t kChunks = DP / 8u;               // 16-byte chunks of a row in fp16
   static constexpr uint32_t kQBytes = kHalf * DP * 2u, kCodeBytes = kStep * DP * 2u;
   static constexpr uint32_t q_at = 0, k_at = 2u * kQBytes, v_at = k_at + kStages * kCodeBytes;
-  static constexpr uint32_t scales = v_at + kStages * kCodeBytes;  // [ring][group] {key scale, log2 value scale, reciprocal}
+  static constexpr uint32_t scales = v_at + kStages * kCodeBytes;  // [ring][group] {key scale, log2 value scale, its reciprocal x kLower}
   static constexpr uint32_t nan_bits = scales + kScaleRing * kGroups * 16u;  // [stage][slot][8 pieces] 16 columns each
   static constexpr uint32_t row_nan = nan_bits + kStages * kStep * 16u;      // [256 rows] the columns that are NaN
   static constexpr uint32_t kSmem = row_nan + kPromptRows * 16u + 1024u;
@@ -287,9 +290,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
         } else if (__builtin_expect(__any_sync(0xffffffffu, now > m + kSlack), 0)) {
           wait(&pv_full[half][(steps - 1u) & 1u], ((steps - 1u) >> 1) & 1u);  // the sums of the step before are in O
           tc_fence_after();
-          const float fade = exp2_fast(m - (now == -CUDART_INF_F ? 0.f : now));
+          const float root = exp2_fast(0.5f * (m - (now == -CUDART_INF_F ? 0.f : now))), fade = root * root;
           m = now;
-          l *= fade;
+          l = l * root * root;
 #pragma unroll 1
           for (uint32_t i = 0; i < DP / 16u; ++i) {
             float v[16];
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           }
         }
         // ---- powers, over S
-        const float base = kCarry - (m == -CUDART_INF_F ? 0.f : m);
+        const float base = kCarry + kRaise - (m == -CUDART_INF_F ? 0.f : m);
 #pragma unroll
         for (uint32_t i = 0; i < 2u; ++i) {
           uint32_t out[16];
@@ -316,9 +319,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
 #pragma unroll
             for (uint32_t e = 0; e < 16u; e += 2u) {
               const float2 y = split(fma(f2(__uint_as_float(s[i][16u * h + e]), __uint_as_float(s[i][16u * h + e + 1u])), by2, plus2));
-              const float2 x = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-              sum = sum + f2(x.x, x.y);
-              out[8u * h + e / 2u] = pack2(x.x, x.y, __half());
+              const F2 x = f2(exp2_fast(y.x), exp2_fast(y.y));
+              sum = sum + x;
+              const float2 power = split(x * f2(kLower, kLower));
+              out[8u * h + e / 2u] = pack2(power.x, power.y, __half());
             }
             const float2 z = split(sum);
             l = fmaf(z.x + z.y, sc.z, l);
@@ -422,7 +426,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
           for (uint32_t i = 0; i < count; ++i) most = fmaxf(most, __ldcg(record_of(i) + row));
           const float from = most == -CUDART_INF_F ? 0.f : most;
           for (uint32_t i = 0; i < count; ++i) {
-            all = fmaf(__ldcg(record_of(i) + kHalf + row), exp2_fast(__ldcg(record_of(i) + row) - from), all);
+            const float root = exp2_fast(0.5f * (__ldcg(record_of(i) + row) - from));
+            all = fmaf(__ldcg(record_of(i) + kHalf + row) * root, root, all);
           }
           const float by = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll 1
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt8_kernel(const Paged8
       if (round != 0u) wait(&k_empty[stage], (round - 1u) & 1u);
       if (lane == 0u) {
         const float to = fminf(fmaxf(vs, 0x1p-60f), 0x1p60f);
-        reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + group] = make_float4(ks, log2f(to), 1.f / to, 0.f);
+        reinterpret_cast<float4*>(smem + Shape::scales)[ring * kGroups + group] = make_float4(ks, log2f(to), kLower / to, 0.f);
       }
       store(tile, kw);
       if (lane == 0u) {

@@ -455,3 +455,37 @@ def test_attend_refuses_bad_workspaces():
     assert qgemv_b200.call(*size, 4, 2, None) == INVALID_VALUE
     a.tokens = 0
     assert qgemv_b200.call("qg_paged_attn8", ctypes.byref(c), ctypes.byref(a), 256, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])  # fp16 does not hold such values
+@pytest.mark.parametrize("dim,group,rows", [(64, 2, 0), (128, 8, 0), (64, 2, 7), (128, 4, 5), (256, 1, 3), (64, 2, 30), (128, 8, 9)])
+def test_values_at_both_ends_of_the_scales(cuda, dim, group, rows, dtype):
+    """One block of the largest scale among 65520 slots of the least one, zeros and others: slots that weigh
+    2^-12 to 2^-40 of one of the block's add up to a part of the softmax's sum, wherever the block lies.
+    `rows` 0 is a call without offsets."""
+    rng = np.random.default_rng(dim + group + rows)
+    n, block, new = 65536, 16, max(rows, 1)
+    table = int32([rng.permutation(n // 64).tolist()])
+    code = lambda x: x.to(torch.float8_e4m3fn)  # noqa: E731
+    scale = torch.full((2, n // 64, 1, 4), 1.0, device="cuda")
+    scale[1] = 2.0 ** -60
+    keys = torch.zeros(n // 64, 1, 64, dim, device="cuda")
+    keys[..., 1] = torch.randint(-2, 3, keys.shape[:-1], device="cuda")
+    for first in (0, n // 2, n - 64):
+        page = int(table[0, first // 64])
+        for small in (0.0, 50.0):
+            k, s = keys.clone(), scale.clone()
+            v = torch.randn(keys.shape, device="cuda") * small
+            k[page, 0, :block, 0], s[1, page, 0, 0] = 16.0, 2.0 ** 60
+            v[page, 0, :block] = torch.randn(block, dim, device="cuda") * 100
+            c = paged8.PagedCache8(code(k), code(v.clamp(-448, 448)), *s, table)
+            plan = paged8.AttentionPlan8(c, group, max_tokens=new)
+            for powers in (0, 12, 18, 23, 40):
+                q = torch.zeros(new, group, dim, dtype=DTYPES[dtype], device="cuda")
+                q[..., 0] = powers * np.log(2) * dim ** 0.5 / 16
+                q[..., 1] = torch.from_numpy(rng.standard_normal((new, group)))
+                off = offsets([rows]) if rows else None
+                out, lse = paged8.attend(plan, q, int32([n]), offsets=off, return_lse=True)
+                check(c, q, [n], [new], out, lse)
+    assert ops.get_error() == 0
