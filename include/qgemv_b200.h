@@ -711,9 +711,10 @@ cudaError_t qg_kv_read8(const qg_kv_pages8* cache, const qg_read8* r, cudaStream
  * q, out: [tokens][n_q_heads][head_dim] with row strides in elements (multiples of 16 bytes),
  * 16-B aligned; lse [tokens][n_q_heads] or NULL; rows of no sequence are left alone.
  * fp32 queries enter the products as sums of two fp16 terms (22 bits) and so do probabilities; 16-bit
- * queries exactly, or as far as 2^-25 of their row's largest value, and probabilities, where a call has
- * more than 8 rows for a kv head, in fp16 (11 bits).  Statistics and sums are fp32; results are
- * deterministic.  The pools' strides nest as in qg_paged_attn.  `workspace` as there:
+ * queries exactly, or as far as 2^-25 of their row's largest value, their probabilities in two terms too where
+ * a call without offsets has at most 8 query heads a kv head, or one with offsets at most 8 rows for a kv head
+ * (tokens times those heads, all sequences counted), else in fp16 (11 bits).  So a token can get other bits in a
+ * call with offsets than in one without.  Statistics and sums are fp32; results are deterministic.  The pools' strides nest as in qg_paged_attn.  `workspace` as there:
  * qg_paged_attn8_workspace_bytes long for the same cache, heads and at least as many tokens, its
  * first QG_PAGED_ATTN_ZEROED bytes zero before its first use; calls that overlap need one each. */
 typedef struct qg_attn8 {

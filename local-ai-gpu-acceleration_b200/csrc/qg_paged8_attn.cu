@@ -34,9 +34,10 @@
 // 85 us (34); 256 x 300, 32/8 heads: 50 us (25); 1 x 511: 12.6 us, all latency.  Two warps a scheduler (255 registers) issue in 40% of the
 // cycles; the rest is the latency of their chains.
 //
-// Rows.  fp32 queries, and any where a kv head has at most 8 rows: eight rows fill rows 0-7 of the A
-// operand and their fp16 errors rows 8-15 (22 bits), probabilities alike.  16-bit queries of more
-// rows: 16 rows whole, probabilities rounded to fp16 once (11 bits, the output's own precision).
+// Rows.  fp32 queries, and any in a call without offsets of at most 8 query heads a kv head or with offsets of
+// at most 8 rows for a kv head in all: eight rows fill rows 0-7 of the A operand and their fp16 errors rows
+// 8-15 (22 bits), probabilities alike.  Other calls with 16-bit queries: 16 rows whole, probabilities rounded
+// to fp16 once (11 bits, the output's own precision).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -1092,9 +1093,9 @@ extern "C" cudaError_t qg_paged_attn8(const qg_kv_pages8* cache, const qg_attn8*
   }
   PoolStrides8 strides;
   if (!pool_strides8(cache, &strides)) return cudaErrorInvalidValue;
-  // rows of a kv head: a call of one row a sequence has its group
+  // rows of a kv head: a call of one row a sequence has its group; of a ragged call only the sum is known here
   const uint32_t group = p->n_q_heads / c.c.n_kv;
-  const bool few = p->offsets == nullptr && group <= 8u, wide = p->dtype == QG_F32;
+  const bool few = (p->offsets == nullptr ? 1ull : p->tokens) * group <= 8u, wide = p->dtype == QG_F32;
   const uint32_t rs = few || (wide && plan.dp == 256u) ? 1u : 2u, terms = few || wide ? 2u : 1u;
   // a box is part of one tile and page
   const uint32_t log_tile = log_tile8(plan.dp, rs, terms);

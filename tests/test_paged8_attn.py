@@ -489,3 +489,34 @@ def test_values_at_both_ends_of_the_scales(cuda, dim, group, rows, dtype):
                 out, lse = paged8.attend(plan, q, int32([n]), offsets=off, return_lse=True)
                 check(c, q, [n], [new], out, lse)
     assert ops.get_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_few_rows_keep_22_bits(cuda, dim, dtype):
+    """Calls of at most 8 rows for a kv head, with and without offsets: two slots whose values cancel but for the
+    difference of their probabilities, which fp16 probabilities would round to 2^-12 of the values.  The head's
+    bound without its fp16 term."""
+    rng = np.random.default_rng(dim)
+    cache_rng = np.random.default_rng(dim)
+    for group, seqs, ragged in ((1, 40, False), (8, 9, False), (5, 3, False), (1, 1, True), (1, 8, True), (4, 2, True), (8, 1, True)):
+        c = make_cache(cache_rng, seqs, 1, 32, 16, 2, dim, power=9)
+        c.k_scale.fill_(2.0 ** -6)
+        c.v_scale.fill_(1.0)
+        page = c.table[:, 0].long()
+        v = torch.randint(100, 400, (seqs, 2, dim), device="cuda").float().to(torch.float8_e4m3fn)
+        codes(c.v)[page, :, 0], codes(c.v)[page, :, 1] = codes(v), codes(v) ^ 0x80
+        q = queries(rng, seqs, 2 * group, dim, DTYPES[dtype], 0.5)
+        plan = paged8.AttentionPlan8(c, 2 * group, max_tokens=seqs)
+        out = paged8.attend(plan, q, int32([2] * seqs), offsets=offsets([1] * seqs) if ragged else None)
+        for b in range(seqs):
+            k, v = (logical(c, name, b, 2) for name in "kv")
+            qd = q[b].double().cpu().view(2, group, dim)
+            p = torch.softmax(torch.einsum("hgd,hjd->hgj", qd, k) * dim ** -0.5, -1)
+            want = torch.einsum("hgj,hjd->hgd", p, v)
+            ds = (qd.norm(dim=-1).max() * k.norm(dim=-1).max()).item() * dim ** -0.5 * 2.0 ** -20
+            tol = (2 * ds + 2.0 ** -16) * v.abs().max() + UNIT[q.dtype] * 1.01 * want.abs() + TINY[q.dtype]
+            off = (out[b].double().cpu().view(2, group, dim) - want).abs()
+            assert (off <= tol).all(), (group, seqs, ragged, b, (off / tol).max())
+    assert ops.get_error() == 0
