@@ -85,8 +85,10 @@ __global__ void __launch_bounds__(kReadThreads) read8_kernel(const Paged8View c,
     before += static_cast<uint32_t>(n);
     if (n < static_cast<int>(kReadThreads)) break;
   }
-  if (blockIdx.x == 0u && threadIdx.x == 0u && a.offsets[c.c.batch] > static_cast<int64_t>(a.tokens)) {
-    atomicOr(&g_error_word, QG_ERR_PAGE);
+  // offsets that do not ascend or lie outside the call; the look-ups below stay inside whatever they are
+  for (uint64_t b = piece0 + threadIdx.x; b < c.c.batch; b += static_cast<uint64_t>(gridDim.x) * kReadThreads) {
+    const int32_t o0 = a.offsets[b], o1 = a.offsets[b + 1u];
+    if (o0 < 0 || o1 < o0 || static_cast<uint32_t>(o1) > a.tokens) atomicOr(&g_error_word, QG_ERR_PAGE);
   }
   const uint32_t p = in0 + threadIdx.x, down = div_by(p, a.row_pieces);  // from the CTA's first row on
   const uint32_t row = row0 + down, in = p - down * a.row_pieces.d;

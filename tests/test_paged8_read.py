@@ -166,3 +166,22 @@ def test_read_rows_that_begin_on_16_bytes(cuda, dtype):
             assert torch.equal(out[:187], x[:187]) and (out[187:] == 9).all()
             assert (w[:, :lead] == 9).all() and (w[:, lead + 240:] == 9).all()
     assert ops.get_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [3, 300])
+def test_read_reports_offsets_that_do_not_ascend(cuda, batch):
+    """Wherever in the list they are: an offset below the one before it, below zero, or past the call's rows."""
+    rng = np.random.default_rng(9)
+    c = make_cache(rng, batch, 1, 32, 16, 1, 64)
+    starts, good = int32([0] * batch), np.arange(batch + 1) * 4
+    tokens = 4 * batch
+    paged8.read(c, starts, int32(good.tolist()), tokens)
+    assert ops.get_error() == 0
+    for at, value in ((1, 9), (1, -1), (1, tokens + 1), (batch - 1, 2), (batch // 2 + 1, tokens + 5), (batch, 0),
+                      (batch, tokens - 5), (batch, tokens + 1), (0, -1), (0, 5)):
+        off = good.copy()
+        off[at] = value
+        for rows in (tokens, 3):  # also where the call has fewer CTAs than sequences
+            paged8.read(c, starts, int32(off.tolist()), rows)
+            assert ops.get_error() == paged.QG_ERR_PAGE, (at, value, rows)
