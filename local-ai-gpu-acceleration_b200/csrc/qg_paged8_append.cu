@@ -528,6 +528,8 @@ extern "C" cudaError_t qg_qk_norm_rope_append8(const qg_kv_pages8* cache, const 
   // a sequence of n new tokens touches at most n / block + 2 blocks
   const uint64_t most = (static_cast<uint64_t>(p->tokens) >> c.log_block) + 2ull * std::min(p->tokens, cache->batch);
   a.block_tasks = static_cast<uint32_t>(std::min<uint64_t>(most, p->tokens));
+  // find_run() stops behind its task's sequences: one more task, so that what does not fit is reported of all
+  if (cache->batch > kThreads8) ++a.block_tasks;
   const bool halves = p->pairs == QG_PAIRS_HALVES;
   if (p->dtype == QG_F32) return launch_append8<float>(c, a, halves, stream);
   if (p->dtype == QG_F16) return launch_append8<__half>(c, a, halves, stream);

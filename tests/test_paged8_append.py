@@ -396,3 +396,26 @@ def test_append_one_row_a_sequence_equals_the_ragged_call(cuda, heads, dim, rot,
             assert torch.equal(codes(getattr(one, name)), codes(getattr(ragged, name)))
             assert torch.equal(getattr(one, name + "_scale"), getattr(ragged, name + "_scale"))
         assert ops.get_error() == paged.QG_ERR_PAGE | (paged.QG_ERR_POSITION if rot and i % 2 else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [16, 64])
+def test_append_reports_what_does_not_fit_behind_the_last_row(cuda, block):
+    """Many sequences, rows of the first three alone: offsets and lengths of the others are looked at too."""
+    rng = np.random.default_rng(8)
+    batch = 400
+    c = make_cache(rng, batch, 1, 64, block, 1, 64)
+    q, k, v = new_rows(rng, 3, 2, 1, 64, torch.float16)
+    pos = int32([0] * 3)
+    off, lens = np.array([0, 1, 2] + [3] * (batch - 2)), np.array([1, 1, 1] + [0] * (batch - 3))
+    paged8.qk_norm_rope_append(c, q, k, v, None, pos, int32(lens.tolist()), offsets=int32(off.tolist()))
+    assert ops.get_error() == 0
+    for at in (60, 127, 128, 129, 300, 399):
+        bad = off.copy()
+        bad[at] = 2
+        paged8.qk_norm_rope_append(c, q, k, v, None, pos, int32(lens.tolist()), offsets=int32(bad.tolist()))
+        assert ops.get_error() == paged.QG_ERR_PAGE, at
+        long = lens.copy()
+        long[at] = 65
+        paged8.qk_norm_rope_append(c, q, k, v, None, pos, int32(long.tolist()), offsets=int32(off.tolist()))
+        assert ops.get_error() == paged.QG_ERR_PAGE, at
