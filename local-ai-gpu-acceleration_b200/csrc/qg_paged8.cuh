@@ -12,7 +12,7 @@ struct Paged8View {
   PagedView c;                      // pools in bytes
   float *ks, *vs;
   uint64_t scale_page, scale_head;  // elements
-  uint32_t log_block, page_blocks;  // slots of a block, blocks of a page
+  uint32_t log_block;               // log2 of the slots of a block
 };
 
 constexpr int kLeastPower = -60, kMostPower = 60;   // of a block's scale
@@ -107,7 +107,6 @@ inline bool paged8_view(const qg_kv_pages8* c, Paged8View* out) {
   out->scale_page = c->scale_page_stride;
   out->scale_head = c->scale_head_stride;
   out->log_block = static_cast<uint32_t>(__builtin_ctz(c->block));
-  out->page_blocks = c->page_size >> out->log_block;
   return true;
 }
 

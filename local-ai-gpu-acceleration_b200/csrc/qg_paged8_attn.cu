@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kAttnThreads, Attn8Shape<DP, RS, TERMS>::kCtas
   constexpr int kMma = TERMS == 2 ? RS : 1;                 // products for a tile
   constexpr int kSteps = kTile / 16;                        // 16-slot steps
   constexpr uint32_t kChunks = DP / 16;                     // 16-dim chunks
-  constexpr uint32_t kSet = 32u / kSteps, kTiles = kEntries / kSteps;  // tiles looked up together; that are kept
+  constexpr uint32_t kSet = 32u / kSteps;                   // tiles looked up together
   const PagedView& c = cache.c;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
