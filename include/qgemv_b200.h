@@ -637,7 +637,8 @@ cudaError_t qg_kv_evict(const qg_kv_pages* cache, const qg_evict* e, cudaStream_
  * head * scale_head_stride + i of k_scale and v_scale.  Scales of blocks that hold slots of a
  * sequence lie between 2^-60 and 2^60, so the cache holds magnitudes up to 5e20 in steps down to
  * 1.7e-21; the append's are powers of two, the readers take any (qg_paged_attn8 takes a scale of
- * values outside that range as its end).
+ * values outside that range as its end; an append to a block that has another keeps it until it grows, and
+ * multiplies by its fp32 reciprocal).
  *
  * New rows.  A call has `tokens` rows, sequence after sequence: rows offsets[b] to
  * offsets[b + 1] - 1 ([batch + 1], ascending) are the new tokens of sequence b, rows before
@@ -706,15 +707,19 @@ cudaError_t qg_kv_read8(const qg_kv_pages8* cache, const qg_read8* r, cudaStream
  * last `window` and the first `sink`.  For query head h of kv head h / (n_q_heads / n_kv_heads)
  * out = softmax over the seen slots of (scale * q . k_j) times v_j, lse the log of the softmax's
  * sum, as in qg_paged_attn; out 0 and lse -inf where nothing is seen (rows of an empty sequence).
- * What a token does not see never reaches its row, whatever the codes and scales there; a NaN
- * code among the seen makes the row (key) or the column (value) NaN.
+ * What a token does not see never reaches its row, whatever the codes there and the scales of blocks that it
+ * sees nothing of; a NaN code among the seen makes the row (key) or the column (value) NaN.
  * q, out: [tokens][n_q_heads][head_dim] with row strides in elements (multiples of 16 bytes),
  * 16-B aligned; lse [tokens][n_q_heads] or NULL; rows of no sequence are left alone.
  * fp32 queries enter the products as sums of two fp16 terms (22 bits) and so do probabilities; 16-bit
  * queries exactly, or as far as 2^-25 of their row's largest value, their probabilities in two terms too where
  * a call without offsets has at most 8 query heads a kv head, or one with offsets at most 8 rows for a kv head
  * (tokens times those heads, all sequences counted), else in fp16 (11 bits).  So a token can get other bits in a
- * call with offsets than in one without.  Statistics and sums are fp32; results are deterministic.  The pools' strides nest as in qg_paged_attn.  `workspace` as there:
+ * call with offsets than in one without.  Probabilities enter the products times their block's value scale, with
+ * these bits down to 2^-21 (16-bit queries, many rows) or 2^-28 of the row's largest such product, with fewer
+ * below: an error is relative to 448 times the largest value scale among the blocks that the token sees any
+ * slot of, also where it sees only small codes of that block.  Statistics and sums are fp32 and hold scales
+ * of the whole range; results are deterministic.  The pools' strides nest as in qg_paged_attn.  `workspace` as there:
  * qg_paged_attn8_workspace_bytes long for the same cache, heads and at least as many tokens, its
  * first QG_PAGED_ATTN_ZEROED bytes zero before its first use; calls that overlap need one each. */
 typedef struct qg_attn8 {

@@ -4,7 +4,7 @@
 //
 // A block's codes depend on the largest of its new values and on the scale that it has, so the
 // unit of work for keys and values is what a call writes to one (block, kv head): a CTA holds
-// those rows in registers (in shared memory where they are more than one pass of its 16 to 32 rows),
+// those rows in registers (in shared memory where they are more than one pass of its 8 to 64 rows),
 // finds their maximum, and only then rounds.  Where the block was begun before and its scale
 // grows, the CTA also scales the block's other codes down, so that they stand for what they stood
 // for: scales are powers of two, so this moves exponents and rounds only what falls below e4m3's
@@ -14,10 +14,10 @@
 // a batch of heads a warp too, without the CTA's barrier: 256 sequences of 64/8 heads x 128 bf16 are
 // 640 CTAs and 10 us on the GPU, against 4608 and 25 us with a CTA for each block.
 //
-// Measured (B200, floor = bytes at 6.56 TB/s): 16384 tokens of 64/8 heads x 128 bf16, blocks of 64: 149 us
-// (floor 98); launched apart the queries took 110 us, 63% of the issue slots, and the blocks 42, a chain of
-// loads in CTAs of 3 to 4 us each.  32 tokens 2.9 us, 2047 of 32/8 x 80 17 us.  Several heads a CTA, one after
-// another, took 157 (2 heads) to 189 us (16).
+// Measured (B200, floor = bytes at 6.56 TB/s): 16384 tokens of 64/8 heads x 128 bf16, blocks of 64: 148 us
+// (floor 98); a launch of the queries alone takes 115 us, one of the blocks alone 41, a chain of loads in CTAs
+// of 3 to 4 us each.  32 tokens 2.9 us, 2047 of 32/8 x 80 17 us (queries 8, blocks 12).  Several heads a CTA, one
+// after another, took 157 (2 heads) to 189 us (16).
 //
 // A row lies in LPR lanes as in qg_paged_append.cu: pairs never leave a lane, the sum of
 // squares is log2(LPR) shuffles.
@@ -152,7 +152,7 @@ __device__ __forceinline__ void put8(uint8_t* to, const float (&x)[8], float by)
                                              float_to_codes(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
 }
 
-// ONE: a row a sequence (no offsets).  Five CTAs an SM: 16384 tokens took 155 us, 178 with four, 176 with six.
+// ONE: a row a sequence (no offsets).  Five CTAs an SM: 16384 tokens take 148 us, 173 with four, 169 with six.
 template <typename T, int LPR, bool HALVES, bool ONE>
 __global__ void __launch_bounds__(kThreads8, 5) append8_kernel(const Paged8View c, const Append8Args a) {
   constexpr uint32_t kSide = 32 / LPR;                 // rows side by side in a warp

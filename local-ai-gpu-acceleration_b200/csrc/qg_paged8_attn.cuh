@@ -114,6 +114,9 @@ constexpr size_t prompt8_bytes(uint32_t dp) {
 // 16-bit queries and heads up to 128 wide, where a sequence has `kPromptFrom` rows or more for a kv head on average;
 // us of this and of the other kernel, 16 sequences of 4000 slots (32/8 heads x 128): 16 rows 104 and 66, 32 rows 105
 // and 94, 64 rows 106 and 149, 512 rows 203 and 919; of 600 slots 43 and 44, 45 and 51, 45 and 70, 78 and 205.
+// The host knows the cache's sequences, not which of them have rows: the average is over all (over as many as
+// rows where those are fewer).  So a lone prompt in a large cache can miss this kernel: 1000 tokens of 4000 slots, 64/8
+// heads x 128, 175 us in a cache of up to 200 sequences, 746 in one of more.
 constexpr uint32_t kPromptFrom = 40;
 inline bool prompt8_fits(uint32_t dp, uint64_t tokens, uint32_t batch, uint32_t group) {
   return dp <= 128u && tokens * group >= static_cast<uint64_t>(kPromptFrom) * (tokens < batch ? tokens : batch);

@@ -11,7 +11,7 @@
 // M is the largest y so far, but only moved (and O scaled) when it has grown by 2^8: powers carry 2^7, so
 // they stay below fp16's largest value, and those down to 2^-21 of the largest keep 11 bits.  For the
 // softmax's sum they are 2^64 times as large (why is in qg_paged8_attn.cu); that costs 3% of the time.  A branch for
-// steps whose scales need it, in any of five forms, cost 5 to 13%.
+// steps whose scales need it cost 9 to 13% in four forms.
 //
 // Codes become fp16 once for 256 rows: seven warps take turns at 16 slots, load their codes into
 // registers a turn ahead, convert them and write them in panels of 64 dims, 128 swizzled bytes a slot.
@@ -24,8 +24,8 @@
 // instruction cache and took twice the time.
 //
 // Measured (B200): 4096 new tokens of 5600 slots, 64/8 heads x 128 bf16: 650 us, 733 TFLOP/s, 0.44 of what
-// cuBLAS reaches; a step takes about 3000 cycles, its products 1024.  Leaving out any one of the powers, the
-// products or the conversions saves under 8%: issuer, rows and codes each take about as long, by latency.
+// cuBLAS reaches; a step takes about 3100 cycles, its products 1024.  Leaving out any one of the powers, the
+// products or the conversions saved under 8%: issuer, rows and codes each take about as long, by latency.
 // 4 ragged prompts of 288 to 2500 tokens, 32/8 heads x 64, window 1000: 120 us.
 //
 // Work.  Segments, blocks, equal ranges for one CTA an SM, records and joins as in
